@@ -418,6 +418,40 @@ int lce_pad_rows(const void* src, int dtype, int64_t rows, int64_t cols, int64_t
 int lce_transpose_rows(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, void* dst, int64_t dst_ld,
                        void* stream);
 
+/*
+ * Distillation from a teacher's top logits.  No counterpart in the reference.  From version 1000 on.
+ *
+ *   z[n][v] = logit_scale * sum_h x[n][h] * W[h][v],  lse[n] = log sum_v exp z[n][v]
+ *   loss    = 1/R * sum_n (lse[n] + sum_k q[n][k] * (log q[n][k] - z[n][index[n][k]])),  R = rows with a target
+ *
+ * the mean over those rows of the divergence KL(q || softmax(z)), and its gradients.  The loss and the gradients take the kernels,
+ * the routes and the scratch bound of the loss against labels; logits reach memory no more than there.  (For a temperature T
+ * logit_scale is the student's factor over T.)
+ *
+ * lce_soft_targets makes the targets: entry k of row n is there if index[n * ld_index + k] >= 0 and its logit is not -inf; what
+ * other entries hold is not looked at.  q = the softmax of logits / temperature over a row's entries; entries of the same column
+ * are added up in the first of them.  Outputs, dense (N, K): out_index (the column, -1: no target) and out_q (0 there); y, N
+ * labels as the other calls take them: the column of a row's first entry, -1 for a row without any, V where an index is not below V.
+ *
+ * lce_distill takes these.  Rows whose y is -1 have dx == 0 and add nothing to dW or to R; a row with an index that is no column of
+ * the weight, or with a NaN or +inf among its logits, makes the loss NaN, as does R == 0 (both gradients are zeros then).
+ *   p          monitoring, z_reg and phases are 0; ignore_index is not looked at (-1 is taken); n_chunk, pack_rows and route as in
+ *              lce_forward_backward
+ *   K          1 <= K <= LCE_MAX_TARGETS, N * K < 2^31
+ *   grad_out   device pointer to 1 float, as in lce_forward_backward (may be NULL without gradients)
+ *   lse        out, N floats, as in lce_forward
+ *   loss       out, 1 float;  n_valid  out, 1 int64: R
+ *   dx, dw     out, either may be NULL
+ *   ws         lce_distill_workspace_bytes(p, K, dx or dw wanted) bytes: those of the loss and 4 bytes per entry
+ */
+#define LCE_MAX_TARGETS 1024
+int lce_soft_targets(int64_t N, int64_t K, int64_t V, const int64_t* index, int64_t ld_index, const void* logits, int logits_dtype,
+                     int64_t ld_logits, float temperature, int32_t* out_index, float* out_q, int64_t* y, void* stream);
+int lce_distill_workspace_bytes(const lce_problem* p, int64_t K, int32_t grads, size_t* bytes);
+int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const float* q, const int64_t* y, const void* x, const void* w,
+                const float* grad_out, float* lse, float* loss, int64_t* n_valid, void* dx, void* dw, void* ws, size_t ws_bytes,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

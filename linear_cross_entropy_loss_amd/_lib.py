@@ -21,6 +21,7 @@ GRADS_NONE, GRADS_LARGE, GRADS_SMALL, GRADS_NARROW = -1, 0, 1, 2  # gradient_ker
 W_HV, W_VH = 0, 1  # lce_problem.w_layout: weight stored (H, V) / (V, H) row-major
 LCE_EINVAL_SHAPE, LCE_EINVAL_DTYPE, LCE_EINVAL_ARG, LCE_EWORKSPACE, LCE_EHIP, LCE_ESTATIC = -1, -2, -3, -4, -5, -6
 STATIC_SCRATCH_BYTES = 64 << 20
+MAX_TARGETS = 1024  # lce_distill: targets of a row
 
 EXPORTS = (
     "lce_version",
@@ -42,6 +43,9 @@ EXPORTS = (
     "lce_stand_in",
     "lce_pad_rows",
     "lce_transpose_rows",
+    "lce_soft_targets",
+    "lce_distill_workspace_bytes",
+    "lce_distill",
 )
 
 _DTYPES = {torch.bfloat16: LCE_BF16, torch.float16: LCE_F16, torch.float32: LCE_F32}
@@ -135,6 +139,13 @@ def load():
     lib.lce_pad_rows.argtypes = [vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_int64, vp]
     lib.lce_transpose_rows.restype = ctypes.c_int
     lib.lce_transpose_rows.argtypes = lib.lce_pad_rows.argtypes
+    i32, i64 = ctypes.c_int32, ctypes.c_int64
+    lib.lce_soft_targets.restype = ctypes.c_int
+    lib.lce_soft_targets.argtypes = [i64, i64, i64, vp, i64, vp, ctypes.c_int, i64, ctypes.c_float, vp, vp, vp, vp]
+    lib.lce_distill_workspace_bytes.restype = ctypes.c_int
+    lib.lce_distill_workspace_bytes.argtypes = [P, i64, i32, ctypes.POINTER(sz)]
+    lib.lce_distill.restype = ctypes.c_int
+    lib.lce_distill.argtypes = [P, i64] + [vp] * 12 + [sz, vp]
     _lib = lib
     return lib
 
@@ -251,3 +262,9 @@ def forward_backward_plan(prob: LceProblem) -> tuple[int, int]:
     raise_for_status(lib.lce_forward_backward_plan(ctypes.byref(prob), ctypes.byref(n), ctypes.byref(r)),
                      "lce_forward_backward_plan")
     return int(n.value), int(r.value)
+
+
+def distill_workspace_bytes(prob: LceProblem, K: int, grads: bool) -> int:
+    b = ctypes.c_size_t(0)
+    raise_for_status(load().lce_distill_workspace_bytes(ctypes.byref(prob), int(K), int(grads), ctypes.byref(b)), "linear_distillation")
+    return b.value

@@ -24,7 +24,10 @@ size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 
 bool is16(int d) { return d == LCE_BF16 || d == LCE_F16; }
 
-int route_of(const lce_problem* p) { return p->route & ~(LCE_ROUTE_EXACT_SUMS | LCE_ROUTE_KEEP_LOGITS); }
+// A flag in the route of the problems that lce_distill plans: a row has several targets, which are put into the staged dz.
+constexpr int kSoftTargets = 1 << 30;
+bool soft(const lce_problem* p) { return (p->route & kSoftTargets) != 0; }
+int route_of(const lce_problem* p) { return p->route & ~(LCE_ROUTE_EXACT_SUMS | LCE_ROUTE_KEEP_LOGITS | kSoftTargets); }
 
 // The last plan of a kind that this thread made.  A call asks for its plan up to three times (whether the route covers the
 // problem, the workspace, the launches), and a training step for the same one as the step before; a plan follows from the
@@ -51,7 +54,7 @@ template <class Plan> struct LastPlan {
 constexpr int64_t kTileLimit = ((int64_t)1 << 31) / 256;  // bytes of a row
 
 int check(const lce_problem* p, bool backward) {
-  if (!p) return LCE_EINVAL_ARG;
+  if (!p || soft(p)) return LCE_EINVAL_ARG;  // (the flag is set after the check)
   if (p->N <= 0 || p->H <= 0 || p->V <= 0 || p->n_chunk <= 0) return LCE_EINVAL_SHAPE;
   // Any N, H, V; only the row strides are constrained (below).
   if (p->N > (int64_t)1 << 30 || p->V > (int64_t)1 << 30 || p->H > (int64_t)1 << 20) return LCE_EINVAL_SHAPE;
@@ -438,7 +441,7 @@ int make_plan_bwd(const lce_problem* p, BwdPlan* b, bool settled) {
 // would take with all they ask for.
 bool plan_narrow(const lce_problem* p, size_t budget, BwdPlan* b, bool* starved) {
   const int64_t tok = lce::pad_to(p->N, 128) / 128, voc = lce::pad_to(p->V, 128) / 128;
-  if (p->H > lce::kNarrowHidden || splits(p) || p->pack_rows == LCE_PACK_ALWAYS || p->max_workgroups != 0 || tok > 1 << 20 || voc > 1 << 20)
+  if (p->H > lce::kNarrowHidden || splits(p) || soft(p) || p->pack_rows == LCE_PACK_ALWAYS || p->max_workgroups != 0 || tok > 1 << 20 || voc > 1 << 20)
     return false;
   // The kernel reaches the rows of whole K tiles of a weight stored (H, V) by 32-bit offsets.  The caller's rows are short enough
   // (check); those of the copy of an fp32 weight, as wide as the vocabulary here, have to be: else slabs of it.
@@ -520,7 +523,8 @@ struct FusedPlan {
 // time at two of them, 13 % at eight.  bf16, ms a step, products / pass: N=8192, V=50304, H=768 2.03 / 2.17, 1024 2.48 /
 // 2.56, 1280 3.12 / 3.17, 1536 3.53 / 3.53, 2048 4.41 / 4.32; N=16384, V=131072 stored (V, H), H=768 9.46 / 10.13, 1024
 // 11.85 / 12.30, 1536 17.57 / 17.58; fp16, N=8192, V=50304, H=768 2.15 / 2.28, 1024 2.65 / 2.73, 1536 3.78 / 3.74.
-bool factors_in_gradients(const lce_problem* p) { return lce::padded_hidden(p->H) <= 1024; }
+// (Several targets a row: each would have its slice of the stage rewritten, so they are put in after the pass.)
+bool factors_in_gradients(const lce_problem* p) { return lce::padded_hidden(p->H) <= 1024 && !soft(p); }
 
 bool plan_fused_with(const lce_problem* p, bool lo8, bool settled, int64_t most_chunks, FusedPlan* f);
 constexpr int64_t kMostChunks = 1024;  // (lce_compact.hip counts the rows of so many)
@@ -955,7 +959,7 @@ int forward_impl(const lce_problem* p, const void* x, const void* w, const int64
 // Body of lce_forward_backward for a problem that plan_fused accepts.
 int fused_impl(const lce_problem* p, const FusedPlan& f, const void* x, const void* w, const int64_t* y,
                const float* grad_out, float* lse, float* out5, int64_t* n_valid, void* dx, void* dw, void* ws,
-               void* stream) {
+               void* stream, const lce::SoftTargets* targets = nullptr) {
   hipStream_t s = (hipStream_t)stream;
   char* base = (char*)ws;
   const PackPlan& k = f.k;
@@ -1102,6 +1106,12 @@ int fused_impl(const lce_problem* p, const FusedPlan& f, const void* x, const vo
     if ((dx || dw) && (ph & LCE_PHASE_BWD_DZ)) {
       e = f.kept ? lce::launch_stage_pairs(a, s) : f.factors ? lce::launch_stage_factors(a, s) : lce::launch_stage_scale(a, s);
       if (e != hipSuccess) return hip_fail(e, f.kept ? "stage_pairs" : f.factors ? "stage_factors" : "stage_scale");
+      if (targets != nullptr) {
+        lce::SoftTargets t = *targets;
+        t.row0 = row0;
+        e = lce::launch_soft_gradient(a, t, s);
+        if (e != hipSuccess) return hip_fail(e, "soft_gradient");
+      }
     }
     if (f.small) {
       lce::SmallGrads g = lce::plan_small_grads(a.N, p->H, p->V, products(p), f.small_blocks);
@@ -1132,11 +1142,185 @@ int fused_impl(const lce_problem* p, const FusedPlan& f, const void* x, const vo
   return LCE_OK;
 }
 
+// Body of lce_backward for a problem and its plan.
+int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const void* w, const int64_t* y, const float* lse,
+                  const int64_t* n_valid, const float* grad_out, void* dx, void* dw, void* ws, void* stream,
+                  const lce::SoftTargets* targets = nullptr) {
+  hipStream_t s = (hipStream_t)stream;
+  char* base = (char*)ws;
+
+  lce::BwdArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = x; a.w = w; a.y = y; a.lse = lse; a.n_valid = n_valid; a.grad_out = grad_out;
+  a.N = p->N; a.H = p->H; a.V = p->V;
+  a.Np = lce::padded_tokens(p->N); a.Hp = lce::padded_hidden(p->H);
+  a.ldx = p->ldx; a.ldw = p->ldw; a.lddx = p->lddx; a.lddw = p->lddw;
+  a.x_dtype = p->x_dtype; a.w_dtype = p->w_dtype; a.dx_dtype = p->dx_dtype; a.dw_dtype = p->dw_dtype;
+  a.w_vh = p->w_layout == LCE_W_VH;
+  a.ignore_index = p->ignore_index;
+  a.scale = p->logit_scale; a.z_reg = p->z_reg;
+  a.dx = dx; a.dw = dw;
+  // fp16 staging of dz: times 2^10, unless z_reg is so large that the factor 1 + 2 * z_reg * lse on top of it would
+  // leave fp16's range for ordinary logits (with the factor 2^10 in place bwd_dz clamps that factor to +-63, which
+  // |lse| < 992 never reaches at z_reg <= 1/32)
+  a.dz_shift = p->x_dtype == LCE_F16 && p->z_reg <= 0.03125f ? 10 : 0;
+  a.dz = base + b.dz;
+  a.dx_acc = b.slabs > 1 ? (float*)(base + b.dx_acc) : nullptr;
+  a.dx_part = b.parts_on ? (float*)(base + b.dx_part) : nullptr;
+  a.dw_part = b.parts_on ? (float*)(base + b.dw_part) : nullptr;
+  int rc = current_num_cus(&a.num_cus, p->max_workgroups, &a.small_wgs);
+  if (rc != LCE_OK) return rc;
+  a.live = lce::live_bands(logit_k_bytes(p));
+  const int ph = p->phases ? p->phases : ~0;
+
+  // Tokens with an ignored label have dz == 0: the kernels run on the other rows only, packed to the front.
+  const PackPlan& k = b.pack;
+  const bool pack = b.pack_on, x32 = p->x_dtype == LCE_F32;
+  const int64_t dxes = p->dx_dtype == LCE_F32 ? 4 : 2;
+  a.xc = base + k.xc;
+  a.ldxc = k.ldxc;
+  if (pack) {
+    a.n_rows = (const int64_t*)(base + k.n_rows);
+    a.perm = (const int*)(base + k.perm);
+    a.dxc = b.stage_dx ? base + b.dxc : nullptr;
+    a.lddxc = b.lddxc;
+    a.y = (const int64_t*)(base + k.yc);
+    a.lse = (const float*)(base + b.lse_c);
+  }
+  if ((pack || x32) && (ph & LCE_PHASE_PACK)) {
+    const int* perm = pack ? (const int*)(base + k.perm) : nullptr;
+    hipError_t e;
+    if (pack) {
+      e = lce::launch_compact_labels(y, p->N, p->ignore_index, (int*)(base + k.cnt), (int64_t*)(base + k.n_rows),
+                                     (int*)(base + k.perm), (int64_t*)(base + k.yc), s);
+      if (e != hipSuccess) return hip_fail(e, "compact_labels");
+    }
+    float* lse_c = pack ? (float*)(base + b.lse_c) : nullptr;
+    e = x32 ? lce::launch_gather_rows_split((const float*)x, p->ldx, p->H, perm, a.n_rows, p->N, base + k.xc, k.ldxc,
+                                            pack ? lse : nullptr, lse_c, a.num_cus, s)
+            : lce::launch_gather_rows(x, p->ldx * 2, p->H * 2, perm, a.n_rows, p->N, base + k.xc, k.ldxc * 2, lse, lse_c,
+                                      a.num_cus, s);
+    if (e != hipSuccess) return hip_fail(e, "gather_rows");
+  }
+  if (x32) {  // fp32 activations reach the tile kernels as copies in bf16 pairs, whether or not rows were dropped
+    a.x = a.xc;
+    a.ldx = a.ldxc;
+    a.x_dtype = lce::DT_PAIR;
+    a.x_lo = a.ldxc / 2;
+  }
+  a.dz_rows = a.Np;  // rows of the dz stage (BwdArgs::dz)
+
+  for (int64_t i = 0; i < b.slabs; ++i) {
+    a.v0 = i * b.vs;
+    a.vw = p->V - a.v0 < b.vs ? p->V - a.v0 : b.vs;   // columns of this slab that exist
+    a.vs = lce::pad_to(a.vw, 256);                    // its padded width: dz row stride and K extent of dx
+    a.dx_grid = a.num_cus;
+    a.dw_grid = a.num_cus;
+    hipError_t e;
+    if (p->w_dtype == LCE_F32) {
+      // dz and dx of this slab read a 16-bit copy of its columns of the fp32 weight
+      if ((ph & LCE_PHASE_BWD_DZ) || (dx && (ph & LCE_PHASE_BWD_DX))) {
+        e = a.w_vh ? lce::launch_convert_w_rows((const float*)w, p->ldw, p->H, a.v0, a.vw, base + b.w16, p->H,
+                                                compute_dtype(p), s)
+                   : lce::launch_convert_w_slab((const float*)w, p->ldw, p->H, a.v0, a.vw, base + b.w16, a.vs,
+                                                compute_dtype(p), s);
+        if (e != hipSuccess) return hip_fail(e, "convert_w");
+      }
+      a.w = base + b.w16; a.ldw = a.w_vh ? p->H : a.vs; a.w_dtype = compute_dtype(p); a.wv0 = a.v0; a.Vw = a.vw;
+    } else {
+      a.wv0 = 0; a.Vw = p->V;
+    }
+    a.first = i == 0;
+    a.last = i == b.slabs - 1;
+    const bool want_dx = dx && (ph & LCE_PHASE_BWD_DX), want_dw = dw && (ph & LCE_PHASE_BWD_DW);
+    if (b.narrow) {
+      lce::SmallGrads g = lce::plan_narrow_grads(p->N, p->H, p->V, b.small_blocks);
+      g.part = (float*)(base + b.dx_part);
+      e = lce::launch_bwd_narrow(a, g, want_dx, want_dw, s);
+      if (e != hipSuccess) return hip_fail(e, "bwd_narrow");
+      continue;
+    }
+    if (ph & LCE_PHASE_BWD_DZ) {
+      e = lce::launch_bwd_dz(a, s);
+      if (e != hipSuccess) return hip_fail(e, "bwd_dz");
+      if (targets != nullptr) {
+        e = lce::launch_soft_gradient(a, *targets, s);
+        if (e != hipSuccess) return hip_fail(e, "soft_gradient");
+      }
+    }
+    if (b.small) {
+      lce::SmallGrads g = lce::plan_small_grads(p->N, p->H, a.vw, products(p), b.small_blocks);
+      g.part = (float*)(base + b.dx_part);
+      e = lce::launch_bwd_grads_small(a, g, want_dx, want_dw, s);
+      if (e != hipSuccess) return hip_fail(e, "bwd_grads_small");
+      continue;
+    }
+    if (want_dx) {
+      e = lce::launch_bwd_dx(a, s);
+      if (e != hipSuccess) return hip_fail(e, "bwd_dx");
+    }
+    if (want_dw) {
+      e = lce::launch_bwd_dw(a, s);
+      if (e != hipSuccess) return hip_fail(e, "bwd_dw");
+    }
+  }
+  if (pack && dx && (ph & LCE_PHASE_BWD_DX)) {
+    // dropped tokens get exact zeros, staged packed rows go to their tokens (nothing to do if none was dropped)
+    hipError_t e = lce::launch_scatter_rows(a.dxc, b.lddxc * dxes, (const int*)(base + k.perm), a.n_rows, p->N, y,
+                                            p->ignore_index, dx, p->lddx * dxes, p->H * dxes, a.num_cus, s);
+    if (e != hipSuccess) return hip_fail(e, "scatter_rows");
+  }
+  return LCE_OK;
+}
+
+// What lce_distill keeps behind the workspace of the loss itself.
+struct DistillPlan {
+  bool grads, one_pass;
+  FusedPlan f;
+  BwdPlan b;
+  size_t out5, part, z, total;
+};
+
+int check_targets(int64_t N, int64_t K) {
+  if (K < 1 || K > lce::kMaxTargets) return LCE_EINVAL_SHAPE;
+  return N * K >= (int64_t)1 << 31 ? LCE_EINVAL_SHAPE : LCE_OK;  // (entries are counted in 32 bits)
+}
+
+// The problem as the loss's planners and kernels see it: labels are columns, -1 stands for none.
+lce_problem soft_problem(const lce_problem* p) {
+  lce_problem q = *p;
+  q.ignore_index = -1;
+  q.route |= kSoftTargets;
+  return q;
+}
+
+int plan_distill(const lce_problem* q, int64_t K, bool grads, DistillPlan* d) {
+  d->grads = grads;
+  d->one_pass = grads && plan_fused(q, &d->f);
+  size_t o;
+  if (d->one_pass) {
+    o = d->f.total;
+  } else {
+    o = plan_fwd(q).total;
+    if (grads) {
+      const int rc = plan_bwd(q, &d->b);
+      if (rc != LCE_OK) return rc;
+      if (d->b.total > o) o = d->b.total;
+    }
+  }
+  o = align_up(o);
+  d->out5 = o; o += 256;
+  d->part = o; o += align_up((size_t)lce::soft_loss_groups() * sizeof(double));
+  d->z = o; o += align_up((size_t)q->N * (size_t)K * 4);
+  d->total = o;
+  return LCE_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
-int lce_version(void) { return 901; }  // 0.9.1: lce_gradient_kernels
+int lce_version(void) { return 1000; }  // 0.10.0: lce_distill
 
 const char* lce_strerror(int status) {
   switch (status) {
@@ -1247,127 +1431,7 @@ int lce_backward(const lce_problem* p, const void* x, const void* w, const int64
   rc = plan_bwd(p, &b);
   if (rc != LCE_OK) return rc;
   if (!ws || ws_bytes < b.total || misaligned(ws)) return LCE_EWORKSPACE;
-  hipStream_t s = (hipStream_t)stream;
-  char* base = (char*)ws;
-
-  lce::BwdArgs a;
-  memset(&a, 0, sizeof(a));
-  a.x = x; a.w = w; a.y = y; a.lse = lse; a.n_valid = n_valid; a.grad_out = grad_out;
-  a.N = p->N; a.H = p->H; a.V = p->V;
-  a.Np = lce::padded_tokens(p->N); a.Hp = lce::padded_hidden(p->H);
-  a.ldx = p->ldx; a.ldw = p->ldw; a.lddx = p->lddx; a.lddw = p->lddw;
-  a.x_dtype = p->x_dtype; a.w_dtype = p->w_dtype; a.dx_dtype = p->dx_dtype; a.dw_dtype = p->dw_dtype;
-  a.w_vh = p->w_layout == LCE_W_VH;
-  a.ignore_index = p->ignore_index;
-  a.scale = p->logit_scale; a.z_reg = p->z_reg;
-  a.dx = dx; a.dw = dw;
-  // fp16 staging of dz: times 2^10, unless z_reg is so large that the factor 1 + 2 * z_reg * lse on top of it would
-  // leave fp16's range for ordinary logits (with the factor 2^10 in place bwd_dz clamps that factor to +-63, which
-  // |lse| < 992 never reaches at z_reg <= 1/32)
-  a.dz_shift = p->x_dtype == LCE_F16 && p->z_reg <= 0.03125f ? 10 : 0;
-  a.dz = base + b.dz;
-  a.dx_acc = b.slabs > 1 ? (float*)(base + b.dx_acc) : nullptr;
-  a.dx_part = b.parts_on ? (float*)(base + b.dx_part) : nullptr;
-  a.dw_part = b.parts_on ? (float*)(base + b.dw_part) : nullptr;
-  rc = current_num_cus(&a.num_cus, p->max_workgroups, &a.small_wgs);
-  if (rc != LCE_OK) return rc;
-  a.live = lce::live_bands(logit_k_bytes(p));
-  const int ph = p->phases ? p->phases : ~0;
-
-  // Tokens with an ignored label have dz == 0: the kernels run on the other rows only, packed to the front.
-  const PackPlan& k = b.pack;
-  const bool pack = b.pack_on, x32 = p->x_dtype == LCE_F32;
-  const int64_t dxes = p->dx_dtype == LCE_F32 ? 4 : 2;
-  a.xc = base + k.xc;
-  a.ldxc = k.ldxc;
-  if (pack) {
-    a.n_rows = (const int64_t*)(base + k.n_rows);
-    a.perm = (const int*)(base + k.perm);
-    a.dxc = b.stage_dx ? base + b.dxc : nullptr;
-    a.lddxc = b.lddxc;
-    a.y = (const int64_t*)(base + k.yc);
-    a.lse = (const float*)(base + b.lse_c);
-  }
-  if ((pack || x32) && (ph & LCE_PHASE_PACK)) {
-    const int* perm = pack ? (const int*)(base + k.perm) : nullptr;
-    hipError_t e;
-    if (pack) {
-      e = lce::launch_compact_labels(y, p->N, p->ignore_index, (int*)(base + k.cnt), (int64_t*)(base + k.n_rows),
-                                     (int*)(base + k.perm), (int64_t*)(base + k.yc), s);
-      if (e != hipSuccess) return hip_fail(e, "compact_labels");
-    }
-    float* lse_c = pack ? (float*)(base + b.lse_c) : nullptr;
-    e = x32 ? lce::launch_gather_rows_split((const float*)x, p->ldx, p->H, perm, a.n_rows, p->N, base + k.xc, k.ldxc,
-                                            pack ? lse : nullptr, lse_c, a.num_cus, s)
-            : lce::launch_gather_rows(x, p->ldx * 2, p->H * 2, perm, a.n_rows, p->N, base + k.xc, k.ldxc * 2, lse, lse_c,
-                                      a.num_cus, s);
-    if (e != hipSuccess) return hip_fail(e, "gather_rows");
-  }
-  if (x32) {  // fp32 activations reach the tile kernels as copies in bf16 pairs, whether or not rows were dropped
-    a.x = a.xc;
-    a.ldx = a.ldxc;
-    a.x_dtype = lce::DT_PAIR;
-    a.x_lo = a.ldxc / 2;
-  }
-  a.dz_rows = a.Np;  // rows of the dz stage (BwdArgs::dz)
-
-  for (int64_t i = 0; i < b.slabs; ++i) {
-    a.v0 = i * b.vs;
-    a.vw = p->V - a.v0 < b.vs ? p->V - a.v0 : b.vs;   // columns of this slab that exist
-    a.vs = lce::pad_to(a.vw, 256);                    // its padded width: dz row stride and K extent of dx
-    a.dx_grid = a.num_cus;
-    a.dw_grid = a.num_cus;
-    hipError_t e;
-    if (p->w_dtype == LCE_F32) {
-      // dz and dx of this slab read a 16-bit copy of its columns of the fp32 weight
-      if ((ph & LCE_PHASE_BWD_DZ) || (dx && (ph & LCE_PHASE_BWD_DX))) {
-        e = a.w_vh ? lce::launch_convert_w_rows((const float*)w, p->ldw, p->H, a.v0, a.vw, base + b.w16, p->H,
-                                                compute_dtype(p), s)
-                   : lce::launch_convert_w_slab((const float*)w, p->ldw, p->H, a.v0, a.vw, base + b.w16, a.vs,
-                                                compute_dtype(p), s);
-        if (e != hipSuccess) return hip_fail(e, "convert_w");
-      }
-      a.w = base + b.w16; a.ldw = a.w_vh ? p->H : a.vs; a.w_dtype = compute_dtype(p); a.wv0 = a.v0; a.Vw = a.vw;
-    } else {
-      a.wv0 = 0; a.Vw = p->V;
-    }
-    a.first = i == 0;
-    a.last = i == b.slabs - 1;
-    const bool want_dx = dx && (ph & LCE_PHASE_BWD_DX), want_dw = dw && (ph & LCE_PHASE_BWD_DW);
-    if (b.narrow) {
-      lce::SmallGrads g = lce::plan_narrow_grads(p->N, p->H, p->V, b.small_blocks);
-      g.part = (float*)(base + b.dx_part);
-      e = lce::launch_bwd_narrow(a, g, want_dx, want_dw, s);
-      if (e != hipSuccess) return hip_fail(e, "bwd_narrow");
-      continue;
-    }
-    if (ph & LCE_PHASE_BWD_DZ) {
-      e = lce::launch_bwd_dz(a, s);
-      if (e != hipSuccess) return hip_fail(e, "bwd_dz");
-    }
-    if (b.small) {
-      lce::SmallGrads g = lce::plan_small_grads(p->N, p->H, a.vw, products(p), b.small_blocks);
-      g.part = (float*)(base + b.dx_part);
-      e = lce::launch_bwd_grads_small(a, g, want_dx, want_dw, s);
-      if (e != hipSuccess) return hip_fail(e, "bwd_grads_small");
-      continue;
-    }
-    if (want_dx) {
-      e = lce::launch_bwd_dx(a, s);
-      if (e != hipSuccess) return hip_fail(e, "bwd_dx");
-    }
-    if (want_dw) {
-      e = lce::launch_bwd_dw(a, s);
-      if (e != hipSuccess) return hip_fail(e, "bwd_dw");
-    }
-  }
-  if (pack && dx && (ph & LCE_PHASE_BWD_DX)) {
-    // dropped tokens get exact zeros, staged packed rows go to their tokens (nothing to do if none was dropped)
-    hipError_t e = lce::launch_scatter_rows(a.dxc, b.lddxc * dxes, (const int*)(base + k.perm), a.n_rows, p->N, y,
-                                            p->ignore_index, dx, p->lddx * dxes, p->H * dxes, a.num_cus, s);
-    if (e != hipSuccess) return hip_fail(e, "scatter_rows");
-  }
-  return LCE_OK;
+  return backward_impl(p, b, x, w, y, lse, n_valid, grad_out, dx, dw, ws, stream);
 }
 
 int lce_unit_gradient(const float** out) {
@@ -1478,6 +1542,76 @@ int lce_forward_backward(const lce_problem* p, const void* x, const void* w, con
   rc = forward_impl(p, x, w, y, lse, out5, n_valid, ws, ws_bytes, stream);
   if (rc != LCE_OK || (!dx && !dw)) return rc;
   return lce_backward(p, x, w, y, lse, n_valid, grad_out, dx, dw, ws, ws_bytes, stream);
+}
+
+int lce_soft_targets(int64_t N, int64_t K, int64_t V, const int64_t* index, int64_t ld_index, const void* logits, int logits_dtype,
+                     int64_t ld_logits, float temperature, int32_t* out_index, float* out_q, int64_t* y, void* stream) {
+  if (N < 1 || N > (int64_t)1 << 30 || V < 1 || V > (int64_t)1 << 30) return LCE_EINVAL_SHAPE;
+  const int rc = check_targets(N, K);
+  if (rc != LCE_OK) return rc;
+  if (logits_dtype != LCE_BF16 && logits_dtype != LCE_F16 && logits_dtype != LCE_F32) return LCE_EINVAL_DTYPE;
+  if (!index || !logits || !out_index || !out_q || !y || ld_index < 0 || ld_logits < 0) return LCE_EINVAL_ARG;
+  if (!(temperature > 0.f) || temperature > 3.4e38f) return LCE_EINVAL_ARG;
+  const hipError_t e = lce::launch_soft_targets(index, ld_index, logits, logits_dtype, ld_logits, N, (int)K, V, temperature, out_index, out_q,
+                                                y, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "soft_targets");
+  return LCE_OK;
+}
+
+int lce_distill_workspace_bytes(const lce_problem* p, int64_t K, int32_t grads, size_t* bytes) {
+  int rc = check(p, grads != 0);
+  if (rc == LCE_OK) rc = check_targets(p->N, K);
+  if (rc != LCE_OK) return rc;
+  if (!bytes || p->monitoring || p->z_reg != 0.f || p->phases) return LCE_EINVAL_ARG;
+  const lce_problem q = soft_problem(p);
+  DistillPlan d;
+  rc = plan_distill(&q, K, grads != 0, &d);
+  if (rc == LCE_OK) *bytes = d.total;
+  return rc;
+}
+
+int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const float* q, const int64_t* y, const void* x, const void* w,
+                const float* grad_out, float* lse, float* loss, int64_t* n_valid, void* dx, void* dw, void* ws, size_t ws_bytes,
+                void* stream) {
+  const bool grads = dx || dw;
+  int rc = check(p, grads);
+  if (rc == LCE_OK) rc = check_targets(p->N, K);
+  if (rc != LCE_OK) return rc;
+  if (!x || !w || !y || !index || !q || !lse || !loss || !n_valid || (grads && !grad_out)) return LCE_EINVAL_ARG;
+  if (misaligned(x) || misaligned(w) || misaligned(dx) || misaligned(dw)) return LCE_EINVAL_ARG;
+  if (p->monitoring || p->z_reg != 0.f || p->phases) return LCE_EINVAL_ARG;
+  const lce_problem soft_p = soft_problem(p);
+  DistillPlan d;
+  rc = plan_distill(&soft_p, K, grads, &d);
+  if (rc != LCE_OK) return rc;
+  if (!ws || ws_bytes < d.total || misaligned(ws)) return LCE_EWORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  char* base = (char*)ws;
+  float* out5 = (float*)(base + d.out5);
+
+  lce::SoftLogits g;
+  memset(&g, 0, sizeof(g));
+  g.x = x; g.w = w; g.N = p->N; g.H = p->H; g.ldx = p->ldx; g.ldw = p->ldw;
+  g.x_dtype = p->x_dtype; g.w_dtype = p->w_dtype; g.w_vh = p->w_layout == LCE_W_VH; g.K = (int)K;
+  g.index = index; g.scale = p->logit_scale; g.z = (float*)(base + d.z);
+  hipError_t e = lce::launch_soft_logits(g, s);
+  if (e != hipSuccess) return hip_fail(e, "soft_logits");
+
+  lce::SoftTargets t;
+  memset(&t, 0, sizeof(t));
+  t.index = index; t.q = q; t.z = g.z; t.N = p->N; t.K = (int)K;
+  if (d.one_pass) {
+    rc = fused_impl(&soft_p, d.f, x, w, y, grad_out, lse, out5, n_valid, dx, dw, ws, stream, &t);
+  } else {
+    lce_problem fwd = soft_p;
+    fwd.route = p->route;
+    rc = forward_impl(&fwd, x, w, y, lse, out5, n_valid, ws, d.out5, stream);
+    if (rc == LCE_OK && grads) rc = backward_impl(&soft_p, d.b, x, w, y, lse, n_valid, grad_out, dx, dw, ws, stream, &t);
+  }
+  if (rc != LCE_OK) return rc;
+  e = lce::launch_soft_loss(t, y, lse, p->V, n_valid, (double*)(base + d.part), loss, s);
+  if (e != hipSuccess) return hip_fail(e, "soft_loss");
+  return LCE_OK;
 }
 
 }  // extern "C"

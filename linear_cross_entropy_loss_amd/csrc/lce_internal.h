@@ -482,6 +482,35 @@ inline SmallGrads plan_narrow_grads(int64_t N, int64_t H, int64_t V, int64_t mos
   g.us = 5.0 + (H <= 64 ? 3.2 : 4.6) * t;
   return g;
 }
+// Distillation (lce_distill.hip): K targets a row in the place of a label, [N][K] each, in the tokens' order.
+constexpr int kMaxTargets = 1024;
+struct SoftTargets {
+  const int* index;  // column, or -1: no target
+  const float* q;    // its probability (0 where there is none)
+  const float* z;    // the scaled logit there
+  int64_t N, row0;   // tokens; the first row of a chunk (rows that are not packed)
+  int K;
+};
+// z[n][k] = scale * x[n] . W[index[n][k]], w rounded to the type of x.
+struct SoftLogits {
+  const void* x;
+  const void* w;
+  int64_t N, H, ldx, ldw;
+  int x_dtype, w_dtype, w_vh, K;
+  const int* index;
+  float scale;
+  float* z;
+};
+hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const void* logits, int dtype, int64_t ld_logits, int64_t N, int K,
+                               int64_t V, float temperature, int* out_index, float* out_q, int64_t* y, hipStream_t s);
+hipError_t launch_soft_logits(const SoftLogits& a, hipStream_t s);
+// dz of the targets' columns of the slab or chunk that `a` describes, over what the label's kernels staged there.
+hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStream_t s);
+// part: soft_loss_groups() doubles.
+hipError_t launch_soft_loss(const SoftTargets& t, const int64_t* y, const float* lse, int64_t V, const int64_t* n_valid, double* part,
+                            float* loss, hipStream_t s);
+int soft_loss_groups();
+
 hipError_t launch_fwd_narrow(const FwdArgs& a, int64_t rows, hipStream_t s);
 hipError_t launch_bwd_narrow(const BwdArgs& a, const SmallGrads& g, bool want_dx, bool want_dw, hipStream_t s);
 hipError_t launch_bwd_grads_small(const BwdArgs& a, const SmallGrads& g, bool want_dx, bool want_dw, hipStream_t s);

@@ -781,5 +781,11 @@ class LinearCrossEntropyLoss(torch.nn.Linear):
             }
         return loss
 
+    def distill(self, x, index, logits, temperature: float = 1.0):
+        """Loss of ``x`` against a teacher's top logits (``linear_distillation``), with this module's weight and logit_scale."""
+        from .distillation import linear_distillation
+
+        return linear_distillation(x, self.weight, index, logits, temperature, self.logit_scale, self.N_chunk_size)
+
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias=False"
