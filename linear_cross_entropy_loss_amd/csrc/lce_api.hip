@@ -1308,6 +1308,9 @@ int plan_distill(const lce_problem* q, int64_t K, bool grads, DistillPlan* d) {
       if (d->b.total > o) o = d->b.total;
     }
   }
+  // (the scratch of the targets' logits is free again before the loss's kernels run)
+  const size_t sorting = lce::soft_logits_bytes(q->N, (int)K, q->V);
+  if (sorting > o) o = sorting;
   o = align_up(o);
   d->out5 = o; o += 256;
   d->part = o; o += align_up((size_t)lce::soft_loss_groups() * sizeof(double));
@@ -1591,10 +1594,10 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
 
   lce::SoftLogits g;
   memset(&g, 0, sizeof(g));
-  g.x = x; g.w = w; g.N = p->N; g.H = p->H; g.ldx = p->ldx; g.ldw = p->ldw;
+  g.x = x; g.w = w; g.N = p->N; g.H = p->H; g.V = p->V; g.ldx = p->ldx; g.ldw = p->ldw;
   g.x_dtype = p->x_dtype; g.w_dtype = p->w_dtype; g.w_vh = p->w_layout == LCE_W_VH; g.K = (int)K;
   g.index = index; g.scale = p->logit_scale; g.z = (float*)(base + d.z);
-  hipError_t e = lce::launch_soft_logits(g, s);
+  hipError_t e = lce::launch_soft_logits(g, base, s);
   if (e != hipSuccess) return hip_fail(e, "soft_logits");
 
   lce::SoftTargets t;

@@ -145,9 +145,13 @@ __global__ __launch_bounds__(64 * kTargetWaves) void soft_targets_kernel(const i
   }
 }
 
-// The student's logits at the teacher's columns, in fp32 from operands of the compute type.  A wave per entry.
+// The student's logits at the teacher's columns, in fp32 from operands of the compute type: z[e] = s x[n] . W[:, v] for every entry
+// e = (n, v).
+//
+// Few entries: a wave per entry.  A weight stored (H, V) then costs a line of 128 bytes for every element, which is what bounds it
+// (N=16384, K=64, H=2048: 31.7 ms).
 template <class XT, class WT, bool WVH>
-__global__ __launch_bounds__(256) void soft_logits_kernel(const SoftLogits a) {
+__global__ __launch_bounds__(256) void soft_logits_direct_kernel(const SoftLogits a) {
   const int lane = threadIdx.x & 63;
   for (int64_t e = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); e < a.N * a.K; e += (int64_t)gridDim.x * 4) {
     const int v = a.index[e];
@@ -162,6 +166,239 @@ __global__ __launch_bounds__(256) void soft_logits_kernel(const SoftLogits a) {
       z = wave_sum(z);
     }
     if (lane == 0) a.z[e] = z * a.scale;
+  }
+}
+
+// More: the entries are sorted by groups of 64 columns (one line of a 16-bit W), whose part of W then passes through LDS once for
+// all of them.  Counting sort: counts of every group, their prefix sums and from them the list of work items -- up to kItemEntries
+// entries of one group --, then the places.  The order within a group is not the same in every call; a logit does not depend on it.
+constexpr int kGroupCols = 64, kItemEntries = 256;
+constexpr int kSortThreads = 1024, kSortPer = 8;
+constexpr int64_t kSortedEntries = 16384;  // from here on
+constexpr int64_t kMostColGroups = 16384;  // counts of a workgroup: 64 KiB of LDS
+
+__global__ __launch_bounds__(kSortThreads) void soft_clear_kernel(int* counts, int groups) {
+  const int i = blockIdx.x * kSortThreads + threadIdx.x;
+  if (i < groups) counts[i] = 0;
+}
+
+__global__ __launch_bounds__(kSortThreads) void soft_count_kernel(const int* index, int64_t M, int* counts, int groups) {
+  extern __shared__ int sh_count[];
+  for (int g = threadIdx.x; g < groups; g += kSortThreads) sh_count[g] = 0;
+  __syncthreads();
+  const int64_t e0 = (int64_t)blockIdx.x * kSortThreads * kSortPer + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < kSortPer; ++i) {
+    const int64_t e = e0 + i * kSortThreads;
+    const int v = e < M ? index[e] : -1;
+    if (v >= 0) atomicAdd(&sh_count[v / kGroupCols], 1);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < groups; g += kSortThreads)
+    if (sh_count[g] != 0) atomicAdd(&counts[g], sh_count[g]);
+}
+
+// One workgroup: counts[] becomes its own exclusive prefix sum, items[] the list of work items (column group, first entry, entries),
+// *num_items their number.
+__global__ __launch_bounds__(kSortThreads) void soft_items_kernel(int* counts, int groups, int4* items, int* num_items) {
+  __shared__ int sh_entries[kSortThreads / 64], sh_items[kSortThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int entries_before = 0, items_before = 0;
+  for (int g0 = 0; g0 < groups; g0 += kSortThreads) {
+    const int g = g0 + threadIdx.x;
+    const int n = g < groups ? counts[g] : 0, m = (n + kItemEntries - 1) / kItemEntries;
+    int en = n, it = m;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int ue = __shfl_up(en, d), ui = __shfl_up(it, d);
+      if (lane >= d) {
+        en += ue;
+        it += ui;
+      }
+    }
+    if (lane == 63) {
+      sh_entries[wave] = en;
+      sh_items[wave] = it;
+    }
+    __syncthreads();
+    int be = entries_before, bi = items_before;
+    for (int w = 0; w < kSortThreads / 64; ++w) {
+      if (w < wave) {
+        be += sh_entries[w];
+        bi += sh_items[w];
+      }
+      entries_before += sh_entries[w];
+      items_before += sh_items[w];
+    }
+    __syncthreads();
+    const int first = be + en - n, item = bi + it - m;
+    if (g < groups) counts[g] = first;
+    for (int i = 0; i < m; ++i) {
+      const int left = n - i * kItemEntries;
+      items[item + i] = make_int4(g, first + i * kItemEntries, left < kItemEntries ? left : kItemEntries, 0);
+    }
+  }
+  if (threadIdx.x == 0) num_items[0] = items_before;
+}
+
+// entries[place] = (e, column); place: counts[group] and up, in stretches that a workgroup takes for its own entries.
+__global__ __launch_bounds__(kSortThreads) void soft_place_kernel(const int* index, int64_t M, int* counts, int groups, int2* entries) {
+  extern __shared__ int sh_count[];
+  for (int g = threadIdx.x; g < groups; g += kSortThreads) sh_count[g] = 0;
+  __syncthreads();
+  const int64_t e0 = (int64_t)blockIdx.x * kSortThreads * kSortPer + threadIdx.x;
+  int v[kSortPer], rank[kSortPer];
+#pragma unroll
+  for (int i = 0; i < kSortPer; ++i) {
+    const int64_t e = e0 + i * kSortThreads;
+    v[i] = e < M ? index[e] : -1;
+    if (v[i] >= 0) rank[i] = atomicAdd(&sh_count[v[i] / kGroupCols], 1);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < groups; g += kSortThreads)
+    if (sh_count[g] != 0) sh_count[g] = atomicAdd(&counts[g], sh_count[g]);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSortPer; ++i)
+    if (v[i] >= 0) entries[sh_count[v[i] / kGroupCols] + rank[i]] = make_int2((int)(e0 + i * kSortThreads), v[i]);
+}
+
+// a . b over the elements of 16 bytes, on top of c.
+template <class XT> LCE_DEV float dot16(u32x4_t a, u32x4_t b, float c);
+template <> LCE_DEV float dot16<__bf16>(u32x4_t a, u32x4_t b, float c) {
+  typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned ai = a[i], bi = b[i];
+    c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, ai), __builtin_bit_cast(pair_t, bi), c, false);
+  }
+  return c;
+}
+template <> LCE_DEV float dot16<_Float16>(u32x4_t a, u32x4_t b, float c) {
+  typedef _Float16 pair_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned ai = a[i], bi = b[i];
+    c = __builtin_amdgcn_fdot2(__builtin_bit_cast(pair_t, ai), __builtin_bit_cast(pair_t, bi), c, false);
+  }
+  return c;
+}
+template <> LCE_DEV float dot16<float>(u32x4_t a, u32x4_t b, float c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned ai = a[i], bi = b[i];
+    c = fmaf(__builtin_bit_cast(float, ai), __builtin_bit_cast(float, bi), c);
+  }
+  return c;
+}
+
+// to[0 .. n) = from[0 .. n) in the compute type, zeros from `valid` on.  from + n lies in the matrix where valid >= n; there the
+// address is one of 16 bytes.
+template <class XT, class WT, int n> LCE_DEV void load_as(XT (&to)[n], const WT* from, int64_t valid) {
+  if (valid >= n) {
+    WT raw[n];
+    constexpr int kPer = 16 / sizeof(WT);
+#pragma unroll
+    for (int i = 0; i < n / kPer; ++i) {
+      const u32x4_t v = reinterpret_cast<const u32x4_t*>(from)[i];
+      __builtin_memcpy(raw + i * kPer, &v, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < n; ++i) to[i] = (XT)raw[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i) to[i] = i < valid ? (XT)from[i] : (XT)0.f;
+  }
+}
+
+// A workgroup per item: the 64 columns of W come through LDS 128 bytes of each at a time (64 or 32 hidden indices), and eight lanes
+// take such a stretch of one entry's row of x, a whole line, against the entry's column: 32 entries at a time, eight times.  The
+// column's line is read by eight neighbouring lanes, which meets every bank once.
+//   Traffic: W once for every 256 entries of a group, 2 H bytes for every entry, from the caches where x fits those.
+template <class XT, class WT, bool WVH>
+__global__ __launch_bounds__(256) void soft_logits_kernel(const SoftLogits a, const int4* items, const int* num_items, const int2* entries) {
+  constexpr int kPiece = 16 / sizeof(XT), kDeep = 8 * kPiece;  // elements of a lane's piece, of a stretch
+  constexpr int kSets = kItemEntries / 32;
+  __shared__ __attribute__((aligned(16))) XT tile[2][kGroupCols * kDeep];
+  if ((int)blockIdx.x >= num_items[0]) return;
+  const int4 item = items[blockIdx.x];
+  const int t = threadIdx.x, j = t & 7;
+  const XT* x[kSets];
+  int column[kSets];
+  float z[kSets];
+#pragma unroll
+  for (int g = 0; g < kSets; ++g) {
+    const int at = g * 32 + (t >> 3);
+    const int2 e = entries[item.y + (at < item.z ? at : 0)];
+    x[g] = reinterpret_cast<const XT*>(a.x) + e.x / a.K * a.ldx + j * kPiece;
+    column[g] = (e.y & (kGroupCols - 1)) * kDeep + j * kPiece;
+    z[g] = 0.f;
+  }
+  const WT* w = reinterpret_cast<const WT*>(a.w);
+  const int64_t v0 = (int64_t)item.x * kGroupCols;
+  // (V, H): thread = quarter of a column's stretch; (H, V): thread = eight columns of one or two hidden indices
+  constexpr int kRows = kDeep / 32, kOfW = WVH ? kDeep / 4 : 8;
+  XT part[WVH ? 1 : kRows][kOfW];
+  auto fetch = [&](int64_t h0) {
+    if constexpr (WVH) {
+      const int64_t v = v0 + (t >> 2), h = h0 + (t & 3) * kOfW;
+#pragma unroll
+      for (int i = 0; i < kOfW; i += kPiece) {
+        XT some[kPiece];
+        load_as<XT, WT, kPiece>(some, w + v * a.ldw + h + i, v < a.V ? a.H - h - i : 0);
+#pragma unroll
+        for (int u = 0; u < kPiece; ++u) part[0][i + u] = some[u];
+      }
+    } else {
+      const int64_t v = v0 + (t >> 5) * 8;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int64_t h = h0 + (t & 31) * kRows + r;
+        load_as<XT, WT, 8>(part[r], w + h * a.ldw + v, h < a.H ? a.V - v : 0);
+      }
+    }
+  };
+  fetch(0);
+  int buffer = 0;
+  for (int64_t h0 = 0; h0 < a.H; h0 += kDeep, buffer ^= 1) {
+    u32x4_t piece[kSets];
+#pragma unroll
+    for (int g = 0; g < kSets; ++g)
+      if (g * 32 < item.z) {
+        XT some[kPiece];
+        load_as<XT, XT, kPiece>(some, x[g] + h0, a.H - h0 - j * kPiece);
+        __builtin_memcpy(&piece[g], some, 16);
+      }
+    if constexpr (WVH) {
+#pragma unroll
+      for (int i = 0; i < kOfW; i += kPiece) {
+        u32x4_t v;
+        __builtin_memcpy(&v, &part[0][i], 16);
+        *reinterpret_cast<u32x4_t*>(&tile[buffer][(t >> 2) * kDeep + (t & 3) * kOfW + i]) = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        XT both[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) both[r] = part[r][i];
+        unsigned v;
+        __builtin_memcpy(&v, both, 4);
+        *reinterpret_cast<unsigned*>(&tile[buffer][((t >> 5) * 8 + i) * kDeep + (t & 31) * kRows]) = v;
+      }
+    }
+    if (h0 + kDeep < a.H) fetch(h0 + kDeep);
+    __syncthreads();  // (the other buffer is written next: by then every wave is past this one's reads of the round before)
+#pragma unroll
+    for (int g = 0; g < kSets; ++g)
+      if (g * 32 < item.z) z[g] = dot16<XT>(piece[g], *reinterpret_cast<const u32x4_t*>(&tile[buffer][column[g]]), z[g]);
+  }
+#pragma unroll
+  for (int g = 0; g < kSets; ++g) {
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) z[g] += __shfl_xor(z[g], d);
+    const int at = g * 32 + (t >> 3);
+    if (j == 0 && at < item.z) a.z[entries[item.y + at].x] = z[g] * a.scale;
   }
 }
 
@@ -225,11 +462,48 @@ __global__ __launch_bounds__(64) void soft_loss_sum_kernel(const double* part, i
   if (threadIdx.x == 0) loss[0] = (float)(sum / (double)n_valid[0]);
 }
 
-template <class XT, class WT> void launch_logits(const SoftLogits& a, hipStream_t s) {
-  const int64_t groups = (a.N * a.K + 3) / 4;
-  const dim3 grid((unsigned)(groups < kMostGroups ? groups : kMostGroups));
-  if (a.w_vh) hipLaunchKernelGGL((soft_logits_kernel<XT, WT, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((soft_logits_kernel<XT, WT, false>), grid, dim3(256), 0, s, a);
+// Scratch of the sorted kernels, after `base`: counts, number of items, items, entries.
+struct SortPlan {
+  bool sorted;
+  int groups;
+  int64_t most_items;
+  size_t num_items, items, entries, total;
+};
+SortPlan plan_sort(int64_t N, int K, int64_t V) {
+  SortPlan p;
+  const int64_t M = N * K, groups = (V + kGroupCols - 1) / kGroupCols;
+  auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+  p.sorted = M >= kSortedEntries && groups <= kMostColGroups;
+  p.groups = (int)(groups <= kMostColGroups ? groups : 0);
+  p.most_items = groups + M / kItemEntries;
+  p.num_items = up((size_t)p.groups * 4);
+  p.items = p.num_items + 256;
+  p.entries = p.items + up((size_t)p.most_items * sizeof(int4));
+  p.total = p.sorted ? p.entries + up((size_t)M * sizeof(int2)) : 0;
+  return p;
+}
+
+template <class XT, class WT, bool WVH> hipError_t launch_logits(const SoftLogits& a, void* ws, hipStream_t s) {
+  const SortPlan p = plan_sort(a.N, a.K, a.V);
+  const int64_t M = a.N * a.K;
+  if (!p.sorted) {
+    const int64_t groups = (M + 3) / 4;
+    hipLaunchKernelGGL((soft_logits_direct_kernel<XT, WT, WVH>), dim3((unsigned)(groups < kMostGroups ? groups : kMostGroups)), dim3(256), 0,
+                       s, a);
+    return hipGetLastError();
+  }
+  char* base = reinterpret_cast<char*>(ws);
+  int* counts = reinterpret_cast<int*>(base);
+  int* num_items = reinterpret_cast<int*>(base + p.num_items);
+  int4* items = reinterpret_cast<int4*>(base + p.items);
+  int2* entries = reinterpret_cast<int2*>(base + p.entries);
+  const dim3 grid((unsigned)((M + kSortThreads * kSortPer - 1) / (kSortThreads * kSortPer))), block(kSortThreads);
+  hipLaunchKernelGGL(soft_clear_kernel, dim3((unsigned)((p.groups + kSortThreads - 1) / kSortThreads)), block, 0, s, counts, p.groups);
+  hipLaunchKernelGGL(soft_count_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups);
+  hipLaunchKernelGGL(soft_items_kernel, dim3(1), block, 0, s, counts, p.groups, items, num_items);
+  hipLaunchKernelGGL(soft_place_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups, entries);
+  hipLaunchKernelGGL((soft_logits_kernel<XT, WT, WVH>), dim3((unsigned)p.most_items), dim3(256), 0, s, a, items, num_items, entries);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -251,14 +525,19 @@ hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const voi
   return hipGetLastError();
 }
 
-hipError_t launch_soft_logits(const SoftLogits& a, hipStream_t s) {
-  if (a.x_dtype == DT_BF16 && a.w_dtype == DT_BF16) launch_logits<__bf16, __bf16>(a, s);
-  else if (a.x_dtype == DT_BF16 && a.w_dtype == DT_F32) launch_logits<__bf16, float>(a, s);
-  else if (a.x_dtype == DT_F16 && a.w_dtype == DT_F16) launch_logits<_Float16, _Float16>(a, s);
-  else if (a.x_dtype == DT_F16 && a.w_dtype == DT_F32) launch_logits<_Float16, float>(a, s);
-  else if (a.x_dtype == DT_F32 && a.w_dtype == DT_F32) launch_logits<float, float>(a, s);
-  else return hipErrorInvalidValue;
-  return hipGetLastError();
+size_t soft_logits_bytes(int64_t N, int K, int64_t V) { return plan_sort(N, K, V).total; }
+
+hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s) {
+  if (a.x_dtype == DT_BF16 && a.w_dtype == DT_BF16)
+    return a.w_vh ? launch_logits<__bf16, __bf16, true>(a, ws, s) : launch_logits<__bf16, __bf16, false>(a, ws, s);
+  if (a.x_dtype == DT_BF16 && a.w_dtype == DT_F32)
+    return a.w_vh ? launch_logits<__bf16, float, true>(a, ws, s) : launch_logits<__bf16, float, false>(a, ws, s);
+  if (a.x_dtype == DT_F16 && a.w_dtype == DT_F16)
+    return a.w_vh ? launch_logits<_Float16, _Float16, true>(a, ws, s) : launch_logits<_Float16, _Float16, false>(a, ws, s);
+  if (a.x_dtype == DT_F16 && a.w_dtype == DT_F32)
+    return a.w_vh ? launch_logits<_Float16, float, true>(a, ws, s) : launch_logits<_Float16, float, false>(a, ws, s);
+  if (a.x_dtype == DT_F32 && a.w_dtype == DT_F32 && !a.w_vh) return launch_logits<float, float, false>(a, ws, s);
+  return hipErrorInvalidValue;
 }
 
 hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStream_t s) {

@@ -495,7 +495,7 @@ struct SoftTargets {
 struct SoftLogits {
   const void* x;
   const void* w;
-  int64_t N, H, ldx, ldw;
+  int64_t N, H, V, ldx, ldw;
   int x_dtype, w_dtype, w_vh, K;
   const int* index;
   float scale;
@@ -503,7 +503,8 @@ struct SoftLogits {
 };
 hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const void* logits, int dtype, int64_t ld_logits, int64_t N, int K,
                                int64_t V, float temperature, int* out_index, float* out_q, int64_t* y, hipStream_t s);
-hipError_t launch_soft_logits(const SoftLogits& a, hipStream_t s);
+size_t soft_logits_bytes(int64_t N, int K, int64_t V);  // scratch (may be 0)
+hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s);
 // dz of the targets' columns of the slab or chunk that `a` describes, over what the label's kernels staged there.
 hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStream_t s);
 // part: soft_loss_groups() doubles.
