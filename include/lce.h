@@ -452,6 +452,40 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
                 const float* grad_out, float* lse, float* loss, int64_t* n_valid, void* dx, void* dw, void* ws, size_t ws_bytes,
                 void* stream);
 
+/*
+ * Selections from rows of logits that are in memory (row stride ld in elements, any; rows at any element boundary).  No
+ * counterpart in the reference.  The order of a row: value descending, equal values by column (-0 equals 0; NaN comes first).
+ * 0 <= rows <= 2^30, 1 <= cols <= 2^30; with no rows nothing is done.  From version 1000 on.
+ *
+ * lce_top_logits: the first k of each row, 1 <= k <= min(cols, LCE_MAX_TARGETS): values (rows, k) in the type of the logits, index
+ * (rows, k), and -- lse not NULL -- log sum exp of the whole row (-inf where all are, NaN where one is).  What lce_soft_targets
+ * reads of a teacher.
+ *
+ * lce_sample: one token a row from the uniform number u[row] in [0, 1).  With w[j] = exp((z[j] - max z) / temperature), summed in 64
+ * bits, in the order above:
+ *   top_k   (0: all) keeps the first k
+ *   top_p   (1: all) keeps column j while sum_{i<j} w[i] < top_p * the sum over what top_k kept
+ *   min_p   (0: all) keeps the columns with w >= min_p
+ * each of them the first column at least, and of what all three keep the token is the first column whose sum of w up to and
+ * with it exceeds u * the whole sum.  temperature 0: the first column.  Columns of -inf are never drawn; a row of nothing else, or
+ * with a NaN, gives -1.  Settings by row (a pointer that is not NULL) replace the number; there top_k <= 0, top_p >= 1 or NaN and
+ * min_p <= 0 or NaN keep all, top_p <= 0 keeps the first column, and a temperature that is not positive stands for 0.
+ */
+typedef struct lce_sampling {
+  float temperature; /* 0 <= temperature < inf */
+  float top_p;       /* 0 < top_p <= 1         */
+  float min_p;       /* 0 <= min_p <= 1        */
+  int64_t top_k;     /* >= 0                   */
+  const float* temperature_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  const int64_t* top_k_rows;
+} lce_sampling;
+int lce_top_logits(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, int64_t k, void* values, int64_t* index, float* lse,
+                   void* stream);
+int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* u, const lce_sampling* s, int64_t* token,
+               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

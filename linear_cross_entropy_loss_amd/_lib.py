@@ -46,6 +46,8 @@ EXPORTS = (
     "lce_soft_targets",
     "lce_distill_workspace_bytes",
     "lce_distill",
+    "lce_top_logits",
+    "lce_sample",
 )
 
 _DTYPES = {torch.bfloat16: LCE_BF16, torch.float16: LCE_F16, torch.float32: LCE_F32}
@@ -76,6 +78,21 @@ class LceProblem(ctypes.Structure):
         ("max_workgroups", ctypes.c_int32),
         ("w_layout", ctypes.c_int32),
         ("route", ctypes.c_int32),
+    ]
+
+
+class LceSampling(ctypes.Structure):
+    """Mirror of ``struct lce_sampling``."""
+
+    _fields_ = [
+        ("temperature", ctypes.c_float),
+        ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float),
+        ("top_k", ctypes.c_int64),
+        ("temperature_rows", ctypes.c_void_p),
+        ("top_p_rows", ctypes.c_void_p),
+        ("min_p_rows", ctypes.c_void_p),
+        ("top_k_rows", ctypes.c_void_p),
     ]
 
 
@@ -146,6 +163,10 @@ def load():
     lib.lce_distill_workspace_bytes.argtypes = [P, i64, i32, ctypes.POINTER(sz)]
     lib.lce_distill.restype = ctypes.c_int
     lib.lce_distill.argtypes = [P, i64] + [vp] * 12 + [sz, vp]
+    lib.lce_top_logits.restype = ctypes.c_int
+    lib.lce_top_logits.argtypes = [vp, ctypes.c_int, i64, i64, i64, i64, vp, vp, vp, vp]
+    lib.lce_sample.restype = ctypes.c_int
+    lib.lce_sample.argtypes = [vp, ctypes.c_int, i64, i64, i64, vp, ctypes.POINTER(LceSampling), vp, vp]
     _lib = lib
     return lib
 

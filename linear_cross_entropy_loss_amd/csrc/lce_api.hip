@@ -1617,4 +1617,43 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
   return LCE_OK;
 }
 
+namespace {
+int check_logits(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld) {
+  if (dtype != LCE_BF16 && dtype != LCE_F16 && dtype != LCE_F32) return LCE_EINVAL_DTYPE;
+  if (rows < 0 || rows > (int64_t)1 << 30 || cols < 1 || cols > (int64_t)1 << 30) return LCE_EINVAL_SHAPE;
+  if (rows > 0 && (!logits || ld < 0 || ((uintptr_t)logits & (dtype == LCE_F32 ? 3 : 1)))) return LCE_EINVAL_ARG;
+  return LCE_OK;
+}
+}  // namespace
+
+int lce_top_logits(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, int64_t k, void* values, int64_t* index, float* lse,
+                   void* stream) {
+  const int rc = check_logits(logits, dtype, rows, cols, ld);
+  if (rc != LCE_OK) return rc;
+  if (k < 1 || k > cols || k > LCE_MAX_TARGETS) return LCE_EINVAL_SHAPE;
+  if (rows == 0) return LCE_OK;
+  if (!values || !index) return LCE_EINVAL_ARG;
+  const hipError_t e = lce::launch_top(logits, dtype, rows, cols, ld, (int)k, values, index, lse, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "top_logits");
+  return LCE_OK;
+}
+
+int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* u, const lce_sampling* s, int64_t* token,
+               void* stream) {
+  const int rc = check_logits(logits, dtype, rows, cols, ld);
+  if (rc != LCE_OK) return rc;
+  if (!s) return LCE_EINVAL_ARG;
+  // (numbers that are not there for each row are checked; those that are, lce.h says what they stand for)
+  if (!s->temperature_rows && !(s->temperature >= 0.f && s->temperature <= 3.4e38f)) return LCE_EINVAL_ARG;
+  if (!s->top_p_rows && !(s->top_p > 0.f && s->top_p <= 1.f)) return LCE_EINVAL_ARG;
+  if (!s->min_p_rows && !(s->min_p >= 0.f && s->min_p <= 1.f)) return LCE_EINVAL_ARG;
+  if (!s->top_k_rows && s->top_k < 0) return LCE_EINVAL_ARG;
+  if (rows == 0) return LCE_OK;
+  if (!u || !token) return LCE_EINVAL_ARG;
+  const lce::Sampling a = {s->temperature, s->top_p, s->min_p, s->top_k, s->temperature_rows, s->top_p_rows, s->min_p_rows, s->top_k_rows};
+  const hipError_t e = lce::launch_sample(logits, dtype, rows, cols, ld, u, a, token, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "sample");
+  return LCE_OK;
+}
+
 }  // extern "C"

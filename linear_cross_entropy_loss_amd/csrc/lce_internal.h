@@ -512,6 +512,20 @@ hipError_t launch_soft_loss(const SoftTargets& t, const int64_t* y, const float*
                             float* loss, hipStream_t s);
 int soft_loss_groups();
 
+// Selections from rows of logits (lce_select.hip).  A pointer that is not null has one setting for each row.
+struct Sampling {
+  float temperature, top_p, min_p;
+  int64_t top_k;
+  const float* temperature_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  const int64_t* top_k_rows;
+};
+hipError_t launch_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* u, const Sampling& s,
+                         int64_t* token, hipStream_t stream);
+hipError_t launch_top(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, int k, void* values, int64_t* index, float* lse,
+                      hipStream_t stream);
+
 hipError_t launch_fwd_narrow(const FwdArgs& a, int64_t rows, hipStream_t s);
 hipError_t launch_bwd_narrow(const BwdArgs& a, const SmallGrads& g, bool want_dx, bool want_dw, hipStream_t s);
 hipError_t launch_bwd_grads_small(const BwdArgs& a, const SmallGrads& g, bool want_dx, bool want_dw, hipStream_t s);
