@@ -469,7 +469,7 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
  * each of them the first column at least, and of what all three keep the token is the first column whose sum of w up to and
  * with it exceeds u * the whole sum.  temperature 0: the first column.  Columns of -inf are never drawn; a row of nothing else, or
  * with a NaN, gives -1.  Settings by row (a pointer that is not NULL) replace the number; there top_k <= 0, top_p >= 1 or NaN and
- * min_p <= 0 or NaN keep all, top_p <= 0 keeps the first column, and a temperature that is not positive stands for 0.
+ * min_p <= 0 or NaN keep all, top_p <= 0 and min_p > 1 keep the first column, and a temperature that is not positive stands for 0.
  */
 typedef struct lce_sampling {
   float temperature; /* 0 <= temperature < inf */

@@ -72,17 +72,17 @@ template <class E> struct RowUnits {
     }
     return u32x4_t{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
   }
-  // f(unit, elements, how many of them are there) for the units of this lane, two loads in flight; every lane of a wave makes
+  // f(unit, elements, how many of them are there) for the units of this lane, four loads in flight; every lane of a wave makes
   // the same number of calls.
   template <class F> LCE_DEV void each(F f) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t u0 = wave * share + lane;
-    for (int64_t i = 0; i < share && wave * share + i < units; i += 128) {
-      u32x4_t v[2];
+    for (int64_t i = 0; i < share && wave * share + i < units; i += 256) {
+      u32x4_t v[4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) v[r] = i + r * 64 < share ? load(u0 + i + r * 64) : u32x4_t{};
+      for (int r = 0; r < 4; ++r) v[r] = i + r * 64 < share ? load(u0 + i + r * 64) : u32x4_t{};
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 4; ++r)
         if (i + r * 64 < share) {
           E e[kPer];
           __builtin_memcpy(e, &v[r], 16);
@@ -92,75 +92,120 @@ template <class E> struct RowUnits {
   }
 };
 
-template <class F, class Join> LCE_DEV F wave_all(F v, Join join) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = join(v, (F)__shfl_xor(v, d));
+// v of the lane that the DPP control names, 0 where there is none (or the row is not in ROWS).
+template <int CTRL, int ROWS> LCE_DEV unsigned from_lane(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> LCE_DEV int from_lane(int v) { return (int)from_lane<CTRL, ROWS>((unsigned)v); }
+template <int CTRL, int ROWS> LCE_DEV u64 from_lane(u64 v) {
+  return (u64)from_lane<CTRL, ROWS>((unsigned)(v >> 32)) << 32 | from_lane<CTRL, ROWS>((unsigned)v);
+}
+template <int CTRL, int ROWS> LCE_DEV double from_lane(double v) {
+  return __builtin_bit_cast(double, from_lane<CTRL, ROWS>(__builtin_bit_cast(u64, v)));
+}
+LCE_DEV u64 read_lane(u64 v, int lane) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+LCE_DEV int read_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+LCE_DEV unsigned read_lane(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
+LCE_DEV double read_lane(double v, int lane) { return __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, v), lane)); }
+struct Sum {
+  template <class F> LCE_DEV static F join(F a, F b) { return a + b; }
+};
+struct Largest {  // (of unsigned numbers: 0 stands for none)
+  template <class F> LCE_DEV static F join(F a, F b) { return a > b ? a : b; }
+};
+// Joined over the lanes up to and with this one (every lane of the wave takes part).  ROW: over the 16 lanes of a row only.
+template <class J, class F, bool ROW = false> LCE_DEV F wave_upto(F v) {
+  v = J::join(v, from_lane<0x111, 0xf>(v));
+  v = J::join(v, from_lane<0x112, 0xf>(v));
+  v = J::join(v, from_lane<0x114, 0xf>(v));
+  v = J::join(v, from_lane<0x118, 0xf>(v));
+  if constexpr (!ROW) {
+    v = J::join(v, from_lane<0x142, 0xa>(v));
+    v = J::join(v, from_lane<0x143, 0xc>(v));
+  }
   return v;
 }
-// Over the workgroup; `sh`: room for one value of each wave.  Ends with a barrier.
-template <class F, class Join> LCE_DEV F block_all(F v, F* sh, Join join) {
-  v = wave_all(v, join);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+// Over the workgroup; `sh`: room for one value of each wave.  *before (sums): over the threads before this one.  Ends with a barrier.
+static_assert(kSelectWaves == 16, "a row of lanes joins the waves' values");
+template <class J, class F> LCE_DEV F block_all(F v, F* sh, F* before = nullptr) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const F upto = wave_upto<J>(v);
+  if (lane == 63) sh[wave] = upto;
   __syncthreads();
-  F r = sh[0];
-  for (int w = 1; w < kSelectWaves; ++w) r = join(r, sh[w]);
+  const F waves = wave_upto<J, F, true>(sh[lane & 15]);
   __syncthreads();
-  return r;
-}
-// Sum over the threads before this one.  Ends with a barrier.
-template <class F> LCE_DEV F block_before(F v, F* sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  F up = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const F o = __shfl_up(up, d);
-    if (lane >= d) up += o;
-  }
-  if (lane == 63) sh[wave] = up;
-  __syncthreads();
-  F before = up - v;
-  for (int w = 0; w < wave; ++w) before += sh[w];
-  __syncthreads();
-  return before;
+  if (before != nullptr) *before = upto - v + (wave > 0 ? read_lane(waves, wave - 1) : F(0));
+  return read_lane(waves, 15);
 }
 
-// The column of the r-th (from 0) element with the key; -1 if there are no more than r.  All threads take part and get it.
-template <class E> LCE_DEV int64_t column_of(const RowUnits<E>& row, unsigned key, int64_t r, int64_t* sh /* [kSelectWaves + 1] */) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int mine = 0;
-  row.each([&](int64_t, const E* e, int c) {
+// The column of the r-th (from 0) element with the key; -1 if there are no more than r.  All threads take part and get it.  The waves
+// count such elements, by parts of their share of the row, and the one that has the r-th looks for it in its part.
+constexpr int kParts = 32;
+struct ColumnShared {
+  int count[kSelectWaves][kParts];
+  int64_t of_wave[kSelectWaves];
+  int64_t column;
+};
+template <class E> LCE_DEV int64_t column_of(const RowUnits<E>& row, unsigned key, int64_t r, ColumnShared* sh) {
+  constexpr int kPer = RowUnits<E>::kPer;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t u0 = wave * row.share, rounds = row.share / 64, per = (rounds + kParts - 1) / kParts;
+  if (threadIdx.x == 0) sh->column = -1;
+  int64_t mine = 0;
+#pragma unroll 1
+  for (int part = 0; part < kParts; ++part) {
+    int count = 0;
+#pragma unroll 1
+    for (int64_t i = part * per; i < (part + 1) * per && i < rounds && u0 + i * 64 < row.units; i += 4) {
+      u32x4_t v[4];
 #pragma unroll
-    for (int i = 0; i < RowUnits<E>::kPer; ++i) mine += i < c && key_of(as_float(e[i])) == key ? 1 : 0;
-  });
-  const int64_t of_wave = wave_all((int64_t)mine, [](int64_t a, int64_t b) { return a + b; });
-  if (lane == 0) sh[wave] = of_wave;
-  if (threadIdx.x == 0) sh[kSelectWaves] = -1;
+      for (int q = 0; q < 4; ++q) v[q] = i + q < (part + 1) * per && i + q < rounds ? row.load(u0 + (i + q) * 64 + lane) : u32x4_t{};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (!(i + q < (part + 1) * per && i + q < rounds)) continue;
+        E e[kPer];
+        __builtin_memcpy(e, &v[q], 16);
+        const int c = row.count(u0 + (i + q) * 64 + lane);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) count += __popcll(__ballot(k < c && key_of(as_float(e[k])) == key));
+      }
+    }
+    if (lane == 0) sh->count[wave][part] = count;
+    mine += count;
+  }
+  if (lane == 0) sh->of_wave[wave] = mine;
   __syncthreads();
   int64_t before = 0;
-  for (int w = 0; w < wave; ++w) before += sh[w];
-  if (before <= r && r < before + of_wave) {  // (one wave)
-    row.each([&](int64_t unit, const E* e, int c) {
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) before += w < wave ? sh->of_wave[w] : 0;
+  if (before <= r && r < before + mine) {  // (one wave)
+    int part = 0;
+    while (part < kParts - 1 && before + sh->count[wave][part] <= r) before += sh->count[wave][part++];
+#pragma unroll 1
+    for (int64_t i = part * per; i < (part + 1) * per && i < rounds; ++i) {
+      const int64_t unit = u0 + i * 64 + lane;
+      const u32x4_t v = row.load(unit);
+      E e[kPer];
+      __builtin_memcpy(e, &v, 16);
+      const int c = row.count(unit);
       int here = 0;
 #pragma unroll
-      for (int i = 0; i < RowUnits<E>::kPer; ++i) here += i < c && key_of(as_float(e[i])) == key ? 1 : 0;
-      int up = here;
+      for (int k = 0; k < kPer; ++k) here += k < c && key_of(as_float(e[k])) == key ? 1 : 0;
+      const int upto = wave_upto<Sum>(here);
+      int64_t at = before + upto - here;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(up, d);
-        if (lane >= d) up += o;
-      }
-      int64_t at = before + up - here;
-#pragma unroll
-      for (int i = 0; i < RowUnits<E>::kPer; ++i)
-        if (i < c && key_of(as_float(e[i])) == key) {
-          if (at == r) sh[kSelectWaves] = row.column(unit) + i;
+      for (int k = 0; k < kPer; ++k)
+        if (k < c && key_of(as_float(e[k])) == key) {
+          if (at == r) sh->column = row.column(unit) + k;
           ++at;
         }
-      before += __shfl(up, 63);
-    });
+      before += read_lane(upto, 63);
+    }
   }
   __syncthreads();
-  const int64_t at = sh[kSelectWaves];
+  const int64_t at = sh->column;
   __syncthreads();
   return at;
 }
@@ -193,7 +238,8 @@ struct Weights {
     return exp2_series(t);
   }
   // (rounded by the sum with 2^52, whose last place is 1)
-  LCE_DEV u64 of(float z) const { return __builtin_bit_cast(u64, fma(real(z), one, 4503599627370496.0)) & 0xfffffffffffffull; }
+  LCE_DEV u64 fixed(double w) const { return __builtin_bit_cast(u64, fma(w, one, 4503599627370496.0)) & 0xfffffffffffffull; }
+  LCE_DEV u64 of(float z) const { return fixed(real(z)); }
 };
 struct NoWeights {
   LCE_DEV u64 of(float) const { return 0; }
@@ -245,7 +291,7 @@ struct SelectShared {
   Histogram first, next;
   Place place;
   u64 of_wave[kSelectWaves];
-  int64_t of_wave_count[kSelectWaves + 1];
+  ColumnShared columns;
 };
 
 // The histogram of the first digit; returns the weight of the elements with a key of `least` and above.
@@ -269,7 +315,7 @@ template <class E> LCE_DEV u64 fill_first(const RowUnits<E>& row, const Weights&
       atomicAdd(&sh->first.count[digit_of(key, 0)], 1);
     }
   });
-  return block_all(mine, sh->of_wave, [](u64 a, u64 b) { return a + b; });
+  return block_all<Sum>(mine, sh->of_wave);
 }
 
 // What a place is looked for by: the k-th element; the last key with an element before which there is less than `most` weight; the
@@ -300,8 +346,12 @@ LCE_DEV Place find_place(const RowUnits<E>& row, const W& weights, SelectShared*
     const int d1 = kDigits - 1 - 2 * (int)threadIdx.x, d0 = d1 - 1;  // this thread's digits, the larger first
     const int c1 = h->count[d1], c0 = h->count[d0];
     const u64 w1 = WEIGHTED ? h->weight[d1] : 0, w0 = WEIGHTED ? h->weight[d0] : 0;
-    int64_t cb = p.count + block_before((int64_t)(c1 + c0), sh->of_wave_count);
-    u64 wb = WEIGHTED ? p.weight + block_before(w1 + w0, sh->of_wave) : 0;
+    int c_before;
+    u64 w_before = 0;
+    block_all<Sum>(c1 + c0, reinterpret_cast<int*>(sh->of_wave), &c_before);
+    if (WEIGHTED) block_all<Sum>(w1 + w0, sh->of_wave, &w_before);
+    int64_t cb = p.count + c_before;
+    u64 wb = p.weight + w_before;
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
     if (want.here(cb, wb, c1, w1)) sh->place = {p.key | (unsigned)d1 << shift, cb, wb, c1};
     cb += c1;
@@ -324,173 +374,740 @@ template <class E> LCE_DEV unsigned largest_key(const RowUnits<E>& row, unsigned
       top = i < c && k > top ? k : top;
     }
   });
-  return block_all(top, sh, [](unsigned a, unsigned b) { return a > b ? a : b; });
+  return block_all<Largest>(top, sh);
 }
 
-template <class E>
-__global__ __launch_bounds__(kSelectThreads) void sample_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
-                                                                const Sampling s, int bits, int64_t* token) {
-  __shared__ SelectShared sh;
-  for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
-    const RowUnits<E> row(logits + n * ld, cols);
-    const float temperature = s.temperature_rows ? s.temperature_rows[n] : s.temperature;
-    const float top_p = s.top_p_rows ? s.top_p_rows[n] : s.top_p, min_p = s.min_p_rows ? s.min_p_rows[n] : s.min_p;
-    const int64_t top_k = s.top_k_rows ? s.top_k_rows[n] : s.top_k;
-    const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh.of_wave));
-    if (top == kNanKey || top == kLowKey) {  // a NaN, or no column left
-      if (threadIdx.x == 0) token[n] = -1;
-      continue;
-    }
-    Place at = {top, 0, 0, 0};
-    int64_t r = 0;
-    if (threadIdx.x == 0) sh.place = at;
-    if (temperature > 0.f && top_k != 1) {
-      const Weights weights = {(double)value_of(top), 1.4426950408889634074 / (double)temperature, (double)((u64)1 << bits)};
-      // the smallest key that min_p keeps: the weights are monotone in the keys
-      unsigned least = top;
-      if (min_p > 0.f) {
-        unsigned lo = kLowKey;  // (`least` has such a weight: the first column always stays)
-        while (least - lo > 1) {
-          const unsigned mid = lo + (least - lo) / 2;
-          if (weights.real(value_of(mid)) >= (double)min_p) least = mid;
-          else lo = mid;
-        }
-      }
-      const u64 by_min = fill_first(row, weights, min_p > 0.f ? least : 0, &sh);
-      const int t2 = 2 * (int)threadIdx.x;
-      auto add = [](u64 a, u64 b) { return a + b; };
-      const u64 all = block_all(sh.first.weight[t2] + sh.first.weight[t2 + 1], sh.of_wave, add);
-      const int64_t counted = (int64_t)block_all((u64)(sh.first.count[t2] + sh.first.count[t2 + 1]), sh.of_wave, add);
-      u64 stays = all;
-#pragma unroll 1
-      for (int step = kByCount; step <= kByWeight; ++step) {
-        if (step == kByCount && !(top_k > 0 && top_k < counted)) continue;
-        if (step == kByShare && !(top_p < 1.f)) continue;
-        Want want = {(Wanted)step, top_k, (double)top_p * (double)stays, 0};
-        if (step == kByWeight) {
-          if (by_min < stays) stays = by_min;
-          const double some = (double)u[n] * (double)stays;
-          want.target = some > 0.0 ? (u64)some : 0;
-          if (want.target >= stays) want.target = stays - 1;
-        }
-        at = find_place<true>(row, weights, &sh, want);
-        u64 w = weights.of(value_of(at.key));
-        w = w == 0 ? 1 : w;  // (not of an element that was counted)
-        if (step == kByCount) {
-          stays = at.weight + (u64)(top_k - at.count) * w;
-        } else if (step == kByShare) {
-          const double some = (want.most - (double)at.weight) / (double)w;
-          int64_t kept = some > 0.0 ? (int64_t)some : 0;
-          if (kept > at.same) kept = at.same;
-          if (kept < at.same && (double)(at.weight + (u64)kept * w) < want.most) ++kept;  // (`some` rounded down)
-          if (at.weight == 0 && kept == 0) kept = 1;
-          const u64 by_p = at.weight + (u64)kept * w;
-          if (by_p < stays) stays = by_p;
-        } else {
-          r = (int64_t)((want.target - at.weight) / w);
-        }
-      }
-    }
-    const int64_t column = column_of(row, at.key, r, sh.of_wave_count);
-    if (threadIdx.x == 0) token[n] = column;
+// Settings of a row.
+struct RowSettings {
+  float temperature, top_p, min_p, u;
+  int64_t top_k;
+  int bits;
+  LCE_DEV RowSettings(const Sampling& s, const float* u_, int64_t n, int bits_) : bits(bits_) {
+    temperature = s.temperature_rows ? s.temperature_rows[n] : s.temperature;
+    top_p = s.top_p_rows ? s.top_p_rows[n] : s.top_p;
+    min_p = s.min_p_rows ? s.min_p_rows[n] : s.min_p;
+    top_k = s.top_k_rows ? s.top_k_rows[n] : s.top_k;
+    u = u_[n];
   }
+  LCE_DEV bool greedy() const { return !(temperature > 0.f) || top_k == 1; }
+  LCE_DEV Weights weights(float top) const {
+    return {(double)top, 1.4426950408889634074 / (double)temperature, (double)((u64)1 << bits)};
+  }
+};
+
+// The place of the token, and which of the place's elements it is, from `find`, which looks up places, the number of elements
+// with a weight, the sum of their weights and of those that min_p keeps.
+template <class Find, class WeightAt>
+LCE_DEV Place draw_place(const RowSettings& s, int64_t counted, u64 all, u64 by_min, Place at, int64_t* which, Find find, WeightAt weight_at) {
+  u64 stays = all;
+  if (s.min_p > 1.f) by_min = (u64)1 << s.bits;  // (the first column alone)
+#pragma unroll 1
+  for (int step = kByCount; step <= kByWeight; ++step) {
+    if (step == kByCount && !(s.top_k > 0 && s.top_k < counted)) continue;
+    if (step == kByShare && !(s.top_p < 1.f)) continue;
+    Want want = {(Wanted)step, s.top_k, (double)s.top_p * (double)stays, 0};
+    if (step == kByWeight) {
+      if (by_min < stays) stays = by_min;
+      const double some = (double)s.u * (double)stays;
+      want.target = some > 0.0 ? (u64)some : 0;
+      if (want.target >= stays) want.target = stays - 1;
+    }
+    at = find(want);
+    u64 w = weight_at(at);
+    w = w == 0 ? 1 : w;  // (not of an element that was counted)
+    if (step == kByCount) {
+      stays = at.weight + (u64)(s.top_k - at.count) * w;
+    } else if (step == kByShare) {
+      const double some = (want.most - (double)at.weight) / (double)w;
+      int64_t kept = some > 0.0 ? (int64_t)some : 0;
+      if (kept > at.same) kept = at.same;
+      if (kept < at.same && (double)(at.weight + (u64)kept * w) < want.most) ++kept;  // (`some` rounded down)
+      if (at.weight == 0 && kept == 0) kept = 1;
+      const u64 by_p = at.weight + (u64)kept * w;
+      if (by_p < stays) stays = by_p;
+    } else {
+      *which = (int64_t)((want.target - at.weight) / w);
+    }
+  }
+  return at;
+}
+
+// The token of a row by digits, any type; -1 where there is none.
+template <class E> LCE_DEV int64_t sample_by_digits(const RowUnits<E>& row, const RowSettings& s, SelectShared* sh) {
+  const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh->of_wave));
+  if (top == kNanKey || top == kLowKey) return -1;  // a NaN, or no column left
+  Place at = {top, 0, 0, 0};
+  int64_t which = 0;
+  if (threadIdx.x == 0) sh->place = at;
+  if (!s.greedy()) {
+    const Weights weights = s.weights(value_of(top));
+    // the smallest key that min_p keeps: the weights are monotone in the keys
+    unsigned least = top;
+    if (s.min_p > 0.f) {
+      unsigned lo = kLowKey;  // (`least` has such a weight: the first column always stays)
+      while (least - lo > 1) {
+        const unsigned mid = lo + (least - lo) / 2;
+        if (weights.real(value_of(mid)) >= (double)s.min_p) least = mid;
+        else lo = mid;
+      }
+    }
+    const u64 by_min = fill_first(row, weights, s.min_p > 0.f ? least : 0, sh);
+    const int t2 = 2 * (int)threadIdx.x;
+    const u64 all = block_all<Sum>(sh->first.weight[t2] + sh->first.weight[t2 + 1], sh->of_wave);
+    const int64_t counted = (int64_t)block_all<Sum>((u64)(sh->first.count[t2] + sh->first.count[t2 + 1]), sh->of_wave);
+    at = draw_place(s, counted, all, by_min, at, &which, [&](const Want& want) { return find_place<true>(row, weights, sh, want); },
+                    [&](const Place& p) { return weights.of(value_of(p.key)); });
+  }
+  return column_of(row, at.key, which, &sh->columns);
 }
 
 constexpr int kMostTop = 1024;
 
-template <class E>
-__global__ __launch_bounds__(kSelectThreads) void top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, int sorted,
-                                                             E* values, int64_t* index, float* lse) {
-  __shared__ SelectShared sh;
-  __shared__ u64 list[kMostTop];
-  __shared__ int listed;
-  for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
-    const RowUnits<E> row(logits + n * ld, cols);
-    const NoWeights none;
-    if (lse != nullptr) {
-      const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh.of_wave));
-      const float m = top == kNanKey ? __builtin_nanf("") : value_of(top);
-      float sum = 0.f;
-      row.each([&](int64_t, const E* e, int c) {
-#pragma unroll
-        for (int i = 0; i < RowUnits<E>::kPer; ++i) {
-          const float z = as_float(e[i]);
-          if (i < c) sum += z == m ? 1.f : __expf(z - m);  // (equal infinities have no difference)
-        }
-      });
-      const double all = block_all((double)sum, reinterpret_cast<double*>(sh.of_wave), [](double a, double b) { return a + b; });
-      if (threadIdx.x == 0) lse[n] = top == kLowKey ? m : (float)((double)m + log(all));
-    }
-    const Place p = find_place<false>(row, none, &sh, Want{kByCount, k, 0.0, 0});
-    // what is larger, in any order, and the first k - p.count of the key
-    if (threadIdx.x == 0) listed = 0;
-    if ((int)threadIdx.x < sorted) list[threadIdx.x] = ~(u64)0;
-    int mine = 0;
-    __syncthreads();
-    row.each([&](int64_t unit, const E* e, int c) {
-#pragma unroll
-      for (int i = 0; i < RowUnits<E>::kPer; ++i) {
-        const unsigned key = key_of(as_float(e[i]));
-        if (i < c && key > p.key) {
-          const int to = atomicAdd(&listed, 1);  // (p.count of them)
-          if (to < kMostTop) list[to] = (u64)~key << 32 | (u64)(row.column(unit) + i);
-        }
-        mine += i < c && key == p.key ? 1 : 0;
-      }
-    });
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t of_wave = wave_all((int64_t)mine, [](int64_t a, int64_t b) { return a + b; });
-    if (lane == 0) sh.of_wave_count[wave] = of_wave;
-    __syncthreads();
-    const int64_t want = k - p.count;
-    int64_t before = 0;
-    for (int w = 0; w < wave; ++w) before += sh.of_wave_count[w];
-    if (of_wave > 0 && before < want) {
-      row.each([&](int64_t unit, const E* e, int c) {
-        int here = 0;
-#pragma unroll
-        for (int i = 0; i < RowUnits<E>::kPer; ++i) here += i < c && key_of(as_float(e[i])) == p.key ? 1 : 0;
-        int up = here;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const int o = __shfl_up(up, d);
-          if (lane >= d) up += o;
-        }
-        int64_t at = before + up - here;
-#pragma unroll
-        for (int i = 0; i < RowUnits<E>::kPer; ++i)
-          if (i < c && key_of(as_float(e[i])) == p.key) {
-            if (at < want) list[p.count + at] = (u64)~p.key << 32 | (u64)(row.column(unit) + i);
-            ++at;
-          }
-        before += __shfl(up, 63);
-      });
-    }
-    // in order: by key, then by column (a bitonic network over `sorted`, a power of two)
+// An entry of a list that is sorted: by key, the larger first, then by column.
+LCE_DEV u64 entry_of(unsigned key, int64_t column) { return (u64)~key << 32 | (u64)column; }
+LCE_DEV unsigned key_in(u64 entry) { return ~(unsigned)(entry >> 32); }
+LCE_DEV int64_t column_in(u64 entry) { return (int64_t)(entry & 0xffffffffu); }
+
+// A bitonic network over list[0 .. sorted), a power of two from 2 on; up to 128 entries by one wave, without barriers in between.
+// Starts and ends with a barrier.
+LCE_DEV void sort_list(u64* list, int sorted) {
+  __syncthreads();
+  const bool one_wave = sorted <= 128;
+  if (!one_wave || threadIdx.x < 64) {
+#pragma unroll 1
     for (int size = 2; size <= sorted; size <<= 1)
+#pragma unroll 1
       for (int d = size >> 1; d > 0; d >>= 1) {
-        __syncthreads();
-        const int i = threadIdx.x, j = i ^ d;
-        if (i < sorted && j > i) {
+        for (int t = threadIdx.x; t < sorted / 2; t += kSelectThreads) {
+          const int i = ((t & ~(d - 1)) << 1) | (t & (d - 1)), j = i | d;  // the t-th pair
           const u64 a = list[i], b = list[j];
           if ((a > b) == ((i & size) == 0)) {
             list[i] = b;
             list[j] = a;
           }
         }
+        if (one_wave) {
+          __threadfence_block();
+          __builtin_amdgcn_wave_barrier();
+        } else {
+          __syncthreads();
+        }
       }
-    __syncthreads();
-    if ((int)threadIdx.x < k) {
-      int64_t column = (int64_t)(list[threadIdx.x] & 0xffffffffu);
-      column = column < cols ? column : cols - 1;  // (logits that change under the kernel must not lead it astray)
-      index[n * k + threadIdx.x] = column;
-      values[n * k + threadIdx.x] = row.p[column];
+  }
+  __syncthreads();
+}
+LCE_DEV int power_of_two(int n) {
+  int p = 2;
+  while (p < n) p <<= 1;
+  return p;
+}
+// The first k of the list to memory.
+template <class E> LCE_DEV void store_top(const RowUnits<E>& row, const u64* list, int k, E* values, int64_t* index) {
+  for (int i = threadIdx.x; i < k; i += kSelectThreads) {
+    int64_t column = column_in(list[i]);
+    column = column < row.n ? column : row.n - 1;  // (logits that change under the kernel must not lead it astray)
+    index[i] = column;
+    values[i] = row.p[column];
+  }
+}
+
+// The first k of a row by digits, any type.  list: kMostTop entries.
+template <class E>
+LCE_DEV void top_by_digits(const RowUnits<E>& row, int k, E* values, int64_t* index, float* lse, SelectShared* sh, u64* list, int* listed) {
+  constexpr int kPer = RowUnits<E>::kPer;
+  if (lse != nullptr) {
+    const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh->of_wave));
+    const float m = top == kNanKey ? __builtin_nanf("") : value_of(top);
+    float sum = 0.f;
+    row.each([&](int64_t, const E* e, int c) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float z = as_float(e[i]);
+        if (i < c) sum += z == m ? 1.f : __expf(z - m);  // (equal infinities have no difference)
+      }
+    });
+    const double all = block_all<Sum>((double)sum, reinterpret_cast<double*>(sh->of_wave));
+    if (threadIdx.x == 0) *lse = top == kLowKey ? m : (float)((double)m + log(all));
+  }
+  const Place p = find_place<false>(row, NoWeights(), sh, Want{kByCount, k, 0.0, 0});
+  // what is larger, in any order, and the first k - p.count of the key in the order of the columns
+  const int sorted = power_of_two(k), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x == 0) *listed = 0;
+  if ((int)threadIdx.x < sorted) list[threadIdx.x] = ~(u64)0;
+  __syncthreads();
+  int mine = 0;
+  row.each([&](int64_t unit, const E* e, int c) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const unsigned key = key_of(as_float(e[i]));
+      if (i < c && key > p.key) {
+        const int to = atomicAdd(listed, 1);  // (p.count of them)
+        if (to < kMostTop) list[to] = entry_of(key, row.column(unit) + i);
+      }
+      mine += i < c && key == p.key ? 1 : 0;
     }
+  });
+  const int upto = wave_upto<Sum>(mine);
+  if (lane == 63) sh->columns.of_wave[wave] = upto;
+  __syncthreads();
+  const int64_t want = k - p.count;
+  int64_t before = 0;
+  for (int w = 0; w < wave; ++w) before += sh->columns.of_wave[w];
+  if (sh->columns.of_wave[wave] > 0 && before < want) {
+    row.each([&](int64_t unit, const E* e, int c) {
+      int here = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) here += i < c && key_of(as_float(e[i])) == p.key ? 1 : 0;
+      const int of_unit = wave_upto<Sum>(here);
+      int64_t at = before + of_unit - here;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < c && key_of(as_float(e[i])) == p.key) {
+          if (at < want) list[p.count + at] = entry_of(p.key, row.column(unit) + i);
+          ++at;
+        }
+      before += read_lane(of_unit, 63);
+    });
+  }
+  sort_list(list, sorted);
+  store_top(row, list, k, values, index);
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// The first k, k up to kMostByMaxima, without a histogram: of the largest element of each thread, the k-th is a lower bound of the k-th
+// of the row, and about k (1 + k / 2048) elements are not below it: these are listed and sorted.  Two passes over the row, one that
+// takes maxima, one that compares (and sums the exponentials for lse).  Rows whose list would be too long (most elements equal, or
+// fewer than k threads with one), with a NaN or an infinity on top are done by digits.
+// ---------------------------------------------------------------------------------------------------------------------------
+constexpr int kMostByMaxima = 512, kMostList = 2048;
+struct TopShared {
+  union {
+    SelectShared digits;
+    unsigned of_thread[kSelectThreads];
+  };
+  u64 list[kMostList];
+  u64 of_wave[kSelectWaves];
+  unsigned least, top;
+  int listed;
+};
+
+// 16 bytes of a row as unsigned numbers in the order of the values (-0 just below 0), two of 16 bits or one of 32 bits to a word.
+template <class E> struct Ordered;
+template <> struct Ordered<float> {
+  static constexpr unsigned kLow = 0x007fffffu, kInf = 0xff800000u;
+  LCE_DEV static unsigned word(unsigned w) { return w ^ ((unsigned)((int)w >> 31) | 0x80000000u); }
+  LCE_DEV static unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
+  LCE_DEV static unsigned smaller(unsigned a, unsigned b) { return a < b ? a : b; }
+  LCE_DEV static unsigned largest(unsigned a) { return a; }
+  LCE_DEV static unsigned smallest(unsigned a) { return a; }
+  LCE_DEV static unsigned in_top_bits(unsigned a) { return a >> 16; }
+  LCE_DEV static unsigned from_top_bits(unsigned a) { return a << 16; }
+  LCE_DEV static float value(unsigned a) { return value_of(a); }
+};
+template <class E> struct OrderedHalf {
+  typedef short signed_t __attribute__((ext_vector_type(2)));
+  typedef unsigned short pair_t __attribute__((ext_vector_type(2)));
+  LCE_DEV static unsigned word(unsigned w) {
+    return w ^ (__builtin_bit_cast(unsigned, __builtin_bit_cast(signed_t, w) >> (short)15) | 0x80008000u);
+  }
+  LCE_DEV static unsigned larger(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(pair_t, a), __builtin_bit_cast(pair_t, b)));
+  }
+  LCE_DEV static unsigned smaller(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(pair_t, a), __builtin_bit_cast(pair_t, b)));
+  }
+  LCE_DEV static unsigned largest(unsigned a) { return a >> 16 > (a & 0xffffu) ? a >> 16 : a & 0xffffu; }
+  LCE_DEV static unsigned smallest(unsigned a) { return a >> 16 < (a & 0xffffu) ? a >> 16 : a & 0xffffu; }
+  LCE_DEV static unsigned in_top_bits(unsigned a) { return a; }
+  LCE_DEV static unsigned from_top_bits(unsigned a) { return a; }
+  LCE_DEV static float value(unsigned a) {
+    return (float)__builtin_bit_cast(E, (unsigned short)(a & 0x8000u ? a & 0x7fffu : a ^ 0xffffu));
+  }
+};
+template <> struct Ordered<__bf16> : OrderedHalf<__bf16> { static constexpr unsigned kLow = 0x007f, kInf = 0xff80; };
+template <> struct Ordered<_Float16> : OrderedHalf<_Float16> { static constexpr unsigned kLow = 0x03ff, kInf = 0xfc00; };
+
+// Whole pieces of a row, dealt to the threads one by one, and the elements before and behind them.
+template <class E> struct RowPieces {
+  typedef Ordered<E> O;
+  typedef typename bits_of<sizeof(E)>::type Bits;
+  static constexpr int kPer = 16 / sizeof(E), kFlight = 4;
+  const E* p;
+  int64_t n, head, body;
+  LCE_DEV RowPieces(const E* row, int64_t cols) : p(row), n(cols) {
+    const int64_t off = (int64_t)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E));
+    head = off < n ? off : n;
+    body = (n - head) / kPer;
+  }
+  // f(column, ordered bits) for the elements at the edges, one to a thread.
+  template <class F> LCE_DEV void edges(F f) const {
+    const int64_t tail = n - head - body * kPer, t = threadIdx.x;
+    if (t < head + tail) {
+      const int64_t at = t < head ? t : n - tail + (t - head);
+      const unsigned w = O::word(reinterpret_cast<const Bits*>(p)[at]);
+      f(at, sizeof(E) == 2 ? w & 0xffffu : w);
+    }
+  }
+  // f(column of the first, piece), kFlight pieces in flight.
+  template <class F> LCE_DEV void each(F f) const {
+    const u32x4_t* from = reinterpret_cast<const u32x4_t*>(p + head);
+#pragma unroll 1
+    for (int64_t base = threadIdx.x; base < body; base += kFlight * kSelectThreads) {
+      u32x4_t v[kFlight];
+#pragma unroll
+      for (int r = 0; r < kFlight; ++r) {
+        const int64_t at = base + r * kSelectThreads;
+        v[r] = from[at < body ? at : base];
+      }
+#pragma unroll
+      for (int r = 0; r < kFlight; ++r) {
+        const int64_t at = base + r * kSelectThreads;
+        if (at < body) f(head + at * kPer, v[r]);
+      }
+    }
+  }
+};
+
+// The list of a row's first elements: sh->list, sorted, k of them and more; returns whether it could be made.  sh->top: the ordered bits of the
+// largest element.  sums: sum exp(z - max) of the row for the caller's lse.
+template <class E, bool LSE> LCE_DEV bool list_first(const RowPieces<E>& row, int k, TopShared* sh, double* sums) {
+  typedef Ordered<E> O;
+  constexpr int kPer = RowPieces<E>::kPer;
+  const int t = threadIdx.x, lane = t & 63;
+  unsigned most = 0, least = ~0u;
+  row.edges([&](int64_t, unsigned a) {
+    most = O::larger(most, a);  // (of 16 bits: the upper half stays as it is)
+    least = O::smaller(least, sizeof(E) == 2 ? a | 0xffff0000u : a);
+  });
+  row.each([&](int64_t, u32x4_t v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned a = O::word(v[i]);
+      most = O::larger(most, a);
+      least = O::smaller(least, a);
+    }
+  });
+  most = O::largest(most);
+  least = O::smallest(least);
+  sh->of_thread[t] = O::in_top_bits(most);
+  const unsigned top = block_all<Largest>(most, reinterpret_cast<unsigned*>(sh->of_wave));
+  // (a NaN is above +inf or below -inf)
+  const bool odd = __syncthreads_or(least < O::kLow || top >= O::kInf || top <= O::kLow);
+  if (t == 0) {
+    sh->top = top;
+    sh->listed = 0;
+  }
+  if (odd) {
+    __syncthreads();
+    return false;
+  }
+  // the largest number, of 16 bits, that k threads' maxima are not below
+  if (t < 64) {
+    unsigned of[kSelectThreads / 64];
+#pragma unroll
+    for (int i = 0; i < kSelectThreads / 64; ++i) of[i] = sh->of_thread[i * 64 + lane];
+    unsigned bound = 0;
+#pragma unroll 1
+    for (unsigned bit = 0x8000u; bit != 0; bit >>= 1) {
+      const unsigned mid = bound | bit;
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < kSelectThreads / 64; ++i) count += __popcll(__ballot(of[i] >= mid));
+      if (count >= k) bound = mid;
+    }
+    if (bound == 0x8000u) bound = 0x7fffu;  // (-0 is 0)
+    if (t == 0) sh->least = O::from_top_bits(bound);
+  }
+  __syncthreads();
+  const unsigned from = sh->least;
+  const float m = O::value(top);
+  float sum = 0.f;
+  auto add = [&](int64_t at, unsigned a) {
+    if (a >= from) {
+      const int to = atomicAdd(&sh->listed, 1);
+      if (to < kMostList) sh->list[to] = entry_of(key_of(O::value(a)), at);
+    }
+  };
+  auto term = [&](float z) { sum += __builtin_amdgcn_exp2f((z - m) * 1.4426950408889634f); };
+  row.edges([&](int64_t at, unsigned a) {
+    add(at, a);
+    if (LSE) term(O::value(a));
+  });
+  row.each([&](int64_t at, u32x4_t v) {
+    unsigned best = 0;
+    u32x4_t a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = O::word(v[i]);
+      best = O::larger(best, a[i]);
+    }
+    if (O::largest(best) >= from) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (sizeof(E) == 2) {
+          add(at + 2 * i, a[i] & 0xffffu);
+          add(at + 2 * i + 1, a[i] >> 16);
+        } else {
+          add(at + i, a[i]);
+        }
+      }
+    }
+    if (LSE) {
+      E e[kPer];
+      __builtin_memcpy(e, &v, 16);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) term(as_float(e[i]));
+    }
+  });
+  if (LSE) *sums = block_all<Sum>((double)sum, reinterpret_cast<double*>(sh->of_wave));
+  __syncthreads();
+  const int listed = sh->listed;
+  if (listed > kMostList) {
+    __syncthreads();  // (the caller may use the place of it all)
+    return false;
+  }
+  const int sorted = power_of_two(listed);
+  for (int i = listed + t; i < sorted; i += kSelectThreads) sh->list[i] = ~(u64)0;
+  sort_list(sh->list, sorted);
+  return listed >= k;
+}
+
+// (64 registers a thread: two workgroups to a compute unit, of which one reads while the other sorts)
+template <class E, bool LSE>
+__global__ __launch_bounds__(kSelectThreads, 8) void top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values,
+                                                                int64_t* index, float* lse) {
+  __shared__ TopShared sh;
+  for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
+    const E* from = logits + n * ld;
+    double sums = 0.0;
+    if (k <= kMostByMaxima && list_first<E, LSE>(RowPieces<E>(from, cols), k, &sh, &sums)) {
+      if (LSE && threadIdx.x == 0) lse[n] = (float)((double)Ordered<E>::value(sh.top) + log(sums));
+      store_top(RowUnits<E>(from, cols), sh.list, k, values + n * k, index + n * k);
+      __syncthreads();
+    } else {
+      top_by_digits(RowUnits<E>(from, cols), k, values + n * k, index + n * k, LSE ? lse + n : nullptr, &sh.digits, sh.list, &sh.listed);
+    }
+  }
+}
+
+// The token of a row whose first k are listed, k of them kept by top_k (1: the first column).
+template <class E> LCE_DEV int64_t sample_listed(const RowSettings& s, int k, TopShared* sh) {
+  if (s.greedy()) return column_in(sh->list[0]);
+  const Weights weights = s.weights(value_of(key_in(sh->list[0])));
+  const int t = threadIdx.x;
+  const double real = t < k ? weights.real(value_of(key_in(sh->list[t]))) : 0.0;
+  const u64 w = weights.fixed(real);
+  u64 before;
+  u64 stays = block_all<Sum>(w, sh->of_wave, &before);
+  const double most = (double)s.top_p * (double)stays;
+  // (each keeps a beginning of the list: the weight of those that all keep is their sum)
+  const bool kept = t < k && (t == 0 || ((!(s.top_p < 1.f) || (double)before < most) && (!(s.min_p > 0.f) || real >= (double)s.min_p)));
+  stays = block_all<Sum>(kept ? w : (u64)0, sh->of_wave);
+  const double some = (double)s.u * (double)stays;
+  u64 target = some > 0.0 ? (u64)some : 0;
+  if (target >= stays) target = stays - 1;
+  if (w != 0 && before <= target && target - before < w) sh->least = (unsigned)t;  // (one thread)
+  __syncthreads();
+  const int at = (int)sh->least & (kMostList - 1);
+  const int64_t column = column_in(sh->list[at]);
+  __syncthreads();
+  return column;
+}
+
+// Rows of which the first elements are enough: settings for all of them with 1 <= top_k <= kMostByMaxima or temperature 0.
+template <class E>
+__global__ __launch_bounds__(kSelectThreads, 8) void sample_top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
+                                                                       const Sampling settings, int bits, int64_t* token) {
+  __shared__ TopShared sh;
+  for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
+    const E* from = logits + n * ld;
+    const RowSettings s(settings, u, n, bits);
+    const int64_t k = s.greedy() ? 1 : s.top_k < cols ? s.top_k : cols;
+    int64_t column;
+    if (list_first<E, false>(RowPieces<E>(from, cols), (int)k, &sh, nullptr)) column = sample_listed<E>(s, (int)k, &sh);
+    else column = sample_by_digits(RowUnits<E>(from, cols), s, &sh.digits);
+    if (threadIdx.x == 0) token[n] = column;
+    __syncthreads();
+  }
+}
+
+// float32 rows with any settings.
+__global__ __launch_bounds__(kSelectThreads) void sample_float_kernel(const float* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
+                                                                      const Sampling settings, int bits, int64_t* token) {
+  __shared__ TopShared sh;
+  for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
+    const float* from = logits + n * ld;
+    const RowSettings s(settings, u, n, bits);
+    const int64_t k = s.greedy() ? 1 : s.top_k;
+    int64_t column;
+    if (k >= 1 && k <= kMostByMaxima && k < cols && list_first<float, false>(RowPieces<float>(from, cols), (int)k, &sh, nullptr))
+      column = sample_listed<float>(s, (int)k, &sh);
+    else column = sample_by_digits(RowUnits<float>(from, cols), s, &sh.digits);
+    if (threadIdx.x == 0) token[n] = column;
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// 16-bit rows with any settings.  A row has at most 65536 different values, and a histogram of all of them fits the LDS of a
+// compute unit, with 16 bits a count.  Counts are what a row is read for; weights are worked out for each value that occurs, not for
+// each element, and places found without another look at the row.
+//   A word has the counts of the numbers +m (lower half) and -m (upper half), m its index: the bits of the magnitude.  0 and -0 are
+// one value.  Columns masked by -inf or the type's lowest number, which may be most of a row, would meet in one word: they are
+// counted apart.  A count beyond 65535 overflows into the other half of its word or is lost; either way the sum of all counts is short,
+// and the row, like one with a NaN or with nothing but masked columns, is done by digits.
+//   The values that occur are then listed in the order of the row, over the histogram, and a thread has a stretch of the list.
+// ---------------------------------------------------------------------------------------------------------------------------
+template <class E> struct HalfFormat;
+template <> struct HalfFormat<__bf16> { static constexpr unsigned kInf = 0x7f80; };
+template <> struct HalfFormat<_Float16> { static constexpr unsigned kInf = 0x7c00; };
+template <class E> LCE_DEV float half_value(unsigned bits) { return (float)__builtin_bit_cast(E, (unsigned short)bits); }
+
+constexpr int kHalfWords = 32768;
+constexpr int kWordRows = kHalfWords / 256;  // 256 words: four to a lane
+struct HalfShared {
+  union {
+    unsigned hist[kHalfWords];
+    unsigned values[kHalfWords];  // the values that occur, in order: bits, and the count in the upper half
+    TopShared top;
+    ColumnShared columns;
+  };
+  int row_values[2 * kWordRows], row_first[2 * kWordRows];  // of the positive numbers by rows from the last one, of the negative ones
+  u64 of_wave[kSelectWaves];
+  Place place;  // (its key: the bits)
+};
+
+template <class E> struct HalfRow {
+  static constexpr unsigned kInf = HalfFormat<E>::kInf, kMax = kInf - 1;
+  HalfShared* sh;
+
+  // The counts of the row's values, listed.  Returns whether the list has all of the row's columns that are not masked; *different: how
+  // many values it has.
+  LCE_DEV bool fill(const RowPieces<E>& row, int* different) const {
+    constexpr int kWordRounds = kHalfWords / 4 / kSelectThreads;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    u32x4_t* words = reinterpret_cast<u32x4_t*>(sh->hist);
+#pragma unroll
+    for (int i = 0; i < kWordRounds; ++i) words[i * kSelectThreads + t] = u32x4_t{};
+    __syncthreads();
+    int masked = 0;
+    bool nan = false;
+    auto one = [&](unsigned bits) {
+      const unsigned m = bits & 0x7fffu;
+      if (m > kInf) nan = true;
+      else if (m >= kMax && (bits & 0x8000u)) ++masked;
+      else atomicAdd(&sh->hist[m], bits & 0x8000u ? 0x10000u : 1u);
+    };
+    row.edges([&](int64_t at, unsigned) { one(reinterpret_cast<const unsigned short*>(row.p)[at]); });
+    row.each([&](int64_t, u32x4_t w) {
+      typedef unsigned short pair_t __attribute__((ext_vector_type(2)));
+      pair_t most = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned m = w[i] & 0x7fff7fffu;
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(pair_t, m));
+      }
+      if (most[0] >= kMax || most[1] >= kMax) {
+        u64 some = (u64)w[1] << 32 | w[0];
+        const u64 rest = (u64)w[3] << 32 | w[2];
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          one((unsigned)some & 0xffffu);
+          some = e == 3 ? rest : some >> 16;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          atomicAdd(&sh->hist[w[i] & 0x7fffu], 1u << ((w[i] >> 11) & 16));
+          atomicAdd(&sh->hist[(w[i] >> 16) & 0x7fffu], 1u << ((w[i] >> 27) & 16));
+        }
+      }
+    });
+    const bool any_nan = __syncthreads_or(nan);
+    // the counts leave the histogram, whose place the list takes
+    u32x4_t w[kWordRounds];
+    u64 sum = 0;
+#pragma unroll
+    for (int i = 0; i < kWordRounds; ++i) {
+      w[i] = words[i * kSelectThreads + t];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += (w[i][j] & 0xffffu) + (w[i][j] >> 16);
+    }
+    if (t == 0) {  // 0 and -0
+      w[0][0] = (w[0][0] & 0xffffu) + (w[0][0] >> 16);
+      if (w[0][0] > 0xffffu) --sum;  // (a count that is too large, as any other)
+    }
+    u64 who[2][4];
+    auto occur = [&](u32x4_t some) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        who[0][j] = __ballot((some[j] & 0xffffu) != 0);
+        who[1][j] = __ballot(some[j] >> 16 != 0);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kWordRounds; ++i) {
+      const int at = i * kSelectWaves + wave;
+      int plus = 0, minus = 0;
+      if (__any((w[i][0] | w[i][1] | w[i][2] | w[i][3]) != 0)) {
+        occur(w[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          plus += __popcll(who[0][j]);
+          minus += __popcll(who[1][j]);
+        }
+      }
+      if (lane == 0) {
+        sh->row_values[kWordRows - 1 - at] = plus;
+        sh->row_values[kWordRows + at] = minus;
+      }
+    }
+    const u64 both = block_all<Sum>(sum | (u64)masked << 31, sh->of_wave);
+    const u64 counted = both & 0x7fffffffu;
+    int before;
+    *different = block_all<Sum>(t < 2 * kWordRows ? sh->row_values[t] : 0, reinterpret_cast<int*>(sh->of_wave), &before);
+    if (any_nan || counted == 0 || *different > kHalfWords || (int64_t)(counted + (both >> 31)) != row.n) return false;
+    if (t < 2 * kWordRows) sh->row_first[t] = before;
+    __syncthreads();
+    const u64 above = ~(u64)0 << lane << 1, below = ~(~(u64)0 << lane);
+#pragma unroll
+    for (int i = 0; i < kWordRounds; ++i) {
+      if (!__any((w[i][0] | w[i][1] | w[i][2] | w[i][3]) != 0)) continue;
+      occur(w[i]);
+      const int at = i * kSelectWaves + wave;
+      int plus = sh->row_first[kWordRows - 1 - at], minus = sh->row_first[kWordRows + at];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        plus += __popcll(who[0][j] & above);
+        minus += __popcll(who[1][j] & below);
+      }
+      const unsigned m = (unsigned)(i * kSelectThreads + t) * 4;
+#pragma unroll
+      for (int j = 3; j >= 0; --j)
+        if ((w[i][j] & 0xffffu) != 0) sh->values[plus++] = (m + j) | w[i][j] << 16;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (w[i][j] >> 16 != 0) sh->values[minus++] = (m + j) | 0x8000u | (w[i][j] & 0xffff0000u);
+    }
+    __syncthreads();
+    return true;
+  }
+
+  // f(bits, count) for the values of this thread's stretch of the list.
+  template <class F> LCE_DEV void stretch(int different, F f) const {
+    const int per = (different + kSelectThreads - 1) / kSelectThreads, first = (int)threadIdx.x * per;
+    const int end = first + per < different ? first + per : different;
+#pragma unroll 1
+    for (int i = first; i < end; ++i) f(sh->values[i] & 0xffffu, (int)(sh->values[i] >> 16));
+  }
+
+  // The place that is wanted.  cb, wb: elements and weight before this thread's stretch; c, w: its own.
+  LCE_DEV Place find(const Weights& weights, int different, int64_t cb, u64 wb, int64_t c, u64 w, const Want& want) const {
+    __syncthreads();
+    if (want.here(cb, wb, c, w)) {
+      bool found = false;
+      stretch(different, [&](unsigned bits, int count) {
+        if (found) return;
+        const u64 each = weights.of(half_value<E>(bits));
+        const int n_here = each != 0 ? count : 0;
+        if (want.here(cb, wb, n_here, each * (u64)n_here)) {
+          sh->place = {bits, cb, wb, n_here};
+          found = true;
+        }
+        cb += n_here;
+        wb += each * (u64)n_here;
+      });
+    }
+    __syncthreads();
+    return sh->place;
+  }
+};
+
+// Whether either half of a word equals that of `twice`, a number's bits in both halves, after `mask`.  (Also where the upper half is off by one and
+// the lower half is equal: a filter.)
+LCE_DEV bool equal_half(unsigned word, unsigned twice, unsigned mask) {
+  const unsigned x = (word & mask) ^ twice;
+  return ((x - 0x00010001u) & ~x & 0x80008000u) != 0;
+}
+
+template <class E>
+__global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
+                                                                     const Sampling settings, int bits, int64_t* token) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  HalfShared* sh = reinterpret_cast<HalfShared*>(lds);
+  for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
+    const E* from = logits + n * ld;
+    const RowSettings s(settings, u, n, bits);
+    const RowPieces<E> row(from, cols);
+    const HalfRow<E> half = {sh};
+    const int64_t k = s.greedy() ? 1 : s.top_k;
+    int64_t column;
+    int different;
+    if (k >= 1 && k <= kMostByMaxima && k < cols && list_first<E, false>(row, (int)k, &sh->top, nullptr)) {
+      column = sample_listed<E>(s, (int)k, &sh->top);
+    } else if (!s.greedy() && half.fill(row, &different)) {
+      const unsigned top = sh->values[0] & 0xffffu;
+      const Weights weights = s.weights(half_value<E>(top));
+      const double min_p = s.min_p > 0.f ? (double)s.min_p : 0.0;
+      u64 weight = 0, by_min = 0;
+      int elements = 0;
+      half.stretch(different, [&](unsigned value, int c) {
+        const double real = weights.real(half_value<E>(value));
+        const u64 w = weights.fixed(real);
+        if (w != 0) elements += c;
+        weight += w * (u64)c;
+        if (real >= min_p) by_min += w * (u64)c;
+      });
+      int cb;
+      u64 wb;
+      const int weighed = block_all<Sum>(elements, reinterpret_cast<int*>(sh->of_wave), &cb);
+      const u64 all = block_all<Sum>(weight, sh->of_wave, &wb);
+      by_min = s.min_p > 0.f ? block_all<Sum>(by_min, sh->of_wave) : all;
+      int64_t which = 0;
+      const Place at = draw_place(s, weighed, all, by_min, Place{top, 0, 0, 0}, &which,
+                                  [&](const Want& want) { return half.find(weights, different, cb, wb, elements, weight, want); },
+                                  [&](const Place& p) { return weights.of(half_value<E>(p.key)); });
+      __syncthreads();  // (the list of values is not read any more)
+      column = column_of(RowUnits<E>(from, cols), key_of(half_value<E>(at.key)), which, &sh->columns);
+    } else {
+      __syncthreads();
+      column = sample_by_digits(RowUnits<E>(from, cols), s, &sh->top.digits);
+    }
+    if (threadIdx.x == 0) token[n] = column;
     __syncthreads();
   }
 }
 
 unsigned grid_of(int64_t rows) { return (unsigned)(rows < (int64_t)1 << 20 ? rows : (int64_t)1 << 20); }
+static_assert(sizeof(HalfShared) <= 160 * 1024, "a compute unit has 160 KiB of LDS");
+
+template <class E>
+hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u, const Sampling& s, int bits, int64_t* token,
+                            hipStream_t stream) {
+  const dim3 grid(grid_of(rows)), block(kSelectThreads);
+  const bool first_alone = (!s.temperature_rows && s.temperature == 0.f) || (!s.top_k_rows && s.top_k >= 1 && s.top_k <= kMostByMaxima);
+  if (first_alone) {
+    hipLaunchKernelGGL(sample_top_kernel<E>, grid, block, 0, stream, logits, rows, cols, ld, u, s, bits, token);
+  } else if constexpr (sizeof(E) == 2) {
+    static LdsOptIn optin;
+    const hipError_t e = optin.ensure(reinterpret_cast<const void*>(sample_half_kernel<E>), (int)sizeof(HalfShared));
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(sample_half_kernel<E>, grid, block, sizeof(HalfShared), stream, logits, rows, cols, ld, u, s, bits, token);
+  } else {
+    hipLaunchKernelGGL(sample_float_kernel, grid, block, 0, stream, logits, rows, cols, ld, u, s, bits, token);
+  }
+  return hipGetLastError();
+}
+
+template <class E>
+hipError_t launch_top_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values, int64_t* index, float* lse,
+                         hipStream_t stream) {
+  const dim3 grid(grid_of(rows)), block(kSelectThreads);
+  if (lse != nullptr) hipLaunchKernelGGL((top_kernel<E, true>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
+  else hipLaunchKernelGGL((top_kernel<E, false>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
+  return hipGetLastError();
+}
 
 }  // namespace
 
@@ -499,29 +1116,18 @@ hipError_t launch_sample(const void* logits, int dtype, int64_t rows, int64_t co
   int log2 = 0;
   while ((int64_t)1 << log2 < cols) ++log2;
   const int bits = 62 - log2 < 50 ? 62 - log2 : 50;  // (a double has 53: a weight of one and the half that rounds it fit)
-  const dim3 grid(grid_of(rows)), block(kSelectThreads);
-  if (dtype == DT_BF16) hipLaunchKernelGGL(sample_kernel<__bf16>, grid, block, 0, stream, (const __bf16*)logits, rows, cols, ld, u, s, bits, token);
-  else if (dtype == DT_F16)
-    hipLaunchKernelGGL(sample_kernel<_Float16>, grid, block, 0, stream, (const _Float16*)logits, rows, cols, ld, u, s, bits, token);
-  else if (dtype == DT_F32) hipLaunchKernelGGL(sample_kernel<float>, grid, block, 0, stream, (const float*)logits, rows, cols, ld, u, s, bits, token);
-  else return hipErrorInvalidValue;
-  return hipGetLastError();
+  if (dtype == DT_BF16) return launch_sample_of((const __bf16*)logits, rows, cols, ld, u, s, bits, token, stream);
+  if (dtype == DT_F16) return launch_sample_of((const _Float16*)logits, rows, cols, ld, u, s, bits, token, stream);
+  if (dtype == DT_F32) return launch_sample_of((const float*)logits, rows, cols, ld, u, s, bits, token, stream);
+  return hipErrorInvalidValue;
 }
 
 hipError_t launch_top(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, int k, void* values, int64_t* index, float* lse,
                       hipStream_t stream) {
-  int sorted = 2;
-  while (sorted < k) sorted <<= 1;
-  const dim3 grid(grid_of(rows)), block(kSelectThreads);
-  if (dtype == DT_BF16)
-    hipLaunchKernelGGL(top_kernel<__bf16>, grid, block, 0, stream, (const __bf16*)logits, rows, cols, ld, k, sorted, (__bf16*)values, index, lse);
-  else if (dtype == DT_F16)
-    hipLaunchKernelGGL(top_kernel<_Float16>, grid, block, 0, stream, (const _Float16*)logits, rows, cols, ld, k, sorted, (_Float16*)values, index,
-                       lse);
-  else if (dtype == DT_F32)
-    hipLaunchKernelGGL(top_kernel<float>, grid, block, 0, stream, (const float*)logits, rows, cols, ld, k, sorted, (float*)values, index, lse);
-  else return hipErrorInvalidValue;
-  return hipGetLastError();
+  if (dtype == DT_BF16) return launch_top_of((const __bf16*)logits, rows, cols, ld, k, (__bf16*)values, index, lse, stream);
+  if (dtype == DT_F16) return launch_top_of((const _Float16*)logits, rows, cols, ld, k, (_Float16*)values, index, lse, stream);
+  if (dtype == DT_F32) return launch_top_of((const float*)logits, rows, cols, ld, k, (float*)values, index, lse, stream);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace lce

@@ -131,7 +131,7 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         top_k: 0 keeps all.  top_p: 1 keeps all.  min_p: 0 keeps all.
 
     Each setting is a number, or a tensor (...) on the logits' device with one for every row (in which, without a check, top_k <= 0,
-    top_p >= 1 and min_p <= 0 keep all, top_p <= 0 keeps one column and a temperature that is not positive stands for 0).
+    top_p >= 1 and min_p <= 0 keep all, top_p <= 0 and min_p > 1 keep one column and a temperature that is not positive stands for 0).
     Returns torch.long tokens (...); -1 for a row that is masked altogether or has a NaN.
     """
     if torch.compiler.is_compiling():
