@@ -140,37 +140,75 @@ template <class J, class F> LCE_DEV F block_all(F v, F* sh, F* before = nullptr)
   return read_lane(waves, 15);
 }
 
-// The column of the r-th (from 0) element with the key; -1 if there are no more than r.  All threads take part and get it.  The waves
+// Which elements of 16 bytes equal a value, as bits 0 .. 7 (or 3).  0 and -0 are equal; the value is no NaN.
+template <class E> struct Equal {  // 16-bit elements
+  unsigned twice, mask;
+  LCE_DEV explicit Equal(float value) {
+    const unsigned bits = __builtin_bit_cast(unsigned short, (E)value);
+    mask = (bits & 0x7fffu) == 0 ? 0x7fff7fffu : 0xffffffffu;
+    twice = (bits | bits << 16) & mask;
+  }
+  // (one half equal, or the lower one is and the upper one is off by one)
+  LCE_DEV bool maybe(u32x4_t v) const {
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned x = (v[i] & mask) ^ twice;
+      any |= (x - 0x00010001u) & ~x;
+    }
+    return (any & 0x80008000u) != 0;
+  }
+  LCE_DEV bool is(u32x4_t v, int k) const {
+    const unsigned x = (v[k >> 1] & mask) ^ twice;
+    return (k & 1 ? x >> 16 : x & 0xffffu) == 0;
+  }
+};
+template <> struct Equal<float> {
+  float value;
+  LCE_DEV explicit Equal(float v) : value(v) {}
+  LCE_DEV bool is(u32x4_t v, int k) const {
+    const unsigned w = v[k];
+    return __builtin_bit_cast(float, w) == value;
+  }
+  LCE_DEV bool maybe(u32x4_t v) const { return is(v, 0) || is(v, 1) || is(v, 2) || is(v, 3); }
+};
+
+// The column of the r-th (from 0) element with a value; -1 if there are no more than r.  All threads take part and get it.  The waves
 // count such elements, by parts of their share of the row, and the one that has the r-th looks for it in its part.
-constexpr int kParts = 32;
+constexpr int kParts = 32, kPartRounds = 8;  // rounds that are in flight together
 struct ColumnShared {
   int count[kSelectWaves][kParts];
   int64_t of_wave[kSelectWaves];
   int64_t column;
 };
-template <class E> LCE_DEV int64_t column_of(const RowUnits<E>& row, unsigned key, int64_t r, ColumnShared* sh) {
+template <class E> LCE_DEV int64_t column_of(const RowUnits<E>& row, float value, int64_t r, ColumnShared* sh) {
   constexpr int kPer = RowUnits<E>::kPer;
+  const Equal<E> equal(value);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t u0 = wave * row.share, rounds = row.share / 64, per = (rounds + kParts - 1) / kParts;
+  const int64_t u0 = wave * row.share, left = (row.units - u0 + 63) / 64, share = row.share / 64;
+  const int64_t rounds = left < 0 ? 0 : left < share ? left : share;
+  const int64_t per = (rounds + kParts * kPartRounds - 1) / (kParts * kPartRounds) * kPartRounds;  // rounds of a part
+  auto load = [&](int64_t i, u32x4_t (&v)[kPartRounds]) {
+#pragma unroll
+    for (int q = 0; q < kPartRounds; ++q)
+      if (i + q < rounds) v[q] = row.load(u0 + (i + q) * 64 + lane);
+  };
   if (threadIdx.x == 0) sh->column = -1;
-  int64_t mine = 0;
+  int mine = 0;
 #pragma unroll 1
-  for (int part = 0; part < kParts; ++part) {
+  for (int64_t i = 0, part = 0; i < rounds; ++part) {
     int count = 0;
 #pragma unroll 1
-    for (int64_t i = part * per; i < (part + 1) * per && i < rounds && u0 + i * 64 < row.units; i += 4) {
-      u32x4_t v[4];
+    for (const int64_t end = i + per; i < end && i < rounds; i += kPartRounds) {
+      u32x4_t v[kPartRounds];
+      load(i, v);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = i + q < (part + 1) * per && i + q < rounds ? row.load(u0 + (i + q) * 64 + lane) : u32x4_t{};
+      for (int q = 0; q < kPartRounds; ++q)
+        if (i + q < rounds && __any(equal.maybe(v[q]))) {
+          const int c = row.count(u0 + (i + q) * 64 + lane);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (!(i + q < (part + 1) * per && i + q < rounds)) continue;
-        E e[kPer];
-        __builtin_memcpy(e, &v[q], 16);
-        const int c = row.count(u0 + (i + q) * 64 + lane);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) count += __popcll(__ballot(k < c && key_of(as_float(e[k])) == key));
-      }
+          for (int k = 0; k < kPer; ++k) count += __popcll(__ballot(k < c && equal.is(v[q], k)));
+        }
     }
     if (lane == 0) sh->count[wave][part] = count;
     mine += count;
@@ -181,27 +219,30 @@ template <class E> LCE_DEV int64_t column_of(const RowUnits<E>& row, unsigned ke
 #pragma unroll
   for (int w = 0; w < kSelectWaves; ++w) before += w < wave ? sh->of_wave[w] : 0;
   if (before <= r && r < before + mine) {  // (one wave)
-    int part = 0;
-    while (part < kParts - 1 && before + sh->count[wave][part] <= r) before += sh->count[wave][part++];
+    int64_t i = 0;
+    for (int part = 0; part < kParts - 1 && before + sh->count[wave][part] <= r; ++part, i += per) before += sh->count[wave][part];
 #pragma unroll 1
-    for (int64_t i = part * per; i < (part + 1) * per && i < rounds; ++i) {
-      const int64_t unit = u0 + i * 64 + lane;
-      const u32x4_t v = row.load(unit);
-      E e[kPer];
-      __builtin_memcpy(e, &v, 16);
-      const int c = row.count(unit);
-      int here = 0;
+    for (const int64_t end = i + per; i < end && i < rounds; i += kPartRounds) {
+      u32x4_t v[kPartRounds];
+      load(i, v);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) here += k < c && key_of(as_float(e[k])) == key ? 1 : 0;
-      const int upto = wave_upto<Sum>(here);
-      int64_t at = before + upto - here;
+      for (int q = 0; q < kPartRounds; ++q) {
+        if (!(i + q < rounds && __any(equal.maybe(v[q])))) continue;
+        const int64_t unit = u0 + (i + q) * 64 + lane;
+        const int c = row.count(unit);
+        int here = 0;
 #pragma unroll
-      for (int k = 0; k < kPer; ++k)
-        if (k < c && key_of(as_float(e[k])) == key) {
-          if (at == r) sh->column = row.column(unit) + k;
-          ++at;
-        }
-      before += read_lane(upto, 63);
+        for (int k = 0; k < kPer; ++k) here += k < c && equal.is(v[q], k) ? 1 : 0;
+        const int upto = wave_upto<Sum>(here);
+        int64_t at = before + upto - here;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          if (k < c && equal.is(v[q], k)) {
+            if (at == r) sh->column = row.column(unit) + k;
+            ++at;
+          }
+        before += read_lane(upto, 63);
+      }
     }
   }
   __syncthreads();
@@ -458,7 +499,7 @@ template <class E> LCE_DEV int64_t sample_by_digits(const RowUnits<E>& row, cons
     at = draw_place(s, counted, all, by_min, at, &which, [&](const Want& want) { return find_place<true>(row, weights, sh, want); },
                     [&](const Place& p) { return weights.of(value_of(p.key)); });
   }
-  return column_of(row, at.key, which, &sh->columns);
+  return column_of(row, value_of(at.key), which, &sh->columns);
 }
 
 constexpr int kMostTop = 1024;
@@ -495,6 +536,27 @@ LCE_DEV void sort_list(u64* list, int sorted) {
       }
   }
   __syncthreads();
+}
+// The same into `to` for any number of entries up to kMostRanked, by counting for each those before it.  Starts and ends with a barrier.
+constexpr int kMostRanked = 512;
+LCE_DEV const u64* rank_list(const u64* list, u64* to, int n) {
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t < n) {
+    const u64 mine = list[t];
+    int rank = 0;
+    int j = 0;
+#pragma unroll 1
+    for (; j + 8 <= n; j += 8) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) rank += list[j + q] < mine ? 1 : 0;
+    }
+#pragma unroll 1
+    for (; j < n; ++j) rank += list[j] < mine ? 1 : 0;
+    to[rank] = mine;
+  }
+  __syncthreads();
+  return to;
 }
 LCE_DEV int power_of_two(int n) {
   int p = 2;
@@ -588,8 +650,9 @@ struct TopShared {
   };
   u64 list[kMostList];
   u64 of_wave[kSelectWaves];
-  unsigned least, top;
-  int listed;
+  int at_least[kSelectWaves];
+  unsigned top;
+  int listed, drawn;
 };
 
 // 16 bytes of a row as unsigned numbers in the order of the values (-0 just below 0), two of 16 bits or one of 32 bits to a word.
@@ -669,9 +732,9 @@ template <class E> struct RowPieces {
   }
 };
 
-// The list of a row's first elements: sh->list, sorted, k of them and more; returns whether it could be made.  sh->top: the ordered bits of the
+// The sorted list of a row's first elements, k of them and more; null if it could not be made.  sh->top: the ordered bits of the
 // largest element.  sums: sum exp(z - max) of the row for the caller's lse.
-template <class E, bool LSE> LCE_DEV bool list_first(const RowPieces<E>& row, int k, TopShared* sh, double* sums) {
+template <class E, bool LSE> LCE_DEV const u64* list_first(const RowPieces<E>& row, int k, TopShared* sh, double* sums) {
   typedef Ordered<E> O;
   constexpr int kPer = RowPieces<E>::kPer;
   const int t = threadIdx.x, lane = t & 63;
@@ -696,31 +759,32 @@ template <class E, bool LSE> LCE_DEV bool list_first(const RowPieces<E>& row, in
   const bool odd = __syncthreads_or(least < O::kLow || top >= O::kInf || top <= O::kLow);
   if (t == 0) {
     sh->top = top;
-    sh->listed = 0;
+    sh->listed = sh->drawn = 0;
   }
   if (odd) {
     __syncthreads();
-    return false;
+    return nullptr;
   }
-  // the largest number, of 16 bits, that k threads' maxima are not below
-  if (t < 64) {
-    unsigned of[kSelectThreads / 64];
+  // the largest number, of 16 bits, that k threads' maxima are not below: four bits at a time, a wave for each of their values
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  unsigned of[kSelectThreads / 64];
 #pragma unroll
-    for (int i = 0; i < kSelectThreads / 64; ++i) of[i] = sh->of_thread[i * 64 + lane];
-    unsigned bound = 0;
+  for (int i = 0; i < kSelectThreads / 64; ++i) of[i] = sh->of_thread[i * 64 + lane];
+  unsigned bound = 0;
 #pragma unroll 1
-    for (unsigned bit = 0x8000u; bit != 0; bit >>= 1) {
-      const unsigned mid = bound | bit;
-      int count = 0;
+  for (int shift = 12; shift >= 0; shift -= 4) {
+    const unsigned mid = bound | (unsigned)wave << shift;
+    int count = 0;
 #pragma unroll
-      for (int i = 0; i < kSelectThreads / 64; ++i) count += __popcll(__ballot(of[i] >= mid));
-      if (count >= k) bound = mid;
-    }
-    if (bound == 0x8000u) bound = 0x7fffu;  // (-0 is 0)
-    if (t == 0) sh->least = O::from_top_bits(bound);
+    for (int i = 0; i < kSelectThreads / 64; ++i) count += __popcll(__ballot(of[i] >= mid));
+    if (lane == 0) sh->at_least[wave] = count;
+    __syncthreads();
+    const u64 enough = __ballot(sh->at_least[lane & 15] >= k);  // (of value 0 there are: all that the bits before left)
+    bound |= (unsigned)(63 - __clzll((long long)((enough & 0xffffu) | 1))) << shift;
+    __syncthreads();
   }
-  __syncthreads();
-  const unsigned from = sh->least;
+  if (bound == 0x8000u) bound = 0x7fffu;  // (-0 is 0)
+  const unsigned from = O::from_top_bits(bound);
   const float m = O::value(top);
   float sum = 0.f;
   auto add = [&](int64_t at, unsigned a) {
@@ -765,12 +829,14 @@ template <class E, bool LSE> LCE_DEV bool list_first(const RowPieces<E>& row, in
   const int listed = sh->listed;
   if (listed > kMostList) {
     __syncthreads();  // (the caller may use the place of it all)
-    return false;
+    return nullptr;
   }
+  // (by ranks n^2 comparisons, by the network n log^2 n and a barrier each round)
+  if (listed <= kMostRanked) return rank_list(sh->list, sh->list + kMostRanked, listed);
   const int sorted = power_of_two(listed);
   for (int i = listed + t; i < sorted; i += kSelectThreads) sh->list[i] = ~(u64)0;
   sort_list(sh->list, sorted);
-  return listed >= k;
+  return sh->list;
 }
 
 // (64 registers a thread: two workgroups to a compute unit, of which one reads while the other sorts)
@@ -781,9 +847,10 @@ __global__ __launch_bounds__(kSelectThreads, 8) void top_kernel(const E* logits,
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
     double sums = 0.0;
-    if (k <= kMostByMaxima && list_first<E, LSE>(RowPieces<E>(from, cols), k, &sh, &sums)) {
+    const u64* list = k <= kMostByMaxima ? list_first<E, LSE>(RowPieces<E>(from, cols), k, &sh, &sums) : nullptr;
+    if (list != nullptr) {
       if (LSE && threadIdx.x == 0) lse[n] = (float)((double)Ordered<E>::value(sh.top) + log(sums));
-      store_top(RowUnits<E>(from, cols), sh.list, k, values + n * k, index + n * k);
+      store_top(RowUnits<E>(from, cols), list, k, values + n * k, index + n * k);
       __syncthreads();
     } else {
       top_by_digits(RowUnits<E>(from, cols), k, values + n * k, index + n * k, LSE ? lse + n : nullptr, &sh.digits, sh.list, &sh.listed);
@@ -792,11 +859,15 @@ __global__ __launch_bounds__(kSelectThreads, 8) void top_kernel(const E* logits,
 }
 
 // The token of a row whose first k are listed, k of them kept by top_k (1: the first column).
-template <class E> LCE_DEV int64_t sample_listed(const RowSettings& s, int k, TopShared* sh) {
-  if (s.greedy()) return column_in(sh->list[0]);
-  const Weights weights = s.weights(value_of(key_in(sh->list[0])));
+LCE_DEV int64_t sample_listed(const RowSettings& s, int k, const u64* list, TopShared* sh) {
+  if (s.greedy()) {
+    const int64_t column = column_in(list[0]);
+    __syncthreads();
+    return column;
+  }
+  const Weights weights = s.weights(value_of(key_in(list[0])));
   const int t = threadIdx.x;
-  const double real = t < k ? weights.real(value_of(key_in(sh->list[t]))) : 0.0;
+  const double real = t < k ? weights.real(value_of(key_in(list[t]))) : 0.0;
   const u64 w = weights.fixed(real);
   u64 before;
   u64 stays = block_all<Sum>(w, sh->of_wave, &before);
@@ -807,10 +878,10 @@ template <class E> LCE_DEV int64_t sample_listed(const RowSettings& s, int k, To
   const double some = (double)s.u * (double)stays;
   u64 target = some > 0.0 ? (u64)some : 0;
   if (target >= stays) target = stays - 1;
-  if (w != 0 && before <= target && target - before < w) sh->least = (unsigned)t;  // (one thread)
+  if (w != 0 && before <= target && target - before < w) sh->drawn = t;  // (one thread)
   __syncthreads();
-  const int at = (int)sh->least & (kMostList - 1);
-  const int64_t column = column_in(sh->list[at]);
+  const int at = sh->drawn;
+  const int64_t column = column_in(list[at]);
   __syncthreads();
   return column;
 }
@@ -824,8 +895,9 @@ __global__ __launch_bounds__(kSelectThreads, 8) void sample_top_kernel(const E* 
     const E* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
     const int64_t k = s.greedy() ? 1 : s.top_k < cols ? s.top_k : cols;
+    const u64* list = list_first<E, false>(RowPieces<E>(from, cols), (int)k, &sh, nullptr);
     int64_t column;
-    if (list_first<E, false>(RowPieces<E>(from, cols), (int)k, &sh, nullptr)) column = sample_listed<E>(s, (int)k, &sh);
+    if (list != nullptr) column = sample_listed(s, (int)k, list, &sh);
     else column = sample_by_digits(RowUnits<E>(from, cols), s, &sh.digits);
     if (threadIdx.x == 0) token[n] = column;
     __syncthreads();
@@ -840,9 +912,10 @@ __global__ __launch_bounds__(kSelectThreads) void sample_float_kernel(const floa
     const float* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
     const int64_t k = s.greedy() ? 1 : s.top_k;
+    const u64* list = nullptr;
+    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<float, false>(RowPieces<float>(from, cols), (int)k, &sh, nullptr);
     int64_t column;
-    if (k >= 1 && k <= kMostByMaxima && k < cols && list_first<float, false>(RowPieces<float>(from, cols), (int)k, &sh, nullptr))
-      column = sample_listed<float>(s, (int)k, &sh);
+    if (list != nullptr) column = sample_listed(s, (int)k, list, &sh);
     else column = sample_by_digits(RowUnits<float>(from, cols), s, &sh.digits);
     if (threadIdx.x == 0) token[n] = column;
     __syncthreads();
@@ -1024,13 +1097,6 @@ template <class E> struct HalfRow {
   }
 };
 
-// Whether either half of a word equals that of `twice`, a number's bits in both halves, after `mask`.  (Also where the upper half is off by one and
-// the lower half is equal: a filter.)
-LCE_DEV bool equal_half(unsigned word, unsigned twice, unsigned mask) {
-  const unsigned x = (word & mask) ^ twice;
-  return ((x - 0x00010001u) & ~x & 0x80008000u) != 0;
-}
-
 template <class E>
 __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
                                                                      const Sampling settings, int bits, int64_t* token) {
@@ -1042,10 +1108,12 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
     const RowPieces<E> row(from, cols);
     const HalfRow<E> half = {sh};
     const int64_t k = s.greedy() ? 1 : s.top_k;
+    const u64* list = nullptr;
+    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(row, (int)k, &sh->top, nullptr);
     int64_t column;
     int different;
-    if (k >= 1 && k <= kMostByMaxima && k < cols && list_first<E, false>(row, (int)k, &sh->top, nullptr)) {
-      column = sample_listed<E>(s, (int)k, &sh->top);
+    if (list != nullptr) {
+      column = sample_listed(s, (int)k, list, &sh->top);
     } else if (!s.greedy() && half.fill(row, &different)) {
       const unsigned top = sh->values[0] & 0xffffu;
       const Weights weights = s.weights(half_value<E>(top));
@@ -1069,7 +1137,7 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
                                   [&](const Want& want) { return half.find(weights, different, cb, wb, elements, weight, want); },
                                   [&](const Place& p) { return weights.of(half_value<E>(p.key)); });
       __syncthreads();  // (the list of values is not read any more)
-      column = column_of(RowUnits<E>(from, cols), key_of(half_value<E>(at.key)), which, &sh->columns);
+      column = column_of(RowUnits<E>(from, cols), half_value<E>(at.key), which, &sh->columns);
     } else {
       __syncthreads();
       column = sample_by_digits(RowUnits<E>(from, cols), s, &sh->top.digits);
