@@ -17,8 +17,8 @@ namespace lce {
 
 namespace {
 
-constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kDigits = 2048;  // values of a digit
+constexpr int kMostWaves = 16;  // of a workgroup
 typedef unsigned long long u64;
 
 constexpr unsigned kNanKey = 0xffffffffu, kLowKey = 0x007fffffu;  // NaN; -infinity
@@ -42,8 +42,8 @@ template <> struct bits_of<4> { typedef unsigned type; };
 
 // A row in units of up to 16 bytes: its elements before the first address of 16 bytes, whole pieces, the rest.  Wave w has the units
 // [w * share, (w + 1) * share), 64 neighbouring ones at a time, so that (wave, round, lane, element) is the order of the columns.
-template <class E> struct RowUnits {
-  static constexpr int kPer = 16 / sizeof(E);
+template <class E, int NT> struct RowUnits {
+  static constexpr int kPer = 16 / sizeof(E), kThreads = NT, kWaves = NT / 64;
   const E* p;
   int64_t head, body, n, share, units;
   LCE_DEV RowUnits(const E* row, int64_t cols) : p(row), n(cols) {
@@ -51,7 +51,7 @@ template <class E> struct RowUnits {
     head = off < n ? off : n;
     body = (n - head) / kPer;
     units = body + 2;
-    share = (units + kSelectThreads - 1) / kSelectThreads * 64;
+    share = (units + NT - 1) / NT * 64;
   }
   LCE_DEV int64_t column(int64_t unit) const { return unit == 0 ? 0 : head + (unit - 1) * kPer; }
   LCE_DEV int count(int64_t unit) const {
@@ -128,13 +128,13 @@ template <class J, class F, bool ROW = false> LCE_DEV F wave_upto(F v) {
   return v;
 }
 // Over the workgroup; `sh`: room for one value of each wave.  *before (sums): over the threads before this one.  Ends with a barrier.
-static_assert(kSelectWaves == 16, "a row of lanes joins the waves' values");
-template <class J, class F> LCE_DEV F block_all(F v, F* sh, F* before = nullptr) {
+template <class J, int NT, class F> LCE_DEV F block_all(F v, F* sh, F* before = nullptr) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const F upto = wave_upto<J>(v);
   if (lane == 63) sh[wave] = upto;
   __syncthreads();
-  const F waves = wave_upto<J, F, true>(sh[lane & 15]);
+  static_assert(NT / 64 <= 16, "a row of lanes joins the waves' values");
+  const F waves = wave_upto<J, F, true>((lane & 15) < NT / 64 ? sh[lane & 15] : F(0));
   __syncthreads();
   if (before != nullptr) *before = upto - v + (wave > 0 ? read_lane(waves, wave - 1) : F(0));
   return read_lane(waves, 15);
@@ -177,12 +177,12 @@ template <> struct Equal<float> {
 // count such elements, by parts of their share of the row, and the one that has the r-th looks for it in its part.
 constexpr int kParts = 32, kPartRounds = 8;  // rounds that are in flight together
 struct ColumnShared {
-  int count[kSelectWaves][kParts];
-  int64_t of_wave[kSelectWaves];
+  int count[kMostWaves][kParts];
+  int64_t of_wave[kMostWaves];
   int64_t column;
 };
-template <class E> LCE_DEV int64_t column_of(const RowUnits<E>& row, float value, int64_t r, ColumnShared* sh) {
-  constexpr int kPer = RowUnits<E>::kPer;
+template <class E, int NT> LCE_DEV int64_t column_of(const RowUnits<E, NT>& row, float value, int64_t r, ColumnShared* sh) {
+  constexpr int kPer = RowUnits<E, NT>::kPer;
   const Equal<E> equal(value);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t u0 = wave * row.share, left = (row.units - u0 + 63) / 64, share = row.share / 64;
@@ -217,7 +217,7 @@ template <class E> LCE_DEV int64_t column_of(const RowUnits<E>& row, float value
   __syncthreads();
   int64_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) before += w < wave ? sh->of_wave[w] : 0;
+  for (int w = 0; w < NT / 64; ++w) before += w < wave ? sh->of_wave[w] : 0;
   if (before <= r && r < before + mine) {  // (one wave)
     int64_t i = 0;
     for (int part = 0; part < kParts - 1 && before + sh->count[wave][part] <= r; ++part, i += per) before += sh->count[wave][part];
@@ -286,9 +286,13 @@ struct NoWeights {
   LCE_DEV u64 of(float) const { return 0; }
 };
 
-struct Histogram {
+template <bool WEIGHTED> struct Histogram;
+template <> struct Histogram<false> {
   int count[kDigits];
+};
+template <> struct Histogram<true> {
   u64 weight[kDigits];
+  int count[kDigits];
 };
 LCE_DEV int digit_of(unsigned key, int level) { return level == 0 ? key >> 21 : level == 1 ? (key >> 10) & 2047 : key & 1023; }
 LCE_DEV bool in_prefix(unsigned key, unsigned prefix, int level) {
@@ -297,20 +301,20 @@ LCE_DEV bool in_prefix(unsigned key, unsigned prefix, int level) {
 
 // Histogram of the digit `level` over the elements that agree with `prefix` in the digits before it.  WEIGHTED: elements without
 // a weight, which are never drawn, are left out.  Ends with a barrier.
-template <bool WEIGHTED, class E, class W>
-LCE_DEV void fill_histogram(const RowUnits<E>& row, const W& weights, unsigned prefix, int level, Histogram* h) {
-  for (int i = threadIdx.x; i < kDigits; i += kSelectThreads) {
+template <bool WEIGHTED, class E, int NT, class W>
+LCE_DEV void fill_histogram(const RowUnits<E, NT>& row, const W& weights, unsigned prefix, int level, Histogram<WEIGHTED>* h) {
+  for (int i = threadIdx.x; i < kDigits; i += NT) {
     h->count[i] = 0;
-    if (WEIGHTED) h->weight[i] = 0;
+    if constexpr (WEIGHTED) h->weight[i] = 0;
   }
   __syncthreads();
   row.each([&](int64_t, const E* e, int c) {
 #pragma unroll
-    for (int i = 0; i < RowUnits<E>::kPer; ++i) {
+    for (int i = 0; i < RowUnits<E, NT>::kPer; ++i) {
       const float z = as_float(e[i]);
       const unsigned key = key_of(z);
       if (i >= c || !in_prefix(key, prefix, level)) continue;
-      if (WEIGHTED) {
+      if constexpr (WEIGHTED) {
         const u64 w = key == kLowKey ? 0 : weights.of(z);
         if (w == 0) continue;
         atomicAdd(&h->weight[digit_of(key, level)], w);
@@ -328,35 +332,42 @@ struct Place {
   u64 weight;
   int64_t same;  // elements with the key
 };
-struct SelectShared {
-  Histogram first, next;
+// KEEP: the first digit's histogram stays for the next place that a row asks for.
+template <bool WEIGHTED, bool KEEP> struct SelectShared {
+  Histogram<WEIGHTED> first[1], next[KEEP ? 1 : 0];
+  LCE_DEV Histogram<WEIGHTED>* of_level(int level) {
+    if constexpr (KEEP) return level == 0 ? first : next;
+    else return first;
+  }
   Place place;
-  u64 of_wave[kSelectWaves];
+  u64 of_wave[kMostWaves];
   ColumnShared columns;
 };
 
 // The histogram of the first digit; returns the weight of the elements with a key of `least` and above.
-template <class E> LCE_DEV u64 fill_first(const RowUnits<E>& row, const Weights& weights, unsigned least, SelectShared* sh) {
-  for (int i = threadIdx.x; i < kDigits; i += kSelectThreads) {
-    sh->first.count[i] = 0;
-    sh->first.weight[i] = 0;
+template <class E, int NT, class Shared>
+LCE_DEV u64 fill_first(const RowUnits<E, NT>& row, const Weights& weights, unsigned least, Shared* sh) {
+  Histogram<true>* h = sh->first;
+  for (int i = threadIdx.x; i < kDigits; i += NT) {
+    h->count[i] = 0;
+    h->weight[i] = 0;
   }
   __syncthreads();
   u64 mine = 0;
   row.each([&](int64_t, const E* e, int c) {
 #pragma unroll
-    for (int i = 0; i < RowUnits<E>::kPer; ++i) {
+    for (int i = 0; i < RowUnits<E, NT>::kPer; ++i) {
       const float z = as_float(e[i]);
       const unsigned key = key_of(z);
       if (i >= c || key == kLowKey) continue;
       const u64 w = weights.of(z);
       if (w == 0) continue;
       if (key >= least) mine += w;
-      atomicAdd(&sh->first.weight[digit_of(key, 0)], w);
-      atomicAdd(&sh->first.count[digit_of(key, 0)], 1);
+      atomicAdd(&h->weight[digit_of(key, 0)], w);
+      atomicAdd(&h->count[digit_of(key, 0)], 1);
     }
   });
-  return block_all<Sum>(mine, sh->of_wave);
+  return block_all<Sum, NT>(mine, sh->of_wave);
 }
 
 // What a place is looked for by: the k-th element; the last key with an element before which there is less than `most` weight; the
@@ -376,28 +387,41 @@ struct Want {
   }
 };
 
-// The place that is wanted.  WEIGHTED: the histogram of the first digit is there (fill_first).
-template <bool WEIGHTED, class E, class W>
-LCE_DEV Place find_place(const RowUnits<E>& row, const W& weights, SelectShared* sh, const Want& want) {
+// The place that is wanted.  KEEP: the histogram of the first digit is there (fill_first).
+template <bool WEIGHTED, bool KEEP, class E, int NT, class W>
+LCE_DEV Place find_place(const RowUnits<E, NT>& row, const W& weights, SelectShared<WEIGHTED, KEEP>* sh, const Want& want) {
+  constexpr int kOwn = kDigits / NT;  // digits of a thread, the largest first
   Place p = {0, 0, 0, 0};
 #pragma unroll 1
   for (int level = 0; level < 3; ++level) {
-    Histogram* h = level == 0 ? &sh->first : &sh->next;
-    if (level > 0 || !WEIGHTED) fill_histogram<WEIGHTED>(row, weights, p.key, level, h);
-    const int d1 = kDigits - 1 - 2 * (int)threadIdx.x, d0 = d1 - 1;  // this thread's digits, the larger first
-    const int c1 = h->count[d1], c0 = h->count[d0];
-    const u64 w1 = WEIGHTED ? h->weight[d1] : 0, w0 = WEIGHTED ? h->weight[d0] : 0;
+    Histogram<WEIGHTED>* h = sh->of_level(level);
+    if (level > 0 || !KEEP) fill_histogram<WEIGHTED>(row, weights, p.key, level, h);
+    const int top = kDigits - 1 - kOwn * (int)threadIdx.x;
+    int c = 0;
+    u64 w = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      c += h->count[top - i];
+      if constexpr (WEIGHTED) w += h->weight[top - i];
+    }
     int c_before;
     u64 w_before = 0;
-    block_all<Sum>(c1 + c0, reinterpret_cast<int*>(sh->of_wave), &c_before);
-    if (WEIGHTED) block_all<Sum>(w1 + w0, sh->of_wave, &w_before);
+    block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave), &c_before);
+    if (WEIGHTED) block_all<Sum, NT>(w, sh->of_wave, &w_before);
     int64_t cb = p.count + c_before;
     u64 wb = p.weight + w_before;
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
-    if (want.here(cb, wb, c1, w1)) sh->place = {p.key | (unsigned)d1 << shift, cb, wb, c1};
-    cb += c1;
-    wb += w1;
-    if (want.here(cb, wb, c0, w0)) sh->place = {p.key | (unsigned)d0 << shift, cb, wb, c0};
+    if (want.here(cb, wb, c, w)) {
+#pragma unroll 1
+      for (int d = top; d > top - kOwn; --d) {
+        const int cd = h->count[d];
+        u64 wd = 0;
+        if constexpr (WEIGHTED) wd = h->weight[d];
+        if (want.here(cb, wb, cd, wd)) sh->place = {p.key | (unsigned)d << shift, cb, wb, cd};
+        cb += cd;
+        wb += wd;
+      }
+    }
     __syncthreads();
     p = sh->place;
     __syncthreads();
@@ -406,16 +430,16 @@ LCE_DEV Place find_place(const RowUnits<E>& row, const W& weights, SelectShared*
 }
 
 // The largest key of the row.
-template <class E> LCE_DEV unsigned largest_key(const RowUnits<E>& row, unsigned* sh) {
+template <class E, int NT> LCE_DEV unsigned largest_key(const RowUnits<E, NT>& row, unsigned* sh) {
   unsigned top = 0;
   row.each([&](int64_t, const E* e, int c) {
 #pragma unroll
-    for (int i = 0; i < RowUnits<E>::kPer; ++i) {
+    for (int i = 0; i < RowUnits<E, NT>::kPer; ++i) {
       const unsigned k = key_of(as_float(e[i]));
       top = i < c && k > top ? k : top;
     }
   });
-  return block_all<Largest>(top, sh);
+  return block_all<Largest, NT>(top, sh);
 }
 
 // Settings of a row.
@@ -474,7 +498,8 @@ LCE_DEV Place draw_place(const RowSettings& s, int64_t counted, u64 all, u64 by_
 }
 
 // The token of a row by digits, any type; -1 where there is none.
-template <class E> LCE_DEV int64_t sample_by_digits(const RowUnits<E>& row, const RowSettings& s, SelectShared* sh) {
+template <class E, int NT, bool KEEP>
+LCE_DEV int64_t sample_by_digits(const RowUnits<E, NT>& row, const RowSettings& s, SelectShared<true, KEEP>* sh) {
   const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh->of_wave));
   if (top == kNanKey || top == kLowKey) return -1;  // a NaN, or no column left
   Place at = {top, 0, 0, 0};
@@ -493,10 +518,17 @@ template <class E> LCE_DEV int64_t sample_by_digits(const RowUnits<E>& row, cons
       }
     }
     const u64 by_min = fill_first(row, weights, s.min_p > 0.f ? least : 0, sh);
-    const int t2 = 2 * (int)threadIdx.x;
-    const u64 all = block_all<Sum>(sh->first.weight[t2] + sh->first.weight[t2 + 1], sh->of_wave);
-    const int64_t counted = (int64_t)block_all<Sum>((u64)(sh->first.count[t2] + sh->first.count[t2 + 1]), sh->of_wave);
-    at = draw_place(s, counted, all, by_min, at, &which, [&](const Want& want) { return find_place<true>(row, weights, sh, want); },
+    u64 w = 0;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kDigits / NT; ++i) {
+      w += sh->first->weight[i * NT + threadIdx.x];
+      c += sh->first->count[i * NT + threadIdx.x];
+    }
+    const u64 all = block_all<Sum, NT>(w, sh->of_wave);
+    const int counted = block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave));
+    at = draw_place(s, counted, all, by_min, at, &which,
+                    [&](const Want& want) { return find_place<true, KEEP>(row, weights, sh, want); },
                     [&](const Place& p) { return weights.of(value_of(p.key)); });
   }
   return column_of(row, value_of(at.key), which, &sh->columns);
@@ -511,7 +543,7 @@ LCE_DEV int64_t column_in(u64 entry) { return (int64_t)(entry & 0xffffffffu); }
 
 // A bitonic network over list[0 .. sorted), a power of two from 2 on; up to 128 entries by one wave, without barriers in between.
 // Starts and ends with a barrier.
-LCE_DEV void sort_list(u64* list, int sorted) {
+template <int NT> LCE_DEV void sort_list(u64* list, int sorted) {
   __syncthreads();
   const bool one_wave = sorted <= 128;
   if (!one_wave || threadIdx.x < 64) {
@@ -519,7 +551,7 @@ LCE_DEV void sort_list(u64* list, int sorted) {
     for (int size = 2; size <= sorted; size <<= 1)
 #pragma unroll 1
       for (int d = size >> 1; d > 0; d >>= 1) {
-        for (int t = threadIdx.x; t < sorted / 2; t += kSelectThreads) {
+        for (int t = threadIdx.x; t < sorted / 2; t += NT) {
           const int i = ((t & ~(d - 1)) << 1) | (t & (d - 1)), j = i | d;  // the t-th pair
           const u64 a = list[i], b = list[j];
           if ((a > b) == ((i & size) == 0)) {
@@ -539,10 +571,9 @@ LCE_DEV void sort_list(u64* list, int sorted) {
 }
 // The same into `to` for any number of entries up to kMostRanked, by counting for each those before it.  Starts and ends with a barrier.
 constexpr int kMostRanked = 512;
-LCE_DEV const u64* rank_list(const u64* list, u64* to, int n) {
+template <int NT> LCE_DEV const u64* rank_list(const u64* list, u64* to, int n) {
   __syncthreads();
-  const int t = threadIdx.x;
-  if (t < n) {
+  for (int t = threadIdx.x; t < n; t += NT) {
     const u64 mine = list[t];
     int rank = 0;
     int j = 0;
@@ -564,8 +595,8 @@ LCE_DEV int power_of_two(int n) {
   return p;
 }
 // The first k of the list to memory.
-template <class E> LCE_DEV void store_top(const RowUnits<E>& row, const u64* list, int k, E* values, int64_t* index) {
-  for (int i = threadIdx.x; i < k; i += kSelectThreads) {
+template <class E, int NT> LCE_DEV void store_top(const RowUnits<E, NT>& row, const u64* list, int k, E* values, int64_t* index) {
+  for (int i = threadIdx.x; i < k; i += NT) {
     int64_t column = column_in(list[i]);
     column = column < row.n ? column : row.n - 1;  // (logits that change under the kernel must not lead it astray)
     index[i] = column;
@@ -574,9 +605,10 @@ template <class E> LCE_DEV void store_top(const RowUnits<E>& row, const u64* lis
 }
 
 // The first k of a row by digits, any type.  list: kMostTop entries.
-template <class E>
-LCE_DEV void top_by_digits(const RowUnits<E>& row, int k, E* values, int64_t* index, float* lse, SelectShared* sh, u64* list, int* listed) {
-  constexpr int kPer = RowUnits<E>::kPer;
+template <class E, int NT>
+LCE_DEV void top_by_digits(const RowUnits<E, NT>& row, int k, E* values, int64_t* index, float* lse, SelectShared<false, false>* sh, u64* list,
+                           int* listed) {
+  constexpr int kPer = RowUnits<E, NT>::kPer;
   if (lse != nullptr) {
     const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh->of_wave));
     const float m = top == kNanKey ? __builtin_nanf("") : value_of(top);
@@ -588,14 +620,14 @@ LCE_DEV void top_by_digits(const RowUnits<E>& row, int k, E* values, int64_t* in
         if (i < c) sum += z == m ? 1.f : __expf(z - m);  // (equal infinities have no difference)
       }
     });
-    const double all = block_all<Sum>((double)sum, reinterpret_cast<double*>(sh->of_wave));
+    const double all = block_all<Sum, NT>((double)sum, reinterpret_cast<double*>(sh->of_wave));
     if (threadIdx.x == 0) *lse = top == kLowKey ? m : (float)((double)m + log(all));
   }
-  const Place p = find_place<false>(row, NoWeights(), sh, Want{kByCount, k, 0.0, 0});
+  const Place p = find_place<false, false>(row, NoWeights(), sh, Want{kByCount, k, 0.0, 0});
   // what is larger, in any order, and the first k - p.count of the key in the order of the columns
   const int sorted = power_of_two(k), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (threadIdx.x == 0) *listed = 0;
-  if ((int)threadIdx.x < sorted) list[threadIdx.x] = ~(u64)0;
+  for (int i = threadIdx.x; i < sorted; i += NT) list[i] = ~(u64)0;
   __syncthreads();
   int mine = 0;
   row.each([&](int64_t unit, const E* e, int c) {
@@ -631,7 +663,7 @@ LCE_DEV void top_by_digits(const RowUnits<E>& row, int k, E* values, int64_t* in
       before += read_lane(of_unit, 63);
     });
   }
-  sort_list(list, sorted);
+  sort_list<NT>(list, sorted);
   store_top(row, list, k, values, index);
   __syncthreads();
 }
@@ -642,15 +674,22 @@ LCE_DEV void top_by_digits(const RowUnits<E>& row, int k, E* values, int64_t* in
 // takes maxima, one that compares (and sums the exponentials for lse).  Rows whose list would be too long (most elements equal, or
 // fewer than k threads with one), with a NaN or an infinity on top are done by digits.
 // ---------------------------------------------------------------------------------------------------------------------------
-constexpr int kMostByMaxima = 512, kMostList = 2048;
-struct TopShared {
+constexpr int kMostByMaxima = 512, kMostList = 2048, kMaxima = 1024;
+// Digits: the shared memory of the rows that are done by digits.
+template <class Digits> struct TopShared {
   union {
-    SelectShared digits;
-    unsigned of_thread[kSelectThreads];
+    struct {
+      Digits digits;
+      u64 by_digits[kMostTop];  // (the list of top_by_digits)
+    };
+    struct {
+      u64 list[kMostList];
+      unsigned maxima[kMaxima];
+    };
   };
-  u64 list[kMostList];
-  u64 of_wave[kSelectWaves];
-  int at_least[kSelectWaves];
+  u64 of_wave[kMostWaves];
+  int at_least[2][kMostWaves];
+  double sums[kMostWaves];
   unsigned top;
   int listed, drawn;
 };
@@ -692,10 +731,10 @@ template <> struct Ordered<__bf16> : OrderedHalf<__bf16> { static constexpr unsi
 template <> struct Ordered<_Float16> : OrderedHalf<_Float16> { static constexpr unsigned kLow = 0x03ff, kInf = 0xfc00; };
 
 // Whole pieces of a row, dealt to the threads one by one, and the elements before and behind them.
-template <class E> struct RowPieces {
+template <class E, int NT> struct RowPieces {
   typedef Ordered<E> O;
   typedef typename bits_of<sizeof(E)>::type Bits;
-  static constexpr int kPer = 16 / sizeof(E), kFlight = 4;
+  static constexpr int kPer = 16 / sizeof(E), kFlight = 4, kThreads = NT;
   const E* p;
   int64_t n, head, body;
   LCE_DEV RowPieces(const E* row, int64_t cols) : p(row), n(cols) {
@@ -712,76 +751,74 @@ template <class E> struct RowPieces {
       f(at, sizeof(E) == 2 ? w & 0xffffu : w);
     }
   }
-  // f(column of the first, piece), kFlight pieces in flight.
+  // f(column of the first, piece, which of its round), kFlight pieces in flight.
   template <class F> LCE_DEV void each(F f) const {
     const u32x4_t* from = reinterpret_cast<const u32x4_t*>(p + head);
 #pragma unroll 1
-    for (int64_t base = threadIdx.x; base < body; base += kFlight * kSelectThreads) {
+    for (int64_t base = threadIdx.x; base < body; base += kFlight * NT) {
       u32x4_t v[kFlight];
 #pragma unroll
       for (int r = 0; r < kFlight; ++r) {
-        const int64_t at = base + r * kSelectThreads;
+        const int64_t at = base + r * NT;
         v[r] = from[at < body ? at : base];
       }
 #pragma unroll
       for (int r = 0; r < kFlight; ++r) {
-        const int64_t at = base + r * kSelectThreads;
-        if (at < body) f(head + at * kPer, v[r]);
+        const int64_t at = base + r * NT;
+        if (at < body) f(head + at * kPer, v[r], r);
       }
     }
   }
 };
 
 // The sorted list of a row's first elements, k of them and more; null if it could not be made.  sh->top: the ordered bits of the
-// largest element.  sums: sum exp(z - max) of the row for the caller's lse.
-template <class E, bool LSE> LCE_DEV const u64* list_first(const RowPieces<E>& row, int k, TopShared* sh, double* sums) {
+// largest element; sh->sums: by waves, sum exp(z - max) of the row (LSE).
+template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first(const RowPieces<E, NT>& row, int k, Shared* sh) {
   typedef Ordered<E> O;
-  constexpr int kPer = RowPieces<E>::kPer;
-  const int t = threadIdx.x, lane = t & 63;
-  unsigned most = 0, least = ~0u;
+  constexpr int kPer = RowPieces<E, NT>::kPer, kOwn = kMaxima / NT, kWaves = NT / 64;  // maxima of a thread: of every kOwn-th piece
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  unsigned most[kOwn] = {}, least = ~0u;
   row.edges([&](int64_t, unsigned a) {
-    most = O::larger(most, a);  // (of 16 bits: the upper half stays as it is)
+    most[0] = O::larger(most[0], a);  // (of 16 bits: the upper half stays as it is)
     least = O::smaller(least, sizeof(E) == 2 ? a | 0xffff0000u : a);
   });
-  row.each([&](int64_t, u32x4_t v) {
+  row.each([&](int64_t, u32x4_t v, int r) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const unsigned a = O::word(v[i]);
-      most = O::larger(most, a);
+      most[r % kOwn] = O::larger(most[r % kOwn], a);
       least = O::smaller(least, a);
     }
   });
-  most = O::largest(most);
-  least = O::smallest(least);
-  sh->of_thread[t] = O::in_top_bits(most);
-  const unsigned top = block_all<Largest>(most, reinterpret_cast<unsigned*>(sh->of_wave));
-  // (a NaN is above +inf or below -inf)
-  const bool odd = __syncthreads_or(least < O::kLow || top >= O::kInf || top <= O::kLow);
-  if (t == 0) {
-    sh->top = top;
-    sh->listed = sh->drawn = 0;
-  }
-  if (odd) {
-    __syncthreads();
-    return nullptr;
-  }
-  // the largest number, of 16 bits, that k threads' maxima are not below: four bits at a time, a wave for each of their values
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  unsigned of[kSelectThreads / 64];
+  unsigned largest = 0;
 #pragma unroll
-  for (int i = 0; i < kSelectThreads / 64; ++i) of[i] = sh->of_thread[i * 64 + lane];
+  for (int i = 0; i < kOwn; ++i) {
+    most[i] = O::largest(most[i]);
+    sh->maxima[i * NT + t] = O::in_top_bits(most[i]);
+    largest = most[i] > largest ? most[i] : largest;
+  }
+  if (O::smallest(least) < O::kLow) largest = ~0u;  // (a NaN is above +inf or below -inf)
+  if (t == 0) sh->listed = sh->drawn = 0;
+  const unsigned top = block_all<Largest, NT>(largest, reinterpret_cast<unsigned*>(sh->of_wave));
+  if (top >= O::kInf || top <= O::kLow) return nullptr;
+  // the largest number, of 16 bits, that k maxima are not below: some bits at a time, a wave for each of their values
+  constexpr int kBits = kWaves == 16 ? 4 : 3;
+  static_assert(kWaves == 1 << kBits, "a wave to a value");
+  unsigned of[kMaxima / 64];
+#pragma unroll
+  for (int i = 0; i < kMaxima / 64; ++i) of[i] = sh->maxima[i * 64 + lane];
   unsigned bound = 0;
+  int buffer = 0;
 #pragma unroll 1
-  for (int shift = 12; shift >= 0; shift -= 4) {
+  for (int shift = 15 / kBits * kBits; shift >= 0; shift -= kBits, buffer ^= 1) {
     const unsigned mid = bound | (unsigned)wave << shift;
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < kSelectThreads / 64; ++i) count += __popcll(__ballot(of[i] >= mid));
-    if (lane == 0) sh->at_least[wave] = count;
+    for (int i = 0; i < kMaxima / 64; ++i) count += __popcll(__ballot(of[i] >= mid));
+    if (lane == 0) sh->at_least[buffer][wave] = count;
     __syncthreads();
-    const u64 enough = __ballot(sh->at_least[lane & 15] >= k);  // (of value 0 there are: all that the bits before left)
-    bound |= (unsigned)(63 - __clzll((long long)((enough & 0xffffu) | 1))) << shift;
-    __syncthreads();
+    const u64 enough = __ballot(sh->at_least[buffer][lane & (kWaves - 1)] >= k);  // (of value 0 there are: all that the bits before left)
+    bound |= (unsigned)(63 - __clzll((long long)((enough & ((1u << kWaves) - 1)) | 1))) << shift;
   }
   if (bound == 0x8000u) bound = 0x7fffu;  // (-0 is 0)
   const unsigned from = O::from_top_bits(bound);
@@ -798,7 +835,7 @@ template <class E, bool LSE> LCE_DEV const u64* list_first(const RowPieces<E>& r
     add(at, a);
     if (LSE) term(O::value(a));
   });
-  row.each([&](int64_t at, u32x4_t v) {
+  row.each([&](int64_t at, u32x4_t v, int) {
     unsigned best = 0;
     u32x4_t a;
 #pragma unroll
@@ -807,14 +844,15 @@ template <class E, bool LSE> LCE_DEV const u64* list_first(const RowPieces<E>& r
       best = O::larger(best, a[i]);
     }
     if (O::largest(best) >= from) {
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < 4; ++i) {
         if (sizeof(E) == 2) {
-          add(at + 2 * i, a[i] & 0xffffu);
-          add(at + 2 * i + 1, a[i] >> 16);
+          add(at + 2 * i, a[0] & 0xffffu);
+          add(at + 2 * i + 1, a[0] >> 16);
         } else {
-          add(at + i, a[i]);
+          add(at + i, a[0]);
         }
+        a = u32x4_t{a[1], a[2], a[3], 0};
       }
     }
     if (LSE) {
@@ -824,7 +862,11 @@ template <class E, bool LSE> LCE_DEV const u64* list_first(const RowPieces<E>& r
       for (int i = 0; i < kPer; ++i) term(as_float(e[i]));
     }
   });
-  if (LSE) *sums = block_all<Sum>((double)sum, reinterpret_cast<double*>(sh->of_wave));
+  if (LSE) {
+    const double upto = wave_upto<Sum>((double)sum);
+    if (lane == 63) sh->sums[wave] = upto;
+  }
+  if (t == 0) sh->top = top;
   __syncthreads();
   const int listed = sh->listed;
   if (listed > kMostList) {
@@ -832,49 +874,56 @@ template <class E, bool LSE> LCE_DEV const u64* list_first(const RowPieces<E>& r
     return nullptr;
   }
   // (by ranks n^2 comparisons, by the network n log^2 n and a barrier each round)
-  if (listed <= kMostRanked) return rank_list(sh->list, sh->list + kMostRanked, listed);
+  if (listed <= kMostRanked) return rank_list<NT>(sh->list, sh->list + kMostRanked, listed);
   const int sorted = power_of_two(listed);
-  for (int i = listed + t; i < sorted; i += kSelectThreads) sh->list[i] = ~(u64)0;
-  sort_list(sh->list, sorted);
+  for (int i = listed + t; i < sorted; i += NT) sh->list[i] = ~(u64)0;
+  sort_list<NT>(sh->list, sorted);
   return sh->list;
 }
 
-// (64 registers a thread: two workgroups to a compute unit, of which one reads while the other sorts)
+// (64 registers a thread and little LDS: several workgroups to a compute unit, of which some read while others sort)
+constexpr int kTopThreads = 512;
 template <class E, bool LSE>
-__global__ __launch_bounds__(kSelectThreads, 8) void top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values,
-                                                                int64_t* index, float* lse) {
-  __shared__ TopShared sh;
+__global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values,
+                                                             int64_t* index, float* lse) {
+  constexpr int NT = kTopThreads;
+  __shared__ TopShared<SelectShared<false, false>> sh;
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
-    double sums = 0.0;
-    const u64* list = k <= kMostByMaxima ? list_first<E, LSE>(RowPieces<E>(from, cols), k, &sh, &sums) : nullptr;
+    const u64* list = k <= kMostByMaxima ? list_first<E, LSE>(RowPieces<E, NT>(from, cols), k, &sh) : nullptr;
     if (list != nullptr) {
-      if (LSE && threadIdx.x == 0) lse[n] = (float)((double)Ordered<E>::value(sh.top) + log(sums));
-      store_top(RowUnits<E>(from, cols), list, k, values + n * k, index + n * k);
+      if (LSE && threadIdx.x == NT - 1) {
+        double sums = 0.0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) sums += sh.sums[w];
+        lse[n] = (float)((double)Ordered<E>::value(sh.top) + log(sums));
+      }
+      store_top(RowUnits<E, NT>(from, cols), list, k, values + n * k, index + n * k);
       __syncthreads();
     } else {
-      top_by_digits(RowUnits<E>(from, cols), k, values + n * k, index + n * k, LSE ? lse + n : nullptr, &sh.digits, sh.list, &sh.listed);
+      top_by_digits(RowUnits<E, NT>(from, cols), k, values + n * k, index + n * k, LSE ? lse + n : nullptr, &sh.digits, sh.by_digits, &sh.listed);
     }
   }
 }
 
 // The token of a row whose first k are listed, k of them kept by top_k (1: the first column).
-LCE_DEV int64_t sample_listed(const RowSettings& s, int k, const u64* list, TopShared* sh) {
+template <int NT, class Shared> LCE_DEV int64_t sample_listed(const RowSettings& s, int k, const u64* list, Shared* sh) {
   if (s.greedy()) {
     const int64_t column = column_in(list[0]);
     __syncthreads();
     return column;
   }
+  static_assert(kMostByMaxima <= NT, "an entry to a thread");
   const Weights weights = s.weights(value_of(key_in(list[0])));
   const int t = threadIdx.x;
   const double real = t < k ? weights.real(value_of(key_in(list[t]))) : 0.0;
   const u64 w = weights.fixed(real);
   u64 before;
-  u64 stays = block_all<Sum>(w, sh->of_wave, &before);
+  u64 stays = block_all<Sum, NT>(w, sh->of_wave, &before);
   const double most = (double)s.top_p * (double)stays;
   // (each keeps a beginning of the list: the weight of those that all keep is their sum)
   const bool kept = t < k && (t == 0 || ((!(s.top_p < 1.f) || (double)before < most) && (!(s.min_p > 0.f) || real >= (double)s.min_p)));
-  stays = block_all<Sum>(kept ? w : (u64)0, sh->of_wave);
+  stays = block_all<Sum, NT>(kept ? w : (u64)0, sh->of_wave);
   const double some = (double)s.u * (double)stays;
   u64 target = some > 0.0 ? (u64)some : 0;
   if (target >= stays) target = stays - 1;
@@ -888,35 +937,38 @@ LCE_DEV int64_t sample_listed(const RowSettings& s, int k, const u64* list, TopS
 
 // Rows of which the first elements are enough: settings for all of them with 1 <= top_k <= kMostByMaxima or temperature 0.
 template <class E>
-__global__ __launch_bounds__(kSelectThreads, 8) void sample_top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
-                                                                       const Sampling settings, int bits, int64_t* token) {
-  __shared__ TopShared sh;
+__global__ __launch_bounds__(kTopThreads, 8) void sample_top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
+                                                                    const Sampling settings, int bits, int64_t* token) {
+  constexpr int NT = kTopThreads;
+  __shared__ TopShared<SelectShared<true, false>> sh;
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
     const int64_t k = s.greedy() ? 1 : s.top_k < cols ? s.top_k : cols;
-    const u64* list = list_first<E, false>(RowPieces<E>(from, cols), (int)k, &sh, nullptr);
+    const u64* list = list_first<E, false>(RowPieces<E, NT>(from, cols), (int)k, &sh);
     int64_t column;
-    if (list != nullptr) column = sample_listed(s, (int)k, list, &sh);
-    else column = sample_by_digits(RowUnits<E>(from, cols), s, &sh.digits);
+    if (list != nullptr) column = sample_listed<NT>(s, (int)k, list, &sh);
+    else column = sample_by_digits(RowUnits<E, NT>(from, cols), s, &sh.digits);
     if (threadIdx.x == 0) token[n] = column;
     __syncthreads();
   }
 }
 
-// float32 rows with any settings.
+// Rows with any settings: 1024 threads to a row.
+constexpr int kSelectThreads = 1024;
 __global__ __launch_bounds__(kSelectThreads) void sample_float_kernel(const float* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
                                                                       const Sampling settings, int bits, int64_t* token) {
-  __shared__ TopShared sh;
+  constexpr int NT = kSelectThreads;
+  __shared__ TopShared<SelectShared<true, true>> sh;
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const float* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
     const int64_t k = s.greedy() ? 1 : s.top_k;
     const u64* list = nullptr;
-    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<float, false>(RowPieces<float>(from, cols), (int)k, &sh, nullptr);
+    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<float, false>(RowPieces<float, NT>(from, cols), (int)k, &sh);
     int64_t column;
-    if (list != nullptr) column = sample_listed(s, (int)k, list, &sh);
-    else column = sample_by_digits(RowUnits<float>(from, cols), s, &sh.digits);
+    if (list != nullptr) column = sample_listed<NT>(s, (int)k, list, &sh);
+    else column = sample_by_digits(RowUnits<float, NT>(from, cols), s, &sh.digits);
     if (threadIdx.x == 0) token[n] = column;
     __syncthreads();
   }
@@ -943,11 +995,11 @@ struct HalfShared {
   union {
     unsigned hist[kHalfWords];
     unsigned values[kHalfWords];  // the values that occur, in order: bits, and the count in the upper half
-    TopShared top;
+    TopShared<SelectShared<true, true>> top;
     ColumnShared columns;
   };
   int row_values[2 * kWordRows], row_first[2 * kWordRows];  // of the positive numbers by rows from the last one, of the negative ones
-  u64 of_wave[kSelectWaves];
+  u64 of_wave[kMostWaves];
   Place place;  // (its key: the bits)
 };
 
@@ -957,7 +1009,7 @@ template <class E> struct HalfRow {
 
   // The counts of the row's values, listed.  Returns whether the list has all of the row's columns that are not masked; *different: how
   // many values it has.
-  LCE_DEV bool fill(const RowPieces<E>& row, int* different) const {
+  LCE_DEV bool fill(const RowPieces<E, kSelectThreads>& row, int* different) const {
     constexpr int kWordRounds = kHalfWords / 4 / kSelectThreads;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     u32x4_t* words = reinterpret_cast<u32x4_t*>(sh->hist);
@@ -973,7 +1025,7 @@ template <class E> struct HalfRow {
       else atomicAdd(&sh->hist[m], bits & 0x8000u ? 0x10000u : 1u);
     };
     row.edges([&](int64_t at, unsigned) { one(reinterpret_cast<const unsigned short*>(row.p)[at]); });
-    row.each([&](int64_t, u32x4_t w) {
+    row.each([&](int64_t, u32x4_t w, int) {
       typedef unsigned short pair_t __attribute__((ext_vector_type(2)));
       pair_t most = {};
 #pragma unroll
@@ -1021,7 +1073,7 @@ template <class E> struct HalfRow {
     };
 #pragma unroll
     for (int i = 0; i < kWordRounds; ++i) {
-      const int at = i * kSelectWaves + wave;
+      const int at = i * (kSelectThreads / 64) + wave;
       int plus = 0, minus = 0;
       if (__any((w[i][0] | w[i][1] | w[i][2] | w[i][3]) != 0)) {
         occur(w[i]);
@@ -1036,10 +1088,10 @@ template <class E> struct HalfRow {
         sh->row_values[kWordRows + at] = minus;
       }
     }
-    const u64 both = block_all<Sum>(sum | (u64)masked << 31, sh->of_wave);
+    const u64 both = block_all<Sum, kSelectThreads>(sum | (u64)masked << 31, sh->of_wave);
     const u64 counted = both & 0x7fffffffu;
     int before;
-    *different = block_all<Sum>(t < 2 * kWordRows ? sh->row_values[t] : 0, reinterpret_cast<int*>(sh->of_wave), &before);
+    *different = block_all<Sum, kSelectThreads>(t < 2 * kWordRows ? sh->row_values[t] : 0, reinterpret_cast<int*>(sh->of_wave), &before);
     if (any_nan || counted == 0 || *different > kHalfWords || (int64_t)(counted + (both >> 31)) != row.n) return false;
     if (t < 2 * kWordRows) sh->row_first[t] = before;
     __syncthreads();
@@ -1048,7 +1100,7 @@ template <class E> struct HalfRow {
     for (int i = 0; i < kWordRounds; ++i) {
       if (!__any((w[i][0] | w[i][1] | w[i][2] | w[i][3]) != 0)) continue;
       occur(w[i]);
-      const int at = i * kSelectWaves + wave;
+      const int at = i * (kSelectThreads / 64) + wave;
       int plus = sh->row_first[kWordRows - 1 - at], minus = sh->row_first[kWordRows + at];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -1105,15 +1157,15 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
-    const RowPieces<E> row(from, cols);
+    const RowPieces<E, kSelectThreads> row(from, cols);
     const HalfRow<E> half = {sh};
     const int64_t k = s.greedy() ? 1 : s.top_k;
     const u64* list = nullptr;
-    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(row, (int)k, &sh->top, nullptr);
+    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(row, (int)k, &sh->top);
     int64_t column;
     int different;
     if (list != nullptr) {
-      column = sample_listed(s, (int)k, list, &sh->top);
+      column = sample_listed<kSelectThreads>(s, (int)k, list, &sh->top);
     } else if (!s.greedy() && half.fill(row, &different)) {
       const unsigned top = sh->values[0] & 0xffffu;
       const Weights weights = s.weights(half_value<E>(top));
@@ -1129,18 +1181,18 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
       });
       int cb;
       u64 wb;
-      const int weighed = block_all<Sum>(elements, reinterpret_cast<int*>(sh->of_wave), &cb);
-      const u64 all = block_all<Sum>(weight, sh->of_wave, &wb);
-      by_min = s.min_p > 0.f ? block_all<Sum>(by_min, sh->of_wave) : all;
+      const int weighed = block_all<Sum, kSelectThreads>(elements, reinterpret_cast<int*>(sh->of_wave), &cb);
+      const u64 all = block_all<Sum, kSelectThreads>(weight, sh->of_wave, &wb);
+      by_min = s.min_p > 0.f ? block_all<Sum, kSelectThreads>(by_min, sh->of_wave) : all;
       int64_t which = 0;
       const Place at = draw_place(s, weighed, all, by_min, Place{top, 0, 0, 0}, &which,
                                   [&](const Want& want) { return half.find(weights, different, cb, wb, elements, weight, want); },
                                   [&](const Place& p) { return weights.of(half_value<E>(p.key)); });
       __syncthreads();  // (the list of values is not read any more)
-      column = column_of(RowUnits<E>(from, cols), half_value<E>(at.key), which, &sh->columns);
+      column = column_of(RowUnits<E, kSelectThreads>(from, cols), half_value<E>(at.key), which, &sh->columns);
     } else {
       __syncthreads();
-      column = sample_by_digits(RowUnits<E>(from, cols), s, &sh->top.digits);
+      column = sample_by_digits(RowUnits<E, kSelectThreads>(from, cols), s, &sh->top.digits);
     }
     if (threadIdx.x == 0) token[n] = column;
     __syncthreads();
@@ -1156,7 +1208,7 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
   const dim3 grid(grid_of(rows)), block(kSelectThreads);
   const bool first_alone = (!s.temperature_rows && s.temperature == 0.f) || (!s.top_k_rows && s.top_k >= 1 && s.top_k <= kMostByMaxima);
   if (first_alone) {
-    hipLaunchKernelGGL(sample_top_kernel<E>, grid, block, 0, stream, logits, rows, cols, ld, u, s, bits, token);
+    hipLaunchKernelGGL(sample_top_kernel<E>, grid, dim3(kTopThreads), 0, stream, logits, rows, cols, ld, u, s, bits, token);
   } else if constexpr (sizeof(E) == 2) {
     static LdsOptIn optin;
     const hipError_t e = optin.ensure(reinterpret_cast<const void*>(sample_half_kernel<E>), (int)sizeof(HalfShared));
@@ -1171,7 +1223,7 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
 template <class E>
 hipError_t launch_top_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values, int64_t* index, float* lse,
                          hipStream_t stream) {
-  const dim3 grid(grid_of(rows)), block(kSelectThreads);
+  const dim3 grid(grid_of(rows)), block(kTopThreads);
   if (lse != nullptr) hipLaunchKernelGGL((top_kernel<E, true>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
   else hipLaunchKernelGGL((top_kernel<E, false>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
   return hipGetLastError();
