@@ -1628,19 +1628,22 @@ int check_logits(const void* logits, int dtype, int64_t rows, int64_t cols, int6
 
 int lce_top_logits(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, int64_t k, void* values, int64_t* index, float* lse,
                    void* stream) {
-  const int rc = check_logits(logits, dtype, rows, cols, ld);
+  int rc = check_logits(logits, dtype, rows, cols, ld);
   if (rc != LCE_OK) return rc;
   if (k < 1 || k > cols || k > LCE_MAX_TARGETS) return LCE_EINVAL_SHAPE;
   if (rows == 0) return LCE_OK;
   if (!values || !index) return LCE_EINVAL_ARG;
-  const hipError_t e = lce::launch_top(logits, dtype, rows, cols, ld, (int)k, values, index, lse, (hipStream_t)stream);
+  int num_cus = 0;
+  rc = current_num_cus(&num_cus, 0);
+  if (rc != LCE_OK) return rc;
+  const hipError_t e = lce::launch_top(logits, dtype, rows, cols, ld, (int)k, values, index, lse, num_cus, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "top_logits");
   return LCE_OK;
 }
 
 int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* u, const lce_sampling* s, int64_t* token,
                void* stream) {
-  const int rc = check_logits(logits, dtype, rows, cols, ld);
+  int rc = check_logits(logits, dtype, rows, cols, ld);
   if (rc != LCE_OK) return rc;
   if (!s) return LCE_EINVAL_ARG;
   // (numbers that are not there for each row are checked; those that are, lce.h says what they stand for)
@@ -1651,7 +1654,10 @@ int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_
   if (rows == 0) return LCE_OK;
   if (!u || !token) return LCE_EINVAL_ARG;
   const lce::Sampling a = {s->temperature, s->top_p, s->min_p, s->top_k, s->temperature_rows, s->top_p_rows, s->min_p_rows, s->top_k_rows};
-  const hipError_t e = lce::launch_sample(logits, dtype, rows, cols, ld, u, a, token, (hipStream_t)stream);
+  int num_cus = 0;
+  rc = current_num_cus(&num_cus, 0);
+  if (rc != LCE_OK) return rc;
+  const hipError_t e = lce::launch_sample(logits, dtype, rows, cols, ld, u, a, token, num_cus, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "sample");
   return LCE_OK;
 }

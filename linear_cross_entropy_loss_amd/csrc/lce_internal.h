@@ -522,9 +522,9 @@ struct Sampling {
   const int64_t* top_k_rows;
 };
 hipError_t launch_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* u, const Sampling& s,
-                         int64_t* token, hipStream_t stream);
+                         int64_t* token, int num_cus, hipStream_t stream);
 hipError_t launch_top(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, int k, void* values, int64_t* index, float* lse,
-                      hipStream_t stream);
+                      int num_cus, hipStream_t stream);
 
 hipError_t launch_fwd_narrow(const FwdArgs& a, int64_t rows, hipStream_t s);
 hipError_t launch_bwd_narrow(const BwdArgs& a, const SmallGrads& g, bool want_dx, bool want_dw, hipStream_t s);

@@ -273,11 +273,12 @@ LCE_DEV double exp2_series(double t) {
 struct Weights {
   double top, per;  // the largest value, log2(e) / temperature
   double one;       // 2^bits, bits <= 50
-  LCE_DEV double real(float z) const {
+  LCE_DEV double log2_of(float z) const {
     // (equal infinities have no difference, and one times 0, at an infinite temperature, is no number)
-    const double zd = (double)z, t = zd == top ? 0.0 : fmax((zd - top) * per, -2000.0);
-    return exp2_series(t);
+    const double zd = (double)z;
+    return zd == top ? 0.0 : fmax((zd - top) * per, -2000.0);
   }
+  LCE_DEV double real(float z) const { return exp2_series(log2_of(z)); }
   // (rounded by the sum with 2^52, whose last place is 1)
   LCE_DEV u64 fixed(double w) const { return __builtin_bit_cast(u64, fma(w, one, 4503599627370496.0)) & 0xfffffffffffffull; }
   LCE_DEV u64 of(float z) const { return fixed(real(z)); }
@@ -954,21 +955,218 @@ __global__ __launch_bounds__(kTopThreads, 8) void sample_top_kernel(const E* log
   }
 }
 
-// Rows with any settings: 1024 threads to a row.
 constexpr int kSelectThreads = 1024;
-__global__ __launch_bounds__(kSelectThreads) void sample_float_kernel(const float* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
-                                                                      const Sampling settings, int bits, int64_t* token) {
-  constexpr int NT = kSelectThreads;
-  __shared__ TopShared<SelectShared<true, true>> sh;
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Rows with any settings.  A histogram of counts and weights over 4096 bins of equal width in log2 of the weight, which is what
+// the fixed point of the weights reaches; the few elements of the bin in which a place lies are then listed and sorted.  Passes over the
+// row: its maximum, the histogram, one for every place that is asked for.  A bin with more elements than the list has room for is
+// no matter if they are all equal; else the row is done by digits.
+// ---------------------------------------------------------------------------------------------------------------------------
+constexpr int kBins = 4096;
+constexpr double kBinsPerOctave = 80.0;  // 51 octaves: a weight of 2^-51 rounds to 0 with 50 places
+struct BinShared {
+  union {
+    struct {
+      u64 weight[kBins];
+      int count[kBins];
+      u64 list[kMostList];
+    };
+    SelectShared<true, true> digits;
+  };
+  u64 of_wave[kMostWaves];
+  ColumnShared columns;
+  Place place;
+  int64_t column;
+  int bin, listed;
+};
+template <class E, int NT> struct RowBins {
+  typedef Ordered<E> O;
+  static constexpr int kPer = RowPieces<E, NT>::kPer, kOwn = kBins / NT;
+  const RowPieces<E, NT>& row;
+  const Weights& weights;
+  unsigned top;  // the largest key
+  BinShared* sh;
+
+  LCE_DEV static int bin_of(double log2_weight) {
+    const int b = (int)(log2_weight * -kBinsPerOctave);
+    return b < kBins - 1 ? b : kBins - 1;
+  }
+  // f(element) for all elements.
+  template <class F> LCE_DEV void elements(F f) const {
+    row.edges([&](int64_t at, unsigned) { f(at, as_float(row.p[at])); });
+    row.each([&](int64_t at, u32x4_t v, int) {
+      E e[kPer];
+      __builtin_memcpy(e, &v, 16);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) f(at + i, as_float(e[i]));
+    });
+  }
+  // The histogram; the weight that min_p keeps.
+  LCE_DEV u64 fill(double min_p) const {
+    for (int i = threadIdx.x; i < kBins; i += NT) {
+      sh->count[i] = 0;
+      sh->weight[i] = 0;
+    }
+    __syncthreads();
+    u64 mine = 0;
+    elements([&](int64_t, float z) {
+      const double t = weights.log2_of(z), real = exp2_series(t);
+      const u64 w = weights.fixed(real);
+      if (w == 0) return;
+      if (real >= min_p) mine += w;
+      const int b = bin_of(t);
+      atomicAdd(&sh->weight[b], w);
+      atomicAdd(&sh->count[b], 1);
+    });
+    return block_all<Sum, NT>(mine, sh->of_wave);
+  }
+  // The sums of this thread's bins.
+  LCE_DEV void own(int* c, u64* w) const {
+    *c = 0;
+    *w = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      *c += sh->count[threadIdx.x * kOwn + i];
+      *w += sh->weight[threadIdx.x * kOwn + i];
+    }
+  }
+  // The place that is wanted; *column: its column, where it is one element's, else -1.  c, w: the sums of this thread's bins, cb, wb: those
+  // before.  False: by digits.
+  LCE_DEV bool find(int64_t cb, u64 wb, int c, u64 w, const Want& want, Place* place, int64_t* column) const {
+    const int t = threadIdx.x;
+    if (t == 0) sh->listed = 0;
+    if (want.here(cb, wb, c, w)) {
+#pragma unroll 1
+      for (int b = t * kOwn; b < (t + 1) * kOwn; ++b) {
+        const int cd = sh->count[b];
+        const u64 wd = sh->weight[b];
+        if (want.here(cb, wb, cd, wd)) {
+          sh->bin = b;
+          sh->place = {0, cb, wb, cd};
+        }
+        cb += cd;
+        wb += wd;
+      }
+    }
+    __syncthreads();
+    const Place bin = sh->place;
+    const int b = sh->bin;
+    const bool room = bin.same <= kMostList;
+    // keys between which all of its elements are: the bin's ends, each further out by more than the roundings of either direction
+    const double low_z = weights.top - (double)(b + 1) / (kBinsPerOctave * weights.per), high_z = weights.top - (double)b / (kBinsPerOctave * weights.per);
+    const unsigned low_key = key_of((float)low_z), high_key = key_of((float)high_z);
+    const unsigned low = b == kBins - 1 || low_key < kLowKey + 4 ? kLowKey + 1 : low_key - 2, high = high_key < top - 2 ? high_key + 2 : top;
+    unsigned most = 0, inverse = 0;  // the largest key of the bin, of the inverted keys
+    elements([&](int64_t at, float z) {
+      const unsigned key = key_of(z);
+      if (!(key >= low && key <= high)) return;
+      const double log2 = weights.log2_of(z);
+      if (bin_of(log2) != b || weights.fixed(exp2_series(log2)) == 0) return;  // (without a weight: not counted)
+      if (room) {
+        const int to = atomicAdd(&sh->listed, 1);
+        if (to < kMostList) sh->list[to] = entry_of(key, at);
+      } else {
+        most = key > most ? key : most;
+        inverse = ~key > inverse ? ~key : inverse;
+      }
+    });
+    *column = -1;
+    if (!room) {
+      most = block_all<Largest, NT>(most, reinterpret_cast<unsigned*>(sh->of_wave));
+      inverse = block_all<Largest, NT>(inverse, reinterpret_cast<unsigned*>(sh->of_wave));
+      *place = {most, bin.count, bin.weight, bin.same};
+      return most == ~inverse;
+    }
+    __syncthreads();
+    const int n = sh->listed < kMostList ? sh->listed : kMostList;
+    const u64* list = sh->list;
+    if (n <= kMostRanked) {
+      list = rank_list<NT>(sh->list, sh->list + kMostRanked, n);
+    } else {
+      const int sorted = power_of_two(n);
+      for (int i = n + t; i < sorted; i += NT) sh->list[i] = ~(u64)0;
+      sort_list<NT>(sh->list, sorted);
+    }
+    // (some neighbouring entries to a thread)
+    const int per = (n + NT - 1) / NT;
+    u64 mine = 0;
+    for (int i = t * per; i < (t + 1) * per && i < n; ++i) mine += weights.of(value_of(key_in(list[i])));
+    u64 before;
+    block_all<Sum, NT>(mine, sh->of_wave, &before);
+    before += bin.weight;
+    for (int i = t * per; i < (t + 1) * per && i < n; ++i) {
+      const unsigned key = key_in(list[i]);
+      const u64 one = weights.of(value_of(key));
+      if (want.here(bin.count + i, before, 1, one)) {
+        sh->place = {key, bin.count + i, before, 1};
+        sh->column = column_in(list[i]);
+      }
+      before += one;
+    }
+    __syncthreads();
+    *place = sh->place;
+    *column = sh->column;
+    __syncthreads();
+    return true;
+  }
+};
+
+template <class E, int NT>
+LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s, BinShared* sh) {
+  const RowUnits<E, NT> units(from, cols);
+  const unsigned top = largest_key(units, reinterpret_cast<unsigned*>(sh->of_wave));
+  if (top == kNanKey || top == kLowKey) return -1;  // a NaN, or no column left
+  const float inf = __builtin_inff();
+  if (s.greedy()) return column_of(units, value_of(top), 0, &sh->columns);
+  if (value_of(top) < inf) {
+    const Weights weights = s.weights(value_of(top));
+    const RowPieces<E, NT> row(from, cols);
+    const RowBins<E, NT> bins = {row, weights, top, sh};
+    const u64 by_min = bins.fill(s.min_p > 0.f ? (double)s.min_p : 0.0);
+    int c, cb;
+    u64 w, wb;
+    bins.own(&c, &w);
+    const int counted = block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave), &cb);
+    const u64 all = block_all<Sum, NT>(w, sh->of_wave, &wb);
+    if (threadIdx.x == 0) {
+      sh->place = {top, 0, 0, 0};
+      sh->bin = 0;
+      sh->column = 0;
+    }
+    __syncthreads();
+    bool fine = true;
+    int64_t which = 0, column = -1;
+    const Place at = draw_place(s, counted, all, by_min, Place{top, 0, 0, 0}, &which,
+                                [&](const Want& want) {
+                                  Place p = {top, 0, 0, 0};
+                                  if (fine) fine = bins.find(cb, wb, c, w, want, &p, &column);
+                                  return p;
+                                },
+                                [&](const Place& p) { return weights.of(value_of(p.key)); });
+    if (fine) return column >= 0 ? column : column_of(units, value_of(at.key), which, &sh->columns);
+    __syncthreads();
+  }
+  return sample_by_digits(units, s, &sh->digits);
+}
+
+// NT = 512: two rows to a compute unit; 1024 for rows that have one each.
+template <class E, int NT>
+__global__ __launch_bounds__(NT, 4) void sample_bins_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
+                                                            const Sampling settings, int bits, int64_t* token) {
+  __shared__ union {
+    BinShared bins;
+    TopShared<SelectShared<true, true>> top;
+  } sh;
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
-    const float* from = logits + n * ld;
+    const E* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
     const int64_t k = s.greedy() ? 1 : s.top_k;
     const u64* list = nullptr;
-    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<float, false>(RowPieces<float, NT>(from, cols), (int)k, &sh);
+    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(RowPieces<E, NT>(from, cols), (int)k, &sh.top);
     int64_t column;
-    if (list != nullptr) column = sample_listed<NT>(s, (int)k, list, &sh);
-    else column = sample_by_digits(RowUnits<float, NT>(from, cols), s, &sh.digits);
+    if (list != nullptr) column = sample_listed<NT>(s, (int)k, list, &sh.top);
+    else column = sample_by_bins<E, NT>(from, cols, s, &sh.bins);
     if (threadIdx.x == 0) token[n] = column;
     __syncthreads();
   }
@@ -1199,31 +1397,57 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
   }
 }
 
-unsigned grid_of(int64_t rows) { return (unsigned)(rows < (int64_t)1 << 20 ? rows : (int64_t)1 << 20); }
+// Workgroups: up to `most` rows to a compute unit at a time -- a workgroup takes one after another, its code and constants are then at
+// hand (2048 rows of 32000, one workgroup to each 301 us, 256 in all 258) -- but no more than the Infinity Cache holds of them between
+// the passes (2048 float32 rows of 131072: 1024 at a time 408 us, 512 364, 256 414).
+unsigned grid_of(int64_t rows, int64_t row_bytes, int most, int num_cus) {
+  int64_t n = ((int64_t)256 << 20) / (row_bytes < 1 ? 1 : row_bytes);
+  if (n < num_cus) n = num_cus;
+  if (n > (int64_t)most * num_cus) n = (int64_t)most * num_cus;
+  return (unsigned)(rows < n ? rows : n);
+}
 static_assert(sizeof(HalfShared) <= 160 * 1024, "a compute unit has 160 KiB of LDS");
+
+// 16-bit rows up to this are sampled by bins, longer ones by the histogram of all values: that takes a compute unit for a row, much of its
+// time whatever the row's length, and more for fp16, of which a row has more different values.  us, bins / histogram, temperature alone
+// and with top_p: 2048 rows, bf16 V=4096 74, 94 / 159, 170, 16384 137, 166 / 175, 187, 24000 172, 205 / 189, 200, 32768 213, 252 /
+// 204, 215; fp16 16384 135, 159 / 222, 239, 32768 208, 243 / 253, 274; 64 rows, bf16 16384 25, 31 / 24, 25, 32768 38, 46 / 27, 27; fp16
+// 16384 25, 30 / 30, 32, 32768 37, 43 / 33, 36.
+template <class E> constexpr int64_t kMostBinCols = 16384;
+template <> constexpr int64_t kMostBinCols<_Float16> = 32768;
 
 template <class E>
 hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u, const Sampling& s, int bits, int64_t* token,
-                            hipStream_t stream) {
-  const dim3 grid(grid_of(rows)), block(kSelectThreads);
+                            int num_cus, hipStream_t stream) {
+  const int64_t row_bytes = cols * (int64_t)sizeof(E);
   const bool first_alone = (!s.temperature_rows && s.temperature == 0.f) || (!s.top_k_rows && s.top_k >= 1 && s.top_k <= kMostByMaxima);
   if (first_alone) {
-    hipLaunchKernelGGL(sample_top_kernel<E>, grid, dim3(kTopThreads), 0, stream, logits, rows, cols, ld, u, s, bits, token);
-  } else if constexpr (sizeof(E) == 2) {
-    static LdsOptIn optin;
-    const hipError_t e = optin.ensure(reinterpret_cast<const void*>(sample_half_kernel<E>), (int)sizeof(HalfShared));
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(sample_half_kernel<E>, grid, block, sizeof(HalfShared), stream, logits, rows, cols, ld, u, s, bits, token);
-  } else {
-    hipLaunchKernelGGL(sample_float_kernel, grid, block, 0, stream, logits, rows, cols, ld, u, s, bits, token);
+    hipLaunchKernelGGL(sample_top_kernel<E>, dim3(grid_of(rows, row_bytes, 4, num_cus)), dim3(kTopThreads), 0, stream, logits, rows, cols, ld, u,
+                       s, bits, token);
+    return hipGetLastError();
   }
+  if constexpr (sizeof(E) == 2) {
+    if (cols > kMostBinCols<E>) {
+      static LdsOptIn optin;
+      const hipError_t e = optin.ensure(reinterpret_cast<const void*>(sample_half_kernel<E>), (int)sizeof(HalfShared));
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL(sample_half_kernel<E>, dim3(grid_of(rows, row_bytes, 1, num_cus)), dim3(kSelectThreads), sizeof(HalfShared), stream,
+                         logits, rows, cols, ld, u, s, bits, token);
+      return hipGetLastError();
+    }
+  } else if (rows <= num_cus) {
+    hipLaunchKernelGGL((sample_bins_kernel<E, 1024>), dim3((unsigned)rows), dim3(1024), 0, stream, logits, rows, cols, ld, u, s, bits, token);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((sample_bins_kernel<E, 512>), dim3(grid_of(rows, row_bytes, 2, num_cus)), dim3(512), 0, stream, logits, rows, cols, ld, u, s,
+                     bits, token);
   return hipGetLastError();
 }
 
 template <class E>
-hipError_t launch_top_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values, int64_t* index, float* lse,
+hipError_t launch_top_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values, int64_t* index, float* lse, int num_cus,
                          hipStream_t stream) {
-  const dim3 grid(grid_of(rows)), block(kTopThreads);
+  const dim3 grid(grid_of(rows, cols * (int64_t)sizeof(E), 4, num_cus)), block(kTopThreads);
   if (lse != nullptr) hipLaunchKernelGGL((top_kernel<E, true>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
   else hipLaunchKernelGGL((top_kernel<E, false>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
   return hipGetLastError();
@@ -1232,21 +1456,21 @@ hipError_t launch_top_of(const E* logits, int64_t rows, int64_t cols, int64_t ld
 }  // namespace
 
 hipError_t launch_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* u, const Sampling& s,
-                         int64_t* token, hipStream_t stream) {
+                         int64_t* token, int num_cus, hipStream_t stream) {
   int log2 = 0;
   while ((int64_t)1 << log2 < cols) ++log2;
   const int bits = 62 - log2 < 50 ? 62 - log2 : 50;  // (a double has 53: a weight of one and the half that rounds it fit)
-  if (dtype == DT_BF16) return launch_sample_of((const __bf16*)logits, rows, cols, ld, u, s, bits, token, stream);
-  if (dtype == DT_F16) return launch_sample_of((const _Float16*)logits, rows, cols, ld, u, s, bits, token, stream);
-  if (dtype == DT_F32) return launch_sample_of((const float*)logits, rows, cols, ld, u, s, bits, token, stream);
+  if (dtype == DT_BF16) return launch_sample_of((const __bf16*)logits, rows, cols, ld, u, s, bits, token, num_cus, stream);
+  if (dtype == DT_F16) return launch_sample_of((const _Float16*)logits, rows, cols, ld, u, s, bits, token, num_cus, stream);
+  if (dtype == DT_F32) return launch_sample_of((const float*)logits, rows, cols, ld, u, s, bits, token, num_cus, stream);
   return hipErrorInvalidValue;
 }
 
 hipError_t launch_top(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, int k, void* values, int64_t* index, float* lse,
-                      hipStream_t stream) {
-  if (dtype == DT_BF16) return launch_top_of((const __bf16*)logits, rows, cols, ld, k, (__bf16*)values, index, lse, stream);
-  if (dtype == DT_F16) return launch_top_of((const _Float16*)logits, rows, cols, ld, k, (_Float16*)values, index, lse, stream);
-  if (dtype == DT_F32) return launch_top_of((const float*)logits, rows, cols, ld, k, (float*)values, index, lse, stream);
+                      int num_cus, hipStream_t stream) {
+  if (dtype == DT_BF16) return launch_top_of((const __bf16*)logits, rows, cols, ld, k, (__bf16*)values, index, lse, num_cus, stream);
+  if (dtype == DT_F16) return launch_top_of((const _Float16*)logits, rows, cols, ld, k, (_Float16*)values, index, lse, num_cus, stream);
+  if (dtype == DT_F32) return launch_top_of((const float*)logits, rows, cols, ld, k, (float*)values, index, lse, num_cus, stream);
   return hipErrorInvalidValue;
 }
 
