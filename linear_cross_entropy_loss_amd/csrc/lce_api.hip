@@ -1309,7 +1309,7 @@ int plan_distill(const lce_problem* q, int64_t K, bool grads, DistillPlan* d) {
     }
   }
   // (the scratch of the targets' logits is free again before the loss's kernels run)
-  const size_t sorting = lce::soft_logits_bytes(q->N, (int)K, q->V);
+  const size_t sorting = lce::soft_logits_bytes(q->N, (int)K, q->H, q->V, q->w_layout == LCE_W_VH);
   if (sorting > o) o = sorting;
   o = align_up(o);
   d->out5 = o; o += 256;

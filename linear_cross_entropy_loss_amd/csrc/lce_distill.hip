@@ -172,9 +172,14 @@ __global__ __launch_bounds__(256) void soft_logits_direct_kernel(const SoftLogit
 // More: the entries are sorted by groups of 64 columns (one line of a 16-bit W), whose part of W then passes through LDS once for
 // all of them.  Counting sort: counts of every group, their prefix sums and from them the list of work items -- up to kItemEntries
 // entries of one group --, then the places.  The order within a group is not the same in every call; a logit does not depend on it.
-constexpr int kGroupCols = 64, kItemEntries = 256;
+constexpr int kGroupCols = 64, kItemEntries = 128;
 constexpr int kSortThreads = 1024, kSortPer = 8;
-constexpr int64_t kSortedEntries = 16384;  // from here on
+// Whether so many entries are sorted.  The sort and the passes over the groups cost 20 us and the part of W that has an entry; without, a
+// weight stored (H, V) costs a line for every element.  Loss alone, us, sorted / not: (H, V), bf16, V=32000, H=128 8192 entries 48 / 42,
+// 16384 56 / 58, 32768 69 / 87; H=512 4096 59 / 59, 8192 69 / 87; H=2048 2048 99 / 103, 4096 117 / 153; V=131072, H=2048 2048 229 /
+// 207, 8192 410 / 526; fp32, V=32000, H=512 4096 91 / 92, 8192 118 / 147.  (V, H), V=32000, H=512 32768 120 / 101, 65536 188 / 178;
+// H=2048 65536 521 / 522; V=4096, H=2048 32768 140 / 104, 65536 163 / 169.
+inline bool sorts_entries(int64_t M, int64_t H, bool w_vh) { return w_vh ? M >= 65536 : M * H >= (int64_t)3 << 20; }
 constexpr int64_t kMostColGroups = 16384;  // counts of a workgroup: 64 KiB of LDS
 
 __global__ __launch_bounds__(kSortThreads) void soft_clear_kernel(int* counts, int groups) {
@@ -312,16 +317,22 @@ template <class XT, class WT, int n> LCE_DEV void load_as(XT (&to)[n], const WT*
 }
 
 // A workgroup per item: the 64 columns of W come through LDS 128 bytes of each at a time (64 or 32 hidden indices), and eight lanes
-// take such a stretch of one entry's row of x, a whole line, against the entry's column: 32 entries at a time, eight times.  The
+// take such a stretch of one entry's row of x, a whole line, against the entry's column: 32 entries at a time, four times.  The
 // column's line is read by eight neighbouring lanes, which meets every bank once.
-//   Traffic: W once for every 256 entries of a group, 2 H bytes for every entry, from the caches where x fits those.
+//   Bound by memory traffic: 2 H bytes (4 in fp32) for every entry and W once for every 128 entries of a group, from the caches where
+// they fit.  N=16384, K=64, H=2048, V=131072, 0.9 million entries: 627 us, some 3.7 GB of x and 1.7 of W; with 256 entries to an item 841
+// (registers leave fewer workgroups to hide the waits), 512 1295, 64 882, neighbouring items on different XCDs 690, the next lines of x
+// in flight during the products 791.  N=2048, K=64, H=2048, V=16384 in fp32 142, with 256 entries 134; N=8192, K=32, H=768, V=50257
+// stored (V, H) 49 / 65; N=1999, K=20, H=500, V=10007 23 / 41.
 template <class XT, class WT, bool WVH>
 __global__ __launch_bounds__(256) void soft_logits_kernel(const SoftLogits a, const int4* items, const int* num_items, const int2* entries) {
   constexpr int kPiece = 16 / sizeof(XT), kDeep = 8 * kPiece;  // elements of a lane's piece, of a stretch
   constexpr int kSets = kItemEntries / 32;
   __shared__ __attribute__((aligned(16))) XT tile[2][kGroupCols * kDeep];
-  if ((int)blockIdx.x >= num_items[0]) return;
-  const int4 item = items[blockIdx.x];
+  // (neighbouring items, of one group, go to one XCD, whose L2 then has the group's part of W)
+  const int n_items = num_items[0], per = (n_items + 7) / 8, seq = (int)(blockIdx.x >> 3), id = (int)(blockIdx.x & 7) * per + seq;
+  if (seq >= per || id >= n_items) return;
+  const int4 item = items[id];
   const int t = threadIdx.x, j = t & 7;
   const XT* x[kSets];
   int column[kSets];
@@ -359,16 +370,19 @@ __global__ __launch_bounds__(256) void soft_logits_kernel(const SoftLogits a, co
     }
   };
   fetch(0);
-  int buffer = 0;
-  for (int64_t h0 = 0; h0 < a.H; h0 += kDeep, buffer ^= 1) {
-    u32x4_t piece[kSets];
+  auto take = [&](int64_t h0, u32x4_t (&to)[kSets]) {
 #pragma unroll
     for (int g = 0; g < kSets; ++g)
       if (g * 32 < item.z) {
         XT some[kPiece];
         load_as<XT, XT, kPiece>(some, x[g] + h0, a.H - h0 - j * kPiece);
-        __builtin_memcpy(&piece[g], some, 16);
+        __builtin_memcpy(&to[g], some, 16);
       }
+  };
+  u32x4_t piece[kSets];
+  int buffer = 0;
+  for (int64_t h0 = 0; h0 < a.H; h0 += kDeep, buffer ^= 1) {
+    take(h0, piece);
     if constexpr (WVH) {
 #pragma unroll
       for (int i = 0; i < kOfW; i += kPiece) {
@@ -426,32 +440,28 @@ __global__ __launch_bounds__(256) void soft_gradient_kernel(const BwdArgs a, con
   }
 }
 
-// The rows' terms of the loss, a wave per row, and their sum in doubles: one partial sum to a workgroup, or -- FINAL, a single
-// workgroup -- the loss.
-constexpr int kLossWaves = 16, kLossGroups = 512;
+// The entries' terms of the loss, q (log q - z + lse), and their sum in doubles, in an order that is fixed: one partial sum to a workgroup,
+// or -- FINAL, a single workgroup -- the loss.  A row with an index that is no column makes it NaN.
+constexpr int kLossThreads = 1024, kLossGroups = 512;
 template <bool FINAL>
-__global__ __launch_bounds__(64 * kLossWaves) void soft_loss_kernel(const SoftTargets t, const int64_t* y, const float* lse, int64_t V,
-                                                                    const int64_t* n_valid, double* part, float* loss) {
-  __shared__ double sh[kLossWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(kLossThreads) void soft_loss_kernel(const SoftTargets t, const int64_t* y, const float* lse, int64_t V,
+                                                                 const int64_t* n_valid, double* part, float* loss) {
+  __shared__ double sh[kLossThreads / 64];
   double sum = 0.0;
-  for (int64_t n = (int64_t)blockIdx.x * kLossWaves + wave; n < t.N; n += (int64_t)gridDim.x * kLossWaves) {
-    const int64_t yy = y[n];
-    if (yy < 0) continue;
-    float term = 0.f;
-    const float l = lse[n];
-    for (int k = lane; k < t.K; k += 64) {
-      const float q = t.q[n * t.K + k];
-      if (q != 0.f) term = fmaf(q, logf(q) + (l - t.z[n * t.K + k]), term);
-    }
-    sum += yy < V ? (double)term : (double)__builtin_nanf("");
+  const unsigned M = (unsigned)(t.N * t.K), step = gridDim.x * kLossThreads;
+#pragma unroll 4
+  for (unsigned e = blockIdx.x * kLossThreads + threadIdx.x; e < M; e += step) {
+    const float q = t.q[e];
+    if (q != 0.f) sum += (double)(q * (logf(q) + (lse[e / (unsigned)t.K] - t.z[e])));
   }
+  for (int64_t n = (int64_t)blockIdx.x * kLossThreads + threadIdx.x; n < t.N; n += step)
+    if (y[n] >= V) sum = (double)__builtin_nanf("");
   sum = wave_sum(sum);
-  if (lane == 0) sh[wave] = sum;
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sum;
   __syncthreads();
   if (threadIdx.x != 0) return;
   double total = 0.0;
-  for (int i = 0; i < kLossWaves; ++i) total += sh[i];
+  for (int i = 0; i < kLossThreads / 64; ++i) total += sh[i];
   if (FINAL) loss[0] = (float)(total / (double)n_valid[0]);  // no row with an entry: 0/0 = NaN, as against labels
   else part[blockIdx.x] = total;
 }
@@ -469,11 +479,11 @@ struct SortPlan {
   int64_t most_items;
   size_t num_items, items, entries, total;
 };
-SortPlan plan_sort(int64_t N, int K, int64_t V) {
+SortPlan plan_sort(int64_t N, int K, int64_t H, int64_t V, bool w_vh) {
   SortPlan p;
   const int64_t M = N * K, groups = (V + kGroupCols - 1) / kGroupCols;
   auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
-  p.sorted = M >= kSortedEntries && groups <= kMostColGroups;
+  p.sorted = sorts_entries(M, H, w_vh) && groups <= kMostColGroups;
   p.groups = (int)(groups <= kMostColGroups ? groups : 0);
   p.most_items = groups + M / kItemEntries;
   p.num_items = up((size_t)p.groups * 4);
@@ -484,7 +494,7 @@ SortPlan plan_sort(int64_t N, int K, int64_t V) {
 }
 
 template <class XT, class WT, bool WVH> hipError_t launch_logits(const SoftLogits& a, void* ws, hipStream_t s) {
-  const SortPlan p = plan_sort(a.N, a.K, a.V);
+  const SortPlan p = plan_sort(a.N, a.K, a.H, a.V, a.w_vh != 0);
   const int64_t M = a.N * a.K;
   if (!p.sorted) {
     const int64_t groups = (M + 3) / 4;
@@ -502,7 +512,7 @@ template <class XT, class WT, bool WVH> hipError_t launch_logits(const SoftLogit
   hipLaunchKernelGGL(soft_count_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups);
   hipLaunchKernelGGL(soft_items_kernel, dim3(1), block, 0, s, counts, p.groups, items, num_items);
   hipLaunchKernelGGL(soft_place_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups, entries);
-  hipLaunchKernelGGL((soft_logits_kernel<XT, WT, WVH>), dim3((unsigned)p.most_items), dim3(256), 0, s, a, items, num_items, entries);
+  hipLaunchKernelGGL((soft_logits_kernel<XT, WT, WVH>), dim3((unsigned)((p.most_items + 7) / 8 * 8)), dim3(256), 0, s, a, items, num_items, entries);
   return hipGetLastError();
 }
 
@@ -525,7 +535,7 @@ hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const voi
   return hipGetLastError();
 }
 
-size_t soft_logits_bytes(int64_t N, int K, int64_t V) { return plan_sort(N, K, V).total; }
+size_t soft_logits_bytes(int64_t N, int K, int64_t H, int64_t V, bool w_vh) { return plan_sort(N, K, H, V, w_vh).total; }
 
 hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s) {
   if (a.x_dtype == DT_BF16 && a.w_dtype == DT_BF16)
@@ -552,13 +562,12 @@ hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStrea
 
 hipError_t launch_soft_loss(const SoftTargets& t, const int64_t* y, const float* lse, int64_t V, const int64_t* n_valid, double* part,
                             float* loss, hipStream_t s) {
-  const int64_t blocks = (t.N + kLossWaves - 1) / kLossWaves;
+  const int64_t most = t.N * t.K > t.N ? t.N * t.K : t.N, blocks = (most + 4 * kLossThreads - 1) / (4 * kLossThreads);
   const int grid = (int)(blocks < kLossGroups ? blocks : kLossGroups);
-  // (a workgroup's rows one after another: a second launch where it would be more than a few)
-  if (t.N <= 4 * kLossWaves) {
-    hipLaunchKernelGGL(soft_loss_kernel<true>, dim3(1), dim3(64 * kLossWaves), 0, s, t, y, lse, V, n_valid, part, loss);
+  if (grid <= 4) {  // (a workgroup's rounds are shorter than a second launch)
+    hipLaunchKernelGGL(soft_loss_kernel<true>, dim3(1), dim3(kLossThreads), 0, s, t, y, lse, V, n_valid, part, loss);
   } else {
-    hipLaunchKernelGGL(soft_loss_kernel<false>, dim3((unsigned)grid), dim3(64 * kLossWaves), 0, s, t, y, lse, V, n_valid, part, loss);
+    hipLaunchKernelGGL(soft_loss_kernel<false>, dim3((unsigned)grid), dim3(kLossThreads), 0, s, t, y, lse, V, n_valid, part, loss);
     hipLaunchKernelGGL(soft_loss_sum_kernel, dim3(1), dim3(64), 0, s, part, grid, n_valid, loss);
   }
   return hipGetLastError();

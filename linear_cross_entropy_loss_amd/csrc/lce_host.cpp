@@ -32,6 +32,9 @@ struct Abi {
   decltype(&lce_unit_gradient) unit_gradient;
   decltype(&lce_pad_rows) pad_rows;
   decltype(&lce_transpose_rows) transpose_rows;
+  decltype(&lce_soft_targets) soft_targets;
+  decltype(&lce_distill_workspace_bytes) distill_workspace_bytes;
+  decltype(&lce_distill) distill;
 } abi;
 
 template <class F> void bind_one(const py::dict& d, const char* name, F& f) { f = reinterpret_cast<F>(d[name].cast<uintptr_t>()); }
@@ -47,6 +50,9 @@ void bind(const py::dict& d) {
   bind_one(d, "lce_unit_gradient", abi.unit_gradient);
   bind_one(d, "lce_pad_rows", abi.pad_rows);
   bind_one(d, "lce_transpose_rows", abi.transpose_rows);
+  bind_one(d, "lce_soft_targets", abi.soft_targets);
+  bind_one(d, "lce_distill_workspace_bytes", abi.distill_workspace_bytes);
+  bind_one(d, "lce_distill", abi.distill);
 }
 
 int dtype_code(at::ScalarType t) {
@@ -247,10 +253,75 @@ py::object backward(const at::Tensor& x, const at::Tensor& y1, const at::Tensor&
   return py::make_tuple(tensor_or_none(dx), tensor_or_none(dw));
 }
 
+// Distillation (distillation.py): (loss, dx, dw, pre, x, w, w_layout, columns, q, y), as LinearDistillationImplementation keeps them;
+// (status, name) where the C ABI refused; None: not handled.  index, logits: (..., K), contiguous.  scale: of the student's logits, the
+// temperature in it.
+py::object distill(const at::Tensor& x_in, const at::Tensor& At, const at::Tensor& index, const at::Tensor& logits, double temperature,
+                   double scale, int64_t n_chunk, int pack, int route, bool exact, bool need_dx, bool need_dw, bool copy_w, uintptr_t stream) {
+  Call c;
+  lce_problem& p = c.p;
+  if (!describe(x_in, At, false, c) || (c.w != kInPlace && !copy_w)) return py::none();
+  for (const at::Tensor& t : {index, logits})
+    if (!plain(t) || t.device() != x_in.device() || !t.is_contiguous() || t.dim() < 1) return py::none();
+  const int64_t K = index.size(-1);
+  const int ld = dtype_code(logits.scalar_type());
+  if (index.scalar_type() != at::kLong || ld < 0 || K < 1 || index.numel() != p.N * K || logits.numel() != p.N * K) return py::none();
+  p.ignore_index = -1;
+  p.logit_scale = (float)scale;
+  p.n_chunk = n_chunk;
+  p.pack_rows = pack;
+  p.route = (route == 2 ? LCE_ROUTE_ONE_PASS : route == 0 ? LCE_ROUTE_TWO_PASS : LCE_ROUTE_AUTO) | (exact ? LCE_ROUTE_EXACT_SUMS : 0) |
+            (p.x_dtype == LCE_F32 ? LCE_ROUTE_KEEP_LOGITS : 0);
+  const bool grads = need_dx || need_dw;
+  size_t bytes = 0;
+  if (abi.distill_workspace_bytes(&p, K, grads, &bytes) != LCE_OK) return py::none();
+
+  at::NoGradGuard no_grad;
+  const auto o = x_in.options();
+  const at::Tensor x = c.x != kInPlace ? rows_of(p.N, p.H, p.ldx, o) : x_in.dim() == 2 ? x_in : x_in.view({p.N, p.H});
+  const at::Tensor w = c.w != kInPlace ? rows_of(p.H, p.V, p.ldw, At.options()) : p.w_layout == LCE_W_VH ? At.t() : At;
+  at::Tensor dx, dw, pre;
+  if (need_dx) dx = rows_of(p.N, p.H, p.lddx, o);
+  if (need_dw) dw = rows_of(w.size(0), w.size(1), p.lddw, At.options());
+  const auto f32 = o.dtype(at::kFloat);
+  const at::Tensor columns = at::empty({p.N, K}, o.dtype(at::kInt)), q = at::empty({p.N, K}, f32), y = at::empty({p.N}, o.dtype(at::kLong));
+  const at::Tensor loss = at::empty({}, f32);
+  if (grads && p.x_dtype == LCE_F16) pre = at::empty({1}, f32);
+  const size_t lse_bytes = ((size_t)p.N * 4 + 255) & ~(size_t)255;
+  Workspace ws(bytes), kept(lse_bytes + 256);  // (lse and the number of rows)
+  float* const lse = (float*)kept.data.get();
+  int64_t* const n_valid = (int64_t*)((char*)kept.data.get() + lse_bytes);
+  void* const s = reinterpret_cast<void*>(stream);
+  int rc = LCE_OK;
+  const char* what = "lce_distill";
+  {
+    py::gil_scoped_release release;
+    if (c.x != kInPlace) rc = copy_rows(c.x, x_in, p.N, p.H, x, p.ldx, s);
+    if (rc == LCE_OK && c.w != kInPlace) rc = copy_rows(c.w, At, p.H, p.V, w, p.ldw, s);
+    if (rc != LCE_OK) what = "lce_pad_rows";
+    else if ((rc = abi.soft_targets(p.N, K, p.V, (const int64_t*)index.data_ptr(), K, logits.data_ptr(), ld, K, (float)temperature,
+                                    (int32_t*)columns.data_ptr(), (float*)q.data_ptr(), (int64_t*)y.data_ptr(), s)) != LCE_OK)
+      what = "lce_soft_targets";
+    const float* g = nullptr;
+    if (rc == LCE_OK && pre.defined()) {
+      rc = abi.stand_in((const int64_t*)y.data_ptr(), p.N, -1, (float*)pre.data_ptr(), s);
+      g = (const float*)pre.data_ptr();
+    } else if (rc == LCE_OK) {
+      rc = abi.unit_gradient(&g);
+    }
+    if (rc == LCE_OK)
+      rc = abi.distill(&p, K, (const int32_t*)columns.data_ptr(), (const float*)q.data_ptr(), (const int64_t*)y.data_ptr(), x.data_ptr(),
+                       w.data_ptr(), g, lse, (float*)loss.data_ptr(), n_valid, ptr(dx), ptr(dw), ws.data.get(), bytes, s);
+  }
+  if (rc != LCE_OK) return py::make_tuple(rc, what);
+  return py::make_tuple(loss, tensor_or_none(dx), tensor_or_none(dw), tensor_or_none(pre), x, w, p.w_layout, columns, q, y);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_lce_host, m) {
   m.def("bind", &bind);
   m.def("forward", &forward);
   m.def("backward", &backward);
+  m.def("distill", &distill);
 }

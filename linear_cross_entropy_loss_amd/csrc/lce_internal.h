@@ -503,7 +503,7 @@ struct SoftLogits {
 };
 hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const void* logits, int dtype, int64_t ld_logits, int64_t N, int K,
                                int64_t V, float temperature, int* out_index, float* out_q, int64_t* y, hipStream_t s);
-size_t soft_logits_bytes(int64_t N, int K, int64_t V);  // scratch (may be 0)
+size_t soft_logits_bytes(int64_t N, int K, int64_t H, int64_t V, bool w_vh);  // scratch (may be 0)
 hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s);
 // dz of the targets' columns of the slab or chunk that `a` describes, over what the label's kernels staged there.
 hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStream_t s);

@@ -104,6 +104,18 @@ def _run(x, w, layout, targets, scale, N_chunk_size, pack, route, need_dx, need_
     return loss, dx, dw
 
 
+def _native(x, At, index, logits, temperature, scale, N_chunk_size, pack, route, need_dx, need_dw):
+    """All of the forward by the host extension (csrc/lce_host.cpp), which returns the same bits; None: no ordinary call, or one that
+    has a warning to give."""
+    if x.device.index != torch._C._cuda_getDevice():
+        return None
+    done = _lib.host().distill(x, At, index, logits, temperature, scale, N_chunk_size, pack, route, bool(ops.exact_dw_sums.get()), need_dx,
+                               need_dw, "weight" in ops._copy_warned, _stream(x.device))
+    if done is not None and len(done) == 2:
+        _lib.raise_for_status(*done)
+    return done
+
+
 class LinearDistillationImplementation(torch.autograd.Function):
     """Autograd Function behind ``linear_distillation``; gradients for ``x`` and ``At`` only (the teacher is a constant)."""
 
@@ -111,14 +123,18 @@ class LinearDistillationImplementation(torch.autograd.Function):
     def forward(ctx, x_in, At, index, logits, temperature, logit_scale, N_chunk_size, grad_mode):
         x_in = ops._autocast_x(x_in, At)
         need_dx, need_dw = grad_mode and ctx.needs_input_grad[0], grad_mode and ctx.needs_input_grad[1]
-        with _on_device(x_in.device):
-            x, w, layout = _views(x_in, At)
-            targets = _targets(index, logits, At.shape[1], temperature)
-            cfg = (logit_scale / temperature, N_chunk_size, ops._pack_mode(), ops._route_mode())
-            pre = None
-            if (need_dx or need_dw) and x.dtype == torch.float16:
-                pre = ops._stand_in_gradient(x, targets[2], _NO_LABEL)
-            loss, dx, dw = _run(x, w, layout, targets, *cfg, need_dx, need_dw, pre)
+        cfg = (logit_scale / temperature, N_chunk_size, ops._pack_mode(), ops._route_mode())
+        native = _native(x_in, At, index, logits, temperature, *cfg, need_dx, need_dw)
+        if native is not None:
+            loss, dx, dw, pre, x, w, layout, *targets = native
+        else:
+            with _on_device(x_in.device):
+                x, w, layout = _views(x_in, At)
+                targets = _targets(index, logits, At.shape[1], temperature)
+                pre = None
+                if (need_dx or need_dw) and x.dtype == torch.float16:
+                    pre = ops._stand_in_gradient(x, targets[2], _NO_LABEL)
+                loss, dx, dw = _run(x, w, layout, targets, *cfg, need_dx, need_dw, pre)
         ctx.lce_grads = [dx, dw, pre]  # for the first backward; dropped there
         if need_dx or need_dw:
             ctx.save_for_backward(x, w, *targets)

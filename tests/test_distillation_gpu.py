@@ -344,3 +344,41 @@ def test_model_sizes(N, H, V, K, dtype):
         assert abs(loss.item() - ref.item()) <= 64 * 2.0 ** -22 * max(1.0, ref.item())
         assert rel_errors(xg.grad, dz @ wd.t())[1] <= 1.5 * EPS[dtype]
         assert rel_errors(wg.grad.t() if tied else wg.grad, xd.t() @ dz)[1] <= 1.5 * EPS[dtype]
+
+
+@pytest.mark.parametrize("dtype,w_dtype,tied,shape", [(BF16, None, False, (300, 256, 1000)), (F16, None, True, (100, 64, 511)),
+                                                      (BF16, F32, False, (65, 100, 1001)), (F32, None, False, (40, 130, 700))])
+def test_host_path_gives_the_same_bits(dtype, w_dtype, tied, shape):
+    """The C++ host path against the Python one, which a strided index takes."""
+    from linear_cross_entropy_loss_amd import _lib, distillation, linear_distillation
+
+    N, H, V = shape
+    x, w, index, logits = make(N, H, V, 9, dtype, seed=N, empty=0.1, short=0.1, w_dtype=w_dtype)
+    w = (w.t().contiguous().t() if tied else w).cuda()
+    wide = torch.zeros(N, 12, dtype=torch.int64, device="cuda")
+    wide[:, :9] = index.cuda()
+    taken = []
+    native = distillation._native
+    distillation._native = lambda *a: taken.append(native(*a)) or taken[-1]
+    try:
+        results = []
+        for i in (index.cuda(), index.cuda(), wide[:, :9]):  # (the first call may have a warning to give)
+            xg, wg = x.cuda().requires_grad_(True), w.detach().requires_grad_(True)
+            loss = linear_distillation(xg, wg, i, logits.cuda(), 1.5, 0.7)
+            results.append((loss.detach(), *torch.autograd.grad(loss, (xg, wg))))
+    finally:
+        distillation._native = native
+    assert taken[1] is not None and taken[2] is None
+    for a, b in zip(results[1], results[2]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("w_vh", [False, True])
+def test_sorted_and_unsorted_entries(w_vh):
+    """Both sides of the rule by which the targets' logits are formed, columns that many rows name, small numbers of fp16."""
+    for N, K, H in ((2000, 40, 72), (64, 10, 72), (600, 130, 100)):
+        x, w, index, logits = make(N, H, 900, K, F16, seed=K)
+        index[:, 0] = 17  # a column of every row
+        index[:, 1:][index[:, 1:] == 17] = 18
+        w[:, ::3] *= 2.0 ** -12  # subnormal numbers of the type among them
+        check((x, w, index, logits), tied=w_vh and H % 8 == 0, up=512.0)
