@@ -21,6 +21,15 @@ constexpr int kDigits = 2048;  // values of a digit
 constexpr int kMostWaves = 16;  // of a workgroup
 typedef unsigned long long u64;
 
+// The thread's number, as one that the compiler takes for a new one each time: it would else work out addresses from it before the loop
+// over the rows, for all of a kernel's ways to do a row, and there are no registers to keep them in.
+LCE_DEV int thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  __builtin_assume(t >= 0 && t < 1024);
+  return t;
+}
+
 constexpr unsigned kNanKey = 0xffffffffu, kLowKey = 0x007fffffu;  // NaN; -infinity
 LCE_DEV unsigned key_of(float f) {
   unsigned b = __builtin_bit_cast(unsigned, f);
@@ -42,22 +51,22 @@ template <> struct bits_of<4> { typedef unsigned type; };
 
 // A row in units of up to 16 bytes: its elements before the first address of 16 bytes, whole pieces, the rest.  Wave w has the units
 // [w * share, (w + 1) * share), 64 neighbouring ones at a time, so that (wave, round, lane, element) is the order of the columns.
-template <class E, int NT> struct RowUnits {
+template <class E, int NT, int FLIGHT = 4> struct RowUnits {
   static constexpr int kPer = 16 / sizeof(E), kThreads = NT, kWaves = NT / 64;
   const E* p;
-  int64_t head, body, n, share, units;
-  LCE_DEV RowUnits(const E* row, int64_t cols) : p(row), n(cols) {
-    const int64_t off = (int64_t)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E));
+  int head, body, n, share, units;
+  LCE_DEV RowUnits(const E* row, int64_t cols) : p(row), n((int)cols) {
+    const int off = (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E));
     head = off < n ? off : n;
     body = (n - head) / kPer;
     units = body + 2;
     share = (units + NT - 1) / NT * 64;
   }
-  LCE_DEV int64_t column(int64_t unit) const { return unit == 0 ? 0 : head + (unit - 1) * kPer; }
-  LCE_DEV int count(int64_t unit) const {
+  LCE_DEV int column(int unit) const { return unit == 0 ? 0 : head + (unit - 1) * kPer; }
+  LCE_DEV int count(int unit) const {
     return unit == 0 ? (int)head : unit <= body ? kPer : unit == body + 1 ? (int)(n - head - body * kPer) : 0;
   }
-  LCE_DEV u32x4_t load(int64_t unit) const {
+  LCE_DEV u32x4_t load(int unit) const {
     if (unit >= 1 && unit <= body) return *reinterpret_cast<const u32x4_t*>(p + column(unit));
     // (a loop that is not unrolled: it is for two units of a row)
     typedef typename bits_of<sizeof(E)>::type Bits;
@@ -72,23 +81,47 @@ template <class E, int NT> struct RowUnits {
     }
     return u32x4_t{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
   }
-  // f(unit, elements, how many of them are there) for the units of this lane, four loads in flight; every lane of a wave makes
-  // the same number of calls.
+  // f(unit, its elements, how many of them are there) for the units of this lane, FLIGHT loads in flight; every lane of a wave makes
+  // the same number of calls.  (Loops that are not unrolled, here and over the elements: the kernels that end up here, for the rows that
+  // their own way does not do, have no registers to spare.)
   template <class F> LCE_DEV void each(F f) const {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t u0 = wave * share + lane;
-    for (int64_t i = 0; i < share && wave * share + i < units; i += 256) {
-      u32x4_t v[4];
+    const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int u0 = wave * share + lane;
+#pragma unroll 1
+    for (int i = 0; i < share && wave * share + i < units; i += FLIGHT * 64) {
+      u32x4_t v[FLIGHT];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = i + r * 64 < share ? load(u0 + i + r * 64) : u32x4_t{};
+      for (int r = 0; r < FLIGHT; ++r) v[r] = i + r * 64 < share ? load(u0 + i + r * 64) : u32x4_t{};
+#pragma unroll 1
+      for (int j = i; j < i + FLIGHT * 64 && j < share; j += 64) {
+        f(u0 + j, v[0], count(u0 + j));
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (i + r * 64 < share) {
-          E e[kPer];
-          __builtin_memcpy(e, &v[r], 16);
-          f(u0 + i + r * 64, e, count(u0 + i + r * 64));
-        }
+        for (int r = 0; r + 1 < FLIGHT; ++r) v[r] = v[r + 1];
+      }
     }
+  }
+  // f(which, element) for the elements of a unit.
+  template <class F> LCE_DEV static void elements(u32x4_t v, int c, F f) {
+#pragma unroll 1
+    for (int i = 0; i < c; ++i) {
+      if constexpr (sizeof(E) == 2) {
+        const unsigned w = v[0];
+        f(i, as_float(__builtin_bit_cast(E, (unsigned short)w)));
+        v[0] = i & 1 ? v[1] : w >> 16;
+        if (i & 1) {
+          v[1] = v[2];
+          v[2] = v[3];
+        }
+      } else {
+        const unsigned w = v[0];
+        f(i, __builtin_bit_cast(float, w));
+        v = u32x4_t{v[1], v[2], v[3], 0};
+      }
+    }
+  }
+  // f(element) for the elements of this lane's units.
+  template <class F> LCE_DEV void elements(F f) const {
+    each([&](int, u32x4_t v, int c) { elements(v, c, [&](int, float z) { f(z); }); });
   }
 };
 
@@ -109,6 +142,11 @@ LCE_DEV u64 read_lane(u64 v, int lane) {
 LCE_DEV int read_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 LCE_DEV unsigned read_lane(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
 LCE_DEV double read_lane(double v, int lane) { return __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, v), lane)); }
+// A value that all lanes have, into scalar registers.
+template <class F> LCE_DEV F uniform(F v) {
+  if constexpr (sizeof(F) == 4) return __builtin_bit_cast(F, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  else return read_lane(v, 0);
+}
 struct Sum {
   template <class F> LCE_DEV static F join(F a, F b) { return a + b; }
 };
@@ -129,7 +167,7 @@ template <class J, class F, bool ROW = false> LCE_DEV F wave_upto(F v) {
 }
 // Over the workgroup; `sh`: room for one value of each wave.  *before (sums): over the threads before this one.  Ends with a barrier.
 template <class J, int NT, class F> LCE_DEV F block_all(F v, F* sh, F* before = nullptr) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const F upto = wave_upto<J>(v);
   if (lane == 63) sh[wave] = upto;
   __syncthreads();
@@ -175,78 +213,80 @@ template <> struct Equal<float> {
 
 // The column of the r-th (from 0) element with a value; -1 if there are no more than r.  All threads take part and get it.  The waves
 // count such elements, by parts of their share of the row, and the one that has the r-th looks for it in its part.
-constexpr int kParts = 32, kPartRounds = 8;  // rounds that are in flight together
+// kPartRounds rounds are in flight together.
+constexpr int kParts = 32;
 struct ColumnShared {
   int count[kMostWaves][kParts];
-  int64_t of_wave[kMostWaves];
-  int64_t column;
+  int of_wave[kMostWaves];
+  int column;
 };
-template <class E, int NT> LCE_DEV int64_t column_of(const RowUnits<E, NT>& row, float value, int64_t r, ColumnShared* sh) {
-  constexpr int kPer = RowUnits<E, NT>::kPer;
+template <int kPartRounds = 8, class E, int NT, int FL> LCE_DEV int column_of(const RowUnits<E, NT, FL>& row, float value, int r, ColumnShared* sh) {
+  constexpr int kPer = RowUnits<E, NT, FL>::kPer;
   const Equal<E> equal(value);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t u0 = wave * row.share, left = (row.units - u0 + 63) / 64, share = row.share / 64;
-  const int64_t rounds = left < 0 ? 0 : left < share ? left : share;
-  const int64_t per = (rounds + kParts * kPartRounds - 1) / (kParts * kPartRounds) * kPartRounds;  // rounds of a part
-  auto load = [&](int64_t i, u32x4_t (&v)[kPartRounds]) {
+  const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int u0 = wave * row.share, left = (row.units - u0 + 63) / 64, share = row.share / 64;
+  const int rounds = left < 0 ? 0 : left < share ? left : share;
+  const int per = (rounds + kParts * kPartRounds - 1) / (kParts * kPartRounds) * kPartRounds;  // rounds of a part
+  // f(unit, its elements) for the units of kPartRounds rounds from i that may have the value.  (Few have it: that loop is not unrolled.)
+  auto look = [&](int i, auto f) {
+    u32x4_t v[kPartRounds];
+    unsigned hits = 0;
 #pragma unroll
     for (int q = 0; q < kPartRounds; ++q)
       if (i + q < rounds) v[q] = row.load(u0 + (i + q) * 64 + lane);
+#pragma unroll
+    for (int q = 0; q < kPartRounds; ++q)
+      if (i + q < rounds && __any(equal.maybe(v[q]))) hits |= 1u << q;
+#pragma unroll 1
+    for (int unit = u0 + i * 64 + lane; hits != 0; hits >>= 1, unit += 64) {
+      if (hits & 1) f(unit, v[0]);
+#pragma unroll
+      for (int q = 0; q + 1 < kPartRounds; ++q) v[q] = v[q + 1];
+    }
   };
-  if (threadIdx.x == 0) sh->column = -1;
+  if (t == 0) sh->column = -1;
   int mine = 0;
 #pragma unroll 1
-  for (int64_t i = 0, part = 0; i < rounds; ++part) {
+  for (int i = 0, part = 0; i < rounds; ++part) {
     int count = 0;
 #pragma unroll 1
-    for (const int64_t end = i + per; i < end && i < rounds; i += kPartRounds) {
-      u32x4_t v[kPartRounds];
-      load(i, v);
+    for (const int end = i + per; i < end && i < rounds; i += kPartRounds)
+      look(i, [&](int unit, u32x4_t v) {
+        const int c = row.count(unit);
 #pragma unroll
-      for (int q = 0; q < kPartRounds; ++q)
-        if (i + q < rounds && __any(equal.maybe(v[q]))) {
-          const int c = row.count(u0 + (i + q) * 64 + lane);
-#pragma unroll
-          for (int k = 0; k < kPer; ++k) count += __popcll(__ballot(k < c && equal.is(v[q], k)));
-        }
-    }
+        for (int k = 0; k < kPer; ++k) count += __popcll(__ballot(k < c && equal.is(v, k)));
+      });
     if (lane == 0) sh->count[wave][part] = count;
     mine += count;
   }
   if (lane == 0) sh->of_wave[wave] = mine;
   __syncthreads();
-  int64_t before = 0;
+  int before = 0;
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) before += w < wave ? sh->of_wave[w] : 0;
   if (before <= r && r < before + mine) {  // (one wave)
-    int64_t i = 0;
+    int i = 0;
     for (int part = 0; part < kParts - 1 && before + sh->count[wave][part] <= r; ++part, i += per) before += sh->count[wave][part];
 #pragma unroll 1
-    for (const int64_t end = i + per; i < end && i < rounds; i += kPartRounds) {
-      u32x4_t v[kPartRounds];
-      load(i, v);
-#pragma unroll
-      for (int q = 0; q < kPartRounds; ++q) {
-        if (!(i + q < rounds && __any(equal.maybe(v[q])))) continue;
-        const int64_t unit = u0 + (i + q) * 64 + lane;
+    for (const int end = i + per; i < end && i < rounds; i += kPartRounds)
+      look(i, [&](int unit, u32x4_t v) {
         const int c = row.count(unit);
         int here = 0;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) here += k < c && equal.is(v[q], k) ? 1 : 0;
+        for (int k = 0; k < kPer; ++k) here += k < c && equal.is(v, k) ? 1 : 0;
         const int upto = wave_upto<Sum>(here);
-        int64_t at = before + upto - here;
+        int at = before + upto - here;
 #pragma unroll
         for (int k = 0; k < kPer; ++k)
-          if (k < c && equal.is(v[q], k)) {
+          if (k < c && equal.is(v, k)) {
             if (at == r) sh->column = row.column(unit) + k;
             ++at;
           }
         before += read_lane(upto, 63);
-      }
-    }
+      });
   }
   __syncthreads();
-  const int64_t at = sh->column;
+  const int at = sh->column;
   __syncthreads();
   return at;
 }
@@ -302,26 +342,22 @@ LCE_DEV bool in_prefix(unsigned key, unsigned prefix, int level) {
 
 // Histogram of the digit `level` over the elements that agree with `prefix` in the digits before it.  WEIGHTED: elements without
 // a weight, which are never drawn, are left out.  Ends with a barrier.
-template <bool WEIGHTED, class E, int NT, class W>
-LCE_DEV void fill_histogram(const RowUnits<E, NT>& row, const W& weights, unsigned prefix, int level, Histogram<WEIGHTED>* h) {
-  for (int i = threadIdx.x; i < kDigits; i += NT) {
+template <bool WEIGHTED, class E, int NT, int FL, class W>
+LCE_DEV void fill_histogram(const RowUnits<E, NT, FL>& row, const W& weights, unsigned prefix, int level, Histogram<WEIGHTED>* h) {
+  for (int i = thread(); i < kDigits; i += NT) {
     h->count[i] = 0;
     if constexpr (WEIGHTED) h->weight[i] = 0;
   }
   __syncthreads();
-  row.each([&](int64_t, const E* e, int c) {
-#pragma unroll
-    for (int i = 0; i < RowUnits<E, NT>::kPer; ++i) {
-      const float z = as_float(e[i]);
-      const unsigned key = key_of(z);
-      if (i >= c || !in_prefix(key, prefix, level)) continue;
-      if constexpr (WEIGHTED) {
-        const u64 w = key == kLowKey ? 0 : weights.of(z);
-        if (w == 0) continue;
-        atomicAdd(&h->weight[digit_of(key, level)], w);
-      }
-      atomicAdd(&h->count[digit_of(key, level)], 1);
+  row.elements([&](float z) {
+    const unsigned key = key_of(z);
+    if (!in_prefix(key, prefix, level)) return;
+    if constexpr (WEIGHTED) {
+      const u64 w = key == kLowKey ? 0 : weights.of(z);
+      if (w == 0) return;
+      atomicAdd(&h->weight[digit_of(key, level)], w);
     }
+    atomicAdd(&h->count[digit_of(key, level)], 1);
   });
   __syncthreads();
 }
@@ -329,9 +365,9 @@ LCE_DEV void fill_histogram(const RowUnits<E, NT>& row, const W& weights, unsign
 // A place in the order: the key there, and how many elements and what weight come before the first of that key.
 struct Place {
   unsigned key;
-  int64_t count;
+  int count;
   u64 weight;
-  int64_t same;  // elements with the key
+  int same;  // elements with the key
 };
 // KEEP: the first digit's histogram stays for the next place that a row asks for.
 template <bool WEIGHTED, bool KEEP> struct SelectShared {
@@ -346,27 +382,23 @@ template <bool WEIGHTED, bool KEEP> struct SelectShared {
 };
 
 // The histogram of the first digit; returns the weight of the elements with a key of `least` and above.
-template <class E, int NT, class Shared>
-LCE_DEV u64 fill_first(const RowUnits<E, NT>& row, const Weights& weights, unsigned least, Shared* sh) {
+template <class E, int NT, int FL, class Shared>
+LCE_DEV u64 fill_first(const RowUnits<E, NT, FL>& row, const Weights& weights, unsigned least, Shared* sh) {
   Histogram<true>* h = sh->first;
-  for (int i = threadIdx.x; i < kDigits; i += NT) {
+  for (int i = thread(); i < kDigits; i += NT) {
     h->count[i] = 0;
     h->weight[i] = 0;
   }
   __syncthreads();
   u64 mine = 0;
-  row.each([&](int64_t, const E* e, int c) {
-#pragma unroll
-    for (int i = 0; i < RowUnits<E, NT>::kPer; ++i) {
-      const float z = as_float(e[i]);
-      const unsigned key = key_of(z);
-      if (i >= c || key == kLowKey) continue;
-      const u64 w = weights.of(z);
-      if (w == 0) continue;
-      if (key >= least) mine += w;
-      atomicAdd(&h->weight[digit_of(key, 0)], w);
-      atomicAdd(&h->count[digit_of(key, 0)], 1);
-    }
+  row.elements([&](float z) {
+    const unsigned key = key_of(z);
+    if (key == kLowKey) return;
+    const u64 w = weights.of(z);
+    if (w == 0) return;
+    if (key >= least) mine += w;
+    atomicAdd(&h->weight[digit_of(key, 0)], w);
+    atomicAdd(&h->count[digit_of(key, 0)], 1);
   });
   return block_all<Sum, NT>(mine, sh->of_wave);
 }
@@ -376,11 +408,11 @@ LCE_DEV u64 fill_first(const RowUnits<E, NT>& row, const Weights& weights, unsig
 enum Wanted { kByCount, kByShare, kByWeight };
 struct Want {
   Wanted what;
-  int64_t k;
+  int k;
   double most;
   u64 target;
   // whether it is among c elements of weight w behind cb elements of weight wb
-  LCE_DEV bool here(int64_t cb, u64 wb, int64_t c, u64 w) const {
+  LCE_DEV bool here(int cb, u64 wb, int c, u64 w) const {
     if (c == 0) return false;
     if (what == kByCount) return cb < k && k <= cb + c;
     if (what == kByShare) return (wb == 0 || (double)wb < most) && !((double)(wb + w) < most);
@@ -389,15 +421,15 @@ struct Want {
 };
 
 // The place that is wanted.  KEEP: the histogram of the first digit is there (fill_first).
-template <bool WEIGHTED, bool KEEP, class E, int NT, class W>
-LCE_DEV Place find_place(const RowUnits<E, NT>& row, const W& weights, SelectShared<WEIGHTED, KEEP>* sh, const Want& want) {
+template <bool WEIGHTED, bool KEEP, class E, int NT, int FL, class W>
+LCE_DEV Place find_place(const RowUnits<E, NT, FL>& row, const W& weights, SelectShared<WEIGHTED, KEEP>* sh, const Want& want) {
   constexpr int kOwn = kDigits / NT;  // digits of a thread, the largest first
   Place p = {0, 0, 0, 0};
 #pragma unroll 1
   for (int level = 0; level < 3; ++level) {
     Histogram<WEIGHTED>* h = sh->of_level(level);
     if (level > 0 || !KEEP) fill_histogram<WEIGHTED>(row, weights, p.key, level, h);
-    const int top = kDigits - 1 - kOwn * (int)threadIdx.x;
+    const int top = kDigits - 1 - kOwn * (int)thread();
     int c = 0;
     u64 w = 0;
 #pragma unroll
@@ -409,7 +441,7 @@ LCE_DEV Place find_place(const RowUnits<E, NT>& row, const W& weights, SelectSha
     u64 w_before = 0;
     block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave), &c_before);
     if (WEIGHTED) block_all<Sum, NT>(w, sh->of_wave, &w_before);
-    int64_t cb = p.count + c_before;
+    int cb = p.count + c_before;
     u64 wb = p.weight + w_before;
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
     if (want.here(cb, wb, c, w)) {
@@ -431,14 +463,11 @@ LCE_DEV Place find_place(const RowUnits<E, NT>& row, const W& weights, SelectSha
 }
 
 // The largest key of the row.
-template <class E, int NT> LCE_DEV unsigned largest_key(const RowUnits<E, NT>& row, unsigned* sh) {
+template <class E, int NT, int FL> LCE_DEV unsigned largest_key(const RowUnits<E, NT, FL>& row, unsigned* sh) {
   unsigned top = 0;
-  row.each([&](int64_t, const E* e, int c) {
-#pragma unroll
-    for (int i = 0; i < RowUnits<E, NT>::kPer; ++i) {
-      const unsigned k = key_of(as_float(e[i]));
-      top = i < c && k > top ? k : top;
-    }
+  row.elements([&](float z) {
+    const unsigned k = key_of(z);
+    top = k > top ? k : top;
   });
   return block_all<Largest, NT>(top, sh);
 }
@@ -446,25 +475,26 @@ template <class E, int NT> LCE_DEV unsigned largest_key(const RowUnits<E, NT>& r
 // Settings of a row.
 struct RowSettings {
   float temperature, top_p, min_p, u;
-  int64_t top_k;
+  int top_k;
   int bits;
   LCE_DEV RowSettings(const Sampling& s, const float* u_, int64_t n, int bits_) : bits(bits_) {
-    temperature = s.temperature_rows ? s.temperature_rows[n] : s.temperature;
-    top_p = s.top_p_rows ? s.top_p_rows[n] : s.top_p;
-    min_p = s.min_p_rows ? s.min_p_rows[n] : s.min_p;
-    top_k = s.top_k_rows ? s.top_k_rows[n] : s.top_k;
-    u = u_[n];
+    temperature = uniform(s.temperature_rows ? s.temperature_rows[n] : s.temperature);
+    top_p = uniform(s.top_p_rows ? s.top_p_rows[n] : s.top_p);
+    min_p = uniform(s.min_p_rows ? s.min_p_rows[n] : s.min_p);
+    const int64_t k = s.top_k_rows ? s.top_k_rows[n] : s.top_k;
+    top_k = uniform(k < 0 ? 0 : k > 0x7fffffff ? 0x7fffffff : (int)k);
+    u = uniform(u_[n]);
   }
   LCE_DEV bool greedy() const { return !(temperature > 0.f) || top_k == 1; }
   LCE_DEV Weights weights(float top) const {
-    return {(double)top, 1.4426950408889634074 / (double)temperature, (double)((u64)1 << bits)};
+    return {uniform((double)top), uniform(1.4426950408889634074 / (double)temperature), (double)((u64)1 << bits)};
   }
 };
 
 // The place of the token, and which of the place's elements it is, from `find`, which looks up places, the number of elements
 // with a weight, the sum of their weights and of those that min_p keeps.
 template <class Find, class WeightAt>
-LCE_DEV Place draw_place(const RowSettings& s, int64_t counted, u64 all, u64 by_min, Place at, int64_t* which, Find find, WeightAt weight_at) {
+LCE_DEV Place draw_place(const RowSettings& s, int counted, u64 all, u64 by_min, Place at, int* which, Find find, WeightAt weight_at) {
   u64 stays = all;
   if (s.min_p > 1.f) by_min = (u64)1 << s.bits;  // (the first column alone)
 #pragma unroll 1
@@ -485,27 +515,26 @@ LCE_DEV Place draw_place(const RowSettings& s, int64_t counted, u64 all, u64 by_
       stays = at.weight + (u64)(s.top_k - at.count) * w;
     } else if (step == kByShare) {
       const double some = (want.most - (double)at.weight) / (double)w;
-      int64_t kept = some > 0.0 ? (int64_t)some : 0;
-      if (kept > at.same) kept = at.same;
+      int kept = some > 0.0 ? (some < (double)at.same ? (int)some : at.same) : 0;
       if (kept < at.same && (double)(at.weight + (u64)kept * w) < want.most) ++kept;  // (`some` rounded down)
       if (at.weight == 0 && kept == 0) kept = 1;
       const u64 by_p = at.weight + (u64)kept * w;
       if (by_p < stays) stays = by_p;
     } else {
-      *which = (int64_t)((want.target - at.weight) / w);
+      *which = (int)((want.target - at.weight) / w);
     }
   }
   return at;
 }
 
 // The token of a row by digits, any type; -1 where there is none.
-template <class E, int NT, bool KEEP>
-LCE_DEV int64_t sample_by_digits(const RowUnits<E, NT>& row, const RowSettings& s, SelectShared<true, KEEP>* sh) {
+template <class E, int NT, int FL, bool KEEP>
+LCE_DEV int sample_by_digits(const RowUnits<E, NT, FL>& row, const RowSettings& s, SelectShared<true, KEEP>* sh) {
   const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh->of_wave));
   if (top == kNanKey || top == kLowKey) return -1;  // a NaN, or no column left
   Place at = {top, 0, 0, 0};
-  int64_t which = 0;
-  if (threadIdx.x == 0) sh->place = at;
+  int which = 0;
+  if (thread() == 0) sh->place = at;
   if (!s.greedy()) {
     const Weights weights = s.weights(value_of(top));
     // the smallest key that min_p keeps: the weights are monotone in the keys
@@ -521,10 +550,11 @@ LCE_DEV int64_t sample_by_digits(const RowUnits<E, NT>& row, const RowSettings& 
     const u64 by_min = fill_first(row, weights, s.min_p > 0.f ? least : 0, sh);
     u64 w = 0;
     int c = 0;
+    const int t = thread();
 #pragma unroll
     for (int i = 0; i < kDigits / NT; ++i) {
-      w += sh->first->weight[i * NT + threadIdx.x];
-      c += sh->first->count[i * NT + threadIdx.x];
+      w += sh->first->weight[i * NT + t];
+      c += sh->first->count[i * NT + t];
     }
     const u64 all = block_all<Sum, NT>(w, sh->of_wave);
     const int counted = block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave));
@@ -532,27 +562,27 @@ LCE_DEV int64_t sample_by_digits(const RowUnits<E, NT>& row, const RowSettings& 
                     [&](const Want& want) { return find_place<true, KEEP>(row, weights, sh, want); },
                     [&](const Place& p) { return weights.of(value_of(p.key)); });
   }
-  return column_of(row, value_of(at.key), which, &sh->columns);
+  return column_of<FL == 4 ? 8 : 2>(row, value_of(at.key), which, &sh->columns);
 }
 
 constexpr int kMostTop = 1024;
 
 // An entry of a list that is sorted: by key, the larger first, then by column.
-LCE_DEV u64 entry_of(unsigned key, int64_t column) { return (u64)~key << 32 | (u64)column; }
+LCE_DEV u64 entry_of(unsigned key, int column) { return (u64)~key << 32 | (u64)column; }
 LCE_DEV unsigned key_in(u64 entry) { return ~(unsigned)(entry >> 32); }
-LCE_DEV int64_t column_in(u64 entry) { return (int64_t)(entry & 0xffffffffu); }
+LCE_DEV int column_in(u64 entry) { return (int)(entry & 0xffffffffu); }
 
 // A bitonic network over list[0 .. sorted), a power of two from 2 on; up to 128 entries by one wave, without barriers in between.
 // Starts and ends with a barrier.
 template <int NT> LCE_DEV void sort_list(u64* list, int sorted) {
   __syncthreads();
   const bool one_wave = sorted <= 128;
-  if (!one_wave || threadIdx.x < 64) {
+  if (!one_wave || thread() < 64) {
 #pragma unroll 1
     for (int size = 2; size <= sorted; size <<= 1)
 #pragma unroll 1
       for (int d = size >> 1; d > 0; d >>= 1) {
-        for (int t = threadIdx.x; t < sorted / 2; t += NT) {
+        for (int t = thread(); t < sorted / 2; t += NT) {
           const int i = ((t & ~(d - 1)) << 1) | (t & (d - 1)), j = i | d;  // the t-th pair
           const u64 a = list[i], b = list[j];
           if ((a > b) == ((i & size) == 0)) {
@@ -574,7 +604,7 @@ template <int NT> LCE_DEV void sort_list(u64* list, int sorted) {
 constexpr int kMostRanked = 512;
 template <int NT> LCE_DEV const u64* rank_list(const u64* list, u64* to, int n) {
   __syncthreads();
-  for (int t = threadIdx.x; t < n; t += NT) {
+  for (int t = thread(); t < n; t += NT) {
     const u64 mine = list[t];
     int rank = 0;
     int j = 0;
@@ -596,71 +626,61 @@ LCE_DEV int power_of_two(int n) {
   return p;
 }
 // The first k of the list to memory.
-template <class E, int NT> LCE_DEV void store_top(const RowUnits<E, NT>& row, const u64* list, int k, E* values, int64_t* index) {
-  for (int i = threadIdx.x; i < k; i += NT) {
-    int64_t column = column_in(list[i]);
-    column = column < row.n ? column : row.n - 1;  // (logits that change under the kernel must not lead it astray)
+template <class E, int NT, int FL> LCE_DEV void store_top(const RowUnits<E, NT, FL>& row, const u64* list, int k, E* values, int64_t* index) {
+  for (int i = thread(); i < k; i += NT) {
+    int column = column_in(list[i]);
+    column = (unsigned)column < (unsigned)row.n ? column : row.n - 1;  // (logits that change under the kernel must not lead it astray)
     index[i] = column;
     values[i] = row.p[column];
   }
 }
 
 // The first k of a row by digits, any type.  list: kMostTop entries.
-template <class E, int NT>
-LCE_DEV void top_by_digits(const RowUnits<E, NT>& row, int k, E* values, int64_t* index, float* lse, SelectShared<false, false>* sh, u64* list,
+template <class E, int NT, int FL>
+LCE_DEV void top_by_digits(const RowUnits<E, NT, FL>& row, int k, E* values, int64_t* index, float* lse, SelectShared<false, false>* sh, u64* list,
                            int* listed) {
-  constexpr int kPer = RowUnits<E, NT>::kPer;
   if (lse != nullptr) {
     const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh->of_wave));
     const float m = top == kNanKey ? __builtin_nanf("") : value_of(top);
     float sum = 0.f;
-    row.each([&](int64_t, const E* e, int c) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const float z = as_float(e[i]);
-        if (i < c) sum += z == m ? 1.f : __expf(z - m);  // (equal infinities have no difference)
-      }
-    });
+    row.elements([&](float z) { sum += z == m ? 1.f : __expf(z - m); });  // (equal infinities have no difference)
     const double all = block_all<Sum, NT>((double)sum, reinterpret_cast<double*>(sh->of_wave));
-    if (threadIdx.x == 0) *lse = top == kLowKey ? m : (float)((double)m + log(all));
+    if (thread() == 0) *lse = top == kLowKey ? m : (float)((double)m + log(all));
   }
   const Place p = find_place<false, false>(row, NoWeights(), sh, Want{kByCount, k, 0.0, 0});
   // what is larger, in any order, and the first k - p.count of the key in the order of the columns
-  const int sorted = power_of_two(k), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (threadIdx.x == 0) *listed = 0;
-  for (int i = threadIdx.x; i < sorted; i += NT) list[i] = ~(u64)0;
+  const int sorted = power_of_two(k), t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  if (t == 0) *listed = 0;
+  for (int i = t; i < sorted; i += NT) list[i] = ~(u64)0;
   __syncthreads();
   int mine = 0;
-  row.each([&](int64_t unit, const E* e, int c) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const unsigned key = key_of(as_float(e[i]));
-      if (i < c && key > p.key) {
+  row.each([&](int unit, u32x4_t v, int c) {
+    row.elements(v, c, [&](int i, float z) {
+      const unsigned key = key_of(z);
+      if (key > p.key) {
         const int to = atomicAdd(listed, 1);  // (p.count of them)
         if (to < kMostTop) list[to] = entry_of(key, row.column(unit) + i);
       }
-      mine += i < c && key == p.key ? 1 : 0;
-    }
+      mine += key == p.key ? 1 : 0;
+    });
   });
   const int upto = wave_upto<Sum>(mine);
   if (lane == 63) sh->columns.of_wave[wave] = upto;
   __syncthreads();
-  const int64_t want = k - p.count;
-  int64_t before = 0;
+  const int want = k - p.count;
+  int before = 0;
   for (int w = 0; w < wave; ++w) before += sh->columns.of_wave[w];
   if (sh->columns.of_wave[wave] > 0 && before < want) {
-    row.each([&](int64_t unit, const E* e, int c) {
+    row.each([&](int unit, u32x4_t v, int c) {
       int here = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) here += i < c && key_of(as_float(e[i])) == p.key ? 1 : 0;
+      row.elements(v, c, [&](int, float z) { here += key_of(z) == p.key ? 1 : 0; });
       const int of_unit = wave_upto<Sum>(here);
-      int64_t at = before + of_unit - here;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i < c && key_of(as_float(e[i])) == p.key) {
-          if (at < want) list[p.count + at] = entry_of(p.key, row.column(unit) + i);
-          ++at;
-        }
+      int at = before + of_unit - here;
+      row.elements(v, c, [&](int i, float z) {
+        if (key_of(z) != p.key) return;
+        if (at < want) list[p.count + at] = entry_of(p.key, row.column(unit) + i);
+        ++at;
+      });
       before += read_lane(of_unit, 63);
     });
   }
@@ -737,17 +757,17 @@ template <class E, int NT> struct RowPieces {
   typedef typename bits_of<sizeof(E)>::type Bits;
   static constexpr int kPer = 16 / sizeof(E), kFlight = 4, kThreads = NT;
   const E* p;
-  int64_t n, head, body;
-  LCE_DEV RowPieces(const E* row, int64_t cols) : p(row), n(cols) {
-    const int64_t off = (int64_t)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E));
+  int n, head, body;
+  LCE_DEV RowPieces(const E* row, int64_t cols) : p(row), n((int)cols) {
+    const int off = (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E));
     head = off < n ? off : n;
     body = (n - head) / kPer;
   }
   // f(column, ordered bits) for the elements at the edges, one to a thread.
   template <class F> LCE_DEV void edges(F f) const {
-    const int64_t tail = n - head - body * kPer, t = threadIdx.x;
+    const int tail = n - head - body * kPer, t = thread();
     if (t < head + tail) {
-      const int64_t at = t < head ? t : n - tail + (t - head);
+      const int at = t < head ? t : n - tail + (t - head);
       const unsigned w = O::word(reinterpret_cast<const Bits*>(p)[at]);
       f(at, sizeof(E) == 2 ? w & 0xffffu : w);
     }
@@ -756,19 +776,39 @@ template <class E, int NT> struct RowPieces {
   template <class F> LCE_DEV void each(F f) const {
     const u32x4_t* from = reinterpret_cast<const u32x4_t*>(p + head);
 #pragma unroll 1
-    for (int64_t base = threadIdx.x; base < body; base += kFlight * NT) {
+    for (int base = thread(); base < body; base += kFlight * NT) {
       u32x4_t v[kFlight];
 #pragma unroll
       for (int r = 0; r < kFlight; ++r) {
-        const int64_t at = base + r * NT;
+        const int at = base + r * NT;
         v[r] = from[at < body ? at : base];
       }
 #pragma unroll
       for (int r = 0; r < kFlight; ++r) {
-        const int64_t at = base + r * NT;
+        const int at = base + r * NT;
         if (at < body) f(head + at * kPer, v[r], r);
       }
     }
+  }
+  // The largest key.
+  LCE_DEV unsigned largest(unsigned* sh) const {
+    unsigned most = 0, least = ~0u;
+    edges([&](int, unsigned a) {
+      most = O::larger(most, a);  // (of 16 bits: the upper half stays as it is)
+      least = O::smaller(least, sizeof(E) == 2 ? a | 0xffff0000u : a);
+    });
+    each([&](int, u32x4_t v, int) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned a = O::word(v[i]);
+        most = O::larger(most, a);
+        least = O::smaller(least, a);
+      }
+    });
+    most = O::largest(most);
+    if (O::smallest(least) < O::kLow) most = ~0u;  // (a NaN is above +inf or below -inf)
+    most = block_all<Largest, NT>(most, sh);
+    return most > O::kInf ? kNanKey : key_of(O::value(most));
   }
 };
 
@@ -777,13 +817,13 @@ template <class E, int NT> struct RowPieces {
 template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first(const RowPieces<E, NT>& row, int k, Shared* sh) {
   typedef Ordered<E> O;
   constexpr int kPer = RowPieces<E, NT>::kPer, kOwn = kMaxima / NT, kWaves = NT / 64;  // maxima of a thread: of every kOwn-th piece
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   unsigned most[kOwn] = {}, least = ~0u;
-  row.edges([&](int64_t, unsigned a) {
+  row.edges([&](int, unsigned a) {
     most[0] = O::larger(most[0], a);  // (of 16 bits: the upper half stays as it is)
     least = O::smaller(least, sizeof(E) == 2 ? a | 0xffff0000u : a);
   });
-  row.each([&](int64_t, u32x4_t v, int r) {
+  row.each([&](int, u32x4_t v, int r) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const unsigned a = O::word(v[i]);
@@ -825,18 +865,18 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
   const unsigned from = O::from_top_bits(bound);
   const float m = O::value(top);
   float sum = 0.f;
-  auto add = [&](int64_t at, unsigned a) {
+  auto add = [&](int at, unsigned a) {
     if (a >= from) {
       const int to = atomicAdd(&sh->listed, 1);
       if (to < kMostList) sh->list[to] = entry_of(key_of(O::value(a)), at);
     }
   };
   auto term = [&](float z) { sum += __builtin_amdgcn_exp2f((z - m) * 1.4426950408889634f); };
-  row.edges([&](int64_t at, unsigned a) {
+  row.edges([&](int at, unsigned a) {
     add(at, a);
     if (LSE) term(O::value(a));
   });
-  row.each([&](int64_t at, u32x4_t v, int) {
+  row.each([&](int at, u32x4_t v, int) {
     unsigned best = 0;
     u32x4_t a;
 #pragma unroll
@@ -893,7 +933,7 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const E* logits, in
     const E* from = logits + n * ld;
     const u64* list = k <= kMostByMaxima ? list_first<E, LSE>(RowPieces<E, NT>(from, cols), k, &sh) : nullptr;
     if (list != nullptr) {
-      if (LSE && threadIdx.x == NT - 1) {
+      if (LSE && thread() == NT - 1) {
         double sums = 0.0;
 #pragma unroll
         for (int w = 0; w < NT / 64; ++w) sums += sh.sums[w];
@@ -908,15 +948,15 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const E* logits, in
 }
 
 // The token of a row whose first k are listed, k of them kept by top_k (1: the first column).
-template <int NT, class Shared> LCE_DEV int64_t sample_listed(const RowSettings& s, int k, const u64* list, Shared* sh) {
+template <int NT, class Shared> LCE_DEV int sample_listed(const RowSettings& s, int k, const u64* list, Shared* sh) {
   if (s.greedy()) {
-    const int64_t column = column_in(list[0]);
+    const int column = column_in(list[0]);
     __syncthreads();
     return column;
   }
   static_assert(kMostByMaxima <= NT, "an entry to a thread");
   const Weights weights = s.weights(value_of(key_in(list[0])));
-  const int t = threadIdx.x;
+  const int t = thread();
   const double real = t < k ? weights.real(value_of(key_in(list[t]))) : 0.0;
   const u64 w = weights.fixed(real);
   u64 before;
@@ -931,7 +971,7 @@ template <int NT, class Shared> LCE_DEV int64_t sample_listed(const RowSettings&
   if (w != 0 && before <= target && target - before < w) sh->drawn = t;  // (one thread)
   __syncthreads();
   const int at = sh->drawn;
-  const int64_t column = column_in(list[at]);
+  const int column = column_in(list[at]);
   __syncthreads();
   return column;
 }
@@ -945,12 +985,12 @@ __global__ __launch_bounds__(kTopThreads, 8) void sample_top_kernel(const E* log
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
-    const int64_t k = s.greedy() ? 1 : s.top_k < cols ? s.top_k : cols;
-    const u64* list = list_first<E, false>(RowPieces<E, NT>(from, cols), (int)k, &sh);
-    int64_t column;
-    if (list != nullptr) column = sample_listed<NT>(s, (int)k, list, &sh);
-    else column = sample_by_digits(RowUnits<E, NT>(from, cols), s, &sh.digits);
-    if (threadIdx.x == 0) token[n] = column;
+    const int k = s.greedy() ? 1 : s.top_k < cols ? s.top_k : (int)cols;
+    const u64* list = list_first<E, false>(RowPieces<E, NT>(from, cols), k, &sh);
+    int column;
+    if (list != nullptr) column = sample_listed<NT>(s, k, list, &sh);
+    else column = sample_by_digits(RowUnits<E, NT, 2>(from, cols), s, &sh.digits);  // (64 registers: no more in flight)
+    if (thread() == 0) token[n] = column;
     __syncthreads();
   }
 }
@@ -977,7 +1017,7 @@ struct BinShared {
   u64 of_wave[kMostWaves];
   ColumnShared columns;
   Place place;
-  int64_t column;
+  int column;
   int bin, listed;
 };
 template <class E, int NT> struct RowBins {
@@ -994,8 +1034,8 @@ template <class E, int NT> struct RowBins {
   }
   // f(element) for all elements.
   template <class F> LCE_DEV void elements(F f) const {
-    row.edges([&](int64_t at, unsigned) { f(at, as_float(row.p[at])); });
-    row.each([&](int64_t at, u32x4_t v, int) {
+    row.edges([&](int at, unsigned) { f(at, as_float(row.p[at])); });
+    row.each([&](int at, u32x4_t v, int) {
       E e[kPer];
       __builtin_memcpy(e, &v, 16);
 #pragma unroll
@@ -1004,13 +1044,13 @@ template <class E, int NT> struct RowBins {
   }
   // The histogram; the weight that min_p keeps.
   LCE_DEV u64 fill(double min_p) const {
-    for (int i = threadIdx.x; i < kBins; i += NT) {
+    for (int i = thread(); i < kBins; i += NT) {
       sh->count[i] = 0;
       sh->weight[i] = 0;
     }
     __syncthreads();
     u64 mine = 0;
-    elements([&](int64_t, float z) {
+    elements([&](int, float z) {
       const double t = weights.log2_of(z), real = exp2_series(t);
       const u64 w = weights.fixed(real);
       if (w == 0) return;
@@ -1023,18 +1063,19 @@ template <class E, int NT> struct RowBins {
   }
   // The sums of this thread's bins.
   LCE_DEV void own(int* c, u64* w) const {
+    const int first = thread() * kOwn;
     *c = 0;
     *w = 0;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      *c += sh->count[threadIdx.x * kOwn + i];
-      *w += sh->weight[threadIdx.x * kOwn + i];
+      *c += sh->count[first + i];
+      *w += sh->weight[first + i];
     }
   }
   // The place that is wanted; *column: its column, where it is one element's, else -1.  c, w: the sums of this thread's bins, cb, wb: those
   // before.  False: by digits.
-  LCE_DEV bool find(int64_t cb, u64 wb, int c, u64 w, const Want& want, Place* place, int64_t* column) const {
-    const int t = threadIdx.x;
+  LCE_DEV bool find(int cb, u64 wb, int c, u64 w, const Want& want, Place* place, int* column) const {
+    const int t = thread();
     if (t == 0) sh->listed = 0;
     if (want.here(cb, wb, c, w)) {
 #pragma unroll 1
@@ -1058,7 +1099,7 @@ template <class E, int NT> struct RowBins {
     const unsigned low_key = key_of((float)low_z), high_key = key_of((float)high_z);
     const unsigned low = b == kBins - 1 || low_key < kLowKey + 4 ? kLowKey + 1 : low_key - 2, high = high_key < top - 2 ? high_key + 2 : top;
     unsigned most = 0, inverse = 0;  // the largest key of the bin, of the inverted keys
-    elements([&](int64_t at, float z) {
+    elements([&](int at, float z) {
       const unsigned key = key_of(z);
       if (!(key >= low && key <= high)) return;
       const double log2 = weights.log2_of(z);
@@ -1115,13 +1156,13 @@ template <class E, int NT> struct RowBins {
 template <class E, int NT>
 LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s, BinShared* sh) {
   const RowUnits<E, NT> units(from, cols);
-  const unsigned top = largest_key(units, reinterpret_cast<unsigned*>(sh->of_wave));
+  const RowPieces<E, NT> row(from, cols);
+  const unsigned top = row.largest(reinterpret_cast<unsigned*>(sh->of_wave));
   if (top == kNanKey || top == kLowKey) return -1;  // a NaN, or no column left
   const float inf = __builtin_inff();
   if (s.greedy()) return column_of(units, value_of(top), 0, &sh->columns);
   if (value_of(top) < inf) {
     const Weights weights = s.weights(value_of(top));
-    const RowPieces<E, NT> row(from, cols);
     const RowBins<E, NT> bins = {row, weights, top, sh};
     const u64 by_min = bins.fill(s.min_p > 0.f ? (double)s.min_p : 0.0);
     int c, cb;
@@ -1129,14 +1170,14 @@ LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s
     bins.own(&c, &w);
     const int counted = block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave), &cb);
     const u64 all = block_all<Sum, NT>(w, sh->of_wave, &wb);
-    if (threadIdx.x == 0) {
+    if (thread() == 0) {
       sh->place = {top, 0, 0, 0};
       sh->bin = 0;
       sh->column = 0;
     }
     __syncthreads();
     bool fine = true;
-    int64_t which = 0, column = -1;
+    int which = 0, column = -1;
     const Place at = draw_place(s, counted, all, by_min, Place{top, 0, 0, 0}, &which,
                                 [&](const Want& want) {
                                   Place p = {top, 0, 0, 0};
@@ -1161,13 +1202,13 @@ __global__ __launch_bounds__(NT, 4) void sample_bins_kernel(const E* logits, int
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
     const RowSettings s(settings, u, n, bits);
-    const int64_t k = s.greedy() ? 1 : s.top_k;
+    const int k = s.greedy() ? 1 : s.top_k;
     const u64* list = nullptr;
-    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(RowPieces<E, NT>(from, cols), (int)k, &sh.top);
-    int64_t column;
-    if (list != nullptr) column = sample_listed<NT>(s, (int)k, list, &sh.top);
+    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(RowPieces<E, NT>(from, cols), k, &sh.top);
+    int column;
+    if (list != nullptr) column = sample_listed<NT>(s, k, list, &sh.top);
     else column = sample_by_bins<E, NT>(from, cols, s, &sh.bins);
-    if (threadIdx.x == 0) token[n] = column;
+    if (thread() == 0) token[n] = column;
     __syncthreads();
   }
 }
@@ -1209,7 +1250,7 @@ template <class E> struct HalfRow {
   // many values it has.
   LCE_DEV bool fill(const RowPieces<E, kSelectThreads>& row, int* different) const {
     constexpr int kWordRounds = kHalfWords / 4 / kSelectThreads;
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     u32x4_t* words = reinterpret_cast<u32x4_t*>(sh->hist);
 #pragma unroll
     for (int i = 0; i < kWordRounds; ++i) words[i * kSelectThreads + t] = u32x4_t{};
@@ -1222,8 +1263,8 @@ template <class E> struct HalfRow {
       else if (m >= kMax && (bits & 0x8000u)) ++masked;
       else atomicAdd(&sh->hist[m], bits & 0x8000u ? 0x10000u : 1u);
     };
-    row.edges([&](int64_t at, unsigned) { one(reinterpret_cast<const unsigned short*>(row.p)[at]); });
-    row.each([&](int64_t, u32x4_t w, int) {
+    row.edges([&](int at, unsigned) { one(reinterpret_cast<const unsigned short*>(row.p)[at]); });
+    row.each([&](int, u32x4_t w, int) {
       typedef unsigned short pair_t __attribute__((ext_vector_type(2)));
       pair_t most = {};
 #pragma unroll
@@ -1290,7 +1331,7 @@ template <class E> struct HalfRow {
     const u64 counted = both & 0x7fffffffu;
     int before;
     *different = block_all<Sum, kSelectThreads>(t < 2 * kWordRows ? sh->row_values[t] : 0, reinterpret_cast<int*>(sh->of_wave), &before);
-    if (any_nan || counted == 0 || *different > kHalfWords || (int64_t)(counted + (both >> 31)) != row.n) return false;
+    if (any_nan || counted == 0 || *different > kHalfWords || (int)(counted + (both >> 31)) != row.n) return false;
     if (t < 2 * kWordRows) sh->row_first[t] = before;
     __syncthreads();
     const u64 above = ~(u64)0 << lane << 1, below = ~(~(u64)0 << lane);
@@ -1319,14 +1360,14 @@ template <class E> struct HalfRow {
 
   // f(bits, count) for the values of this thread's stretch of the list.
   template <class F> LCE_DEV void stretch(int different, F f) const {
-    const int per = (different + kSelectThreads - 1) / kSelectThreads, first = (int)threadIdx.x * per;
+    const int per = (different + kSelectThreads - 1) / kSelectThreads, first = (int)thread() * per;
     const int end = first + per < different ? first + per : different;
 #pragma unroll 1
     for (int i = first; i < end; ++i) f(sh->values[i] & 0xffffu, (int)(sh->values[i] >> 16));
   }
 
   // The place that is wanted.  cb, wb: elements and weight before this thread's stretch; c, w: its own.
-  LCE_DEV Place find(const Weights& weights, int different, int64_t cb, u64 wb, int64_t c, u64 w, const Want& want) const {
+  LCE_DEV Place find(const Weights& weights, int different, int cb, u64 wb, int c, u64 w, const Want& want) const {
     __syncthreads();
     if (want.here(cb, wb, c, w)) {
       bool found = false;
@@ -1357,13 +1398,13 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
     const RowSettings s(settings, u, n, bits);
     const RowPieces<E, kSelectThreads> row(from, cols);
     const HalfRow<E> half = {sh};
-    const int64_t k = s.greedy() ? 1 : s.top_k;
+    const int k = s.greedy() ? 1 : s.top_k;
     const u64* list = nullptr;
-    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(row, (int)k, &sh->top);
-    int64_t column;
+    if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(row, k, &sh->top);
+    int column;
     int different;
     if (list != nullptr) {
-      column = sample_listed<kSelectThreads>(s, (int)k, list, &sh->top);
+      column = sample_listed<kSelectThreads>(s, k, list, &sh->top);
     } else if (!s.greedy() && half.fill(row, &different)) {
       const unsigned top = sh->values[0] & 0xffffu;
       const Weights weights = s.weights(half_value<E>(top));
@@ -1382,7 +1423,7 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
       const int weighed = block_all<Sum, kSelectThreads>(elements, reinterpret_cast<int*>(sh->of_wave), &cb);
       const u64 all = block_all<Sum, kSelectThreads>(weight, sh->of_wave, &wb);
       by_min = s.min_p > 0.f ? block_all<Sum, kSelectThreads>(by_min, sh->of_wave) : all;
-      int64_t which = 0;
+      int which = 0;
       const Place at = draw_place(s, weighed, all, by_min, Place{top, 0, 0, 0}, &which,
                                   [&](const Want& want) { return half.find(weights, different, cb, wb, elements, weight, want); },
                                   [&](const Place& p) { return weights.of(half_value<E>(p.key)); });
@@ -1392,7 +1433,7 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
       __syncthreads();
       column = sample_by_digits(RowUnits<E, kSelectThreads>(from, cols), s, &sh->top.digits);
     }
-    if (threadIdx.x == 0) token[n] = column;
+    if (thread() == 0) token[n] = column;
     __syncthreads();
   }
 }
