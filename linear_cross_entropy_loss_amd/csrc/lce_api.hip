@@ -1565,7 +1565,7 @@ int lce_distill_workspace_bytes(const lce_problem* p, int64_t K, int32_t grads, 
   int rc = check(p, grads != 0);
   if (rc == LCE_OK) rc = check_targets(p->N, K);
   if (rc != LCE_OK) return rc;
-  if (!bytes || p->monitoring || p->z_reg != 0.f || p->phases) return LCE_EINVAL_ARG;
+  if (!bytes || p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale <= 3.4e38f)) return LCE_EINVAL_ARG;
   const lce_problem q = soft_problem(p);
   DistillPlan d;
   rc = plan_distill(&q, K, grads != 0, &d);
@@ -1582,7 +1582,7 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
   if (rc != LCE_OK) return rc;
   if (!x || !w || !y || !index || !q || !lse || !loss || !n_valid || (grads && !grad_out)) return LCE_EINVAL_ARG;
   if (misaligned(x) || misaligned(w) || misaligned(dx) || misaligned(dw)) return LCE_EINVAL_ARG;
-  if (p->monitoring || p->z_reg != 0.f || p->phases) return LCE_EINVAL_ARG;
+  if (p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale <= 3.4e38f)) return LCE_EINVAL_ARG;
   const lce_problem soft_p = soft_problem(p);
   DistillPlan d;
   rc = plan_distill(&soft_p, K, grads, &d);

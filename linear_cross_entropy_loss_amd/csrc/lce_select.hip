@@ -102,21 +102,17 @@ template <class E, int NT, int FLIGHT = 4> struct RowUnits {
   }
   // f(which, element) for the elements of a unit.
   template <class F> LCE_DEV static void elements(u32x4_t v, int c, F f) {
+    constexpr int kHalves = 4 / sizeof(E);
 #pragma unroll 1
-    for (int i = 0; i < c; ++i) {
-      if constexpr (sizeof(E) == 2) {
-        const unsigned w = v[0];
+    for (int i = 0; i < c; i += kHalves) {
+      const unsigned w = v[0];
+      if constexpr (kHalves == 2) {
         f(i, as_float(__builtin_bit_cast(E, (unsigned short)w)));
-        v[0] = i & 1 ? v[1] : w >> 16;
-        if (i & 1) {
-          v[1] = v[2];
-          v[2] = v[3];
-        }
+        if (i + 1 < c) f(i + 1, as_float(__builtin_bit_cast(E, (unsigned short)(w >> 16))));
       } else {
-        const unsigned w = v[0];
         f(i, __builtin_bit_cast(float, w));
-        v = u32x4_t{v[1], v[2], v[3], 0};
       }
+      v = u32x4_t{v[1], v[2], v[3], 0};
     }
   }
   // f(element) for the elements of this lane's units.

@@ -382,3 +382,77 @@ def test_sorted_and_unsorted_entries(w_vh):
         index[:, 1:][index[:, 1:] == 17] = 18
         w[:, ::3] *= 2.0 ** -12  # subnormal numbers of the type among them
         check((x, w, index, logits), tied=w_vh and H % 8 == 0, up=512.0)
+
+
+@pytest.mark.pack_auto
+def test_refusals():
+    from linear_cross_entropy_loss_amd import LinearCrossEntropyLoss, linear_distillation
+
+    x, w, index, logits = (t.cuda() for t in make(6, 16, 40, 5, BF16, seed=40))
+    for bad in ((x, w[:8], index, logits), (x, w[0], index, logits), (x, w, index[:5], logits[:5]), (x, w, index, logits[:, :4]),
+                (x, w, index.int(), logits), (x, w, index, logits.double()), (x, w, index, logits.long()), (x, w, index[:, :0], logits[:, :0]),
+                (x, w.half(), index, logits), (x.double(), w.double(), index, logits), (x[:0], w, index[:0], logits[:0]),
+                (x, w, index.repeat(1, 205)[:, :1025], logits.repeat(1, 205)[:, :1025])):
+        with pytest.raises(ValueError):
+            linear_distillation(*bad)
+    for bad in ((x.cpu(), w, index, logits), (x, w.cpu(), index, logits), (x, w, index.cpu(), logits), (x, w, index, logits.cpu())):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            linear_distillation(*bad)
+    for numbers in ({"temperature": 0.0}, {"temperature": -1.0}, {"temperature": math.inf}, {"temperature": math.nan}, {"temperature": 1e-60},
+                    {"logit_scale": 0.0}, {"logit_scale": math.inf}, {"logit_scale": math.nan}, {"logit_scale": 1e30, "temperature": 1e-30},
+                    {"N_chunk_size": 0}, {"N_chunk_size": -4}):
+        with pytest.raises(ValueError):
+            linear_distillation(x, w, index, logits, **numbers)
+    module = LinearCrossEntropyLoss(16, 40, device="cuda", dtype=BF16)
+    with pytest.raises(ValueError):
+        module.distill(x, index.int(), logits)
+
+
+def test_two_streams_at_once():
+    from linear_cross_entropy_loss_amd import linear_distillation
+
+    sets = [[t.cuda() for t in make(700, 256, 5000, 24, BF16, seed=41 + i, empty=0.2, twice=True)] for i in range(2)]
+
+    def call(x, w, index, logits):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = linear_distillation(x, w, index, logits, 1.5)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    ref = [call(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = call(*sets[i])
+    torch.cuda.synchronize()
+    for a, b in zip(ref, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.pack_auto
+def test_opcheck():
+    from linear_cross_entropy_loss_amd import ops  # noqa: F401 (registers the operators)
+    from linear_cross_entropy_loss_amd import distillation  # noqa: F401
+
+    x, w, index, logits = (t.cuda() for t in make(10, 32, 100, 5, BF16, seed=43))
+    for needs in ((True, True), (False, True), (True, False), (False, False)):
+        torch.library.opcheck(torch.ops.lce_amd.distill.default, (x, w, index, logits, 1.5, 0.7, 4096, *needs),
+                              test_utils=("test_schema", "test_faketensor"))
+
+
+def test_beside_the_loss_on_labels():
+    """Both losses on the same hidden states and weight, weighed and added, as a step would: the gradients add up."""
+    from linear_cross_entropy_loss_amd import linear_cross_entropy, linear_distillation
+
+    x, w, index, logits = (t.cuda() for t in make(200, 128, 1500, 10, BF16, seed=44, empty=0.3))
+    y = torch.randint(0, 1500, (200,), device="cuda")
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    T = 2.0
+    labels, teacher = lambda: 0.3 * linear_cross_entropy(x, y, w)[0], lambda: T * T * linear_distillation(x, w, index, logits, T)
+    parts = [torch.autograd.grad(loss(), (x, w)) for loss in (labels, teacher)]
+    both = torch.autograd.grad(labels() + teacher(), (x, w))
+    for got, a, b in zip(both, *parts):
+        assert torch.equal(got, a + b)

@@ -343,3 +343,118 @@ def test_distillation_on_policy():
     p = torch.log_softmax(x[kept].double() @ student.weight.detach().cpu().double() / 1.5, -1)
     ref = (torch.special.xlogy(q, q) - q * p.gather(-1, index[kept])).sum(-1).mean()
     assert abs(first[0].item() - ref.item()) <= 64 * 2.0 ** -22 * max(1.0, ref.item())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("N,V", [(3001, 1009), (1100, 20011), (600, 33003)])
+def test_more_rows_than_workgroups(N, V, dtype):
+    """A workgroup takes rows one after another, and neighbours are done in different ways: ordinary, all equal, masked, with a NaN, with
+    infinities, one column alone."""
+    z = rows(N, V, dtype, seed=16)
+    kind = torch.randint(0, 8, (N,), generator=torch.Generator().manual_seed(17))
+    z[kind == 0] = 1.5
+    z[kind == 1] = -math.inf
+    z[kind == 2, V // 2] = math.nan
+    z[kind == 3, V // 3] = math.inf
+    z[kind == 4, 5:] = -math.inf
+    u = torch.rand(N, generator=torch.Generator().manual_seed(18))
+    check_top(z, 20)
+    check_sample(z, u)
+    check_sample(z, u, top_p=0.7)
+    check_sample(z, u, temperature=0.9, top_k=33)
+    g = torch.Generator().manual_seed(19)
+    check_sample(z, u, temperature=torch.rand(N, generator=g), top_k=torch.randint(-1, 60, (N,), generator=g),
+                 top_p=torch.rand(N, generator=g) * 1.2, min_p=torch.rand(N, generator=g) * 0.1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_long_lists(dtype):
+    """More than the way by maxima takes, and rows of fewer columns than threads."""
+    for N, V in ((5, 5003), (3, 40000)):
+        z, u = rows(N, V, dtype, seed=20), torch.rand(N, generator=torch.Generator().manual_seed(21))
+        for k in (511, 512, 513, 1000, 1024):
+            check_top(z, k)
+            check_sample(z, u, top_k=k, temperature=3.0)
+        check_sample(z, u, top_k=3000, temperature=5.0, top_p=0.9, min_p=0.01)
+    z, u = rows(4, 700, dtype, seed=22), torch.rand(4, generator=torch.Generator().manual_seed(23))
+    for k in (300, 512, 699, 700):
+        check_top(z, k)
+        check_sample(z, u, top_k=k)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("V", [1000, 9000, 40000])
+def test_temperatures(V, dtype):
+    """From the largest column alone to the same weight for all; at 1e-3 of V = 40000 values between 2 and 8 more than one column counts."""
+    z = rows(6, V, dtype, seed=24)
+    u = torch.rand(6, generator=torch.Generator().manual_seed(25))
+    for t in (1e-38, 1e-6, 1e-3, 0.1, 30.0, 1e6, 1e30, 3e38):
+        check_sample(z, u, temperature=t)
+        check_sample(z, u, temperature=t, top_p=0.37)
+        check_sample(z, u, temperature=t, min_p=0.8, top_k=V // 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_values_close_together(dtype):
+    """Thousands of different values within a few bins of the weight, and as many equal ones beside them."""
+    V = 15000
+    g = torch.Generator().manual_seed(26)
+    near = (1.0 + torch.rand(4, V, generator=g) / 300).to(dtype)
+    near[1, ::2] = 1.0
+    near[2, :100] += 3
+    near[3, 5000:] -= 40
+    u = torch.rand(4, generator=g)
+    for settings in ({}, {"top_p": 0.5}, {"top_k": 4000}, {"min_p": 0.999}, {"temperature": 0.001, "top_p": 0.6}):
+        check_sample(near, u, **settings)
+    check_top(near, 100)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_row_of_millions(dtype):
+    V = (1 << 22) + 5
+    z, u = rows(1, V, dtype, seed=27), torch.tensor([0.8125])
+    check_top(z, 1024)
+    check_top(z, 10)
+    check_sample(z, u, top_p=0.9)
+    check_sample(z, u, top_k=50)
+
+
+def test_two_streams_and_two_threads_at_once():
+    import threading
+
+    from linear_cross_entropy_loss_amd import sample_logits, top_logits
+
+    sets = [(rows(300, 33000, BF16, seed=28 + i).cuda(), torch.rand(300, device="cuda")) for i in range(2)]
+    sets.append((rows(300, 9000, F32, seed=30).cuda(), torch.rand(300, device="cuda")))
+    call = lambda z, u: (sample_logits(z, u, 0.9, 0, 0.9), sample_logits(z, u, top_k=40), *top_logits(z, 30))
+    ref = [call(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = [None] * len(sets)
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                got[i] = call(*sets[i])
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sets))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(ref, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_no_gradient_and_opcheck():
+    from linear_cross_entropy_loss_amd import sample_logits, top_logits
+
+    z, u = rows(4, 300, BF16, seed=31).cuda().requires_grad_(True), torch.rand(4, device="cuda")
+    values, _, lse = top_logits(z, 5)
+    assert not values.requires_grad and not lse.requires_grad and not sample_logits(z, u).requires_grad
+    z = z.detach()
+    torch.library.opcheck(torch.ops.lce_amd.top_logits.default, (z, 5), test_utils=("test_schema", "test_faketensor"))
+    one = torch.ones((), device="cuda")
+    torch.library.opcheck(torch.ops.lce_amd.sample_logits.default, (z, u, one, torch.zeros((), dtype=torch.int64, device="cuda"), one, 0 * one),
+                          test_utils=("test_schema", "test_faketensor"))
