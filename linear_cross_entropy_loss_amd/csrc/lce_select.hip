@@ -174,7 +174,104 @@ template <class J, int NT, class F> LCE_DEV F block_all(F v, F* sh, F* before = 
   return read_lane(waves, 15);
 }
 
-// Which elements of 16 bytes equal a value, as bits 0 .. 7 (or 3).  0 and -0 are equal; the value is no NaN.
+// 16 bytes of a row as unsigned numbers in the order of the values (-0 just below 0), two of 16 bits or one of 32 bits to a word.
+template <class E> struct Ordered;
+template <> struct Ordered<float> {
+  static constexpr unsigned kLow = 0x007fffffu, kInf = 0xff800000u;
+  LCE_DEV static unsigned word(unsigned w) { return w ^ ((unsigned)((int)w >> 31) | 0x80000000u); }
+  LCE_DEV static unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
+  LCE_DEV static unsigned smaller(unsigned a, unsigned b) { return a < b ? a : b; }
+  LCE_DEV static unsigned largest(unsigned a) { return a; }
+  LCE_DEV static unsigned smallest(unsigned a) { return a; }
+  LCE_DEV static unsigned in_top_bits(unsigned a) { return a >> 16; }
+  LCE_DEV static unsigned from_top_bits(unsigned a) { return a << 16; }
+  LCE_DEV static float value(unsigned a) { return value_of(a); }
+};
+template <class E> struct OrderedHalf {
+  typedef short signed_t __attribute__((ext_vector_type(2)));
+  typedef unsigned short pair_t __attribute__((ext_vector_type(2)));
+  LCE_DEV static unsigned word(unsigned w) {
+    return w ^ (__builtin_bit_cast(unsigned, __builtin_bit_cast(signed_t, w) >> (short)15) | 0x80008000u);
+  }
+  LCE_DEV static unsigned larger(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(pair_t, a), __builtin_bit_cast(pair_t, b)));
+  }
+  LCE_DEV static unsigned smaller(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(pair_t, a), __builtin_bit_cast(pair_t, b)));
+  }
+  LCE_DEV static unsigned largest(unsigned a) { return a >> 16 > (a & 0xffffu) ? a >> 16 : a & 0xffffu; }
+  LCE_DEV static unsigned smallest(unsigned a) { return a >> 16 < (a & 0xffffu) ? a >> 16 : a & 0xffffu; }
+  LCE_DEV static unsigned in_top_bits(unsigned a) { return a; }
+  LCE_DEV static unsigned from_top_bits(unsigned a) { return a; }
+  LCE_DEV static float value(unsigned a) {
+    return (float)__builtin_bit_cast(E, (unsigned short)(a & 0x8000u ? a & 0x7fffu : a ^ 0xffffu));
+  }
+};
+template <> struct Ordered<__bf16> : OrderedHalf<__bf16> { static constexpr unsigned kLow = 0x007f, kInf = 0xff80; };
+template <> struct Ordered<_Float16> : OrderedHalf<_Float16> { static constexpr unsigned kLow = 0x03ff, kInf = 0xfc00; };
+
+// Whole pieces of a row, dealt to the threads one by one, and the elements before and behind them.
+template <class E, int NT> struct RowPieces {
+  typedef Ordered<E> O;
+  typedef typename bits_of<sizeof(E)>::type Bits;
+  static constexpr int kPer = 16 / sizeof(E), kFlight = 4, kThreads = NT;
+  const E* p;
+  int n, head, body;
+  LCE_DEV RowPieces(const E* row, int64_t cols) : p(row), n((int)cols) {
+    const int off = (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E));
+    head = off < n ? off : n;
+    body = (n - head) / kPer;
+  }
+  // f(column, ordered bits) for the elements at the edges, one to a thread.
+  template <class F> LCE_DEV void edges(F f) const {
+    const int tail = n - head - body * kPer, t = thread();
+    if (t < head + tail) {
+      const int at = t < head ? t : n - tail + (t - head);
+      const unsigned w = O::word(reinterpret_cast<const Bits*>(p)[at]);
+      f(at, sizeof(E) == 2 ? w & 0xffffu : w);
+    }
+  }
+  // f(column of the first, piece, which of its round), kFlight pieces in flight.
+  template <class F> LCE_DEV void each(F f) const {
+    const u32x4_t* from = reinterpret_cast<const u32x4_t*>(p + head);
+#pragma unroll 1
+    for (int base = thread(); base < body; base += kFlight * NT) {
+      u32x4_t v[kFlight];
+#pragma unroll
+      for (int r = 0; r < kFlight; ++r) {
+        const int at = base + r * NT;
+        v[r] = from[at < body ? at : base];
+      }
+#pragma unroll
+      for (int r = 0; r < kFlight; ++r) {
+        const int at = base + r * NT;
+        if (at < body) f(head + at * kPer, v[r], r);
+      }
+    }
+  }
+  // The largest key.
+  LCE_DEV unsigned largest(unsigned* sh) const {
+    unsigned most = 0, least = ~0u;
+    edges([&](int, unsigned a) {
+      most = O::larger(most, a);  // (of 16 bits: the upper half stays as it is)
+      least = O::smaller(least, sizeof(E) == 2 ? a | 0xffff0000u : a);
+    });
+    each([&](int, u32x4_t v, int) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned a = O::word(v[i]);
+        most = O::larger(most, a);
+        least = O::smaller(least, a);
+      }
+    });
+    most = O::largest(most);
+    if (O::smallest(least) < O::kLow) most = ~0u;  // (a NaN is above +inf or below -inf)
+    most = block_all<Largest, NT>(most, sh);
+    return most > O::kInf ? kNanKey : key_of(O::value(most));
+  }
+};
+
+// The elements of 16 bytes that equal a value: how many, and which.  0 and -0 are equal; the value is no NaN.
 template <class E> struct Equal {  // 16-bit elements
   unsigned twice, mask;
   LCE_DEV explicit Equal(float value) {
@@ -182,15 +279,15 @@ template <class E> struct Equal {  // 16-bit elements
     mask = (bits & 0x7fffu) == 0 ? 0x7fff7fffu : 0xffffffffu;
     twice = (bits | bits << 16) & mask;
   }
-  // (one half equal, or the lower one is and the upper one is off by one)
-  LCE_DEV bool maybe(u32x4_t v) const {
-    unsigned any = 0;
+  LCE_DEV int count(u32x4_t v) const {
+    typedef unsigned short pair_t __attribute__((ext_vector_type(2)));
+    pair_t others = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const unsigned x = (v[i] & mask) ^ twice;
-      any |= (x - 0x00010001u) & ~x;
+      others += __builtin_elementwise_min(__builtin_bit_cast(pair_t, x), pair_t{1, 1});
     }
-    return (any & 0x80008000u) != 0;
+    return 8 - (others[0] + others[1]);
   }
   LCE_DEV bool is(u32x4_t v, int k) const {
     const unsigned x = (v[k >> 1] & mask) ^ twice;
@@ -204,82 +301,106 @@ template <> struct Equal<float> {
     const unsigned w = v[k];
     return __builtin_bit_cast(float, w) == value;
   }
-  LCE_DEV bool maybe(u32x4_t v) const { return is(v, 0) || is(v, 1) || is(v, 2) || is(v, 3); }
+  LCE_DEV int count(u32x4_t v) const { return is(v, 0) + is(v, 1) + is(v, 2) + is(v, 3); }
 };
 
-// The column of the r-th (from 0) element with a value; -1 if there are no more than r.  All threads take part and get it.  The waves
-// count such elements, by parts of their share of the row, and the one that has the r-th looks for it in its part.
-// kPartRounds rounds are in flight together.
+// The column of the r-th (from 0) element with a value, which is no NaN; -1 if there are no more than r.  All threads take part and get it.
+// The waves count such elements, by parts of their share of the row's pieces, and the one that has the r-th looks for it in its part.
+// kPartRounds loads of 1 KiB a wave are in flight together.
 constexpr int kParts = 32;
 struct ColumnShared {
   int count[kMostWaves][kParts];
   int of_wave[kMostWaves];
   int column;
 };
-template <int kPartRounds = 8, class E, int NT, int FL> LCE_DEV int column_of(const RowUnits<E, NT, FL>& row, float value, int r, ColumnShared* sh) {
-  constexpr int kPer = RowUnits<E, NT, FL>::kPer;
+template <int kPartRounds = 8, class E, int NT> LCE_DEV int column_of(const RowPieces<E, NT>& row, float value, int r, ColumnShared* sh) {
+  constexpr int kPer = RowPieces<E, NT>::kPer;
   const Equal<E> equal(value);
   const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int u0 = wave * row.share, left = (row.units - u0 + 63) / 64, share = row.share / 64;
-  const int rounds = left < 0 ? 0 : left < share ? left : share;
+  const int all = (row.body + 63) / 64, share = (all + NT / 64 - 1) / (NT / 64);  // in rounds: 64 pieces
+  const int first = wave * share, left = all - first, rounds = left < 0 ? 0 : left < share ? left : share;
   const int per = (rounds + kParts * kPartRounds - 1) / (kParts * kPartRounds) * kPartRounds;  // rounds of a part
-  // f(unit, its elements) for the units of kPartRounds rounds from i that may have the value.  (Few have it: that loop is not unrolled.)
-  auto look = [&](int i, auto f) {
-    u32x4_t v[kPartRounds];
-    unsigned hits = 0;
+  const u32x4_t* from = reinterpret_cast<const u32x4_t*>(row.p + row.head);
+  const int last = (first + rounds) * 64 < row.body ? (first + rounds) * 64 : row.body;
+  // v, c: the pieces of kPartRounds rounds from i, and how many elements of each have the value
+  u32x4_t v[kPartRounds];
+  int c[kPartRounds];
+  auto look = [&](int i) {
+    const int piece = (first + i) * 64 + lane;
 #pragma unroll
-    for (int q = 0; q < kPartRounds; ++q)
-      if (i + q < rounds) v[q] = row.load(u0 + (i + q) * 64 + lane);
+    for (int q = 0; q < kPartRounds; ++q) {
+      const int at = piece + q * 64;
+      v[q] = from[at < last ? at : last - 1];
+    }
 #pragma unroll
-    for (int q = 0; q < kPartRounds; ++q)
-      if (i + q < rounds && __any(equal.maybe(v[q]))) hits |= 1u << q;
-#pragma unroll 1
-    for (int unit = u0 + i * 64 + lane; hits != 0; hits >>= 1, unit += 64) {
-      if (hits & 1) f(unit, v[0]);
-#pragma unroll
-      for (int q = 0; q + 1 < kPartRounds; ++q) v[q] = v[q + 1];
+    for (int q = 0; q < kPartRounds; ++q) {
+      const int equals = equal.count(v[q]);
+      c[q] = piece + q * 64 < last ? equals : 0;
     }
   };
+  // the elements before and behind the pieces (fewer than 8 each): in every wave
+  const int tail = row.n - row.head - row.body * kPer;
+  const E before_all = row.p[lane < row.head ? lane : 0], behind_all = row.p[row.n - 1 - (lane < tail ? tail - 1 - lane : 0)];
   if (t == 0) sh->column = -1;
   int mine = 0;
 #pragma unroll 1
   for (int i = 0, part = 0; i < rounds; ++part) {
     int count = 0;
 #pragma unroll 1
-    for (const int end = i + per; i < end && i < rounds; i += kPartRounds)
-      look(i, [&](int unit, u32x4_t v) {
-        const int c = row.count(unit);
+    for (const int end = i + per; i < end && i < rounds; i += kPartRounds) {
+      look(i);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) count += __popcll(__ballot(k < c && equal.is(v, k)));
-      });
+      for (int q = 0; q < kPartRounds; ++q) count += c[q];
+    }
+    count = read_lane(wave_upto<Sum>(count), 63);
     if (lane == 0) sh->count[wave][part] = count;
     mine += count;
   }
   if (lane == 0) sh->of_wave[wave] = mine;
+  const u64 in_head = __ballot(lane < row.head && as_float(before_all) == value), in_tail = __ballot(lane < tail && as_float(behind_all) == value);
   __syncthreads();
-  int before = 0;
+  int before = __popcll(in_head), upto = before;
 #pragma unroll
-  for (int w = 0; w < NT / 64; ++w) before += w < wave ? sh->of_wave[w] : 0;
-  if (before <= r && r < before + mine) {  // (one wave)
+  for (int w = 0; w < NT / 64; ++w) {
+    before += w < wave ? sh->of_wave[w] : 0;
+    upto += sh->of_wave[w];
+  }
+  if (before <= r && r < before + mine) {  // (one wave, or none)
     int i = 0;
     for (int part = 0; part < kParts - 1 && before + sh->count[wave][part] <= r; ++part, i += per) before += sh->count[wave][part];
 #pragma unroll 1
-    for (const int end = i + per; i < end && i < rounds; i += kPartRounds)
-      look(i, [&](int unit, u32x4_t v) {
-        const int c = row.count(unit);
-        int here = 0;
+    for (const int end = i + per; i < end && i < rounds; i += kPartRounds) {
+      u32x4_t in = {};
+      int round = -1, here = 0, upto_here = 0, before_round = 0;
+      if (rounds > kPartRounds) look(i);  // (else they are still there)
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) here += k < c && equal.is(v, k) ? 1 : 0;
-        const int upto = wave_upto<Sum>(here);
-        int at = before + upto - here;
+      for (int q = 0; q < kPartRounds; ++q) {
+        if (i + q >= rounds) continue;
+        const int sum = wave_upto<Sum>(c[q]), of_round = read_lane(sum, 63);
+        if (before <= r && r < before + of_round) {  // (one round)
+          round = q;
+          in = v[q];
+          here = c[q];
+          upto_here = sum;
+          before_round = before;
+        }
+        before += of_round;
+      }
+      if (round < 0) continue;
+      int at = before_round + upto_here - here;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k)
-          if (k < c && equal.is(v, k)) {
-            if (at == r) sh->column = row.column(unit) + k;
-            ++at;
-          }
-        before += read_lane(upto, 63);
-      });
+      for (int k = 0; k < kPer; ++k)
+        if (here != 0 && equal.is(in, k)) {
+          if (at == r) sh->column = row.head + ((first + i + round) * 64 + lane) * kPer + k;
+          ++at;
+        }
+      break;
+    }
+  } else if (t < 64 && (r < __popcll(in_head) || r >= upto)) {
+    const bool head = r < __popcll(in_head);
+    const int which = head ? r : r - upto;
+    const u64 in = head ? in_head : in_tail;
+    if ((in >> lane & 1) && __popcll(in & ((u64(1) << lane) - 1)) == which) sh->column = head ? lane : row.n - tail + lane;
   }
   __syncthreads();
   const int at = sh->column;
@@ -558,7 +679,7 @@ LCE_DEV int sample_by_digits(const RowUnits<E, NT, FL>& row, const RowSettings& 
                     [&](const Want& want) { return find_place<true, KEEP>(row, weights, sh, want); },
                     [&](const Place& p) { return weights.of(value_of(p.key)); });
   }
-  return column_of<FL == 4 ? 8 : 2>(row, value_of(at.key), which, &sh->columns);
+  return column_of<FL == 4 ? 8 : 2>(RowPieces<E, NT>(row.p, row.n), value_of(at.key), which, &sh->columns);
 }
 
 constexpr int kMostTop = 1024;
@@ -709,103 +830,6 @@ template <class Digits> struct TopShared {
   double sums[kMostWaves];
   unsigned top;
   int listed, drawn;
-};
-
-// 16 bytes of a row as unsigned numbers in the order of the values (-0 just below 0), two of 16 bits or one of 32 bits to a word.
-template <class E> struct Ordered;
-template <> struct Ordered<float> {
-  static constexpr unsigned kLow = 0x007fffffu, kInf = 0xff800000u;
-  LCE_DEV static unsigned word(unsigned w) { return w ^ ((unsigned)((int)w >> 31) | 0x80000000u); }
-  LCE_DEV static unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
-  LCE_DEV static unsigned smaller(unsigned a, unsigned b) { return a < b ? a : b; }
-  LCE_DEV static unsigned largest(unsigned a) { return a; }
-  LCE_DEV static unsigned smallest(unsigned a) { return a; }
-  LCE_DEV static unsigned in_top_bits(unsigned a) { return a >> 16; }
-  LCE_DEV static unsigned from_top_bits(unsigned a) { return a << 16; }
-  LCE_DEV static float value(unsigned a) { return value_of(a); }
-};
-template <class E> struct OrderedHalf {
-  typedef short signed_t __attribute__((ext_vector_type(2)));
-  typedef unsigned short pair_t __attribute__((ext_vector_type(2)));
-  LCE_DEV static unsigned word(unsigned w) {
-    return w ^ (__builtin_bit_cast(unsigned, __builtin_bit_cast(signed_t, w) >> (short)15) | 0x80008000u);
-  }
-  LCE_DEV static unsigned larger(unsigned a, unsigned b) {
-    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(pair_t, a), __builtin_bit_cast(pair_t, b)));
-  }
-  LCE_DEV static unsigned smaller(unsigned a, unsigned b) {
-    return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(pair_t, a), __builtin_bit_cast(pair_t, b)));
-  }
-  LCE_DEV static unsigned largest(unsigned a) { return a >> 16 > (a & 0xffffu) ? a >> 16 : a & 0xffffu; }
-  LCE_DEV static unsigned smallest(unsigned a) { return a >> 16 < (a & 0xffffu) ? a >> 16 : a & 0xffffu; }
-  LCE_DEV static unsigned in_top_bits(unsigned a) { return a; }
-  LCE_DEV static unsigned from_top_bits(unsigned a) { return a; }
-  LCE_DEV static float value(unsigned a) {
-    return (float)__builtin_bit_cast(E, (unsigned short)(a & 0x8000u ? a & 0x7fffu : a ^ 0xffffu));
-  }
-};
-template <> struct Ordered<__bf16> : OrderedHalf<__bf16> { static constexpr unsigned kLow = 0x007f, kInf = 0xff80; };
-template <> struct Ordered<_Float16> : OrderedHalf<_Float16> { static constexpr unsigned kLow = 0x03ff, kInf = 0xfc00; };
-
-// Whole pieces of a row, dealt to the threads one by one, and the elements before and behind them.
-template <class E, int NT> struct RowPieces {
-  typedef Ordered<E> O;
-  typedef typename bits_of<sizeof(E)>::type Bits;
-  static constexpr int kPer = 16 / sizeof(E), kFlight = 4, kThreads = NT;
-  const E* p;
-  int n, head, body;
-  LCE_DEV RowPieces(const E* row, int64_t cols) : p(row), n((int)cols) {
-    const int off = (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E));
-    head = off < n ? off : n;
-    body = (n - head) / kPer;
-  }
-  // f(column, ordered bits) for the elements at the edges, one to a thread.
-  template <class F> LCE_DEV void edges(F f) const {
-    const int tail = n - head - body * kPer, t = thread();
-    if (t < head + tail) {
-      const int at = t < head ? t : n - tail + (t - head);
-      const unsigned w = O::word(reinterpret_cast<const Bits*>(p)[at]);
-      f(at, sizeof(E) == 2 ? w & 0xffffu : w);
-    }
-  }
-  // f(column of the first, piece, which of its round), kFlight pieces in flight.
-  template <class F> LCE_DEV void each(F f) const {
-    const u32x4_t* from = reinterpret_cast<const u32x4_t*>(p + head);
-#pragma unroll 1
-    for (int base = thread(); base < body; base += kFlight * NT) {
-      u32x4_t v[kFlight];
-#pragma unroll
-      for (int r = 0; r < kFlight; ++r) {
-        const int at = base + r * NT;
-        v[r] = from[at < body ? at : base];
-      }
-#pragma unroll
-      for (int r = 0; r < kFlight; ++r) {
-        const int at = base + r * NT;
-        if (at < body) f(head + at * kPer, v[r], r);
-      }
-    }
-  }
-  // The largest key.
-  LCE_DEV unsigned largest(unsigned* sh) const {
-    unsigned most = 0, least = ~0u;
-    edges([&](int, unsigned a) {
-      most = O::larger(most, a);  // (of 16 bits: the upper half stays as it is)
-      least = O::smaller(least, sizeof(E) == 2 ? a | 0xffff0000u : a);
-    });
-    each([&](int, u32x4_t v, int) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned a = O::word(v[i]);
-        most = O::larger(most, a);
-        least = O::smaller(least, a);
-      }
-    });
-    most = O::largest(most);
-    if (O::smallest(least) < O::kLow) most = ~0u;  // (a NaN is above +inf or below -inf)
-    most = block_all<Largest, NT>(most, sh);
-    return most > O::kInf ? kNanKey : key_of(O::value(most));
-  }
 };
 
 // The sorted list of a row's first elements, k of them and more; null if it could not be made.  sh->top: the ordered bits of the
@@ -1151,12 +1175,11 @@ template <class E, int NT> struct RowBins {
 
 template <class E, int NT>
 LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s, BinShared* sh) {
-  const RowUnits<E, NT> units(from, cols);
   const RowPieces<E, NT> row(from, cols);
   const unsigned top = row.largest(reinterpret_cast<unsigned*>(sh->of_wave));
   if (top == kNanKey || top == kLowKey) return -1;  // a NaN, or no column left
   const float inf = __builtin_inff();
-  if (s.greedy()) return column_of(units, value_of(top), 0, &sh->columns);
+  if (s.greedy()) return column_of(row, value_of(top), 0, &sh->columns);
   if (value_of(top) < inf) {
     const Weights weights = s.weights(value_of(top));
     const RowBins<E, NT> bins = {row, weights, top, sh};
@@ -1181,10 +1204,10 @@ LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s
                                   return p;
                                 },
                                 [&](const Place& p) { return weights.of(value_of(p.key)); });
-    if (fine) return column >= 0 ? column : column_of(units, value_of(at.key), which, &sh->columns);
+    if (fine) return column >= 0 ? column : column_of(row, value_of(at.key), which, &sh->columns);
     __syncthreads();
   }
-  return sample_by_digits(units, s, &sh->digits);
+  return sample_by_digits(RowUnits<E, NT>(from, cols), s, &sh->digits);
 }
 
 // NT = 512: two rows to a compute unit; 1024 for rows that have one each.
@@ -1424,7 +1447,7 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
                                   [&](const Want& want) { return half.find(weights, different, cb, wb, elements, weight, want); },
                                   [&](const Place& p) { return weights.of(half_value<E>(p.key)); });
       __syncthreads();  // (the list of values is not read any more)
-      column = column_of(RowUnits<E, kSelectThreads>(from, cols), half_value<E>(at.key), which, &sh->columns);
+      column = column_of(row, half_value<E>(at.key), which, &sh->columns);
     } else {
       __syncthreads();
       column = sample_by_digits(RowUnits<E, kSelectThreads>(from, cols), s, &sh->top.digits);
