@@ -408,22 +408,23 @@ template <int kPartRounds = 8, class E, int NT> LCE_DEV int column_of(const RowP
   return at;
 }
 
-// 2^t for t <= 0: 2^(t - rint t) by its Taylor series in the 64-bit unit, whose first term left out is below 7e-15, times a power of two.
-LCE_DEV double exp2_series(double t) {
-  const double n = rint(t), x = (t - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, x, 1.0 / 3628800.0);
-  p = fma(p, x, 1.0 / 362880.0);
-  p = fma(p, x, 1.0 / 40320.0);
-  p = fma(p, x, 1.0 / 5040.0);
-  p = fma(p, x, 1.0 / 720.0);
-  p = fma(p, x, 1.0 / 120.0);
-  p = fma(p, x, 1.0 / 24.0);
-  p = fma(p, x, 1.0 / 6.0);
-  p = fma(p, x, 0.5);
+// 2^t for -2000 <= t <= 0: 2^(t - rint t) by the polynomial of degree 10 whose largest relative error over half a unit to either side is
+// smallest (2.1e-16; 2^0 is 1), times a power of two.
+LCE_DEV double exp2_poly(double t) {
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: the sum's last place is 1
+  const double m = t + kWhole, x = t - (m - kWhole);
+  double p = 7.037278846726901e-09;
+  p = fma(p, x, 1.0208537929657404e-07);
+  p = fma(p, x, 1.3215662835959238e-06);
+  p = fma(p, x, 1.5252658116409854e-05);
+  p = fma(p, x, 0.00015403529961127076);
+  p = fma(p, x, 0.0013333558228561767);
+  p = fma(p, x, 0.009618129108034596);
+  p = fma(p, x, 0.05550410866445883);
+  p = fma(p, x, 0.24022650695908768);
+  p = fma(p, x, 0.6931471805599497);
   p = fma(p, x, 1.0);
-  p = fma(p, x, 1.0);
-  return ldexp(p, (int)n);
+  return ldexp(p, (int)(unsigned)__builtin_bit_cast(u64, m));
 }
 
 // Weights of a row as fixed-point numbers.
@@ -435,7 +436,9 @@ struct Weights {
     const double zd = (double)z;
     return zd == top ? 0.0 : fmax((zd - top) * per, -2000.0);
   }
-  LCE_DEV double real(float z) const { return exp2_series(log2_of(z)); }
+  // (of a finite top)
+  LCE_DEV double log2_below(float z) const { return fmax(((double)z - top) * per, -2000.0); }
+  LCE_DEV double real(float z) const { return exp2_poly(log2_of(z)); }
   // (rounded by the sum with 2^52, whose last place is 1)
   LCE_DEV u64 fixed(double w) const { return __builtin_bit_cast(u64, fma(w, one, 4503599627370496.0)) & 0xfffffffffffffull; }
   LCE_DEV u64 of(float z) const { return fixed(real(z)); }
@@ -530,8 +533,8 @@ struct Want {
   u64 target;
   // whether it is among c elements of weight w behind cb elements of weight wb
   LCE_DEV bool here(int cb, u64 wb, int c, u64 w) const {
-    if (c == 0) return false;
     if (what == kByCount) return cb < k && k <= cb + c;
+    if (w == 0) return false;
     if (what == kByShare) return (wb == 0 || (double)wb < most) && !((double)(wb + w) < most);
     return wb <= target && target - wb < w;
   }
@@ -1052,34 +1055,32 @@ template <class E, int NT> struct RowBins {
     const int b = (int)(log2_weight * -kBinsPerOctave);
     return b < kBins - 1 ? b : kBins - 1;
   }
-  // f(element) for all elements.
-  template <class F> LCE_DEV void elements(F f) const {
-    row.edges([&](int at, unsigned) { f(at, as_float(row.p[at])); });
-    row.each([&](int at, u32x4_t v, int) {
-      E e[kPer];
-      __builtin_memcpy(e, &v, 16);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) f(at + i, as_float(e[i]));
-    });
-  }
-  // The histogram; the weight that min_p keeps.
-  LCE_DEV u64 fill(double min_p) const {
+  // The histogram (of weights, and of counts if they are `counted`); the weight that min_p keeps.
+  LCE_DEV u64 fill(double min_p, bool counted) const {
     for (int i = thread(); i < kBins; i += NT) {
       sh->count[i] = 0;
       sh->weight[i] = 0;
     }
     __syncthreads();
     u64 mine = 0;
-    elements([&](int, float z) {
-      const double t = weights.log2_of(z), real = exp2_series(t);
+    auto one = [&](float z) {
+      const double t = weights.log2_below(z), real = exp2_poly(t);
       const u64 w = weights.fixed(real);
       if (w == 0) return;
-      if (real >= min_p) mine += w;
       const int b = bin_of(t);
       atomicAdd(&sh->weight[b], w);
-      atomicAdd(&sh->count[b], 1);
+      if (counted) atomicAdd(&sh->count[b], 1);
+      if (min_p > 0.0 && real >= min_p) mine += w;
+    };
+    row.edges([&](int at, unsigned) { one(as_float(row.p[at])); });
+    row.each([&](int, u32x4_t v, int) {
+      E e[kPer];
+      __builtin_memcpy(e, &v, 16);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) one(as_float(e[i]));
     });
-    return block_all<Sum, NT>(mine, sh->of_wave);
+    __syncthreads();
+    return min_p > 0.0 ? block_all<Sum, NT>(mine, sh->of_wave) : 0;
   }
   // The sums of this thread's bins.
   LCE_DEV void own(int* c, u64* w) const {
@@ -1104,7 +1105,7 @@ template <class E, int NT> struct RowBins {
         const u64 wd = sh->weight[b];
         if (want.here(cb, wb, cd, wd)) {
           sh->bin = b;
-          sh->place = {0, cb, wb, cd};
+          sh->place = {0, cb, wb, 0};
         }
         cb += cd;
         wb += wd;
@@ -1113,34 +1114,41 @@ template <class E, int NT> struct RowBins {
     __syncthreads();
     const Place bin = sh->place;
     const int b = sh->bin;
-    const bool room = bin.same <= kMostList;
-    // keys between which all of its elements are: the bin's ends, each further out by more than the roundings of either direction
+    // values between which all of its elements are: the bin's ends, each further out by more than the roundings of either direction
     const double low_z = weights.top - (double)(b + 1) / (kBinsPerOctave * weights.per), high_z = weights.top - (double)b / (kBinsPerOctave * weights.per);
     const unsigned low_key = key_of((float)low_z), high_key = key_of((float)high_z);
-    const unsigned low = b == kBins - 1 || low_key < kLowKey + 4 ? kLowKey + 1 : low_key - 2, high = high_key < top - 2 ? high_key + 2 : top;
+    const float low = uniform(value_of(b == kBins - 1 || low_key < kLowKey + 4 ? kLowKey + 1 : low_key - 2));
+    const float high = uniform(value_of(high_key < top - 2 ? high_key + 2 : top));
     unsigned most = 0, inverse = 0;  // the largest key of the bin, of the inverted keys
-    elements([&](int at, float z) {
+    auto one = [&](int at, float z) {
+      if (!(z >= low && z <= high)) return;
+      const double log2 = weights.log2_below(z);
+      if (bin_of(log2) != b || weights.fixed(exp2_poly(log2)) == 0) return;  // (without a weight: not in the histogram)
       const unsigned key = key_of(z);
-      if (!(key >= low && key <= high)) return;
-      const double log2 = weights.log2_of(z);
-      if (bin_of(log2) != b || weights.fixed(exp2_series(log2)) == 0) return;  // (without a weight: not counted)
-      if (room) {
-        const int to = atomicAdd(&sh->listed, 1);
-        if (to < kMostList) sh->list[to] = entry_of(key, at);
-      } else {
-        most = key > most ? key : most;
-        inverse = ~key > inverse ? ~key : inverse;
-      }
+      const int to = atomicAdd(&sh->listed, 1);
+      if (to < kMostList) sh->list[to] = entry_of(key, at);
+      most = key > most ? key : most;
+      inverse = ~key > inverse ? ~key : inverse;
+    };
+    row.edges([&](int at, unsigned) { one(at, as_float(row.p[at])); });
+    row.each([&](int at, u32x4_t v, int) {
+      E e[kPer];
+      __builtin_memcpy(e, &v, 16);
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) any |= as_float(e[i]) >= low && as_float(e[i]) <= high;
+      if (any) RowUnits<E, NT>::elements(v, kPer, [&](int i, float z) { one(at + i, z); });
     });
+    __syncthreads();
+    const int in_bin = sh->listed;
     *column = -1;
-    if (!room) {
+    if (in_bin > kMostList) {
       most = block_all<Largest, NT>(most, reinterpret_cast<unsigned*>(sh->of_wave));
       inverse = block_all<Largest, NT>(inverse, reinterpret_cast<unsigned*>(sh->of_wave));
-      *place = {most, bin.count, bin.weight, bin.same};
+      *place = {most, bin.count, bin.weight, in_bin};
       return most == ~inverse;
     }
-    __syncthreads();
-    const int n = sh->listed < kMostList ? sh->listed : kMostList;
+    const int n = in_bin;
     const u64* list = sh->list;
     if (n <= kMostRanked) {
       list = rank_list<NT>(sh->list, sh->list + kMostRanked, n);
@@ -1183,11 +1191,12 @@ LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s
   if (value_of(top) < inf) {
     const Weights weights = s.weights(value_of(top));
     const RowBins<E, NT> bins = {row, weights, top, sh};
-    const u64 by_min = bins.fill(s.min_p > 0.f ? (double)s.min_p : 0.0);
-    int c, cb;
+    const bool by_count = s.top_k > 0 && s.top_k < row.n;
+    const u64 by_min = bins.fill(s.min_p > 0.f ? (double)s.min_p : 0.0, by_count);
+    int c, cb = 0;
     u64 w, wb;
     bins.own(&c, &w);
-    const int counted = block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave), &cb);
+    const int counted = by_count ? block_all<Sum, NT>(c, reinterpret_cast<int*>(sh->of_wave), &cb) : 0;
     const u64 all = block_all<Sum, NT>(w, sh->of_wave, &wb);
     if (thread() == 0) {
       sh->place = {top, 0, 0, 0};
@@ -1197,7 +1206,7 @@ LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s
     __syncthreads();
     bool fine = true;
     int which = 0, column = -1;
-    const Place at = draw_place(s, counted, all, by_min, Place{top, 0, 0, 0}, &which,
+    const Place at = draw_place(s, counted, all, s.min_p > 0.f ? by_min : all, Place{top, 0, 0, 0}, &which,
                                 [&](const Want& want) {
                                   Place p = {top, 0, 0, 0};
                                   if (fine) fine = bins.find(cb, wb, c, w, want, &p, &column);
