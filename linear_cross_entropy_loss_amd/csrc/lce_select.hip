@@ -408,21 +408,27 @@ template <int kPartRounds = 8, class E, int NT> LCE_DEV int column_of(const RowP
   return at;
 }
 
+// a * b + c with c in scalar registers.  (With constants in vector registers the compiler copies each before it adds to it.)
+LCE_DEV double fma_scalar(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+}
 // 2^t for -2000 <= t <= 0: 2^(t - rint t) by the polynomial of degree 10 whose largest relative error over half a unit to either side is
 // smallest (2.1e-16; 2^0 is 1), times a power of two.
 LCE_DEV double exp2_poly(double t) {
   constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: the sum's last place is 1
   const double m = t + kWhole, x = t - (m - kWhole);
   double p = 7.037278846726901e-09;
-  p = fma(p, x, 1.0208537929657404e-07);
-  p = fma(p, x, 1.3215662835959238e-06);
-  p = fma(p, x, 1.5252658116409854e-05);
-  p = fma(p, x, 0.00015403529961127076);
-  p = fma(p, x, 0.0013333558228561767);
-  p = fma(p, x, 0.009618129108034596);
-  p = fma(p, x, 0.05550410866445883);
-  p = fma(p, x, 0.24022650695908768);
-  p = fma(p, x, 0.6931471805599497);
+  p = fma_scalar(p, x, 1.0208537929657404e-07);
+  p = fma_scalar(p, x, 1.3215662835959238e-06);
+  p = fma_scalar(p, x, 1.5252658116409854e-05);
+  p = fma_scalar(p, x, 0.00015403529961127076);
+  p = fma_scalar(p, x, 0.0013333558228561767);
+  p = fma_scalar(p, x, 0.009618129108034596);
+  p = fma_scalar(p, x, 0.05550410866445883);
+  p = fma_scalar(p, x, 0.24022650695908768);
+  p = fma_scalar(p, x, 0.6931471805599497);
   p = fma(p, x, 1.0);
   return ldexp(p, (int)(unsigned)__builtin_bit_cast(u64, m));
 }
@@ -431,13 +437,16 @@ LCE_DEV double exp2_poly(double t) {
 struct Weights {
   double top, per;  // the largest value, log2(e) / temperature
   double one;       // 2^bits, bits <= 50
+  double least;     // -bits - 1 + 2^-10
   LCE_DEV double log2_of(float z) const {
     // (equal infinities have no difference, and one times 0, at an infinite temperature, is no number)
     const double zd = (double)z;
     return zd == top ? 0.0 : fmax((zd - top) * per, -2000.0);
   }
-  // (of a finite top)
-  LCE_DEV double log2_below(float z) const { return fmax(((double)z - top) * per, -2000.0); }
+  // The same for a finite top, without a bound below; and whether such an element is taken to have a weight at all: one above half a
+  // place rounds to one or more.
+  LCE_DEV double log2_below(float z) const { return ((double)z - top) * per; }
+  LCE_DEV bool has_weight(double log2) const { return log2 >= least; }
   LCE_DEV double real(float z) const { return exp2_poly(log2_of(z)); }
   // (rounded by the sum with 2^52, whose last place is 1)
   LCE_DEV u64 fixed(double w) const { return __builtin_bit_cast(u64, fma(w, one, 4503599627370496.0)) & 0xfffffffffffffull; }
@@ -607,7 +616,7 @@ struct RowSettings {
   }
   LCE_DEV bool greedy() const { return !(temperature > 0.f) || top_k == 1; }
   LCE_DEV Weights weights(float top) const {
-    return {uniform((double)top), uniform(1.4426950408889634074 / (double)temperature), (double)((u64)1 << bits)};
+    return {uniform((double)top), uniform(1.4426950408889634074 / (double)temperature), (double)((u64)1 << bits), -1023.0 / 1024.0 - bits};
   }
 };
 
@@ -1028,6 +1037,7 @@ constexpr int kSelectThreads = 1024;
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kBins = 4096;
 constexpr double kBinsPerOctave = 80.0;  // 51 octaves: a weight of 2^-51 rounds to 0 with 50 places
+static_assert(51 * 80 < kBins);
 struct BinShared {
   union {
     struct {
@@ -1052,8 +1062,7 @@ template <class E, int NT> struct RowBins {
   BinShared* sh;
 
   LCE_DEV static int bin_of(double log2_weight) {
-    const int b = (int)(log2_weight * -kBinsPerOctave);
-    return b < kBins - 1 ? b : kBins - 1;
+    return (int)(log2_weight * -kBinsPerOctave);  // (< 51 * 80)
   }
   // The histogram (of weights, and of counts if they are `counted`); the weight that min_p keeps.
   LCE_DEV u64 fill(double min_p, bool counted) const {
@@ -1064,13 +1073,17 @@ template <class E, int NT> struct RowBins {
     __syncthreads();
     u64 mine = 0;
     auto one = [&](float z) {
-      const double t = weights.log2_below(z), real = exp2_poly(t);
+      const double t = weights.log2_below(z);
+      if (!weights.has_weight(t)) return;
+      const double real = exp2_poly(t);
       const u64 w = weights.fixed(real);
-      if (w == 0) return;
       const int b = bin_of(t);
       atomicAdd(&sh->weight[b], w);
       if (counted) atomicAdd(&sh->count[b], 1);
-      if (min_p > 0.0 && real >= min_p) mine += w;
+      if (min_p > 0.0) {
+        asm volatile("");  // (a branch)
+        if (real >= min_p) mine += w;
+      }
     };
     row.edges([&](int at, unsigned) { one(as_float(row.p[at])); });
     row.each([&](int, u32x4_t v, int) {
@@ -1117,13 +1130,13 @@ template <class E, int NT> struct RowBins {
     // values between which all of its elements are: the bin's ends, each further out by more than the roundings of either direction
     const double low_z = weights.top - (double)(b + 1) / (kBinsPerOctave * weights.per), high_z = weights.top - (double)b / (kBinsPerOctave * weights.per);
     const unsigned low_key = key_of((float)low_z), high_key = key_of((float)high_z);
-    const float low = uniform(value_of(b == kBins - 1 || low_key < kLowKey + 4 ? kLowKey + 1 : low_key - 2));
+    const float low = uniform(value_of(low_key < kLowKey + 4 ? kLowKey + 1 : low_key - 2));
     const float high = uniform(value_of(high_key < top - 2 ? high_key + 2 : top));
     unsigned most = 0, inverse = 0;  // the largest key of the bin, of the inverted keys
     auto one = [&](int at, float z) {
       if (!(z >= low && z <= high)) return;
       const double log2 = weights.log2_below(z);
-      if (bin_of(log2) != b || weights.fixed(exp2_poly(log2)) == 0) return;  // (without a weight: not in the histogram)
+      if (!weights.has_weight(log2) || bin_of(log2) != b) return;
       const unsigned key = key_of(z);
       const int to = atomicAdd(&sh->listed, 1);
       if (to < kMostList) sh->list[to] = entry_of(key, at);
