@@ -650,7 +650,12 @@ LCE_DEV Place draw_place(const RowSettings& s, int counted, u64 all, u64 by_min,
       const u64 by_p = at.weight + (u64)kept * w;
       if (by_p < stays) stays = by_p;
     } else {
-      *which = (int)((want.target - at.weight) / w);
+      // the whole part of the quotient, which is below at.same: by a double and a look at what it leaves
+      const u64 rest = want.target - at.weight;
+      int whole = (int)((double)rest / (double)w);
+      if ((u64)whole * w > rest) --whole;
+      else if (rest - (u64)whole * w >= w) ++whole;
+      *which = whole;
     }
   }
   return at;
@@ -903,6 +908,7 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
       if (to < kMostList) sh->list[to] = entry_of(key_of(O::value(a)), at);
     }
   };
+  // (one fma of z and m log2 e would do, but for logits of 10^30, where the product's rounding is no small number)
   auto term = [&](float z) { sum += __builtin_amdgcn_exp2f((z - m) * 1.4426950408889634f); };
   row.edges([&](int at, unsigned a) {
     add(at, a);
@@ -1490,11 +1496,13 @@ unsigned grid_of(int64_t rows, int64_t row_bytes, int most, int num_cus) {
 }
 static_assert(sizeof(HalfShared) <= 160 * 1024, "a compute unit has 160 KiB of LDS");
 
-// 16-bit rows up to this are sampled by bins, longer ones by the histogram of all values: that takes a compute unit for a row, much of its
-// time whatever the row's length, and more for fp16, of which a row has more different values.  us, bins / histogram, temperature alone
-// and with top_p: 2048 rows, bf16 V=4096 74, 94 / 159, 170, 16384 137, 166 / 175, 187, 24000 172, 205 / 189, 200, 32768 213, 252 /
-// 204, 215; fp16 16384 135, 159 / 222, 239, 32768 208, 243 / 253, 274; 64 rows, bf16 16384 25, 31 / 24, 25, 32768 38, 46 / 27, 27; fp16
-// 16384 25, 30 / 30, 32, 32768 37, 43 / 33, 36.
+// 16-bit rows up to this, or half of it where there is no more than one for each compute unit, are sampled by bins, longer ones by the
+// histogram of all values: that takes a compute unit for a row, much of its time whatever the row's length, and more for fp16, of which a
+// row has more different values.  us, bins / histogram, temperature alone and with top_p:
+//   2048 rows   bf16 V=4096 52/97, 76/109; 16384 87/117, 120/127; 24000 113/124, 147/135; 32768 138/130, 181/141
+//               fp16 V=16384 85/159, 115/180; 32768 133/178, 171/203; 50257 183/195, 226/219; 65536 222/206, 277/237
+//   64 rows     bf16 V=8192 14/16, 20/18; 16384 18/17, 25/18; 32768 27/18, 36/20
+//               fp16 V=8192 14/20, 19/23; 16384 18/22, 24/25; 24000 22/23, 30/27; 32768 26/25, 34/28
 template <class E> constexpr int64_t kMostBinCols = 16384;
 template <> constexpr int64_t kMostBinCols<_Float16> = 32768;
 
@@ -1509,7 +1517,7 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
     return hipGetLastError();
   }
   if constexpr (sizeof(E) == 2) {
-    if (cols > kMostBinCols<E>) {
+    if (cols > (rows > num_cus ? kMostBinCols<E> : kMostBinCols<E> / 2)) {
       static LdsOptIn optin;
       const hipError_t e = optin.ensure(reinterpret_cast<const void*>(sample_half_kernel<E>), (int)sizeof(HalfShared));
       if (e != hipSuccess) return e;
