@@ -1294,8 +1294,8 @@ template <class E> struct HalfRow {
   HalfShared* sh;
 
   // The counts of the row's values, listed.  Returns whether the list has all of the row's columns that are not masked; *different: how
-  // many values it has.
-  LCE_DEV bool fill(const RowPieces<E, kSelectThreads>& row, int* different) const {
+  // many values it has, *any_masked: whether there are masked columns.
+  LCE_DEV bool fill(const RowPieces<E, kSelectThreads>& row, int* different, bool* any_masked) const {
     constexpr int kWordRounds = kHalfWords / 4 / kSelectThreads;
     const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     u32x4_t* words = reinterpret_cast<u32x4_t*>(sh->hist);
@@ -1376,6 +1376,7 @@ template <class E> struct HalfRow {
     }
     const u64 both = block_all<Sum, kSelectThreads>(sum | (u64)masked << 31, sh->of_wave);
     const u64 counted = both & 0x7fffffffu;
+    *any_masked = both >> 31 != 0;
     int before;
     *different = block_all<Sum, kSelectThreads>(t < 2 * kWordRows ? sh->row_values[t] : 0, reinterpret_cast<int*>(sh->of_wave), &before);
     if (any_nan || counted == 0 || *different > kHalfWords || (int)(counted + (both >> 31)) != row.n) return false;
@@ -1449,12 +1450,16 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
     const u64* list = nullptr;
     if (k >= 1 && k <= kMostByMaxima && k < cols) list = list_first<E, false>(row, k, &sh->top);
     int column;
-    int different;
+    int different = 0;
+    bool masked = false;
+    bool filled = list == nullptr && !s.greedy() && half.fill(row, &different, &masked);
+    const unsigned top = filled ? sh->values[0] & 0xffffu : 0;
+    const Weights weights = s.weights(half_value<E>(top));
+    // (at a temperature that leaves the lowest number a weight it masks nothing)
+    if (filled && masked && weights.of(half_value<E>(0x8000u | HalfRow<E>::kMax)) != 0) filled = false;
     if (list != nullptr) {
       column = sample_listed<kSelectThreads>(s, k, list, &sh->top);
-    } else if (!s.greedy() && half.fill(row, &different)) {
-      const unsigned top = sh->values[0] & 0xffffu;
-      const Weights weights = s.weights(half_value<E>(top));
+    } else if (filled) {
       const double min_p = s.min_p > 0.f ? (double)s.min_p : 0.0;
       u64 weight = 0, by_min = 0;
       int elements = 0;

@@ -456,3 +456,28 @@ def test_beside_the_loss_on_labels():
     both = torch.autograd.grad(labels() + teacher(), (x, w))
     for got, a, b in zip(both, *parts):
         assert torch.equal(got, a + b)
+
+
+@pytest.mark.pack_auto
+@pytest.mark.parametrize("V", [1 << 20, (1 << 20) + 8])
+def test_as_many_column_groups_as_are_sorted(V):
+    """A vocabulary with the most groups of columns that the sort of the entries has room for, and one more; oracle on the GPU."""
+    from linear_cross_entropy_loss_amd import linear_distillation
+
+    print(f"distill V={V}", flush=True)
+    N, H, K = 64, 64, 1024
+    g = torch.Generator(device="cuda").manual_seed(45)
+    x = torch.randn(N, H, generator=g, device="cuda").to(BF16).requires_grad_(True)
+    w = (torch.randn(H, V, generator=g, device="cuda") / 8).to(BF16).requires_grad_(True)
+    index = torch.randint(0, V, (N, K), generator=g, device="cuda")
+    index[:, 0] = V - 1
+    logits = 4.0 * torch.randn(N, K, generator=g, device="cuda")
+    loss = linear_distillation(x, w, index, logits)
+    loss.backward()
+    q = torch.zeros(N, V, dtype=torch.float64, device="cuda").scatter_add_(1, index, torch.softmax(logits.double(), 1))
+    p = torch.log_softmax(x.detach().double() @ w.detach().double(), 1)
+    ref = ((torch.special.xlogy(q, q) - q * p).sum(1)).mean()
+    dz = (p.exp() - q) / N
+    assert abs(loss.item() - ref.item()) <= 64 * 2.0 ** -22 * max(1.0, ref.item())
+    assert rel_errors(x.grad, dz @ w.detach().double().t())[1] <= 1.5 * EPS[BF16]
+    assert rel_errors(w.grad, x.detach().double().t() @ dz)[1] <= 1.5 * EPS[BF16]

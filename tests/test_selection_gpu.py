@@ -458,3 +458,36 @@ def test_no_gradient_and_opcheck():
     one = torch.ones((), device="cuda")
     torch.library.opcheck(torch.ops.lce_amd.sample_logits.default, (z, u, one, torch.zeros((), dtype=torch.int64, device="cuda"), one, 0 * one),
                           test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("V", [9000, 40000])
+@pytest.mark.parametrize("dtype,temperature", [(BF16, 1e38), (F16, 3000.0), (F16, 1e5), (F32, 2e38), (F16, 1.0), (BF16, 1.0)])
+def test_the_lowest_number_with_a_weight(dtype, temperature, V):
+    """Columns masked by the type's lowest number count like any other where the temperature leaves them a weight."""
+    z = rows(6, V, dtype, seed=32)
+    z[:3, V // 3:] = torch.finfo(dtype).min
+    z[1, ::2] = -math.inf
+    u = torch.tensor([0.1, 0.6, 0.99, 0.1, 0.6, 0.99])
+    check_sample(z, u, temperature=temperature)
+    check_sample(z, u, temperature=temperature, top_p=0.7)
+
+
+def test_captured_long_rows():
+    """The way that takes a whole compute unit's LDS, captured without a call before, two graphs replayed in turn."""
+    from linear_cross_entropy_loss_amd import sample_logits
+
+    z = [rows(40, 50257, dtype, seed=33).cuda() for dtype in (BF16, F16)]
+    u = torch.rand(40, generator=torch.Generator().manual_seed(34)).cuda()
+    graphs, tokens = [], []
+    for one in z:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            tokens.append(sample_logits(one, u, 0.8, 0, 0.9))
+    for seed in range(3):
+        u.copy_(torch.rand(40, generator=torch.Generator().manual_seed(35 + seed)))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for one, got in zip(z, tokens):
+            assert torch.equal(got.cpu(), ref_sample(one.cpu(), u.cpu(), 0.8, 0, 0.9))
+            assert torch.equal(got, sample_logits(one, u, 0.8, 0, 0.9))
