@@ -960,7 +960,9 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
   return sh->list;
 }
 
-// (64 registers a thread and little LDS: several workgroups to a compute unit, of which some read while others sort)
+// Bound by memory traffic for long rows (2048 rows of 50257 bf16 64 us, 3.2 TB/s of one reading; 2048 of 131072 float32 317, 3.4), by the
+// latency of its steps for short ones: 48 rows of 50304 14 us, of which 4 read and 2 look for the bound, 6 list and sum, 1 sorts.
+// (64 registers a thread and little LDS: four workgroups to a compute unit, of which some read while others sort)
 constexpr int kTopThreads = 512;
 template <class E, bool LSE>
 __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values,
@@ -1040,6 +1042,8 @@ constexpr int kSelectThreads = 1024;
 // the fixed point of the weights reaches; the few elements of the bin in which a place lies are then listed and sorted.  Passes over the
 // row: its maximum, the histogram, one for every place that is asked for.  A bin with more elements than the list has room for is
 // no matter if they are all equal; else the row is done by digits.
+//   Bound by the vector work of the weights, 24 instructions for an element, most of them of 64 bits: 2048 rows of 32000 fp16 113 us, of
+// which the histogram takes half, a place 25, the maximum, from memory, 15.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kBins = 4096;
 constexpr double kBinsPerOctave = 80.0;  // 51 octaves: a weight of 2^-51 rounds to 0 with 50 places
@@ -1238,7 +1242,7 @@ LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s
   return sample_by_digits(RowUnits<E, NT>(from, cols), s, &sh->digits);
 }
 
-// NT = 512: two rows to a compute unit; 1024 for rows that have one each.
+// NT = 512: two rows to a compute unit; 1024 for rows that have one each (256 rows of 131072 float32 82 us with 512, 75 with 1024).
 template <class E, int NT>
 __global__ __launch_bounds__(NT, 4) void sample_bins_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
                                                             const Sampling settings, int bits, int64_t* token) {
@@ -1269,6 +1273,8 @@ __global__ __launch_bounds__(NT, 4) void sample_bins_kernel(const E* logits, int
 // counted apart.  A count beyond 65535 overflows into the other half of its word or is lost; either way the sum of all counts is short,
 // and the row, like one with a NaN or with nothing but masked columns, is done by digits.
 //   The values that occur are then listed in the order of the row, over the histogram, and a thread has a stretch of the list.
+//   Bound by latencies, the passes by LDS atomics and the caches: a row of 131072 bf16 28 us, of which the histogram 9, its reading and the
+// list 6, weights and places 4, the drawn value's column 7; 256 such rows 39 us, the two passes 11 each.
 // ---------------------------------------------------------------------------------------------------------------------------
 template <class E> struct HalfFormat;
 template <> struct HalfFormat<__bf16> { static constexpr unsigned kInf = 0x7f80; };
@@ -1490,15 +1496,21 @@ __global__ __launch_bounds__(kSelectThreads) void sample_half_kernel(const E* lo
   }
 }
 
-// Workgroups: up to `most` rows to a compute unit at a time -- a workgroup takes one after another, its code and constants are then at
-// hand (2048 rows of 32000, one workgroup to each 301 us, 256 in all 258) -- but no more than the Infinity Cache holds of them between
-// the passes (2048 float32 rows of 131072: 1024 at a time 408 us, 512 364, 256 414).
-unsigned grid_of(int64_t rows, int64_t row_bytes, int most, int num_cus) {
-  int64_t n = ((int64_t)256 << 20) / (row_bytes < 1 ? 1 : row_bytes);
-  if (n < num_cus) n = num_cus;
-  if (n > (int64_t)most * num_cus) n = (int64_t)most * num_cus;
+// Workgroups: one for a row (65536 rows of 1000 bf16, us, one for each / 1024 that take one row after another: top_logits 494 / 612,
+// sampling by bins 1307 / 1380; 4096 rows of 32000 80 / 87, 223 / 240), up to a number that a launch can have.
+unsigned grid_of(int64_t rows) { return (unsigned)(rows < (int64_t)1 << 22 ? rows : (int64_t)1 << 22); }
+// The two passes over the first elements, four workgroups to a compute unit, are bound by memory: where so many rows are more than the
+// 256 MiB Infinity Cache holds, as many workgroups as it has room for, so that the second pass finds them there (1500 rows of 131072
+// float32 249 us, 512 at a time 228; 1024 rows of 262144 bf16 180, 165).
+unsigned grid_of_top(int64_t rows, int64_t row_bytes, int num_cus) {
+  const int64_t cached = ((int64_t)256 << 20) / row_bytes;
+  if (cached >= (int64_t)4 * num_cus) return grid_of(rows);
+  const int64_t n = cached < num_cus ? num_cus : cached;
   return (unsigned)(rows < n ? rows : n);
 }
+// The histogram of all values: a workgroup to a compute unit, whose code and constants are at hand for its next row (4096 rows of 32000
+// bf16 260 us, by 512 workgroups 252).
+unsigned grid_of_half(int64_t rows, int num_cus) { return (unsigned)(rows < (int64_t)2 * num_cus ? rows : (int64_t)2 * num_cus); }
 static_assert(sizeof(HalfShared) <= 160 * 1024, "a compute unit has 160 KiB of LDS");
 
 // 16-bit rows up to this, or half of it where there is no more than one for each compute unit, are sampled by bins, longer ones by the
@@ -1517,7 +1529,7 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
   const int64_t row_bytes = cols * (int64_t)sizeof(E);
   const bool first_alone = (!s.temperature_rows && s.temperature == 0.f) || (!s.top_k_rows && s.top_k >= 1 && s.top_k <= kMostByMaxima);
   if (first_alone) {
-    hipLaunchKernelGGL(sample_top_kernel<E>, dim3(grid_of(rows, row_bytes, 4, num_cus)), dim3(kTopThreads), 0, stream, logits, rows, cols, ld, u,
+    hipLaunchKernelGGL(sample_top_kernel<E>, dim3(grid_of_top(rows, row_bytes, num_cus)), dim3(kTopThreads), 0, stream, logits, rows, cols, ld, u,
                        s, bits, token);
     return hipGetLastError();
   }
@@ -1526,7 +1538,7 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
       static LdsOptIn optin;
       const hipError_t e = optin.ensure(reinterpret_cast<const void*>(sample_half_kernel<E>), (int)sizeof(HalfShared));
       if (e != hipSuccess) return e;
-      hipLaunchKernelGGL(sample_half_kernel<E>, dim3(grid_of(rows, row_bytes, 1, num_cus)), dim3(kSelectThreads), sizeof(HalfShared), stream,
+      hipLaunchKernelGGL(sample_half_kernel<E>, dim3(grid_of_half(rows, num_cus)), dim3(kSelectThreads), sizeof(HalfShared), stream,
                          logits, rows, cols, ld, u, s, bits, token);
       return hipGetLastError();
     }
@@ -1534,7 +1546,7 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
     hipLaunchKernelGGL((sample_bins_kernel<E, 1024>), dim3((unsigned)rows), dim3(1024), 0, stream, logits, rows, cols, ld, u, s, bits, token);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((sample_bins_kernel<E, 512>), dim3(grid_of(rows, row_bytes, 2, num_cus)), dim3(512), 0, stream, logits, rows, cols, ld, u, s,
+  hipLaunchKernelGGL((sample_bins_kernel<E, 512>), dim3(grid_of(rows)), dim3(512), 0, stream, logits, rows, cols, ld, u, s,
                      bits, token);
   return hipGetLastError();
 }
@@ -1542,7 +1554,7 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
 template <class E>
 hipError_t launch_top_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values, int64_t* index, float* lse, int num_cus,
                          hipStream_t stream) {
-  const dim3 grid(grid_of(rows, cols * (int64_t)sizeof(E), 4, num_cus)), block(kTopThreads);
+  const dim3 grid(grid_of_top(rows, cols * (int64_t)sizeof(E), num_cus)), block(kTopThreads);
   if (lse != nullptr) hipLaunchKernelGGL((top_kernel<E, true>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
   else hipLaunchKernelGGL((top_kernel<E, false>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
   return hipGetLastError();

@@ -491,3 +491,27 @@ def test_captured_long_rows():
         for one, got in zip(z, tokens):
             assert torch.equal(got.cpu(), ref_sample(one.cpu(), u.cpu(), 0.8, 0, 0.9))
             assert torch.equal(got, sample_logits(one, u, 0.8, 0, 0.9))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_beyond_the_cache(dtype):
+    """So many long rows that a workgroup takes several: what each part of them gives by itself, where it takes one."""
+    from linear_cross_entropy_loss_amd import sample_logits, top_logits
+
+    N, V = 600, 300001 if dtype == F32 else 600001
+    g = torch.Generator(device="cuda").manual_seed(38)
+    z = (2.0 * torch.randn(N, V, generator=g, device="cuda")).to(dtype)
+    z[7] = 0.0
+    z[300, 5] = math.nan
+    z[500, 20:] = -math.inf
+    u = torch.rand(N, generator=g, device="cuda")
+    top, token = top_logits(z, 20), sample_logits(z, u, 0.9, 30)
+    for i in range(0, N, 200):
+        part = top_logits(z[i:i + 200], 20)
+        assert torch.equal(top[1][i:i + 200], part[1])
+        assert torch.equal(top[0][i:i + 200].nan_to_num(nan=9e9), part[0].nan_to_num(nan=9e9))
+        assert torch.equal(top[2][i:i + 200].nan_to_num(nan=9e9), part[2].nan_to_num(nan=9e9))
+        assert torch.equal(token[i:i + 200], sample_logits(z[i:i + 200], u[i:i + 200], 0.9, 30))
+    check_top(z[:2].cpu(), 20)
+    check_top(z[596:].cpu(), 20)
+    assert torch.equal(top[1][596:].cpu(), ref_top(z[596:].cpu(), 20)[1])
