@@ -437,7 +437,7 @@ int lce_transpose_rows(const void* src, int dtype, int64_t rows, int64_t cols, i
  * the weight, or with a NaN or +inf among its logits, makes the loss NaN, as does R == 0 (both gradients are zeros then).
  *   p          monitoring, z_reg and phases are 0; ignore_index is not looked at (-1 is taken); n_chunk, pack_rows and route as in
  *              lce_forward_backward
- *   K          1 <= K <= LCE_MAX_TARGETS, N * K < 2^31
+ *   K          1 <= K <= LCE_MAX_TARGETS, N * K <= 2^30
  *   grad_out   device pointer to 1 float, as in lce_forward_backward (may be NULL without gradients)
  *   lse        out, N floats, as in lce_forward
  *   loss       out, 1 float;  n_valid  out, 1 int64: R

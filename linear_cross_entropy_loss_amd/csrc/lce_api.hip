@@ -1283,7 +1283,7 @@ struct DistillPlan {
 
 int check_targets(int64_t N, int64_t K) {
   if (K < 1 || K > lce::kMaxTargets) return LCE_EINVAL_SHAPE;
-  return N * K >= (int64_t)1 << 31 ? LCE_EINVAL_SHAPE : LCE_OK;  // (entries are counted in 32 bits)
+  return N * K > (int64_t)1 << 30 ? LCE_EINVAL_SHAPE : LCE_OK;  // (entries are counted in 32 bits, launches have fewer than 2^32 threads)
 }
 
 // The problem as the loss's planners and kernels see it: labels are columns, -1 stands for none.

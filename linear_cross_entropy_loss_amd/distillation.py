@@ -209,8 +209,8 @@ def linear_distillation(x, At, index, logits, temperature: float = 1.0, logit_sc
     Args:
         x: hidden states (..., H): bfloat16, float16 or float32.
         At: weight (H, V) with the strides that ``linear_cross_entropy`` takes: of x's dtype, or float32 under 16-bit x.
-        index: (..., K) columns, torch.long, 1 <= K <= 1024.  A negative one, whatever its logit, is no target; one of V and above
-            makes the loss NaN.  A column may be named twice: its probabilities add up.
+        index: (..., K) columns, torch.long, 1 <= K <= 1024, 2^30 of them at most.  A negative one, whatever its logit, is no
+            target; one of V and above makes the loss NaN.  A column may be named twice: its probabilities add up.
         logits: (..., K) the teacher's logits there: bfloat16, float16 or float32.  -inf is no target, NaN and +inf make the loss NaN.
         temperature: divides both sides' logits.
         N_chunk_size: as of ``LinearCrossEntropyLoss``.

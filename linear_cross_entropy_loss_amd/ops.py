@@ -782,7 +782,8 @@ class LinearCrossEntropyLoss(torch.nn.Linear):
         return loss
 
     def distill(self, x, index, logits, temperature: float = 1.0):
-        """Loss of ``x`` against a teacher's top logits (``linear_distillation``), with this module's weight and logit_scale."""
+        """Loss of ``x`` against a teacher's top logits (``linear_distillation``), with this module's weight, logit_scale and
+        N_chunk_size; z-regularisation and monitoring belong to the loss against labels."""
         from .distillation import linear_distillation
 
         return linear_distillation(x, self.weight, index, logits, temperature, self.logit_scale, self.N_chunk_size)

@@ -63,7 +63,7 @@ def _soft(lib, N=4, K=8, V=100, index=PTR, ld_index=8, logits=PTR, dtype=BF16, l
 def test_soft_targets_refusals(lib):
     L = _codes()
     for bad in (dict(N=0), dict(N=(1 << 30) + 1), dict(V=0), dict(V=(1 << 30) + 1), dict(K=0), dict(K=1025), dict(K=-1),
-                dict(N=1 << 29, K=4), dict(N=1 << 21, K=1024)):
+                dict(N=1 << 29, K=4), dict(N=(1 << 20) + 1, K=1024)):
         assert _soft(lib, **bad) == L.LCE_EINVAL_SHAPE, bad
     for bad in (3, -1):
         assert _soft(lib, dtype=bad) == L.LCE_EINVAL_DTYPE
@@ -80,7 +80,7 @@ def test_distill_refusals(lib):
     L = _codes()
     for bad in (0, 1025, -3):
         assert _distill(lib, _prob(), K=bad) == L.LCE_EINVAL_SHAPE
-    assert _distill(lib, _prob(N=1 << 21), K=1024) == L.LCE_EINVAL_SHAPE
+    assert _distill(lib, _prob(N=(1 << 20) + 1), K=1024) == L.LCE_EINVAL_SHAPE
     assert _distill(lib, _prob(N=0)) == L.LCE_EINVAL_SHAPE
     for bad in (dict(index=None), dict(q=None), dict(y=None), dict(x=None), dict(w=None), dict(g=None), dict(lse=None), dict(loss=None),
                 dict(n_valid=None), dict(x=PTR + 2), dict(w=PTR + 8), dict(dx=PTR + 4), dict(dw=PTR + 4)):
