@@ -1104,6 +1104,12 @@ int fused_impl(const lce_problem* p, const FusedPlan& f, const void* x, const vo
       if (e != hipSuccess) return hip_fail(e, "fwd_rows");
     }
     if ((dx || dw) && (ph & LCE_PHASE_BWD_DZ)) {
+      if (targets != nullptr && f.kept) {  // (before dz takes the logits' place)
+        lce::SoftTargets t = *targets;
+        t.row0 = row0;
+        e = lce::launch_soft_pick(a, t, s);
+        if (e != hipSuccess) return hip_fail(e, "soft_pick");
+      }
       e = f.kept ? lce::launch_stage_pairs(a, s) : f.factors ? lce::launch_stage_factors(a, s) : lce::launch_stage_scale(a, s);
       if (e != hipSuccess) return hip_fail(e, f.kept ? "stage_pairs" : f.factors ? "stage_factors" : "stage_scale");
       if (targets != nullptr) {
@@ -1279,6 +1285,7 @@ struct DistillPlan {
   FusedPlan f;
   BwdPlan b;
   size_t out5, part, z, total;
+  bool picks() const { return one_pass && f.kept; }
 };
 
 int check_targets(int64_t N, int64_t K) {
@@ -1308,8 +1315,8 @@ int plan_distill(const lce_problem* q, int64_t K, bool grads, DistillPlan* d) {
       if (d->b.total > o) o = d->b.total;
     }
   }
-  // (the scratch of the targets' logits is free again before the loss's kernels run)
-  const size_t sorting = lce::soft_logits_bytes(q->N, (int)K, q->H, q->V, q->w_layout == LCE_W_VH);
+  // (the scratch of the targets' logits is free again before the loss's kernels run; where the stage keeps the logits they are read there)
+  const size_t sorting = d->picks() ? 0 : lce::soft_logits_bytes(q->N, (int)K, q->H, q->V, q->w_layout == LCE_W_VH);
   if (sorting > o) o = sorting;
   o = align_up(o);
   d->out5 = o; o += 256;
@@ -1592,17 +1599,18 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
   char* base = (char*)ws;
   float* out5 = (float*)(base + d.out5);
 
+  float* const z = (float*)(base + d.z);
   lce::SoftLogits g;
   memset(&g, 0, sizeof(g));
   g.x = x; g.w = w; g.N = p->N; g.H = p->H; g.V = p->V; g.ldx = p->ldx; g.ldw = p->ldw;
   g.x_dtype = p->x_dtype; g.w_dtype = p->w_dtype; g.w_vh = p->w_layout == LCE_W_VH; g.K = (int)K;
-  g.index = index; g.scale = p->logit_scale; g.z = (float*)(base + d.z);
-  hipError_t e = lce::launch_soft_logits(g, base, s);
+  g.index = index; g.scale = p->logit_scale; g.z = z;
+  hipError_t e = d.picks() ? hipSuccess : lce::launch_soft_logits(g, base, s);
   if (e != hipSuccess) return hip_fail(e, "soft_logits");
 
   lce::SoftTargets t;
   memset(&t, 0, sizeof(t));
-  t.index = index; t.q = q; t.z = g.z; t.N = p->N; t.K = (int)K;
+  t.index = index; t.q = q; t.z = z; t.N = p->N; t.K = (int)K;
   if (d.one_pass) {
     rc = fused_impl(&soft_p, d.f, x, w, y, grad_out, lse, out5, n_valid, dx, dw, ws, stream, &t);
   } else {

@@ -7,7 +7,7 @@
 //
 // lse, the softmax and the two contractions of dz are those of the loss against labels, and so are their kernels: a row's first
 // entry serves as its label, a row without an entry has none.  Here are the pieces that know of more than one target: the teacher's
-// distribution (soft_targets_kernel), the student's logits at its columns (soft_logits_kernel), the loss from both, and the
+// distribution (soft_targets_kernel), the student's logits at its columns (soft_logits_kernel, soft_pick_kernel), the loss from both, and the
 // columns' values in the staged dz (soft_gradient_kernel), each the rounding of one fp32 value as at a label.
 #include "lce_gemm.h"
 #include "lce_internal.h"
@@ -416,16 +416,36 @@ __global__ __launch_bounds__(256) void soft_logits_kernel(const SoftLogits a, co
   }
 }
 
-// The staged dz at the teacher's columns: 2^shift * (softmax - q), rounded once.  A thread per entry; rows in the order of the stage.
+// A thread per entry of the staged rows, in the stage's order: whether its column lies in the stage, the entry, the row and the
+// column from the stage's first on.
+LCE_DEV bool staged_entry(const BwdArgs& a, const SoftTargets& t, int64_t* i, int64_t* row, int64_t* rel) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  *row = e / t.K;
+  if (*row >= packed_rows(a.n_rows, a.N)) return false;
+  const int64_t n = a.perm != nullptr ? packed_token(a.perm, *row, t.N) : t.row0 + *row;
+  *i = n * t.K + (e - *row * t.K);
+  const int64_t v = t.index[*i];
+  *rel = v - a.v0;
+  return v >= 0 && *rel >= 0 && *rel < a.vw;
+}
+
+// The student's logits at the teacher's columns where the stage holds them all, in fp32 (fp32 tensors on one pass): the logits that lse is
+// the sum of, so that p = exp(z - lse) is of one arithmetic.  Bound by lines of which it needs 2 bytes, two for an entry (N=2048, K=64:
+// two launches of 6 us, where the kernels above take 165).
+__global__ __launch_bounds__(256) void soft_pick_kernel(const BwdArgs a, const SoftTargets t) {
+  int64_t i, row, rel;
+  if (!staged_entry(a, t, &i, &row, &rel)) return;
+  const unsigned short* z = reinterpret_cast<const unsigned short*>(a.dz) + 2 * dz_block_offset(row / kTile, rel / 64, a.vs) +
+                            (row & (kTile - 1)) * 64 + (rel & 63);
+  t.z[i] = a.scale * __builtin_bit_cast(float, (unsigned)z[0] << 16 | z[kDzBlockElems]);
+}
+
+// The staged dz at the teacher's columns: 2^shift * (softmax - q), rounded once.
 // Bound by the partial lines that it writes: 64 to 128 bytes of memory traffic per entry.
 template <class T>
 __global__ __launch_bounds__(256) void soft_gradient_kernel(const BwdArgs a, const SoftTargets t) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, row = e / t.K;
-  if (row >= packed_rows(a.n_rows, a.N)) return;
-  const int64_t n = a.perm != nullptr ? packed_token(a.perm, row, t.N) : t.row0 + row;
-  const int64_t i = n * t.K + (e - row * t.K);
-  const int64_t v = t.index[i], rel = v - a.v0;
-  if (v < 0 || rel < 0 || rel >= a.vw) return;
+  int64_t i, row, rel;
+  if (!staged_entry(a, t, &i, &row, &rel)) return;
   const float q = t.q[i];
   const float p = __builtin_amdgcn_exp2f(fmaf(t.z[i] - a.lse[row], kLog2e, (float)a.dz_shift));
   const float d = p - q * __builtin_bit_cast(float, (127 + a.dz_shift) << 23);
@@ -548,6 +568,12 @@ hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s) {
     return a.w_vh ? launch_logits<_Float16, float, true>(a, ws, s) : launch_logits<_Float16, float, false>(a, ws, s);
   if (a.x_dtype == DT_F32 && a.w_dtype == DT_F32 && !a.w_vh) return launch_logits<float, float, false>(a, ws, s);
   return hipErrorInvalidValue;
+}
+
+hipError_t launch_soft_pick(const BwdArgs& a, const SoftTargets& t, hipStream_t s) {
+  const int64_t rows = a.Np < a.N ? a.Np : a.N;
+  hipLaunchKernelGGL(soft_pick_kernel, dim3((unsigned)((rows * t.K + 255) / 256)), dim3(256), 0, s, a, t);
+  return hipGetLastError();
 }
 
 hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStream_t s) {

@@ -487,7 +487,7 @@ constexpr int kMaxTargets = 1024;
 struct SoftTargets {
   const int* index;  // column, or -1: no target
   const float* q;    // its probability (0 where there is none)
-  const float* z;    // the scaled logit there
+  float* z;          // the scaled logit there
   int64_t N, row0;   // tokens; the first row of a chunk (rows that are not packed)
   int K;
 };
@@ -505,6 +505,8 @@ hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const voi
                                int64_t V, float temperature, int* out_index, float* out_q, int64_t* y, hipStream_t s);
 size_t soft_logits_bytes(int64_t N, int K, int64_t H, int64_t V, bool w_vh);  // scratch (may be 0)
 hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s);
+// z of a chunk whose stage holds the fp32 logits (BwdArgs of the pairs): read from there.
+hipError_t launch_soft_pick(const BwdArgs& a, const SoftTargets& t, hipStream_t s);
 // dz of the targets' columns of the slab or chunk that `a` describes, over what the label's kernels staged there.
 hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStream_t s);
 // part: soft_loss_groups() doubles.
