@@ -431,7 +431,7 @@ LCE_DEV bool staged_entry(const BwdArgs& a, const SoftTargets& t, int64_t* i, in
 
 // The student's logits at the teacher's columns where the stage holds them all, in fp32 (fp32 tensors on one pass): the logits that lse is
 // the sum of, so that p = exp(z - lse) is of one arithmetic.  Bound by lines of which it needs 2 bytes, two for an entry (N=2048, K=64:
-// two launches of 6 us, where the kernels above take 165).
+// two launches of 7 us, where the kernels above take 165).
 __global__ __launch_bounds__(256) void soft_pick_kernel(const BwdArgs a, const SoftTargets t) {
   int64_t i, row, rel;
   if (!staged_entry(a, t, &i, &row, &rel)) return;
