@@ -769,17 +769,59 @@ template <class E, int NT, int FL> LCE_DEV void store_top(const RowUnits<E, NT, 
   }
 }
 
-// The first k of a row by digits, any type.  list: kMostTop entries.
+// sum exp(z - m) of a row, the same bits from 512 and from 1024 threads: a thread adds up the pieces of one (or, apart, of two) of 1024
+// places, the waves' sums are doubles, in the order of the places.  A term equal to m is 1, also of an infinite m.
+template <class E, int NT> struct ExpSum {
+  static constexpr int kOwn = 1024 / NT, kPer = RowPieces<E, NT>::kPer;
+  float m, sum[kOwn];
+  LCE_DEV explicit ExpSum(float m_) : m(m_) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) sum[i] = 0.f;
+  }
+  template <bool FINITE> LCE_DEV float term(float z) const {
+    // (one fma of z and m log2 e would do, but for logits of 10^30, where the product's rounding is no small number)
+    const float e = __builtin_amdgcn_exp2f((z - m) * 1.4426950408889634f);
+    return FINITE || z != m ? e : 1.f;
+  }
+  template <bool FINITE> LCE_DEV void edge(float z) { sum[0] += term<FINITE>(z); }
+  // r: which of its round
+  template <bool FINITE> LCE_DEV void piece(u32x4_t v, int r) {
+    E e[kPer];
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum[r % kOwn] += term<FINITE>(as_float(e[i]));
+  }
+  // 16 sums; no barrier.
+  LCE_DEV void store(double* sums) const {
+    const int t = thread();
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const double upto = wave_upto<Sum>((double)sum[i]);
+      if ((t & 63) == 63) sums[i * (NT / 64) + (t >> 6)] = upto;
+    }
+  }
+};
+LCE_DEV float log_sum(float m, const double* sums) {
+  double all = 0.0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) all += sums[w];
+  return (float)((double)m + log(all));
+}
+
+// The first k of a row by digits, any type.  list: kMostTop entries; sums: 16.
 template <class E, int NT, int FL>
 LCE_DEV void top_by_digits(const RowUnits<E, NT, FL>& row, int k, E* values, int64_t* index, float* lse, SelectShared<false, false>* sh, u64* list,
-                           int* listed) {
+                           int* listed, double* sums) {
   if (lse != nullptr) {
     const unsigned top = largest_key(row, reinterpret_cast<unsigned*>(sh->of_wave));
     const float m = top == kNanKey ? __builtin_nanf("") : value_of(top);
-    float sum = 0.f;
-    row.elements([&](float z) { sum += z == m ? 1.f : __expf(z - m); });  // (equal infinities have no difference)
-    const double all = block_all<Sum, NT>((double)sum, reinterpret_cast<double*>(sh->of_wave));
-    if (thread() == 0) *lse = top == kLowKey ? m : (float)((double)m + log(all));
+    const RowPieces<E, NT> pieces(row.p, row.n);
+    ExpSum<E, NT> sum(m);
+    pieces.edges([&](int at, unsigned) { sum.template edge<false>(as_float(row.p[at])); });
+    pieces.each([&](int, u32x4_t v, int r) { sum.template piece<false>(v, r); });
+    sum.store(sums);
+    __syncthreads();
+    if (thread() == 0) *lse = top == kLowKey ? m : log_sum(m, sums);
   }
   const Place p = find_place<false, false>(row, NoWeights(), sh, Want{kByCount, k, 0.0, 0});
   // what is larger, in any order, and the first k - p.count of the key in the order of the columns
@@ -853,7 +895,7 @@ template <class Digits> struct TopShared {
 // largest element; sh->sums: by waves, sum exp(z - max) of the row (LSE).
 template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first(const RowPieces<E, NT>& row, int k, Shared* sh) {
   typedef Ordered<E> O;
-  constexpr int kPer = RowPieces<E, NT>::kPer, kOwn = kMaxima / NT, kWaves = NT / 64;  // maxima of a thread: of every kOwn-th piece
+  constexpr int kOwn = kMaxima / NT, kWaves = NT / 64;  // maxima of a thread: of every kOwn-th piece
   const int t = thread(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   unsigned most[kOwn] = {}, least = ~0u;
   row.edges([&](int, unsigned a) {
@@ -901,20 +943,18 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
   if (bound == 0x8000u) bound = 0x7fffu;  // (-0 is 0)
   const unsigned from = O::from_top_bits(bound);
   const float m = O::value(top);
-  float sum = 0.f;
+  ExpSum<E, NT> sum(m);
   auto add = [&](int at, unsigned a) {
     if (a >= from) {
       const int to = atomicAdd(&sh->listed, 1);
       if (to < kMostList) sh->list[to] = entry_of(key_of(O::value(a)), at);
     }
   };
-  // (one fma of z and m log2 e would do, but for logits of 10^30, where the product's rounding is no small number)
-  auto term = [&](float z) { sum += __builtin_amdgcn_exp2f((z - m) * 1.4426950408889634f); };
   row.edges([&](int at, unsigned a) {
     add(at, a);
-    if (LSE) term(O::value(a));
+    if (LSE) sum.template edge<true>(O::value(a));
   });
-  row.each([&](int at, u32x4_t v, int) {
+  row.each([&](int at, u32x4_t v, int r) {
     unsigned best = 0;
     u32x4_t a;
 #pragma unroll
@@ -934,17 +974,9 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
         a = u32x4_t{a[1], a[2], a[3], 0};
       }
     }
-    if (LSE) {
-      E e[kPer];
-      __builtin_memcpy(e, &v, 16);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) term(as_float(e[i]));
-    }
+    if (LSE) sum.template piece<true>(v, r);
   });
-  if (LSE) {
-    const double upto = wave_upto<Sum>((double)sum);
-    if (lane == 63) sh->sums[wave] = upto;
-  }
+  if (LSE) sum.store(sh->sums);
   if (t == 0) sh->top = top;
   __syncthreads();
   const int listed = sh->listed;
@@ -961,28 +993,24 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
 }
 
 // Bound by memory traffic for long rows (2048 rows of 50257 bf16 64 us, 3.2 TB/s of one reading; 2048 of 131072 float32 317, 3.4), by the
-// latency of its steps for short ones: 48 rows of 50304 14 us, of which 4 read and 2 look for the bound, 6 list and sum, 1 sorts.
-// (64 registers a thread and little LDS: four workgroups to a compute unit, of which some read while others sort)
-constexpr int kTopThreads = 512;
-template <class E, bool LSE>
-__global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values,
+// latency of its steps for short ones: 48 rows of 50304 12 us, of which 3 read and 2 look for the bound, 5 list and sum, 1 sorts.
+//   NT = 512: 64 registers a thread and little LDS, four rows to a compute unit, of which some are read while others are sorted; 1024 where
+// each row has a compute unit to itself.  us, 512 / 1024: top_logits, 64 rows, V=4096 bf16 7.7 / 7.8, float32 7.7 / 8.4, 50257 bf16
+// 13 / 12, 131072 21 / 19, float32 25 / 20; 256 rows, 131072 29 / 27, float32 42 / 42; 400 rows, 50257 21 / 25, 29 / 34.  sample_top_kernel,
+// 64 rows, 131072 20 / 17, float32 26 / 20; sample_bins_kernel, 64 rows, float32 75 / 58, 256 rows 98 / 84, 400 rows, 50257 61 / 67.
+template <class E, bool LSE, int NT>
+__global__ __launch_bounds__(NT, NT == 1024 ? 4 : 8) void top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values,
                                                              int64_t* index, float* lse) {
-  constexpr int NT = kTopThreads;
   __shared__ TopShared<SelectShared<false, false>> sh;
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
     const u64* list = k <= kMostByMaxima ? list_first<E, LSE>(RowPieces<E, NT>(from, cols), k, &sh) : nullptr;
     if (list != nullptr) {
-      if (LSE && thread() == NT - 1) {
-        double sums = 0.0;
-#pragma unroll
-        for (int w = 0; w < NT / 64; ++w) sums += sh.sums[w];
-        lse[n] = (float)((double)Ordered<E>::value(sh.top) + log(sums));
-      }
+      if (LSE && thread() == NT - 1) lse[n] = log_sum(Ordered<E>::value(sh.top), sh.sums);
       store_top(RowUnits<E, NT>(from, cols), list, k, values + n * k, index + n * k);
       __syncthreads();
     } else {
-      top_by_digits(RowUnits<E, NT>(from, cols), k, values + n * k, index + n * k, LSE ? lse + n : nullptr, &sh.digits, sh.by_digits, &sh.listed);
+      top_by_digits(RowUnits<E, NT>(from, cols), k, values + n * k, index + n * k, LSE ? lse + n : nullptr, &sh.digits, sh.by_digits, &sh.listed, sh.sums);
     }
   }
 }
@@ -1017,10 +1045,9 @@ template <int NT, class Shared> LCE_DEV int sample_listed(const RowSettings& s, 
 }
 
 // Rows of which the first elements are enough: settings for all of them with 1 <= top_k <= kMostByMaxima or temperature 0.
-template <class E>
-__global__ __launch_bounds__(kTopThreads, 8) void sample_top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
+template <class E, int NT>
+__global__ __launch_bounds__(NT, NT == 1024 ? 4 : 8) void sample_top_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
                                                                     const Sampling settings, int bits, int64_t* token) {
-  constexpr int NT = kTopThreads;
   __shared__ TopShared<SelectShared<true, false>> sh;
   for (int64_t n = blockIdx.x; n < rows; n += gridDim.x) {
     const E* from = logits + n * ld;
@@ -1242,7 +1269,7 @@ LCE_DEV int64_t sample_by_bins(const E* from, int64_t cols, const RowSettings& s
   return sample_by_digits(RowUnits<E, NT>(from, cols), s, &sh->digits);
 }
 
-// NT = 512: two rows to a compute unit; 1024 for rows that have one each (256 rows of 131072 float32 82 us with 512, 75 with 1024).
+// (NT: as in top_kernel; two rows to a compute unit, or one)
 template <class E, int NT>
 __global__ __launch_bounds__(NT, 4) void sample_bins_kernel(const E* logits, int64_t rows, int64_t cols, int64_t ld, const float* u,
                                                             const Sampling settings, int bits, int64_t* token) {
@@ -1529,8 +1556,11 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
   const int64_t row_bytes = cols * (int64_t)sizeof(E);
   const bool first_alone = (!s.temperature_rows && s.temperature == 0.f) || (!s.top_k_rows && s.top_k >= 1 && s.top_k <= kMostByMaxima);
   if (first_alone) {
-    hipLaunchKernelGGL(sample_top_kernel<E>, dim3(grid_of_top(rows, row_bytes, num_cus)), dim3(kTopThreads), 0, stream, logits, rows, cols, ld, u,
-                       s, bits, token);
+    if (rows <= num_cus)
+      hipLaunchKernelGGL((sample_top_kernel<E, 1024>), dim3((unsigned)rows), dim3(1024), 0, stream, logits, rows, cols, ld, u, s, bits, token);
+    else
+      hipLaunchKernelGGL((sample_top_kernel<E, 512>), dim3(grid_of_top(rows, row_bytes, num_cus)), dim3(512), 0, stream, logits, rows, cols, ld,
+                         u, s, bits, token);
     return hipGetLastError();
   }
   if constexpr (sizeof(E) == 2) {
@@ -1542,21 +1572,24 @@ hipError_t launch_sample_of(const E* logits, int64_t rows, int64_t cols, int64_t
                          logits, rows, cols, ld, u, s, bits, token);
       return hipGetLastError();
     }
-  } else if (rows <= num_cus) {
-    hipLaunchKernelGGL((sample_bins_kernel<E, 1024>), dim3((unsigned)rows), dim3(1024), 0, stream, logits, rows, cols, ld, u, s, bits, token);
-    return hipGetLastError();
   }
-  hipLaunchKernelGGL((sample_bins_kernel<E, 512>), dim3(grid_of(rows)), dim3(512), 0, stream, logits, rows, cols, ld, u, s,
-                     bits, token);
+  if (rows <= num_cus)
+    hipLaunchKernelGGL((sample_bins_kernel<E, 1024>), dim3((unsigned)rows), dim3(1024), 0, stream, logits, rows, cols, ld, u, s, bits, token);
+  else
+    hipLaunchKernelGGL((sample_bins_kernel<E, 512>), dim3(grid_of(rows)), dim3(512), 0, stream, logits, rows, cols, ld, u, s, bits, token);
   return hipGetLastError();
 }
 
 template <class E>
 hipError_t launch_top_of(const E* logits, int64_t rows, int64_t cols, int64_t ld, int k, E* values, int64_t* index, float* lse, int num_cus,
                          hipStream_t stream) {
-  const dim3 grid(grid_of_top(rows, cols * (int64_t)sizeof(E), num_cus)), block(kTopThreads);
-  if (lse != nullptr) hipLaunchKernelGGL((top_kernel<E, true>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
-  else hipLaunchKernelGGL((top_kernel<E, false>), grid, block, 0, stream, logits, rows, cols, ld, k, values, index, lse);
+  const dim3 grid(rows <= num_cus ? (unsigned)rows : grid_of_top(rows, cols * (int64_t)sizeof(E), num_cus));
+#define LCE_TOP(LSE, NT) hipLaunchKernelGGL((top_kernel<E, LSE, NT>), grid, dim3(NT), 0, stream, logits, rows, cols, ld, k, values, index, lse)
+  if (rows <= num_cus && lse != nullptr) LCE_TOP(true, 1024);
+  else if (rows <= num_cus) LCE_TOP(false, 1024);
+  else if (lse != nullptr) LCE_TOP(true, 512);
+  else LCE_TOP(false, 512);
+#undef LCE_TOP
   return hipGetLastError();
 }
 

@@ -515,3 +515,19 @@ def test_rows_beyond_the_cache(dtype):
     check_top(z[:2].cpu(), 20)
     check_top(z[596:].cpu(), 20)
     assert torch.equal(top[1][596:].cpu(), ref_top(z[596:].cpu(), 20)[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_a_row_does_not_depend_on_the_others(dtype):
+    """Bit for bit the same values, columns and lse alone, among few and among many rows, by either way to do a row."""
+    from linear_cross_entropy_loss_amd import sample_logits, top_logits
+
+    for V in (777, 30011):
+        z, u = rows(700, V, dtype, seed=39).cuda(), torch.rand(700, generator=torch.Generator().manual_seed(40)).cuda()
+        many, token = top_logits(z, 30), sample_logits(z, u, 0.7, 0, 0.9)
+        for n in (1, 100):
+            few = top_logits(z[:n], 30)
+            assert all(torch.equal(a, b[:n]) for a, b in zip(few, many))
+            assert torch.equal(sample_logits(z[:n], u[:n], 0.7, 0, 0.9), token[:n])
+        assert torch.equal(top_logits(z, 700)[2], many[2])  # (by digits)
+        assert torch.equal(top_logits(z[:3], 700)[2], many[2][:3])
