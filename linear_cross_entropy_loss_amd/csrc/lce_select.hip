@@ -52,7 +52,7 @@ template <> struct bits_of<4> { typedef unsigned type; };
 // A row in units of up to 16 bytes: its elements before the first address of 16 bytes, whole pieces, the rest.  Wave w has the units
 // [w * share, (w + 1) * share), 64 neighbouring ones at a time, so that (wave, round, lane, element) is the order of the columns.
 template <class E, int NT, int FLIGHT = 4> struct RowUnits {
-  static constexpr int kPer = 16 / sizeof(E), kThreads = NT, kWaves = NT / 64;
+  static constexpr int kPer = 16 / sizeof(E);
   const E* p;
   int head, body, n, share, units;
   LCE_DEV RowUnits(const E* row, int64_t cols) : p(row), n((int)cols) {
@@ -64,7 +64,7 @@ template <class E, int NT, int FLIGHT = 4> struct RowUnits {
   }
   LCE_DEV int column(int unit) const { return unit == 0 ? 0 : head + (unit - 1) * kPer; }
   LCE_DEV int count(int unit) const {
-    return unit == 0 ? (int)head : unit <= body ? kPer : unit == body + 1 ? (int)(n - head - body * kPer) : 0;
+    return unit == 0 ? head : unit <= body ? kPer : unit == body + 1 ? n - head - body * kPer : 0;
   }
   LCE_DEV u32x4_t load(int unit) const {
     if (unit >= 1 && unit <= body) return *reinterpret_cast<const u32x4_t*>(p + column(unit));
@@ -214,7 +214,7 @@ template <> struct Ordered<_Float16> : OrderedHalf<_Float16> { static constexpr 
 template <class E, int NT> struct RowPieces {
   typedef Ordered<E> O;
   typedef typename bits_of<sizeof(E)>::type Bits;
-  static constexpr int kPer = 16 / sizeof(E), kFlight = 4, kThreads = NT;
+  static constexpr int kPer = 16 / sizeof(E), kFlight = 4;
   const E* p;
   int n, head, body;
   LCE_DEV RowPieces(const E* row, int64_t cols) : p(row), n((int)cols) {

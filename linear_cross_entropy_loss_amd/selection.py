@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import numbers
 
 import torch
 
@@ -36,7 +37,18 @@ def _(logits, k):
             logits.new_empty(shape, dtype=torch.float32))
 
 
+def _here(t):
+    """Whether t lies on the current device (whose calls the host extension, csrc/lce_host.cpp, takes)."""
+    return t.is_cuda and t.device.index == torch._C._cuda_getDevice()
+
+
 def _top_logits(logits, k):
+    if _here(logits):
+        done = _lib.host().top_logits(logits, k, _stream(logits.device))
+        if done is not None and len(done) == 2:
+            _lib.raise_for_status(*done)
+        if done is not None:
+            return done
     rows = _rows_of(logits, "top_logits")
     N, V = rows.shape
     shape, dev = logits.shape[:-1], rows.device
@@ -79,6 +91,8 @@ def _number_or_rows(value, name, shape, device, dtype, low, high, open_low=False
         if value.is_floating_point() != dtype.is_floating_point or value.is_complex():
             raise ValueError(f"sample_logits: {name} cannot be {value.dtype}")
         return 1, value.detach().to(dtype).expand(shape).contiguous()
+    if not isinstance(value, numbers.Real):
+        raise ValueError(f"sample_logits: {name} must be a number or a tensor, got {type(value).__name__}")
     number = float(value) if dtype.is_floating_point else int(value)
     if not (low < number if open_low else low <= number) or not (number <= high) or number == math.inf:
         raise ValueError(f"sample_logits: {name} = {value} is out of range")
@@ -97,6 +111,10 @@ def _(logits, u, temperature, top_k, top_p, min_p):
 
 
 def _sample_logits(logits, u, temperature, top_k, top_p, min_p):
+    if isinstance(u, torch.Tensor) and _here(logits):
+        tokens = _lib.host().sample_logits(logits, u, temperature, top_k, top_p, min_p, _stream(logits.device))
+        if tokens is not None:
+            return tokens
     rows = _rows_of(logits, "sample_logits")
     N, V = rows.shape
     shape, dev = logits.shape[:-1], rows.device

@@ -531,3 +531,36 @@ def test_a_row_does_not_depend_on_the_others(dtype):
             assert torch.equal(sample_logits(z[:n], u[:n], 0.7, 0, 0.9), token[:n])
         assert torch.equal(top_logits(z, 700)[2], many[2])  # (by digits)
         assert torch.equal(top_logits(z[:3], 700)[2], many[2][:3])
+
+
+def test_host_path_gives_the_same_and_knows_its_limits(monkeypatch):
+    """What the C++ host path takes gives what Python gives; what it does not take gets there by itself."""
+    from linear_cross_entropy_loss_amd import sample_logits, selection, top_logits
+
+    z = rows(12, 301, BF16, seed=41).cuda()
+    u = torch.rand(12, generator=torch.Generator().manual_seed(42)).cuda()
+    g = torch.Generator().manual_seed(43)
+    T, P = torch.rand(12, generator=g).cuda(), torch.rand(12, generator=g).cuda()
+    K = torch.randint(0, 40, (12,), generator=g).cuda()
+    wide = torch.zeros(12, 400, dtype=BF16, device="cuda")
+    wide[:, 50:351] = z
+    calls = [lambda: sample_logits(z, u), lambda: sample_logits(z, u, 0.7, 30, 0.9, 0.01), lambda: sample_logits(z, u, 1, 0, 1, 0),
+             lambda: sample_logits(z, u, T, K, P, 0.02), lambda: sample_logits(z, u, T[0], K.int(), P[3], 0), lambda: sample_logits(
+                 wide[:, 50:351], u, 0.9), lambda: sample_logits(z.reshape(3, 4, 301), u.reshape(3, 4), 0.9, K.reshape(3, 4)),
+             lambda: sample_logits(z.t().contiguous().t(), u), lambda: sample_logits(z[0], u[0]), lambda: sample_logits(z[::2], u[::2], T[::2]),
+             lambda: sample_logits(z.expand(2, 12, 301), u.expand(2, 12)), lambda: sample_logits(z[:, :1], u),
+             lambda: torch.cat([t.reshape(-1).float() for t in top_logits(z, 9)]),
+             lambda: torch.cat([t.reshape(-1).float() for t in top_logits(wide[:, 50:351], 9)]),
+             lambda: torch.cat([t.reshape(-1).float() for t in top_logits(z.reshape(2, 6, 301), 9)]),
+             lambda: torch.cat([t.reshape(-1).float() for t in top_logits(z[3], 2)])]
+    native = [call() for call in calls]
+    monkeypatch.setattr(selection, "_here", lambda t: False)
+    for call, a in zip(calls, native):
+        b = call()
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+    monkeypatch.undo()
+    values, index, lse = top_logits(z.requires_grad_(True).reshape(2, 6, 301), 4)
+    assert values.shape == index.shape == (2, 6, 4) and lse.shape == (2, 6) and values.dtype == BF16 and not values.requires_grad
+    for bad in ({"temperature": "1"}, {"top_k": 1 << 70}, {"top_k": None}):
+        with pytest.raises((ValueError, TypeError, OverflowError)):
+            sample_logits(z, u, **bad)
