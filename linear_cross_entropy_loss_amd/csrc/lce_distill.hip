@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void soft_logits_direct_kernel(const SoftLogit
   for (int64_t e = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); e < a.N * a.K; e += (int64_t)gridDim.x * 4) {
     const int v = a.index[e];
     float z = 0.f;
-    if (v >= 0) {
+    if (v >= 0 && v < a.V) {
       const XT* x = reinterpret_cast<const XT*>(a.x) + e / a.K * a.ldx;
       const WT* w = reinterpret_cast<const WT*>(a.w);
       for (int64_t h = lane; h < a.H; h += 64) {
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kSortThreads) void soft_count_kernel(const int* ind
   for (int i = 0; i < kSortPer; ++i) {
     const int64_t e = e0 + i * kSortThreads;
     const int v = e < M ? index[e] : -1;
-    if (v >= 0) atomicAdd(&sh_count[v / kGroupCols], 1);
+    if (v >= 0 && v / kGroupCols < groups) atomicAdd(&sh_count[v / kGroupCols], 1);
   }
   __syncthreads();
   for (int g = threadIdx.x; g < groups; g += kSortThreads)
@@ -257,6 +257,7 @@ __global__ __launch_bounds__(kSortThreads) void soft_place_kernel(const int* ind
   for (int i = 0; i < kSortPer; ++i) {
     const int64_t e = e0 + i * kSortThreads;
     v[i] = e < M ? index[e] : -1;
+    if (v[i] / kGroupCols >= groups) v[i] = -1;
     if (v[i] >= 0) rank[i] = atomicAdd(&sh_count[v[i] / kGroupCols], 1);
   }
   __syncthreads();

@@ -481,3 +481,29 @@ def test_as_many_column_groups_as_are_sorted(V):
     assert abs(loss.item() - ref.item()) <= 64 * 2.0 ** -22 * max(1.0, ref.item())
     assert rel_errors(x.grad, dz @ w.detach().double().t())[1] <= 1.5 * EPS[BF16]
     assert rel_errors(w.grad, x.detach().double().t() @ dz)[1] <= 1.5 * EPS[BF16]
+
+
+@pytest.mark.pack_auto
+@pytest.mark.parametrize("N,K", [(40, 6), (2048, 64)])
+def test_columns_beyond_the_weight_are_not_read(N, K):
+    """lce_distill given columns that lce_soft_targets would not give: they are left alone, by either way to the logits, and the labels
+    of those rows make the loss NaN; without them in the labels the other rows' gradients are what they are without such entries."""
+    from linear_cross_entropy_loss_amd import distillation, ops
+
+    H, V = 64, 1003
+    x, w, index, logits = (t.cuda() for t in make(N, H, V, K, BF16, seed=46))
+    x2, w2, layout = distillation._views(x, w)
+    columns, q, y = distillation._targets(index, logits, V, 1.0)
+    cfg = (1.0, 4096, ops._pack_mode(), ops._route_mode())
+    odd, q_odd = columns.clone(), q.clone()
+    odd[::3, 1] = torch.tensor([V, V + 63, V + 64, 2 ** 31 - 1], dtype=torch.int32, device="cuda").repeat(N)[: odd[::3].shape[0]]
+    plain, q_plain = columns.clone(), q.clone()
+    plain[::3, 1] = -1
+    q_odd[::3, 1] = q_plain[::3, 1] = 0.0
+    print(f"columns beyond N={N} K={K}", flush=True)
+    got = distillation._run(x2, w2, layout, (odd, q_odd, y), *cfg, True, True, None)
+    ref = distillation._run(x2, w2, layout, (plain, q_plain, y), *cfg, True, True, None)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref)) and torch.isfinite(got[0])
+    y = y.clone()
+    y[0] = V
+    assert distillation._run(x2, w2, layout, (odd, q_odd, y), *cfg, True, True, None)[0].isnan()
