@@ -462,7 +462,8 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
  * reads of a teacher.
  *
  * lce_sample: one token a row from the uniform number u[row] in [0, 1).  With w[j] = exp((z[j] - max z) / temperature), summed in 64
- * bits, in the order above:
+ * bits -- as whole multiples of 2^-b, b = min(50, 62 - ceil(log2 cols)), so that sums do not depend on their order and what is less than
+ * half of one counts as 0 --, in the order above:
  *   top_k   (0: all) keeps the first k
  *   top_p   (1: all) keeps column j while sum_{i<j} w[i] < top_p * the sum over what top_k kept
  *   min_p   (0: all) keeps the columns with w >= min_p

@@ -868,10 +868,12 @@ LCE_DEV void top_by_digits(const RowUnits<E, NT, FL>& row, int k, E* values, int
 // ---------------------------------------------------------------------------------------------------------------------------
 // The first k, k up to kMostByMaxima, without a histogram: of the largest element of each thread, the k-th is a lower bound of the k-th
 // of the row, and about k (1 + k / 2048) elements are not below it: these are listed and sorted.  Two passes over the row, one that
-// takes maxima, one that compares (and sums the exponentials for lse).  Rows whose list would be too long (most elements equal, or
-// fewer than k threads with one), with a NaN or an infinity on top are done by digits.
+// takes maxima, one that compares (and sums the exponentials for lse).  Where many of the maxima equal the bound -- all but a few
+// columns masked, or one value almost everywhere -- only what is larger is listed, and the first columns of that value are added.  Rows whose list
+// would be too long all the same, with a NaN or an infinity on top are done by digits.  (All but 10 columns masked, k = 32, us, here / by
+// digits: a row of 32000 bf16 11 / 72, 2048 of them 48 / 391; what the question costs other rows is half a microsecond.)
 // ---------------------------------------------------------------------------------------------------------------------------
-constexpr int kMostByMaxima = 512, kMostList = 2048, kMaxima = 1024;
+constexpr int kMostByMaxima = 512, kMostList = 2048, kMaxima = 1024, kMostTied = 256;
 // Digits: the shared memory of the rows that are done by digits.
 template <class Digits> struct TopShared {
   union {
@@ -890,6 +892,56 @@ template <class Digits> struct TopShared {
   unsigned top;
   int listed, drawn;
 };
+
+// Adds to the `listed` entries of the list those of the first elements, in the order of the columns, with ordered bits from `from` up to but not
+// with `above`, until there are k.  Returns how many there are.  A block's scan for each piece of a thread: the value is a frequent one.
+template <class E, int NT, class Shared>
+LCE_DEV int list_ties(const RowPieces<E, NT>& row, unsigned from, unsigned above, int listed, int k, Shared* sh) {
+  typedef Ordered<E> O;
+  typedef typename bits_of<sizeof(E)>::type Bits;
+  constexpr int kPer = RowPieces<E, NT>::kPer, kHalves = 4 / sizeof(E);
+  const int t = thread(), tail = row.n - row.head - row.body * kPer;
+  auto in = [&](unsigned a) { return a >= from && a < above; };
+  auto put = [&](int place, unsigned a, int column) {
+    if (place < k) sh->list[place] = entry_of(key_of(O::value(a)), column);
+  };
+  auto edge = [&](int first, int n) {
+    const unsigned w = O::word(reinterpret_cast<const Bits*>(row.p)[first + (t < n ? t : 0)]), a = sizeof(E) == 2 ? w & 0xffffu : w;
+    const bool is = t < n && in(a);
+    int before;
+    const int all = block_all<Sum, NT>(is ? 1 : 0, reinterpret_cast<int*>(sh->of_wave), &before);
+    if (is) put(listed + before, a, first + t);
+    listed += all;
+  };
+  if (row.head > 0) edge(0, row.head);
+#pragma unroll 1
+  for (int base = 0; base < row.body && listed < k; base += NT) {
+    const bool there = base + t < row.body;
+    const int piece = there ? base + t : 0;
+    u32x4_t v = reinterpret_cast<const u32x4_t*>(row.p + row.head)[piece];
+    int mine = 0;
+    auto each = [&](auto f) {
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const unsigned a = O::word(v[0]);
+        f(i * kHalves, sizeof(E) == 2 ? a & 0xffffu : a);
+        if (kHalves == 2) f(i * kHalves + 1, a >> 16);
+        v = u32x4_t{v[1], v[2], v[3], v[0]};
+      }
+    };
+    each([&](int, unsigned a) { mine += there && in(a) ? 1 : 0; });
+    int before;
+    const int all = block_all<Sum, NT>(mine, reinterpret_cast<int*>(sh->of_wave), &before);
+    int place = listed + before;
+    if (mine != 0 && place < k)
+      each([&](int i, unsigned a) {
+        if (in(a)) put(place++, a, row.head + piece * kPer + i);
+      });
+    listed += all;
+  }
+  if (tail > 0 && listed < k) edge(row.n - tail, tail);
+  return listed < k ? listed : k;
+}
 
 // The sorted list of a row's first elements, k of them and more; null if it could not be made.  sh->top: the ordered bits of the
 // largest element; sh->sums: by waves, sum exp(z - max) of the row (LSE).
@@ -942,16 +994,32 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
   }
   if (bound == 0x8000u) bound = 0x7fffu;  // (-0 is 0)
   const unsigned from = O::from_top_bits(bound);
+  // (the numbers that may equal it: of float32 those of the same upper half, which has to be found out)
+  const unsigned group = bound == 0x7fffu ? 0x8000u : bound, above = O::from_top_bits(group + 1);
+  int in_group = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxima / 64; ++i) in_group += __popcll(__ballot(of[i] >= bound && of[i] <= group));
+  const bool tied = in_group > kMostTied;
+  const unsigned limit = tied ? above : from;
+  unsigned tied_most = 0, tied_inverse = 0;  // float32: the largest key of those that may be equal, of the inverted keys
+  auto tie = [&](unsigned a) {
+    if (sizeof(E) == 4 && tied && a >= from && a < above) {
+      const unsigned key = key_of(O::value(a));
+      tied_most = key > tied_most ? key : tied_most;
+      tied_inverse = ~key > tied_inverse ? ~key : tied_inverse;
+    }
+  };
   const float m = O::value(top);
   ExpSum<E, NT> sum(m);
   auto add = [&](int at, unsigned a) {
-    if (a >= from) {
+    if (a >= limit) {
       const int to = atomicAdd(&sh->listed, 1);
       if (to < kMostList) sh->list[to] = entry_of(key_of(O::value(a)), at);
     }
   };
   row.edges([&](int at, unsigned a) {
     add(at, a);
+    tie(a);
     if (LSE) sum.template edge<true>(O::value(a));
   });
   row.each([&](int at, u32x4_t v, int r) {
@@ -962,7 +1030,11 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
       a[i] = O::word(v[i]);
       best = O::larger(best, a[i]);
     }
-    if (O::largest(best) >= from) {
+    if (sizeof(E) == 4 && tied) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tie(a[i]);
+    }
+    if (O::largest(best) >= limit) {
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
         if (sizeof(E) == 2) {
@@ -979,8 +1051,17 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
   if (LSE) sum.store(sh->sums);
   if (t == 0) sh->top = top;
   __syncthreads();
-  const int listed = sh->listed;
-  if (listed > kMostList) {
+  int listed = sh->listed;
+  bool fits = listed <= kMostList;
+  if (fits && tied && listed < k) {
+    if (sizeof(E) == 4) {
+      tied_most = block_all<Largest, NT>(tied_most, reinterpret_cast<unsigned*>(sh->of_wave));
+      tied_inverse = block_all<Largest, NT>(tied_inverse, reinterpret_cast<unsigned*>(sh->of_wave));
+      fits = tied_most == ~tied_inverse;
+    }
+    if (fits) listed = list_ties<E, NT>(row, from, above, listed, k, sh);
+  }
+  if (!fits) {
     __syncthreads();  // (the caller may use the place of it all)
     return nullptr;
   }

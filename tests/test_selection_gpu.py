@@ -564,3 +564,25 @@ def test_host_path_gives_the_same_and_knows_its_limits(monkeypatch):
     for bad in ({"temperature": "1"}, {"top_k": 1 << 70}, {"top_k": None}):
         with pytest.raises((ValueError, TypeError, OverflowError)):
             sample_logits(z, u, **bad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("N,V,offset", [(3, 9001, 0), (3, 9001, 3), (300, 5003, 1), (2, 40000, 5)])
+def test_fewer_large_columns_than_are_asked_for(N, V, offset, dtype):
+    """Rows of which the first k reach into columns that are all equal: masked but for a few, constant, zeros of either sign, and -- float32 --
+    numbers that differ in their last places alone."""
+    base = rows(N, V, dtype, seed=44)
+    few = torch.rand(N, V, generator=torch.Generator().manual_seed(45)) < 12 / V
+    u = torch.rand(N, generator=torch.Generator().manual_seed(46))
+    signs = torch.where(torch.rand(N, V, generator=torch.Generator().manual_seed(47)) < 0.5, 0.0, -0.0).to(dtype)
+    close = (1.0 + torch.arange(V) % 7 * 2.0 ** -20).to(dtype).expand(N, V)
+    for floor in (-math.inf, torch.finfo(dtype).min, -1e4, 0.0, 1.5, signs, close):
+        z = torch.where(few, base, torch.as_tensor(floor).to(dtype))
+        buffer = torch.full((N, V + 11), 7.0, dtype=dtype, device="cuda")
+        zg = buffer[:, offset:offset + V]
+        zg.copy_(z.cuda())
+        for k in (1, 5, 32, 512):
+            check_top(z, k, zg)
+            check_sample(z, u, zg, top_k=k)
+        check_sample(z, u, zg, top_k=50, temperature=2.0, top_p=0.9)
+        check_sample(z, u, zg, top_k=torch.full((N,), 40), temperature=0.5, min_p=0.01)
