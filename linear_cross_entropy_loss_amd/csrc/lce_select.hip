@@ -1245,8 +1245,11 @@ template <class E, int NT> struct RowBins {
     __syncthreads();
     const Place bin = sh->place;
     const int b = sh->bin;
-    // values between which all of its elements are: the bin's ends, each further out by more than the roundings of either direction
-    const double low_z = weights.top - (double)(b + 1) / (kBinsPerOctave * weights.per), high_z = weights.top - (double)b / (kBinsPerOctave * weights.per);
+    // values between which all of its elements are: the bin's ends, each further out by more than the roundings of either direction -- some
+    // 2^-52 of the distance to the top, whose share is large next to 0, and of the top itself, and those to float32
+    const double low_off = (double)(b + 1) / (kBinsPerOctave * weights.per), high_off = (double)b / (kBinsPerOctave * weights.per);
+    const double eps = 1.0 / (1ull << 49), some = fabs(weights.top) * eps;
+    const double low_z = weights.top - low_off - (low_off * eps + some), high_z = weights.top - high_off + (high_off * eps + some);
     const unsigned low_key = key_of((float)low_z), high_key = key_of((float)high_z);
     const float low = uniform(value_of(low_key < kLowKey + 4 ? kLowKey + 1 : low_key - 2));
     const float high = uniform(value_of(high_key < top - 2 ? high_key + 2 : top));
