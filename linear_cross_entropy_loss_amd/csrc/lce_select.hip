@@ -437,16 +437,16 @@ LCE_DEV double exp2_poly(double t) {
 struct Weights {
   double top, per;  // the largest value, log2(e) / temperature
   double one;       // 2^bits, bits <= 50
-  double least;     // -bits - 1 + 2^-10
+  double least;     // -bits - 1 - 2^-10
   LCE_DEV double log2_of(float z) const {
     // (equal infinities have no difference, and one times 0, at an infinite temperature, is no number)
     const double zd = (double)z;
     return zd == top ? 0.0 : fmax((zd - top) * per, -2000.0);
   }
-  // The same for a finite top, without a bound below; and whether such an element is taken to have a weight at all: one above half a
-  // place rounds to one or more.
+  // The same for a finite top, without a bound below; and whether such an element can have a weight at all: one above half a place
+  // rounds to one, and what is below by more than the series may be off is left out without a look at it.
   LCE_DEV double log2_below(float z) const { return ((double)z - top) * per; }
-  LCE_DEV bool has_weight(double log2) const { return log2 >= least; }
+  LCE_DEV bool may_weigh(double log2) const { return log2 >= least; }
   LCE_DEV double real(float z) const { return exp2_poly(log2_of(z)); }
   // (rounded by the sum with 2^52, whose last place is 1)
   LCE_DEV u64 fixed(double w) const { return __builtin_bit_cast(u64, fma(w, one, 4503599627370496.0)) & 0xfffffffffffffull; }
@@ -616,7 +616,7 @@ struct RowSettings {
   }
   LCE_DEV bool greedy() const { return !(temperature > 0.f) || top_k == 1; }
   LCE_DEV Weights weights(float top) const {
-    return {uniform((double)top), uniform(1.4426950408889634074 / (double)temperature), (double)((u64)1 << bits), -1023.0 / 1024.0 - bits};
+    return {uniform((double)top), uniform(1.4426950408889634074 / (double)temperature), (double)((u64)1 << bits), -1025.0 / 1024.0 - bits};
   }
 };
 
@@ -1154,8 +1154,8 @@ constexpr int kSelectThreads = 1024;
 // which the histogram takes half, a place 25, the maximum, from memory, 15.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kBins = 4096;
-constexpr double kBinsPerOctave = 80.0;  // 51 octaves: a weight of 2^-51 rounds to 0 with 50 places
-static_assert(51 * 80 < kBins);
+constexpr double kBinsPerOctave = 80.0;  // 51 octaves and 2^-10: a weight of 2^-51 rounds to 0 with 50 places
+static_assert(51 * 80 + 1 < kBins);
 struct BinShared {
   union {
     struct {
@@ -1180,7 +1180,7 @@ template <class E, int NT> struct RowBins {
   BinShared* sh;
 
   LCE_DEV static int bin_of(double log2_weight) {
-    return (int)(log2_weight * -kBinsPerOctave);  // (< 51 * 80)
+    return (int)(log2_weight * -kBinsPerOctave);  // (<= 51 * 80)
   }
   // The histogram (of weights, and of counts if they are `counted`); the weight that min_p keeps.
   LCE_DEV u64 fill(double min_p, bool counted) const {
@@ -1192,12 +1192,12 @@ template <class E, int NT> struct RowBins {
     u64 mine = 0;
     auto one = [&](float z) {
       const double t = weights.log2_below(z);
-      if (!weights.has_weight(t)) return;
+      if (!weights.may_weigh(t)) return;
       const double real = exp2_poly(t);
       const u64 w = weights.fixed(real);
       const int b = bin_of(t);
       atomicAdd(&sh->weight[b], w);
-      if (counted) atomicAdd(&sh->count[b], 1);
+      if (counted) atomicAdd(&sh->count[b], w != 0 ? 1 : 0);
       if (min_p > 0.0) {
         asm volatile("");  // (a branch)
         if (real >= min_p) mine += w;
@@ -1257,7 +1257,7 @@ template <class E, int NT> struct RowBins {
     auto one = [&](int at, float z) {
       if (!(z >= low && z <= high)) return;
       const double log2 = weights.log2_below(z);
-      if (!weights.has_weight(log2) || bin_of(log2) != b) return;
+      if (!weights.may_weigh(log2) || bin_of(log2) != b) return;  // (some without a weight do no harm: they come last)
       const unsigned key = key_of(z);
       const int to = atomicAdd(&sh->listed, 1);
       if (to < kMostList) sh->list[to] = entry_of(key, at);

@@ -1,8 +1,10 @@
-"""Sampling where a border decides: a bin's border next to zero."""
+"""Sampling where a border decides: a bin's border next to zero, weights next to half a place."""
+import math
+
 import pytest
 import torch
 
-from test_selection_gpu import check_sample
+from test_selection_gpu import BF16, F16, F32, check_sample
 
 pytestmark = [pytest.mark.gpu, pytest.mark.pack_auto]
 
@@ -28,3 +30,32 @@ def test_a_bin_border_at_zero(top, temperature, N):
         for settings in ({}, {"top_p": 0.75}, {"top_k": 3001}, {"top_k": 6001, "top_p": 0.9}, {"min_p": 0.25}):
             check_sample(z[row:row + 1].expand(N, V), u[row:row + 1].expand(N), z[row:row + 1].cuda().expand(N, V), temperature=temperature,
                          **settings)
+
+
+def fixed_point_token(z, u, temperature):
+    """The definition with weights as whole multiples of 2^-b, b = min(50, 62 - ceil(log2 V)), in exact sums; one row, no filter."""
+    bits = min(50, 62 - math.ceil(math.log2(z.numel())))
+    order = torch.sort(z.double(), descending=True, stable=True)
+    w = torch.round(torch.exp((order.values - order.values[0]) / temperature) * 2.0 ** bits).long()
+    upto = torch.cumsum(w, 0)
+    target = min(int(u * float(upto[-1])), int(upto[-1]) - 1)
+    return order.indices[(upto > target).to(torch.uint8).argmax()].item()
+
+
+@pytest.mark.parametrize("N", [1, 300])
+@pytest.mark.parametrize("dtype,V,u", [(F32, 1 << 20, 1 - 2.0 ** -24), (F32, 5000, 1.0), (BF16, 5000, 1.0), (F16, 12000, 1.0), (BF16, 20000, 1.0),
+                                       (F16, 40000, 1.0)])
+def test_weights_next_to_half_a_place(dtype, V, u, N):
+    """What is above half a place counts as one, what is below as none, whichever way a row is done.  (u = 1 takes the last column with
+    a weight; a million columns of half a place are 2^-22 of the whole, which a number below 1 reaches.)"""
+    from linear_cross_entropy_loss_amd import sample_logits
+
+    bits = min(50, 62 - math.ceil(math.log2(V)))
+    # weights of the others by their logarithm: -(bits + 1) and 2^-11 more or less, 3e-4 of half a place
+    for more in (2.0 ** -11, -(2.0 ** -11)):
+        temperature = torch.tensor(64.0 * 1.4426950408889634 / (bits + 1 - more)).item()
+        z = torch.full((V,), -64.0).to(dtype)
+        z[V // 3] = 0.0
+        got = sample_logits(z.cuda().expand(N, V), torch.full((N,), u, device="cuda"), temperature=temperature).cpu()
+        print(f"{dtype} V={V} N={N} {more}: {got[0].item()}", flush=True)
+        assert torch.equal(got, torch.full((N,), fixed_point_token(z, u, temperature)))
