@@ -171,6 +171,10 @@ def load():
     return lib
 
 
+# Numbers that the library takes as float32: the largest that rounds to 0 there and the smallest that rounds to infinity.  (Comparisons, which
+# torch.compile traces, in the place of a conversion, which it does not.)
+F32_ZERO, F32_INF = 2.0 ** -150, 2.0 ** 128 - 2.0 ** 103
+
 _host = None
 
 

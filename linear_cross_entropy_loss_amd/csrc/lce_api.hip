@@ -1561,7 +1561,7 @@ int lce_soft_targets(int64_t N, int64_t K, int64_t V, const int64_t* index, int6
   if (rc != LCE_OK) return rc;
   if (logits_dtype != LCE_BF16 && logits_dtype != LCE_F16 && logits_dtype != LCE_F32) return LCE_EINVAL_DTYPE;
   if (!index || !logits || !out_index || !out_q || !y || ld_index < 0 || ld_logits < 0) return LCE_EINVAL_ARG;
-  if (!(temperature > 0.f) || temperature > 3.4e38f) return LCE_EINVAL_ARG;
+  if (!(temperature > 0.f && temperature < INFINITY)) return LCE_EINVAL_ARG;
   const hipError_t e = lce::launch_soft_targets(index, ld_index, logits, logits_dtype, ld_logits, N, (int)K, V, temperature, out_index, out_q,
                                                 y, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "soft_targets");
@@ -1572,7 +1572,7 @@ int lce_distill_workspace_bytes(const lce_problem* p, int64_t K, int32_t grads, 
   int rc = check(p, grads != 0);
   if (rc == LCE_OK) rc = check_targets(p->N, K);
   if (rc != LCE_OK) return rc;
-  if (!bytes || p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale <= 3.4e38f)) return LCE_EINVAL_ARG;
+  if (!bytes || p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale < INFINITY)) return LCE_EINVAL_ARG;
   const lce_problem q = soft_problem(p);
   DistillPlan d;
   rc = plan_distill(&q, K, grads != 0, &d);
@@ -1589,7 +1589,7 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
   if (rc != LCE_OK) return rc;
   if (!x || !w || !y || !index || !q || !lse || !loss || !n_valid || (grads && !grad_out)) return LCE_EINVAL_ARG;
   if (misaligned(x) || misaligned(w) || misaligned(dx) || misaligned(dw)) return LCE_EINVAL_ARG;
-  if (p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale <= 3.4e38f)) return LCE_EINVAL_ARG;
+  if (p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale < INFINITY)) return LCE_EINVAL_ARG;
   const lce_problem soft_p = soft_problem(p);
   DistillPlan d;
   rc = plan_distill(&soft_p, K, grads, &d);
@@ -1655,7 +1655,7 @@ int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_
   if (rc != LCE_OK) return rc;
   if (!s) return LCE_EINVAL_ARG;
   // (numbers that are not there for each row are checked; those that are, lce.h says what they stand for)
-  if (!s->temperature_rows && !(s->temperature >= 0.f && s->temperature <= 3.4e38f)) return LCE_EINVAL_ARG;
+  if (!s->temperature_rows && !(s->temperature >= 0.f && s->temperature < INFINITY)) return LCE_EINVAL_ARG;
   if (!s->top_p_rows && !(s->top_p > 0.f && s->top_p <= 1.f)) return LCE_EINVAL_ARG;
   if (!s->min_p_rows && !(s->min_p >= 0.f && s->min_p <= 1.f)) return LCE_EINVAL_ARG;
   if (!s->top_k_rows && s->top_k < 0) return LCE_EINVAL_ARG;

@@ -39,10 +39,12 @@ def _check_inputs(x, At, index, logits):
 
 
 def _check_numbers(temperature, logit_scale):
-    if not (0.0 < temperature < math.inf):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not (_lib.F32_ZERO < temperature < _lib.F32_INF):
+        raise ValueError(f"temperature must be positive and finite in float32, got {temperature}")
     if not (0.0 < logit_scale < math.inf):
         raise ValueError(f"logit_scale must be positive and finite, got {logit_scale}")
+    if not (_lib.F32_ZERO < logit_scale / temperature < _lib.F32_INF):
+        raise ValueError(f"logit_scale / temperature must be positive and finite in float32, got {logit_scale} / {temperature}")
 
 
 def _rows_of(t):

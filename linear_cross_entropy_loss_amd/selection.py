@@ -6,7 +6,6 @@ Both go by one order of a row: value descending, equal values by column.  Neithe
 from __future__ import annotations
 
 import ctypes
-import math
 import numbers
 
 import torch
@@ -81,7 +80,23 @@ def top_logits(logits, k: int):
     return _top_logits(logits, k)
 
 
-def _number_or_rows(value, name, shape, device, dtype, low, high, open_low=False):
+# What a setting may be once it has been rounded to float32 (top_k: a whole number): as the definition and lce.h have it.
+_FINE = {
+    "temperature": lambda v: -_lib.F32_ZERO <= v < _lib.F32_INF,
+    "top_k": lambda v: 0 <= v < 2 ** 63 and v == int(v),
+    "top_p": lambda v: _lib.F32_ZERO < v <= 1.0 + 2.0 ** -24,
+    "min_p": lambda v: -_lib.F32_ZERO <= v <= 1.0 + 2.0 ** -24,
+}
+
+
+def _check_number(value, name):
+    if not (isinstance(value, (int, float)) or isinstance(value, numbers.Real)):
+        raise ValueError(f"sample_logits: {name} must be a number or a tensor, got {type(value).__name__}")
+    if not _FINE[name](value):
+        raise ValueError(f"sample_logits: {name} = {value} is out of range")
+
+
+def _number_or_rows(value, name, shape, device, dtype):
     """(number, None), or (a number that is not looked at, a tensor with one entry a row)."""
     if isinstance(value, torch.Tensor):
         if value.device != device:
@@ -91,12 +106,7 @@ def _number_or_rows(value, name, shape, device, dtype, low, high, open_low=False
         if value.is_floating_point() != dtype.is_floating_point or value.is_complex():
             raise ValueError(f"sample_logits: {name} cannot be {value.dtype}")
         return 1, value.detach().to(dtype).expand(shape).contiguous()
-    if not isinstance(value, numbers.Real):
-        raise ValueError(f"sample_logits: {name} must be a number or a tensor, got {type(value).__name__}")
-    number = float(value) if dtype.is_floating_point else int(value)
-    if not (low < number if open_low else low <= number) or not (number <= high) or number == math.inf:
-        raise ValueError(f"sample_logits: {name} = {value} is out of range")
-    return number, None
+    return float(value) if dtype.is_floating_point else int(value), None
 
 
 @torch.library.custom_op("lce_amd::sample_logits", mutates_args=(), device_types="cuda")
@@ -115,16 +125,19 @@ def _sample_logits(logits, u, temperature, top_k, top_p, min_p):
         tokens = _lib.host().sample_logits(logits, u, temperature, top_k, top_p, min_p, _stream(logits.device))
         if tokens is not None:
             return tokens
+    for value, name in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p")):
+        if not isinstance(value, torch.Tensor):
+            _check_number(value, name)
     rows = _rows_of(logits, "sample_logits")
     N, V = rows.shape
     shape, dev = logits.shape[:-1], rows.device
     if not isinstance(u, torch.Tensor) or u.dtype != torch.float32 or u.shape != shape or u.device != dev:
         raise ValueError("sample_logits: u must be a float32 tensor with one number for each row, on the logits' device")
     u = u.detach().contiguous()
-    t, t_rows = _number_or_rows(temperature, "temperature", shape, dev, torch.float32, 0.0, math.inf)
-    k, k_rows = _number_or_rows(top_k, "top_k", shape, dev, torch.int64, 0, 2 ** 63 - 1)
-    p, p_rows = _number_or_rows(top_p, "top_p", shape, dev, torch.float32, 0.0, 1.0, open_low=True)
-    m, m_rows = _number_or_rows(min_p, "min_p", shape, dev, torch.float32, 0.0, 1.0)
+    t, t_rows = _number_or_rows(temperature, "temperature", shape, dev, torch.float32)
+    k, k_rows = _number_or_rows(top_k, "top_k", shape, dev, torch.int64)
+    p, p_rows = _number_or_rows(top_p, "top_p", shape, dev, torch.float32)
+    m, m_rows = _number_or_rows(min_p, "min_p", shape, dev, torch.float32)
     s = _lib.LceSampling(t, p, m, k, _ptr(t_rows), _ptr(p_rows), _ptr(m_rows), _ptr(k_rows))
     tokens = torch.empty(shape, dtype=torch.int64, device=dev)
     with _on_device(dev):
@@ -148,8 +161,9 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         temperature: positive, or 0 for the first column of the order (the largest logit).
         top_k: 0 keeps all.  top_p: 1 keeps all.  min_p: 0 keeps all.
 
-    Each setting is a number, or a tensor (...) on the logits' device with one for every row (in which, without a check, top_k <= 0,
-    top_p >= 1 and min_p <= 0 keep all, top_p <= 0 and min_p > 1 keep one column and a temperature that is not positive stands for 0).
+    Each setting is a number (rounded to float32; a whole one for top_k), or a tensor (...) on the logits' device with one for every row
+    (in which, without a check, top_k <= 0, top_p >= 1 and min_p <= 0 keep all, top_p <= 0 and min_p > 1 keep one column and a temperature
+    that is not positive stands for 0).
     Returns torch.long tokens (...); -1 for a row that is masked altogether or has a NaN.
     """
     if torch.compiler.is_compiling():
