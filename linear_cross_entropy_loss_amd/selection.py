@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import numbers
+from typing import Optional
 
 import torch
 
@@ -89,11 +90,14 @@ _FINE = {
 }
 
 
-def _check_number(value, name):
-    if not (isinstance(value, (int, float)) or isinstance(value, numbers.Real)):
-        raise ValueError(f"sample_logits: {name} must be a number or a tensor, got {type(value).__name__}")
-    if not _FINE[name](value):
-        raise ValueError(f"sample_logits: {name} = {value} is out of range")
+def _check_numbers(temperature, top_k, top_p, min_p):
+    for value, name in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p")):
+        if isinstance(value, torch.Tensor):
+            continue
+        if not (isinstance(value, (int, float)) or isinstance(value, numbers.Real)):
+            raise ValueError(f"sample_logits: {name} must be a number or a tensor, got {type(value).__name__}")
+        if not _FINE[name](value):
+            raise ValueError(f"sample_logits: {name} = {value} is out of range")
 
 
 def _number_or_rows(value, name, shape, device, dtype):
@@ -109,14 +113,18 @@ def _number_or_rows(value, name, shape, device, dtype):
     return float(value) if dtype.is_floating_point else int(value), None
 
 
+# (A tensor in the place of a number: settings by row.  What is a number stays one, so that the library chooses its kernel by it.)
 @torch.library.custom_op("lce_amd::sample_logits", mutates_args=(), device_types="cuda")
-def _op_sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor,
-                      min_p: torch.Tensor) -> torch.Tensor:
-    return _sample_logits(logits, u, temperature, top_k, top_p, min_p)
+def _op_sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature_rows: Optional[torch.Tensor] = None,
+                      top_k_rows: Optional[torch.Tensor] = None, top_p_rows: Optional[torch.Tensor] = None,
+                      min_p_rows: Optional[torch.Tensor] = None, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                      min_p: float = 0.0) -> torch.Tensor:
+    return _sample_logits(logits, u, temperature if temperature_rows is None else temperature_rows, top_k if top_k_rows is None else top_k_rows,
+                          top_p if top_p_rows is None else top_p_rows, min_p if min_p_rows is None else min_p_rows)
 
 
 @_op_sample_logits.register_fake
-def _(logits, u, temperature, top_k, top_p, min_p):
+def _(logits, u, temperature_rows=None, top_k_rows=None, top_p_rows=None, min_p_rows=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return logits.new_empty(logits.shape[:-1], dtype=torch.int64)
 
 
@@ -125,9 +133,7 @@ def _sample_logits(logits, u, temperature, top_k, top_p, min_p):
         tokens = _lib.host().sample_logits(logits, u, temperature, top_k, top_p, min_p, _stream(logits.device))
         if tokens is not None:
             return tokens
-    for value, name in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p")):
-        if not isinstance(value, torch.Tensor):
-            _check_number(value, name)
+    _check_numbers(temperature, top_k, top_p, min_p)
     rows = _rows_of(logits, "sample_logits")
     N, V = rows.shape
     shape, dev = logits.shape[:-1], rows.device
@@ -167,9 +173,9 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     Returns torch.long tokens (...); -1 for a row that is masked altogether or has a NaN.
     """
     if torch.compiler.is_compiling():
-        def tensor(v, dtype):
-            return v if isinstance(v, torch.Tensor) else torch.full((), v, dtype=dtype, device=logits.device)
-
-        return _op_sample_logits(logits.detach(), u, tensor(temperature, torch.float32), tensor(top_k, torch.int64),
-                                 tensor(top_p, torch.float32), tensor(min_p, torch.float32))
+        _check_numbers(temperature, top_k, top_p, min_p)
+        settings = (temperature, top_k, top_p, min_p)
+        rows = [v.detach() if isinstance(v, torch.Tensor) else None for v in settings]
+        t, k, p, m = (default if isinstance(v, torch.Tensor) else v for v, default in zip(settings, (1.0, 0, 1.0, 0.0)))
+        return _op_sample_logits(logits.detach(), u, *rows, float(t), int(k), float(p), float(m))
     return _sample_logits(logits, u, temperature, top_k, top_p, min_p)
