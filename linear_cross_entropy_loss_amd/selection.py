@@ -67,15 +67,15 @@ def top_logits(logits, k: int):
 
     Args:
         logits: (..., V) bfloat16, float16 or float32, any row stride.
-        k: 1 <= k <= min(V, 1024).
+        k: a whole number, 1 <= k <= min(V, 1024).
 
     Returns ``(values, index, lse)``: (..., k) in the logits' type, (..., k) torch.long and (...) float32.  Equal logits come by
     column, NaN before all; ``values - lse[..., None]`` are log-probabilities.  ``index`` and ``values`` are what
     ``linear_distillation`` takes; a column of -inf (masked) that gets among the k is no target there.
     """
-    k = int(k)
-    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], _lib.MAX_TARGETS):
+    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], _lib.MAX_TARGETS) or k != int(k):
         raise ValueError(f"top_logits: k must be in 1 ... min(V, {_lib.MAX_TARGETS}), got {k} for logits of shape {tuple(logits.shape)}")
+    k = int(k)
     if torch.compiler.is_compiling():
         return _op_top_logits(logits.detach(), k)
     return _top_logits(logits, k)

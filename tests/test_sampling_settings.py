@@ -1,11 +1,11 @@
-"""Settings of sample_logits and numbers of linear_distillation: which are refused, eager and compiled, and that numbers reach the library as
-numbers."""
+"""Settings of sample_logits, numbers of top_logits and linear_distillation: which are refused, eager and compiled, and that numbers
+reach the library as numbers."""
 import math
 
 import pytest
 import torch
 
-from linear_cross_entropy_loss_amd import sample_logits, selection
+from linear_cross_entropy_loss_amd import sample_logits, selection, top_logits
 
 BAD = [{"temperature": -1.0}, {"temperature": math.nan}, {"temperature": math.inf}, {"top_p": 0.0}, {"top_p": 1.5}, {"top_p": math.nan},
        {"min_p": -0.1}, {"min_p": 2.0}, {"min_p": math.nan}, {"top_k": -3}, {"top_k": 1 << 70}]
@@ -18,6 +18,14 @@ BAD_ROUNDED = [{"temperature": 1e39}, {"top_p": 1e-50}, {"top_p": 1.0 + 1e-7}, {
 def test_refused_by_name_before_all_else(settings):
     with pytest.raises(ValueError, match=next(iter(settings))):
         sample_logits(torch.zeros(4, 50), torch.zeros(4), **settings)
+
+
+@pytest.mark.parametrize("k", [0, 0.5, 2.7, 51, 1e30, math.nan, math.inf])
+def test_top_logits_takes_whole_numbers(k):
+    with pytest.raises(ValueError, match="k must be in 1"):
+        top_logits(torch.zeros(4, 50), k)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        top_logits(torch.zeros(4, 50), 7.0)
 
 
 # (numbers that float32 rounds to one that is fine)
