@@ -442,7 +442,9 @@ int lce_transpose_rows(const void* src, int dtype, int64_t rows, int64_t cols, i
  *   lse        out, N floats, as in lce_forward
  *   loss       out, 1 float;  n_valid  out, 1 int64: R
  *   dx, dw     out, either may be NULL
- *   ws         lce_distill_workspace_bytes(p, K, dx or dw wanted) bytes: those of the loss and 4 bytes per entry
+ *   ws         lce_distill_workspace_bytes(p, K, dx or dw wanted) bytes: those of the loss -- lce_forward's, or with a gradient
+ *              lce_forward_backward's (of a backward that stages dz, for hidden sizes up to 128 too) --, or up to 16 MiB where the
+ *              loss takes less and the entries' sort more (it goes by stretches of rows that fit), and 4 bytes per entry
  */
 #define LCE_MAX_TARGETS 1024
 int lce_soft_targets(int64_t N, int64_t K, int64_t V, const int64_t* index, int64_t ld_index, const void* logits, int logits_dtype,

@@ -1284,7 +1284,7 @@ struct DistillPlan {
   bool grads, one_pass;
   FusedPlan f;
   BwdPlan b;
-  size_t out5, part, z, total;
+  size_t loss, out5, part, z, total;  // loss: the scratch of the loss itself
   bool picks() const { return one_pass && f.kept; }
 };
 
@@ -1316,7 +1316,8 @@ int plan_distill(const lce_problem* q, int64_t K, bool grads, DistillPlan* d) {
     }
   }
   // (the scratch of the targets' logits is free again before the loss's kernels run; where the stage keeps the logits they are read there)
-  const size_t sorting = d->picks() ? 0 : lce::soft_logits_bytes(q->N, (int)K, q->H, q->V, q->w_layout == LCE_W_VH);
+  d->loss = o;
+  const size_t sorting = d->picks() ? 0 : lce::soft_logits_bytes(q->N, (int)K, q->H, q->V, q->w_layout == LCE_W_VH, d->loss);
   if (sorting > o) o = sorting;
   o = align_up(o);
   d->out5 = o; o += 256;
@@ -1605,7 +1606,7 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
   g.x = x; g.w = w; g.N = p->N; g.H = p->H; g.V = p->V; g.ldx = p->ldx; g.ldw = p->ldw;
   g.x_dtype = p->x_dtype; g.w_dtype = p->w_dtype; g.w_vh = p->w_layout == LCE_W_VH; g.K = (int)K;
   g.index = index; g.scale = p->logit_scale; g.z = z;
-  hipError_t e = d.picks() ? hipSuccess : lce::launch_soft_logits(g, base, s);
+  hipError_t e = d.picks() ? hipSuccess : lce::launch_soft_logits(g, base, d.loss, s);
   if (e != hipSuccess) return hip_fail(e, "soft_logits");
 
   lce::SoftTargets t;

@@ -493,32 +493,51 @@ __global__ __launch_bounds__(64) void soft_loss_sum_kernel(const double* part, i
   if (threadIdx.x == 0) loss[0] = (float)(sum / (double)n_valid[0]);
 }
 
-// Scratch of the sorted kernels, after `base`: counts, number of items, items, entries.
+// Scratch of the sorted kernels, after `base`: counts, number of items, items, entries -- of as many rows at a time as the scratch has room
+// for, some 8.1 bytes an entry: memory that does not grow with N K.  (kSortScratch holds 2 million.  Loss alone, ms, by stretches / all at
+// once: N=65536, H=64, V=4096, K=256, 9 of them, 1.61 / 1.58; N=16384, H=512, V=32000, 3, 1.32 / 1.28; N=8192, H=2048, K=512 3.25 / 3.21.)
 struct SortPlan {
   bool sorted;
   int groups;
-  int64_t most_items;
+  int64_t rows, most_items;  // of a stretch
   size_t num_items, items, entries, total;
 };
-SortPlan plan_sort(int64_t N, int K, int64_t H, int64_t V, bool w_vh) {
+SortPlan plan_sort(int64_t N, int K, int64_t H, int64_t V, bool w_vh, size_t room) {
   SortPlan p;
-  const int64_t M = N * K, groups = (V + kGroupCols - 1) / kGroupCols;
+  const int64_t groups = (V + kGroupCols - 1) / kGroupCols;
   auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
-  p.sorted = sorts_entries(M, H, w_vh) && groups <= kMostColGroups;
+  p.sorted = sorts_entries(N * K, H, w_vh) && groups <= kMostColGroups;
   p.groups = (int)(groups <= kMostColGroups ? groups : 0);
-  p.most_items = groups + M / kItemEntries;
   p.num_items = up((size_t)p.groups * 4);
   p.items = p.num_items + 256;
-  p.entries = p.items + up((size_t)p.most_items * sizeof(int4));
-  p.total = p.sorted ? p.entries + up((size_t)M * sizeof(int2)) : 0;
+  auto stretch = [&](int64_t rows) {
+    p.rows = rows;
+    p.most_items = groups + rows * K / kItemEntries;
+    p.entries = p.items + up((size_t)p.most_items * sizeof(int4));
+    return p.entries + up((size_t)(rows * K) * sizeof(int2));
+  };
+  p.total = stretch(N);
+  if (room < kSortScratch) room = kSortScratch;
+  if (p.sorted && p.total > room) {
+    int64_t lo = 1, hi = N;  // (`lo` rows fit)
+    while (hi - lo > 1) {
+      const int64_t mid = lo + (hi - lo) / 2;
+      (stretch(mid) <= room ? lo : hi) = mid;
+    }
+    stretch(lo);
+    p.total = room;
+  }
+  if (!p.sorted) p.total = 0;
   return p;
 }
+// A row's entries, the groups' counts and their items fit, so that every plan has a row at least.
+static_assert(kMostColGroups * 4 + 256 + (kMostColGroups + kMaxTargets) * 16 + 256 + kMaxTargets * 8 + 256 <= kSortScratch);
 
-template <class XT, class WT, bool WVH> hipError_t launch_logits(const SoftLogits& a, void* ws, hipStream_t s) {
-  const SortPlan p = plan_sort(a.N, a.K, a.H, a.V, a.w_vh != 0);
-  const int64_t M = a.N * a.K;
+template <class XT, class WT, bool WVH> hipError_t launch_logits(const SoftLogits& all, void* ws, size_t room, hipStream_t s) {
+  const SortPlan p = plan_sort(all.N, all.K, all.H, all.V, all.w_vh != 0, room);
   if (!p.sorted) {
-    const int64_t groups = (M + 3) / 4;
+    const SoftLogits& a = all;
+    const int64_t M = a.N * a.K, groups = (M + 3) / 4;
     hipLaunchKernelGGL((soft_logits_direct_kernel<XT, WT, WVH>), dim3((unsigned)(groups < kMostGroups ? groups : kMostGroups)), dim3(256), 0,
                        s, a);
     return hipGetLastError();
@@ -528,13 +547,24 @@ template <class XT, class WT, bool WVH> hipError_t launch_logits(const SoftLogit
   int* num_items = reinterpret_cast<int*>(base + p.num_items);
   int4* items = reinterpret_cast<int4*>(base + p.items);
   int2* entries = reinterpret_cast<int2*>(base + p.entries);
-  const dim3 grid((unsigned)((M + kSortThreads * kSortPer - 1) / (kSortThreads * kSortPer))), block(kSortThreads);
-  hipLaunchKernelGGL(soft_clear_kernel, dim3((unsigned)((p.groups + kSortThreads - 1) / kSortThreads)), block, 0, s, counts, p.groups);
-  hipLaunchKernelGGL(soft_count_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups);
-  hipLaunchKernelGGL(soft_items_kernel, dim3(1), block, 0, s, counts, p.groups, items, num_items);
-  hipLaunchKernelGGL(soft_place_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups, entries);
-  hipLaunchKernelGGL((soft_logits_kernel<XT, WT, WVH>), dim3((unsigned)((p.most_items + 7) / 8 * 8)), dim3(256), 0, s, a, items, num_items, entries);
-  return hipGetLastError();
+  for (int64_t row0 = 0; row0 < all.N; row0 += p.rows) {
+    SoftLogits a = all;
+    a.N = all.N - row0 < p.rows ? all.N - row0 : p.rows;
+    a.x = reinterpret_cast<const XT*>(all.x) + row0 * all.ldx;
+    a.index = all.index + row0 * all.K;
+    a.z = all.z + row0 * all.K;
+    const int64_t M = a.N * a.K;
+    const dim3 grid((unsigned)((M + kSortThreads * kSortPer - 1) / (kSortThreads * kSortPer))), block(kSortThreads);
+    hipLaunchKernelGGL(soft_clear_kernel, dim3((unsigned)((p.groups + kSortThreads - 1) / kSortThreads)), block, 0, s, counts, p.groups);
+    hipLaunchKernelGGL(soft_count_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups);
+    hipLaunchKernelGGL(soft_items_kernel, dim3(1), block, 0, s, counts, p.groups, items, num_items);
+    hipLaunchKernelGGL(soft_place_kernel, grid, block, p.groups * 4, s, a.index, M, counts, p.groups, entries);
+    hipLaunchKernelGGL((soft_logits_kernel<XT, WT, WVH>), dim3((unsigned)((p.most_items + 7) / 8 * 8)), dim3(256), 0, s, a, items, num_items,
+                       entries);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
@@ -556,18 +586,20 @@ hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const voi
   return hipGetLastError();
 }
 
-size_t soft_logits_bytes(int64_t N, int K, int64_t H, int64_t V, bool w_vh) { return plan_sort(N, K, H, V, w_vh).total; }
+size_t soft_logits_bytes(int64_t N, int K, int64_t H, int64_t V, bool w_vh, size_t room) {
+  return plan_sort(N, K, H, V, w_vh, room).total;
+}
 
-hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s) {
+hipError_t launch_soft_logits(const SoftLogits& a, void* ws, size_t room, hipStream_t s) {
   if (a.x_dtype == DT_BF16 && a.w_dtype == DT_BF16)
-    return a.w_vh ? launch_logits<__bf16, __bf16, true>(a, ws, s) : launch_logits<__bf16, __bf16, false>(a, ws, s);
+    return a.w_vh ? launch_logits<__bf16, __bf16, true>(a, ws, room, s) : launch_logits<__bf16, __bf16, false>(a, ws, room, s);
   if (a.x_dtype == DT_BF16 && a.w_dtype == DT_F32)
-    return a.w_vh ? launch_logits<__bf16, float, true>(a, ws, s) : launch_logits<__bf16, float, false>(a, ws, s);
+    return a.w_vh ? launch_logits<__bf16, float, true>(a, ws, room, s) : launch_logits<__bf16, float, false>(a, ws, room, s);
   if (a.x_dtype == DT_F16 && a.w_dtype == DT_F16)
-    return a.w_vh ? launch_logits<_Float16, _Float16, true>(a, ws, s) : launch_logits<_Float16, _Float16, false>(a, ws, s);
+    return a.w_vh ? launch_logits<_Float16, _Float16, true>(a, ws, room, s) : launch_logits<_Float16, _Float16, false>(a, ws, room, s);
   if (a.x_dtype == DT_F16 && a.w_dtype == DT_F32)
-    return a.w_vh ? launch_logits<_Float16, float, true>(a, ws, s) : launch_logits<_Float16, float, false>(a, ws, s);
-  if (a.x_dtype == DT_F32 && a.w_dtype == DT_F32 && !a.w_vh) return launch_logits<float, float, false>(a, ws, s);
+    return a.w_vh ? launch_logits<_Float16, float, true>(a, ws, room, s) : launch_logits<_Float16, float, false>(a, ws, room, s);
+  if (a.x_dtype == DT_F32 && a.w_dtype == DT_F32 && !a.w_vh) return launch_logits<float, float, false>(a, ws, room, s);
   return hipErrorInvalidValue;
 }
 

@@ -503,8 +503,10 @@ struct SoftLogits {
 };
 hipError_t launch_soft_targets(const int64_t* index, int64_t ld_index, const void* logits, int dtype, int64_t ld_logits, int64_t N, int K,
                                int64_t V, float temperature, int* out_index, float* out_q, int64_t* y, hipStream_t s);
-size_t soft_logits_bytes(int64_t N, int K, int64_t H, int64_t V, bool w_vh);  // scratch (may be 0)
-hipError_t launch_soft_logits(const SoftLogits& a, void* ws, hipStream_t s);
+// Scratch (may be 0), no more than the larger of `room` and kSortScratch whatever the number of entries; the same `room` for both.
+constexpr size_t kSortScratch = (size_t)16 << 20;
+size_t soft_logits_bytes(int64_t N, int K, int64_t H, int64_t V, bool w_vh, size_t room);
+hipError_t launch_soft_logits(const SoftLogits& a, void* ws, size_t room, hipStream_t s);
 // z of a chunk whose stage holds the fp32 logits (BwdArgs of the pairs): read from there.
 hipError_t launch_soft_pick(const BwdArgs& a, const SoftTargets& t, hipStream_t s);
 // dz of the targets' columns of the slab or chunk that `a` describes, over what the label's kernels staged there.
