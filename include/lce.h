@@ -460,7 +460,8 @@ int lce_distill(const lce_problem* p, int64_t K, const int32_t* index, const flo
  * 0 <= rows <= 2^30, 1 <= cols <= 2^30; with no rows nothing is done.  From version 1000 on.
  *
  * lce_top_logits: the first k of each row, 1 <= k <= min(cols, LCE_MAX_TARGETS): values (rows, k) in the type of the logits, index
- * (rows, k), and -- lse not NULL -- log sum exp of the whole row (-inf where all are, NaN where one is).  What lce_soft_targets
+ * (rows, k), and -- lse not NULL -- log sum exp of the whole row (-inf where all are, NaN where one is; of
+ * fp32 terms in sums of 130 at most, the rest in doubles: off by some 2^-18 beside its own rounding, whatever cols).  What lce_soft_targets
  * reads of a teacher.
  *
  * lce_sample: one token a row from the uniform number u[row] in [0, 1).  With w[j] = exp((z[j] - max z) / temperature), summed in 64

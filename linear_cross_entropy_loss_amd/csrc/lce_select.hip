@@ -770,13 +770,20 @@ template <class E, int NT, int FL> LCE_DEV void store_top(const RowUnits<E, NT, 
 }
 
 // sum exp(z - m) of a row, the same bits from 512 and from 1024 threads: a thread adds up the pieces of one (or, apart, of two) of 1024
-// places, the waves' sums are doubles, in the order of the places.  A term equal to m is 1, also of an infinite m.
+// places, in fp32 up to kTerms of them (a row of 131072), those sums and the waves' in doubles, in the order of the places.  A term equal to
+// m is 1, also of an infinite m.
 template <class E, int NT> struct ExpSum {
   static constexpr int kOwn = 1024 / NT, kPer = RowPieces<E, NT>::kPer;
+  static constexpr int kFlight = RowPieces<E, NT>::kFlight, kTerms = 128, kRounds = kTerms / kPer * kOwn / kFlight;
   float m, sum[kOwn];
-  LCE_DEV explicit ExpSum(float m_) : m(m_) {
+  double total[kOwn];
+  int rounds;
+  LCE_DEV explicit ExpSum(float m_) : m(m_), rounds(0) {
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) sum[i] = 0.f;
+    for (int i = 0; i < kOwn; ++i) {
+      sum[i] = 0.f;
+      total[i] = 0.0;
+    }
   }
   template <bool FINITE> LCE_DEV float term(float z) const {
     // (one fma of z and m log2 e would do, but for logits of 10^30, where the product's rounding is no small number)
@@ -790,13 +797,20 @@ template <class E, int NT> struct ExpSum {
     __builtin_memcpy(e, &v, 16);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) sum[r % kOwn] += term<FINITE>(as_float(e[i]));
+    if (r == kFlight - 1 && ++rounds % kRounds == 0) {
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        total[i] += (double)sum[i];
+        sum[i] = 0.f;
+      }
+    }
   }
   // 16 sums; no barrier.
   LCE_DEV void store(double* sums) const {
     const int t = thread();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const double upto = wave_upto<Sum>((double)sum[i]);
+      const double upto = wave_upto<Sum>(total[i] + (double)sum[i]);
       if ((t & 63) == 63) sums[i * (NT / 64) + (t >> 6)] = upto;
     }
   }

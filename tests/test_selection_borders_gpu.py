@@ -1,4 +1,4 @@
-"""Sampling where a border decides: a bin's border next to zero, weights next to half a place."""
+"""Sampling and logsumexp where a border decides: a bin's border next to zero, weights next to half a place, sums of very many terms."""
 import math
 
 import pytest
@@ -59,3 +59,20 @@ def test_weights_next_to_half_a_place(dtype, V, u, N):
         got = sample_logits(z.cuda().expand(N, V), torch.full((N,), u, device="cuda"), temperature=temperature).cpu()
         print(f"{dtype} V={V} N={N} {more}: {got[0].item()}", flush=True)
         assert torch.equal(got, torch.full((N,), fixed_point_token(z, u, temperature)))
+
+
+@pytest.mark.parametrize("N", [1, 300])
+@pytest.mark.parametrize("dtype,V", [(BF16, (1 << 22) + 5), (F16, 1 << 23), (F32, (1 << 22) + 5), (F32, 131072), (BF16, 50257)])
+def test_lse_of_long_flat_rows(dtype, V, N):
+    """A term is off by 2 units of 2^-24 and |z - max| <= 2 more; an fp32 sum of at most 130 of them by 65 on top, all to one side; the rest
+    is in doubles and rounded once."""
+    from linear_cross_entropy_loss_amd import top_logits
+
+    for value in (-1.0986, -0.4055, -1.9, -0.01):
+        z = torch.full((1, V), value, device="cuda").to(dtype)
+        z[0, 7] = 0.0
+        ref = torch.logsumexp(z.double(), 1).item()
+        for k in (10, 700):
+            lse = top_logits(z.expand(N, V), k)[2].cpu().double()
+            print(f"{dtype} V={V} N={N} k={k} {value}: off by {(lse[0].item() - ref):.2e}", flush=True)
+            assert ((lse - ref).abs() <= 2.0 ** -24 * (70 + abs(ref))).all()
