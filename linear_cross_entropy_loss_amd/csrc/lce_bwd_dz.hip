@@ -96,8 +96,11 @@ LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const flo
   E* row = wave_base + (lane & 31) * kGroup;
   constexpr bool MON = FUSE && ZREG, KEEP = FUSE && SPLIT;
   // Stores go through a buffer descriptor over this wave's part of the stage (scalar base, one 32-bit offset per
-  // lane, the block's offset as a scalar): no 64-bit vector address arithmetic.  All offsets stay below 2^31
-  // (one block for the second column group, twice that for the pairs' two parts).
+  // lane): no 64-bit vector address arithmetic.  All offsets stay below 2^31 (one block for the second column group,
+  // twice that for the pairs' two parts).  The offset is a vector's, its constant part as far as 12 bits the
+  // instruction's, and not a scalar's: with a scalar offset the compiler lets the next vector instruction write the
+  // registers that a store of 16 bytes is still reading.  (Two such stores in a row, two waves on the SIMD: the first
+  // word of the second went out as the instruction behind it had left it, in the last four of every 16 lanes.)
   const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(wave_base, 0, 0x7fffffff, 0x00020000);
   // staging: this lane's line of a piece when it writes (its token), and line / chunk when it reads back: 8 lines
   // per instruction, 8 lanes each; the upper 32 lanes take their four lines in the order 5, 4, 7, 6 so that lanes
@@ -249,8 +252,8 @@ LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const flo
           const int line = i * 8 + rline;
           const u32x4_t v = *reinterpret_cast<const u32x4_t*>(mine + gi * kPieceBytes + line * (kGroup * 2) +
                                                               ((rchunk ^ (line & 7) ^ ((line >> 3) & 1)) << 4));
-          const unsigned soff = (unsigned)(gi * grp * 2 + part * kDzBlockElems * 2) + qb * (kBlk * kGroup * 2);
-          __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, line * (kGroup * 2) + rchunk * 16, (int)soff, kDzStoreAux);
+          const unsigned off = (unsigned)(gi * grp * 2 + part * kDzBlockElems * 2) + qb * (kBlk * kGroup * 2) + i * (8 * kGroup * 2);
+          __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, rline * (kGroup * 2) + rchunk * 16 + (int)off, 0, kDzStoreAux);
         }
     }
     // The target column of this lane's token, if it lies in this wave's slice: the staged softmax value is
