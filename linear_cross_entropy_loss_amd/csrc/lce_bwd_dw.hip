@@ -244,8 +244,8 @@ template <bool LOAD, bool WVH, bool LO8>
 LCE_DEV void dw_plane_split_io(char* hi, int hi_stride, char* lo, f32x16_t (&acc)[kNB][kNB]) {
   typedef typename std::conditional<LO8, u32x2_t, u32x4_t>::type L;
   constexpr int kLoBytes = LO8 ? 8 : 16;  // of a pair and thread
-  // one descriptor per block, the thread's place as the vector offset, the pair as a scalar offset: no 64-bit
-  // address per pair
+  // one descriptor per block, the thread's place as the vector offset, the pair as a scalar offset -- of loads; on top of the
+  // vector's for stores of 16 bytes (see dz_epilogue_impl in lce_bwd_dz.hip) --: no 64-bit address per pair
   const __amdgpu_buffer_rsrc_t rh = __builtin_amdgcn_make_buffer_rsrc(hi, 0, 255 * hi_stride + 512, 0x00020000);
   const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc(lo, 0, 32 * kThreads * kLoBytes, 0x00020000);
   const int tid = opaque_tid();
@@ -286,7 +286,7 @@ LCE_DEV void dw_plane_split_io(char* hi, int hi_stride, char* lo, f32x16_t (&acc
       u32x4_t nh;
 #pragma unroll
       for (int d = 0; d < 4; ++d) nh[d] = __builtin_amdgcn_perm(r[2 * d + 1], r[2 * d], kSelHigh);
-      __builtin_amdgcn_raw_buffer_store_b128(nh, rh, vh, (rb * kBlk + (cb * 2 + (p & 1)) * 4) * hi_stride, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(nh, rh, vh + (rb * kBlk + (cb * 2 + (p & 1)) * 4) * hi_stride, 0, 0);
       if constexpr (LO8) {
         u32x2_t nl;
 #pragma unroll
@@ -297,7 +297,7 @@ LCE_DEV void dw_plane_split_io(char* hi, int hi_stride, char* lo, f32x16_t (&acc
         u32x4_t nl;
 #pragma unroll
         for (int d = 0; d < 4; ++d) nl[d] = __builtin_amdgcn_perm(r[2 * d + 1], r[2 * d], kSelLow);
-        __builtin_amdgcn_raw_buffer_store_b128(nl, rl, vl, p * (kThreads * kLoBytes), 0);
+        __builtin_amdgcn_raw_buffer_store_b128(nl, rl, vl + p * (kThreads * kLoBytes), 0, 0);
       }
     }
     __builtin_amdgcn_sched_barrier(0);  // (one batch in registers at a time: an operand tile is in flight)
