@@ -321,10 +321,10 @@ template <class XT, class WT, int n> LCE_DEV void load_as(XT (&to)[n], const WT*
 // take such a stretch of one entry's row of x, a whole line, against the entry's column: 32 entries at a time, four times.  The
 // column's line is read by eight neighbouring lanes, which meets every bank once.
 //   Bound by memory traffic: 2 H bytes (4 in fp32) for every entry and W once for every 128 entries of a group, from the caches where
-// they fit.  N=16384, K=64, H=2048, V=131072, 0.9 million entries: 627 us, some 3.7 GB of x and 1.7 of W; with 256 entries to an item 841
-// (registers leave fewer workgroups to hide the waits), 512 1295, 64 882, neighbouring items on different XCDs 690, the next lines of x
-// in flight during the products 791.  N=2048, K=64, H=2048, V=16384 in fp32 142, with 256 entries 134; N=8192, K=32, H=768, V=50257
-// stored (V, H) 49 / 65; N=1999, K=20, H=500, V=10007 23 / 41.
+// they fit.  N=16384, K=64, H=2048, V=131072, 0.9 million entries: 623 us, 3.7 GB of x and 2.1 of W through the L2s, 3.8 of it from beyond
+// them; with 256 entries to an item 841 (registers leave fewer workgroups to hide the waits), 512 1295, 64 882, neighbouring items on
+// different XCDs 690, the next lines of x in flight during the products 791.  N=2048, K=64, H=2048, V=16384 in fp32 142, with 256
+// entries 134; N=8192, K=32, H=768, V=50257 stored (V, H) 49 / 65; N=1999, K=20, H=500, V=10007 23 / 41.
 template <class XT, class WT, bool WVH>
 __global__ __launch_bounds__(256) void soft_logits_kernel(const SoftLogits a, const int4* items, const int* num_items, const int2* entries) {
   constexpr int kPiece = 16 / sizeof(XT), kDeep = 8 * kPiece;  // elements of a lane's piece, of a stretch

@@ -881,7 +881,9 @@ LCE_DEV void top_by_digits(const RowUnits<E, NT, FL>& row, int k, E* values, int
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // The first k, k up to kMostByMaxima, without a histogram: of the largest element of each thread, the k-th is a lower bound of the k-th
-// of the row, and about k (1 + k / 2048) elements are not below it: these are listed and sorted.  Two passes over the row, one that
+// of the row, and about -M ln(1 - k / M) elements of M maxima are not below it: these are listed and sorted.  M is 1024 for rows of 1024 pieces
+// of 16 bytes and more (32 elements for k = 32, 710 for 512), the number of pieces below that; where k is not well below it, the list
+// overflows, in 16-bit rows of 2049 to some 4300 with k from an eighth of the row's length on.  Two passes over the row, one that
 // takes maxima, one that compares (and sums the exponentials for lse).  Where many of the maxima equal the bound -- all but a few
 // columns masked, or one value almost everywhere -- only what is larger is listed, and the first columns of that value are added.  Rows whose list
 // would be too long all the same, with a NaN or an infinity on top are done by digits.  (All but 10 columns masked, k = 32, us, here / by
@@ -1087,8 +1089,9 @@ template <class E, bool LSE, int NT, class Shared> LCE_DEV const u64* list_first
   return sh->list;
 }
 
-// Bound by memory traffic for long rows (2048 rows of 50257 bf16 64 us, 3.2 TB/s of one reading; 2048 of 131072 float32 317, 3.4), by the
-// latency of its steps for short ones: 48 rows of 50304 12 us, of which 3 read and 2 look for the bound, 5 list and sum, 1 sorts.
+// Bound for long rows by memory traffic and vector work beside each other (2048 rows of 50257 bf16 64 us, 3.2 TB/s of one reading; 2048 of
+// 131072 float32 317, 3.4; 8192 of 50257 bf16 234 with the vector units 81 % busy; both readings go beyond the L2s), by the latency of its
+// steps for short ones: 48 rows of 50304 12 us, of which 3 read and 2 look for the bound, 5 list and sum, 1 sorts.
 //   NT = 512: 64 registers a thread and little LDS, four rows to a compute unit, of which some are read while others are sorted; 1024 where
 // each row has a compute unit to itself.  us, 512 / 1024: top_logits, 64 rows, V=4096 bf16 7.7 / 7.8, float32 7.7 / 8.4, 50257 bf16
 // 13 / 12, 131072 21 / 19, float32 25 / 20; 256 rows, 131072 29 / 27, float32 42 / 42; 400 rows, 50257 21 / 25, 29 / 34.  sample_top_kernel,
@@ -1164,8 +1167,8 @@ constexpr int kSelectThreads = 1024;
 // the fixed point of the weights reaches; the few elements of the bin in which a place lies are then listed and sorted.  Passes over the
 // row: its maximum, the histogram, one for every place that is asked for.  A bin with more elements than the list has room for is
 // no matter if they are all equal; else the row is done by digits.
-//   Bound by the vector work of the weights, 24 instructions for an element, most of them of 64 bits: 2048 rows of 32000 fp16 113 us, of
-// which the histogram takes half, a place 25, the maximum, from memory, 15.
+//   Bound by the vector work of the weights, 24 of 42 instructions for an element, most of them of 64 bits: 2048 rows of 32000 fp16 116 us,
+// the vector units 65 % busy; of a row's 25 us the histogram takes 11, the place 7, the maximum, from memory, 5.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kBins = 4096;
 constexpr double kBinsPerOctave = 80.0;  // 51 octaves and 2^-10: a weight of 2^-51 rounds to 0 with 50 places

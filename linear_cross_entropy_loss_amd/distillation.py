@@ -217,6 +217,9 @@ def linear_distillation(x, At, index, logits, temperature: float = 1.0, logit_sc
         temperature: divides both sides' logits.
         N_chunk_size: as of ``LinearCrossEntropyLoss``.
 
+    float32 tensors are multiplied as pairs of bfloat16 (16 bits of mantissa), as by ``linear_cross_entropy``; 16-bit gradients come from a
+    softmax minus target that was rounded to the type.
+
     Rows without a target (prompts, padding) have no gradient and do not count in the mean; no row with one at all gives NaN
     and zero gradients, as a batch without labels does.  Returns the loss (float32); gradients go to ``x`` and ``At``.
     """

@@ -159,7 +159,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     With ``w = exp((z - max z) / temperature)``, in the row's order: ``top_k`` keeps the first k columns, ``top_p`` those
     before which less than ``top_p`` of the weight that ``top_k`` left has gathered, ``min_p`` those of at least ``min_p`` times
     the largest weight -- each the first column at least.  The token is the first column, of what all keep, with which more than
-    ``u`` times the whole weight has gathered.  Weights are summed in 64 bits.
+    ``u`` times the whole weight has gathered.  Weights are whole multiples of ``2 ** -min(50, 62 - ceil(log2(V)))``, summed in 64 bits: the
+    token does not depend on how many rows there are.
 
     Args:
         logits: (..., V) bfloat16, float16 or float32, any row stride; -inf masks a column.
