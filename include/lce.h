@@ -490,6 +490,87 @@ int lce_top_logits(const void* logits, int dtype, int64_t rows, int64_t cols, in
 int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* u, const lce_sampling* s, int64_t* token,
                void* stream);
 
+/*
+ * Logit and logsumexp of one given column for each row, and the gradients for any upstream gradient of either.  No counterpart in the
+ * reference.  From version 1100 on.
+ *
+ *   z[n][v] = logit_scale * sum_h x[n][h] * W[h][v],   lse[n] = log sum_v exp z[n][v],   logits[n] = z[n][y[n]]
+ *   dz[n][v] = grad_lse[n] * exp(z[n][v] - lse[n]) + grad_logits[n] * [v == y[n]],   dx = logit_scale * dz W^T,   dW = logit_scale * x^T dz
+ *
+ * logits - lse is the log-probability of a token.  Where W is one piece of a vocabulary, lse of the whole is the logsumexp of the
+ * pieces' and the logit the sum of theirs.  By the kernels, in the scratch and with the arithmetic of lce_forward and of a
+ * lce_backward that stages dz; an fp16 stage is scaled by the largest |grad_lse| + |grad_logits|.
+ *
+ *   p       as for those calls; monitoring, z_reg and phases are 0, route is not looked at
+ *   y       N labels: a column; p->ignore_index: a row that is not computed, logit and lse 0, without gradients, whatever
+ *           grad_logits and grad_lse hold there; `other`: a column of another piece, logit 0 and no gradient by it; any other
+ *           number: logit NaN, no gradient by it.  lce_token_labels makes them.
+ *   logits, lse   N floats each: out; the backward takes them as the forward gave them
+ *   grad_logits, grad_lse   N floats each
+ *   dx, dw  out, at least one of them
+ *
+ * lce_token_labels: labels[i] = tokens[i] - vocab_start where that is one of V columns, -1 where tokens[i] is ignore_index, V where
+ * it is another token of a vocabulary of vocab_size, V + 1 where it is none (for the two calls: ignore_index -1, other V).
+ * 0 <= vocab_start <= vocab_size - V, 0 <= N <= 2^30.
+ */
+int lce_token_labels(const int64_t* tokens, int64_t N, int64_t ignore_index, int64_t vocab_start, int64_t V, int64_t vocab_size,
+                     int64_t* labels, void* stream);
+int lce_token_logits_workspace_bytes(const lce_problem* p, size_t* fwd_bytes, size_t* bwd_bytes);
+int lce_token_logits(const lce_problem* p, const void* x, const void* w, const int64_t* y, int64_t other, float* logits, float* lse, void* ws,
+                     size_t ws_bytes, void* stream);
+int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w, const int64_t* y, const float* logits, const float* lse,
+                              const float* grad_logits, const float* grad_lse, void* dx, void* dw, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Numbers of 8 bits with a scale for each row: t[r][c] = q[r][c] * scales[r], scales[r] = max_c |t[r][c]| / 127, q the whole number
+ * that is nearest to 127 * t / max |t| (of two the even one; decided exactly).  A row of zeros has a scale of 0; one with a NaN or an
+ * infinity a scale of NaN and zeros.  No counterpart in the reference.  From version 1100 on.
+ *
+ * lce_quantize_rows: of src (rows, cols), any row stride, at any element boundary.  lce_quantize_columns: of its columns, q then
+ * (cols, rows): the transposed copy that lce_int8_logits reads of a weight stored (H, V).
+ *   q       rows on 16-byte boundaries, ldq a multiple of 16; what lies between the end of a row and ldq becomes 0
+ * 1 <= rows, cols; the length of what gets one scale is at most LCE_INT8_DEPTH, the other at most 2^30.
+ *
+ * lce_int8_logits: out[n][v] = logit_scale * sx[n] * w_scales[v] * sum_h qx[n][h] * w[v][h] for v < V, with qx, sx of the rows of x,
+ * which are quantised on the way: the sum in whole numbers, exact; the product with the scales in fp32, rounded once to out's type.
+ *   x       (N, H), any row stride, at any element boundary
+ *   w       (V, H) as the calls above give it, ldw a multiple of 16; what lies behind the end of a row has no effect, and of the last row
+ *           nothing is read past the 4 bytes that hold its last number
+ *   out     (N, V), row stride ldo >= V, at any element boundary
+ *   ws      lce_int8_logits_workspace_bytes(N, H, V) bytes
+ * H <= LCE_INT8_DEPTH (the sums fit 32 bits), 0 <= N <= 2^30 (0: nothing is done), V <= 2^30, ceil(N/256) * ceil(V/256) <= 2^28.
+ */
+#define LCE_INT8_DEPTH ((int64_t)1 << 17)
+int lce_quantize_rows(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* q, int64_t ldq, float* scales, void* stream);
+int lce_quantize_columns(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* q, int64_t ldq, float* scales,
+                         void* stream);
+int lce_int8_logits_workspace_bytes(int64_t N, int64_t H, int64_t V, size_t* bytes);
+int lce_int8_logits(const void* x, int x_dtype, int64_t N, int64_t H, int64_t V, int64_t ldx, const int8_t* w, int64_t ldw,
+                    const float* w_scales, float logit_scale, void* out, int out_dtype, int64_t ldo, void* ws, size_t ws_bytes,
+                    void* stream);
+
+/*
+ * The norm of many tensors together, and the tensors scaled to at most that of max_norm:
+ *   *norm = sqrt(sum over all of them of g^2) / divisor,   out = g * min(1, max_norm / *norm) / divisor
+ * squares and their sum in doubles, in a fixed order; the factor rounded to fp32, each product to out's type.  A norm that is not
+ * finite leaves min(...) at 1: the caller looks at *norm.  No counterpart in the reference.  From version 1100 on.
+ *   t        `count` tensors (host memory, read during the call), n elements each, dense, at any element boundary; grad: in; out: of
+ *            dtype or LCE_F32, may be grad itself; an `out` may overlap no other tensor's memory.  0 <= count <= 2^20
+ *   max_norm > 0 (infinity: no limit);  divisor_ptr: a device pointer to 1 float, or NULL: the number `divisor` > 0
+ *   norm     out, 1 float
+ *   ws       lce_clip_workspace_bytes(t, count) bytes
+ */
+typedef struct lce_tensor {
+  const void* grad;
+  void* out;
+  int64_t n;
+  int32_t dtype;
+  int32_t out_dtype;
+} lce_tensor;
+int lce_clip_workspace_bytes(const lce_tensor* t, int64_t count, size_t* bytes);
+int lce_clip(const lce_tensor* t, int64_t count, float max_norm, float divisor, const float* divisor_ptr, float* norm, void* ws,
+             size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ W_HV, W_VH = 0, 1  # lce_problem.w_layout: weight stored (H, V) / (V, H) row-maj
 LCE_EINVAL_SHAPE, LCE_EINVAL_DTYPE, LCE_EINVAL_ARG, LCE_EWORKSPACE, LCE_EHIP, LCE_ESTATIC = -1, -2, -3, -4, -5, -6
 STATIC_SCRATCH_BYTES = 64 << 20
 MAX_TARGETS = 1024  # lce_distill: targets of a row
+INT8_DEPTH = 1 << 17  # lce_int8_logits: numbers of a row
 
 EXPORTS = (
     "lce_version",
@@ -48,6 +49,16 @@ EXPORTS = (
     "lce_distill",
     "lce_top_logits",
     "lce_sample",
+    "lce_token_labels",
+    "lce_token_logits_workspace_bytes",
+    "lce_token_logits",
+    "lce_token_logits_backward",
+    "lce_quantize_rows",
+    "lce_quantize_columns",
+    "lce_int8_logits_workspace_bytes",
+    "lce_int8_logits",
+    "lce_clip_workspace_bytes",
+    "lce_clip",
 )
 
 _DTYPES = {torch.bfloat16: LCE_BF16, torch.float16: LCE_F16, torch.float32: LCE_F32}
@@ -93,6 +104,18 @@ class LceSampling(ctypes.Structure):
         ("top_p_rows", ctypes.c_void_p),
         ("min_p_rows", ctypes.c_void_p),
         ("top_k_rows", ctypes.c_void_p),
+    ]
+
+
+class LceTensor(ctypes.Structure):
+    """Mirror of ``struct lce_tensor``."""
+
+    _fields_ = [
+        ("grad", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
     ]
 
 
@@ -167,6 +190,20 @@ def load():
     lib.lce_top_logits.argtypes = [vp, ctypes.c_int, i64, i64, i64, i64, vp, vp, vp, vp]
     lib.lce_sample.restype = ctypes.c_int
     lib.lce_sample.argtypes = [vp, ctypes.c_int, i64, i64, i64, vp, ctypes.POINTER(LceSampling), vp, vp]
+    f32, cint = ctypes.c_float, ctypes.c_int
+    lib.lce_token_labels.argtypes = [vp, i64, i64, i64, i64, i64, vp, vp]
+    lib.lce_token_logits_workspace_bytes.argtypes = [P, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+    lib.lce_token_logits.argtypes = [P, vp, vp, vp, i64, vp, vp, vp, sz, vp]
+    lib.lce_token_logits_backward.argtypes = [P] + [vp] * 10 + [sz, vp]
+    lib.lce_quantize_rows.argtypes = [vp, cint, i64, i64, i64, vp, i64, vp, vp]
+    lib.lce_quantize_columns.argtypes = lib.lce_quantize_rows.argtypes
+    lib.lce_int8_logits_workspace_bytes.argtypes = [i64, i64, i64, ctypes.POINTER(sz)]
+    lib.lce_int8_logits.argtypes = [vp, cint, i64, i64, i64, i64, vp, i64, vp, f32, vp, cint, i64, vp, sz, vp]
+    T = ctypes.POINTER(LceTensor)
+    lib.lce_clip_workspace_bytes.argtypes = [T, i64, ctypes.POINTER(sz)]
+    lib.lce_clip.argtypes = [T, i64, f32, f32, vp, vp, vp, sz, vp]
+    for name in EXPORTS[-10:]:
+        getattr(lib, name).restype = ctypes.c_int
     _lib = lib
     return lib
 
@@ -292,4 +329,11 @@ def forward_backward_plan(prob: LceProblem) -> tuple[int, int]:
 def distill_workspace_bytes(prob: LceProblem, K: int, grads: bool) -> int:
     b = ctypes.c_size_t(0)
     raise_for_status(load().lce_distill_workspace_bytes(ctypes.byref(prob), int(K), int(grads), ctypes.byref(b)), "linear_distillation")
+    return b.value
+
+
+def token_logits_workspace_bytes(prob: LceProblem, backward: bool) -> int:
+    b = ctypes.c_size_t(0)
+    where = (None, ctypes.byref(b)) if backward else (ctypes.byref(b), None)
+    raise_for_status(load().lce_token_logits_workspace_bytes(ctypes.byref(prob), *where), "linear_token_logits")
     return b.value

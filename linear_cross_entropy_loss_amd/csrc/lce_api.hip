@@ -4,7 +4,9 @@
 // (linear_cross_entropy/ops.py:681-802) -- minus every allocation, which is the
 // caller's -- and what its backward does (ops.py:804-810).
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <atomic>
+#include <vector>
 #include <stdio.h>
 #include <string.h>
 
@@ -854,8 +856,9 @@ int current_num_cus(int* out, int cap, int* small_wgs = nullptr) {
 }
 
 // Body of lce_forward; `ws` is the caller's workspace or the library's static scratch.
+// (`tok_logits`, `tok_other`: as in FwdArgs; out5 and n_valid may then be left unwritten)
 int forward_impl(const lce_problem* p, const void* x, const void* w, const int64_t* y, float* lse, float* out5,
-                 int64_t* n_valid, void* ws, size_t ws_bytes, void* stream) {
+                 int64_t* n_valid, void* ws, size_t ws_bytes, void* stream, float* tok_logits = nullptr, int64_t tok_other = 0) {
   int rc = check(p, false);
   if (rc != LCE_OK) return rc;
   if (!x || !w || !y || !lse || !out5 || !n_valid) return LCE_EINVAL_ARG;
@@ -875,6 +878,7 @@ int forward_impl(const lce_problem* p, const void* x, const void* w, const int64
   a.ignore_index = p->ignore_index;
   a.scale = p->logit_scale; a.z_reg = p->z_reg; a.monitoring = p->monitoring ? 1 : 0;
   a.lse = lse; a.out5 = out5; a.n_valid = n_valid;
+  a.tok_logits = tok_logits; a.tok_other = tok_other;
   a.part_lse = (float*)(base + f.part_lse);
   a.part_max = (float*)(base + f.part_max);
   a.part_pz = (float*)(base + f.part_pz);
@@ -1151,7 +1155,7 @@ int fused_impl(const lce_problem* p, const FusedPlan& f, const void* x, const vo
 // Body of lce_backward for a problem and its plan.
 int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const void* w, const int64_t* y, const float* lse,
                   const int64_t* n_valid, const float* grad_out, void* dx, void* dw, void* ws, void* stream,
-                  const lce::SoftTargets* targets = nullptr) {
+                  const lce::SoftTargets* targets = nullptr, lce::RowGradients* rows = nullptr) {
   hipStream_t s = (hipStream_t)stream;
   char* base = (char*)ws;
 
@@ -1208,6 +1212,20 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
                                       a.num_cus, s);
     if (e != hipSuccess) return hip_fail(e, "gather_rows");
   }
+  if (rows != nullptr) {
+    // gradients of each row in the place of one upstream gradient
+    rows->perm = pack ? (const int*)(base + k.perm) : nullptr;
+    const hipError_t e = lce::launch_row_gradients(*rows, s);
+    if (e != hipSuccess) return hip_fail(e, "row_gradients");
+    a.row_signs = 1;
+    a.lse = rows->row_lse;
+    a.y = rows->row_y;
+    a.ignore_index = -1;
+    a.grad_out = rows->factor;
+    a.n_valid = nullptr;
+    // (normalised rows: |dz| <= 2, times 2^14 within fp16's range; probabilities stay normal down to 2^-28)
+    a.dz_shift = rows->normalise ? 14 : 0;
+  }
   if (x32) {  // fp32 activations reach the tile kernels as copies in bf16 pairs, whether or not rows were dropped
     a.x = a.xc;
     a.ldx = a.ldxc;
@@ -1252,6 +1270,10 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
       if (targets != nullptr) {
         e = lce::launch_soft_gradient(a, *targets, s);
         if (e != hipSuccess) return hip_fail(e, "soft_gradient");
+      }
+      if (rows != nullptr) {
+        e = lce::launch_row_targets(a, *rows, s);
+        if (e != hipSuccess) return hip_fail(e, "row_targets");
       }
     }
     if (b.small) {
@@ -1331,7 +1353,7 @@ int plan_distill(const lce_problem* q, int64_t K, bool grads, DistillPlan* d) {
 
 extern "C" {
 
-int lce_version(void) { return 1000; }  // 0.10.0: lce_distill
+int lce_version(void) { return 1100; }  // 0.11.0: lce_token_logits, lce_int8_logits, lce_clip
 
 const char* lce_strerror(int status) {
   switch (status) {
@@ -1668,6 +1690,311 @@ int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_
   if (rc != LCE_OK) return rc;
   const hipError_t e = lce::launch_sample(logits, dtype, rows, cols, ld, u, a, token, num_cus, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "sample");
+  return LCE_OK;
+}
+
+int lce_token_labels(const int64_t* tokens, int64_t N, int64_t ignore_index, int64_t vocab_start, int64_t V, int64_t vocab_size,
+                     int64_t* labels, void* stream) {
+  if (N < 0 || N > (int64_t)1 << 30 || V < 1 || V > (int64_t)1 << 30 || vocab_start < 0 || vocab_size < V ||
+      vocab_start > vocab_size - V)
+    return LCE_EINVAL_SHAPE;
+  if (N == 0) return LCE_OK;
+  if (!tokens || !labels) return LCE_EINVAL_ARG;
+  const hipError_t e = lce::launch_token_labels(tokens, N, ignore_index, vocab_start, V, vocab_size, labels, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "token_labels");
+  return LCE_OK;
+}
+
+namespace {
+// What the calls for single tokens keep behind the workspace of the loss's own forward and backward.
+struct TokenPlan {
+  BwdPlan b;
+  size_t fwd, fwd_total;                   // forward: out5 and n_valid, which nobody reads
+  size_t row_lse, row_y, part, bwd_total;  // backward: lce::RowGradients; its factor behind the parts
+};
+
+int check_tokens(const lce_problem* p, bool backward) {
+  const int rc = check(p, backward);
+  if (rc != LCE_OK) return rc;
+  return p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale < INFINITY) ? LCE_EINVAL_ARG : LCE_OK;
+}
+
+// The problem as the planner of the backward sees it: dz is staged (rows have numbers of their own), as for distillation.
+lce_problem token_problem(const lce_problem* p) {
+  lce_problem q = *p;
+  q.route = kSoftTargets;
+  return q;
+}
+
+size_t plan_token_forward(const lce_problem* p, TokenPlan* t) {
+  t->fwd = align_up(plan_fwd(p).total);
+  return t->fwd_total = t->fwd + 256;
+}
+int plan_token_backward(const lce_problem* q, TokenPlan* t) {
+  const int rc = plan_bwd(q, &t->b);
+  if (rc != LCE_OK) return rc;
+  size_t o = align_up(t->b.total);
+  t->row_lse = o; o += align_up((size_t)q->N * 4);
+  t->row_y = o; o += align_up((size_t)q->N * 8);
+  t->part = o; o += align_up((size_t)(lce::kRowGradientParts + 1) * 4);
+  t->bwd_total = o;
+  return LCE_OK;
+}
+}  // namespace
+
+int lce_token_logits_workspace_bytes(const lce_problem* p, size_t* fwd_bytes, size_t* bwd_bytes) {
+  int rc = check_tokens(p, bwd_bytes != nullptr);
+  if (rc != LCE_OK) return rc;
+  TokenPlan t;
+  if (fwd_bytes) *fwd_bytes = plan_token_forward(p, &t);
+  if (bwd_bytes) {
+    const lce_problem q = token_problem(p);
+    rc = plan_token_backward(&q, &t);
+    if (rc == LCE_OK) *bwd_bytes = t.bwd_total;
+  }
+  return rc;
+}
+
+int lce_token_logits(const lce_problem* p, const void* x, const void* w, const int64_t* y, int64_t other, float* logits, float* lse, void* ws,
+                     size_t ws_bytes, void* stream) {
+  const int rc = check_tokens(p, false);
+  if (rc != LCE_OK) return rc;
+  if (!logits) return LCE_EINVAL_ARG;
+  TokenPlan t;
+  if (!ws || ws_bytes < plan_token_forward(p, &t)) return LCE_EWORKSPACE;
+  char* const out = (char*)ws + t.fwd;
+  return forward_impl(p, x, w, y, lse, (float*)out, (int64_t*)(out + 128), ws, t.fwd, stream, logits, other);
+}
+
+int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w, const int64_t* y, const float* logits, const float* lse,
+                              const float* grad_logits, const float* grad_lse, void* dx, void* dw, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_tokens(p, true);
+  if (rc != LCE_OK) return rc;
+  if (!x || !w || !y || !logits || !lse || !grad_logits || !grad_lse || !(dx || dw)) return LCE_EINVAL_ARG;
+  if (misaligned(x) || misaligned(w) || misaligned(dx) || misaligned(dw)) return LCE_EINVAL_ARG;
+  const lce_problem q = token_problem(p);
+  TokenPlan t;
+  rc = plan_token_backward(&q, &t);
+  if (rc != LCE_OK) return rc;
+  if (!ws || ws_bytes < t.bwd_total || misaligned(ws)) return LCE_EWORKSPACE;
+  char* const base = (char*)ws;
+  lce::RowGradients r;
+  memset(&r, 0, sizeof(r));
+  r.grad_lse = grad_lse; r.grad_logits = grad_logits; r.logits = logits; r.lse = lse; r.y = y;
+  r.N = p->N; r.V = p->V; r.ignore_index = p->ignore_index;
+  r.normalise = p->x_dtype == LCE_F16;
+  r.row_lse = (float*)(base + t.row_lse); r.row_y = (int64_t*)(base + t.row_y);
+  r.part = (float*)(base + t.part); r.factor = r.part + lce::kRowGradientParts;
+  return backward_impl(&q, t.b, x, w, y, lse, nullptr, nullptr, dx, dw, ws, stream, nullptr, &r);
+}
+
+namespace {
+int64_t depth_stride(int64_t H) { return lce::pad_to(H, H >= 64 ? 128 : 16); }  // (whole lines, but for short rows)
+
+int check_quantize(const void* src, int dtype, int64_t others, int64_t depth, int64_t least_ld, int64_t ld, const int8_t* q, int64_t ldq,
+                   const float* scales) {
+  if (dtype != LCE_BF16 && dtype != LCE_F16 && dtype != LCE_F32) return LCE_EINVAL_DTYPE;
+  if (others < 1 || others > (int64_t)1 << 30 || depth < 1 || depth > LCE_INT8_DEPTH) return LCE_EINVAL_SHAPE;
+  if (!src || !q || !scales || ld < least_ld || ((uintptr_t)src & (dtype == LCE_F32 ? 3 : 1))) return LCE_EINVAL_ARG;
+  if (misaligned(q) || ldq < depth || ldq % 16 || ldq > 2 * LCE_INT8_DEPTH) return LCE_EINVAL_ARG;
+  return LCE_OK;
+}
+
+struct Int8Plan {
+  int64_t ldx;
+  size_t q, scales, total;
+};
+int plan_int8(int64_t N, int64_t H, int64_t V, Int8Plan* f) {
+  if (N < 0 || N > (int64_t)1 << 30 || H < 1 || H > LCE_INT8_DEPTH || V < 1 || V > (int64_t)1 << 30) return LCE_EINVAL_SHAPE;
+  if ((N + 255) / 256 * ((V + 255) / 256) > (int64_t)1 << 28) return LCE_EINVAL_SHAPE;
+  f->ldx = depth_stride(H);
+  f->q = 0;
+  f->scales = align_up((size_t)N * (size_t)f->ldx);
+  f->total = f->scales + align_up((size_t)N * 4);
+  return LCE_OK;
+}
+}  // namespace
+
+int lce_quantize_rows(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* q, int64_t ldq, float* scales, void* stream) {
+  const int rc = check_quantize(src, dtype, rows, cols, 0, ld, q, ldq, scales);
+  if (rc != LCE_OK) return rc;
+  const hipError_t e = lce::launch_quantize_rows(src, dtype, rows, cols, ld, (signed char*)q, ldq, scales, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "quantize_rows");
+  return LCE_OK;
+}
+
+int lce_quantize_columns(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* q, int64_t ldq, float* scales,
+                         void* stream) {
+  const int rc = check_quantize(src, dtype, cols, rows, 0, ld, q, ldq, scales);
+  if (rc != LCE_OK) return rc;
+  const hipError_t e = lce::launch_quantize_columns(src, dtype, rows, cols, ld, (signed char*)q, ldq, scales, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "quantize_columns");
+  return LCE_OK;
+}
+
+int lce_int8_logits_workspace_bytes(int64_t N, int64_t H, int64_t V, size_t* bytes) {
+  Int8Plan f;
+  const int rc = plan_int8(N, H, V, &f);
+  if (rc != LCE_OK) return rc;
+  if (!bytes) return LCE_EINVAL_ARG;
+  *bytes = f.total;
+  return LCE_OK;
+}
+
+int lce_int8_logits(const void* x, int x_dtype, int64_t N, int64_t H, int64_t V, int64_t ldx, const int8_t* w, int64_t ldw,
+                    const float* w_scales, float logit_scale, void* out, int out_dtype, int64_t ldo, void* ws, size_t ws_bytes,
+                    void* stream) {
+  Int8Plan f;
+  int rc = plan_int8(N, H, V, &f);
+  if (rc != LCE_OK) return rc;
+  for (const int d : {x_dtype, out_dtype})
+    if (d != LCE_BF16 && d != LCE_F16 && d != LCE_F32) return LCE_EINVAL_DTYPE;
+  if (!(logit_scale > 0.f && logit_scale < INFINITY)) return LCE_EINVAL_ARG;
+  if (N == 0) return LCE_OK;
+  if (!x || !w || !w_scales || !out || ldx < 0 || ldo < V || misaligned(w) || ldw < H || ldw % 16 || ldw > 2 * LCE_INT8_DEPTH) return LCE_EINVAL_ARG;
+  if (((uintptr_t)x & (x_dtype == LCE_F32 ? 3 : 1)) || ((uintptr_t)out & (out_dtype == LCE_F32 ? 3 : 1)) || ((uintptr_t)w_scales & 3))
+    return LCE_EINVAL_ARG;
+  if (!ws || ws_bytes < f.total || misaligned(ws)) return LCE_EWORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  lce::Int8Args a;
+  memset(&a, 0, sizeof(a));
+  a.x = (const signed char*)ws + f.q; a.x_scales = (const float*)((char*)ws + f.scales);
+  a.w = (const signed char*)w; a.w_scales = w_scales; a.out = out;
+  a.N = N; a.V = V; a.ldx = f.ldx; a.ldw = ldw; a.ldo = ldo;
+  a.H = (int)H; a.K2 = (int)(lce::pad_to(H, 16) / 2); a.out_dtype = out_dtype; a.scale = logit_scale;
+  rc = current_num_cus(&a.num_cus, 0, &a.small_wgs);
+  if (rc != LCE_OK) return rc;
+  a.live = lce::live_bands(lce::padded_k(a.K2) * 2);
+  hipError_t e = lce::launch_quantize_rows(x, x_dtype, N, H, ldx, (signed char*)ws + f.q, f.ldx, (float*)((char*)ws + f.scales), s);
+  if (e != hipSuccess) return hip_fail(e, "quantize_rows");
+  e = lce::launch_int8_logits(a, s);
+  if (e != hipSuccess) return hip_fail(e, "int8_logits");
+  return LCE_OK;
+}
+
+namespace {
+// Workgroups of a launch, and with them partial sums: eight to a compute unit of 256 keep enough loads in flight.
+constexpr int kClipGroups = 2048;
+int es_of(int dtype) { return dtype == LCE_F32 ? 4 : 2; }
+
+int check_clip(const lce_tensor* t, int64_t count) {
+  if (count < 0 || count > (int64_t)1 << 20) return LCE_EINVAL_SHAPE;
+  if (count > 0 && !t) return LCE_EINVAL_ARG;
+  for (int64_t i = 0; i < count; ++i) {
+    if (t[i].n < 0 || t[i].n > (int64_t)1 << 40) return LCE_EINVAL_SHAPE;
+    const int d = t[i].dtype, o = t[i].out_dtype;
+    if ((d != LCE_BF16 && d != LCE_F16 && d != LCE_F32) || (o != d && o != LCE_F32)) return LCE_EINVAL_DTYPE;
+    if (t[i].n == 0) continue;
+    if (!t[i].grad || !t[i].out || ((uintptr_t)t[i].grad & (es_of(d) - 1)) || ((uintptr_t)t[i].out & (es_of(o) - 1))) return LCE_EINVAL_ARG;
+    if (t[i].grad == t[i].out && o != d) return LCE_EINVAL_ARG;
+  }
+  return LCE_OK;
+}
+
+// Whether an output shares memory with another output, or with a tensor that is not exactly its own input.
+bool clip_overlaps(const lce_tensor* t, int64_t count) {
+  struct Range {
+    uintptr_t from, to;
+    int64_t of;
+  };
+  std::vector<Range> outs;
+  outs.reserve((size_t)count);
+  for (int64_t i = 0; i < count; ++i)
+    if (t[i].n > 0) outs.push_back({(uintptr_t)t[i].out, (uintptr_t)t[i].out + (uintptr_t)t[i].n * (uintptr_t)es_of(t[i].out_dtype), i});
+  std::sort(outs.begin(), outs.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+  for (size_t i = 1; i < outs.size(); ++i)
+    if (outs[i].from < outs[i - 1].to) return true;
+  for (int64_t i = 0; i < count; ++i) {
+    if (t[i].n == 0 || t[i].grad == t[i].out) continue;
+    const uintptr_t from = (uintptr_t)t[i].grad, to = from + (uintptr_t)t[i].n * (uintptr_t)es_of(t[i].dtype);
+    // (the outputs do not overlap: the last one that begins before `to` is the one that reaches furthest)
+    const auto after = std::lower_bound(outs.begin(), outs.end(), to, [](const Range& r, uintptr_t end) { return r.from < end; });
+    if (after != outs.begin() && (after - 1)->to > from) return true;
+  }
+  return false;
+}
+
+// Stretches of a launch: what its tensors have, cut off where the count would leave 31 bits.
+struct ClipLaunch {
+  int64_t first, last;  // tensors
+  int64_t stretches;
+  int grid;
+};
+int64_t next_clip_launch(const lce_tensor* t, int64_t count, int64_t from, ClipLaunch* l) {
+  l->first = from;
+  l->stretches = 0;
+  int64_t i = from;
+  for (; i < count && i - from < lce::kClipEntries; ++i) {
+    const int64_t n = lce::clip_stretches(t[i].n);
+    if (l->stretches + n > (int64_t)1 << 30) break;
+    l->stretches += n;
+  }
+  l->last = i;
+  l->grid = (int)(l->stretches < 1 ? 1 : l->stretches < kClipGroups ? l->stretches : kClipGroups);
+  return i;
+}
+}  // namespace
+
+int lce_clip_workspace_bytes(const lce_tensor* t, int64_t count, size_t* bytes) {
+  const int rc = check_clip(t, count);
+  if (rc != LCE_OK) return rc;
+  if (!bytes) return LCE_EINVAL_ARG;
+  size_t parts = 1;
+  ClipLaunch l;
+  for (int64_t i = 0; i < count;) {
+    i = next_clip_launch(t, count, i, &l);
+    parts += (size_t)l.grid;
+  }
+  *bytes = align_up(parts * sizeof(double));
+  return LCE_OK;
+}
+
+int lce_clip(const lce_tensor* t, int64_t count, float max_norm, float divisor, const float* divisor_ptr, float* norm, void* ws,
+             size_t ws_bytes, void* stream) {
+  size_t need = 0;
+  const int rc = lce_clip_workspace_bytes(t, count, &need);
+  if (rc != LCE_OK) return rc;
+  if (!(max_norm > 0.f) || (!divisor_ptr && !(divisor > 0.f && divisor < INFINITY)) || !norm) return LCE_EINVAL_ARG;
+  if (!ws || ws_bytes < need || misaligned(ws)) return LCE_EWORKSPACE;
+  try {
+    if (clip_overlaps(t, count)) return LCE_EINVAL_ARG;
+  } catch (...) {  // (no memory for the list)
+    return LCE_EWORKSPACE;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  lce::ClipBatch b;
+  memset(&b, 0, sizeof(b));
+  b.part = (double*)ws;
+  const auto fill = [&](const ClipLaunch& l) {
+    b.count = (int)(l.last - l.first);
+    b.stretches = (unsigned)l.stretches;
+    unsigned first = 0;
+    for (int64_t i = l.first; i < l.last; ++i) {
+      b.e[i - l.first] = {t[i].grad, t[i].out, t[i].n, first, (short)t[i].dtype, (short)t[i].out_dtype};
+      first += (unsigned)lce::clip_stretches(t[i].n);
+    }
+  };
+  ClipLaunch l = {0, 0, 0, 1};
+  int parts = 0;
+  for (int64_t i = 0; i < count;) {
+    i = next_clip_launch(t, count, i, &l);
+    fill(l);
+    b.part0 = parts;
+    const hipError_t e = lce::launch_clip_norm(b, l.grid, s);
+    if (e != hipSuccess) return hip_fail(e, "clip_norm");
+    parts += l.grid;
+  }
+  // (the last launch's tensors first: the last ones read)
+  bool first = true;
+  const int64_t last_start = count > 0 ? l.first : 0;
+  for (int64_t start = last_start; first || start < last_start;) {
+    if (count > 0 && !first) next_clip_launch(t, count, start, &l);
+    if (count > 0) fill(l);
+    const hipError_t e = lce::launch_clip_scale(b, l.grid, parts, max_norm, divisor, divisor_ptr, first ? norm : nullptr, s);
+    if (e != hipSuccess) return hip_fail(e, "clip_scale");
+    start = first ? 0 : l.last;
+    first = false;
+  }
   return LCE_OK;
 }
 

@@ -74,6 +74,7 @@ constexpr int kDzStoreAux = LCE_DZ_STORE_AUX;  // cache policy of the dz stores:
 // place): their upper 16 bits where the hi part will be, the lower 16 where the lo part will be.
 constexpr int kNoLabel = -0x7fffffff - 1;  // ignore_index, or no such row
 constexpr int kOffLabel = -1;              // a label that is no column of W (V <= 2^30): matches nothing
+constexpr int kOffNegative = -2;           // the same, and the row's gain is -1 (BwdArgs::row_signs)
 template <class T, bool ZREG, bool VTAIL, bool FUSE, int NQ>
 LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const float (&pf_lse)[NQ], f32x16_t (&acc)[kNB][NQ],
                               int64_t slice_v0, int64_t tw, char* mine) {
@@ -121,6 +122,7 @@ LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const flo
     // (the power-of-two factor of the staged dz rides along in the exponent)
     nlse[qb] = valid ? fmaf(-l, kLog2e, (float)a.dz_shift) : -INFINITY;  // (FUSE: set per block below)
     gain[qb] = 1.f + 2.f * a.z_reg * l;
+    if (ZREG && !FUSE) gain[qb] = yy == kOffNegative ? -1.f : gain[qb];
     // (with the staging factor 2^10 of fp16 in place: |dz| * 2^10 <= 63 * 2^10 stays finite in fp16 whatever lse is)
     if (a.dz_shift != 0) gain[qb] = fminf(fmaxf(gain[qb], -63.f), 63.f);
     // target column inside this wave's slice, only in the lane half that holds it
@@ -320,11 +322,11 @@ LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const flo
 template <bool FUSE> LCE_DEV void dz_row_scalars(const BwdArgs& a, int64_t rows, int64_t tok, int& y, float& lse) {
   const bool exists = tok < rows;
   const int64_t yy = exists ? a.y[tok] : a.ignore_index;
-  y = yy == a.ignore_index ? kNoLabel : (yy >= 0 && yy < a.V ? (int)yy : kOffLabel);
+  y = yy == a.ignore_index ? kNoLabel : (yy >= 0 && yy < a.V ? (int)yy : a.row_signs && yy == kNegativeRow ? kOffNegative : kOffLabel);
   lse = exists && !FUSE ? a.lse[tok] : 0.f;
 }
 
-// ZREG (z_regularization != 0) is a compile-time switch of the kernels rather than a
+// ZREG (z_regularization != 0, or rows with signs of their own) is a compile-time switch of the kernels rather than a
 // branch inside them: with a branch the compiler hoists the accumulator reads of
 // both arms above it and needs every vector register at once.
 // The launch covers `tiles_p` tile columns of the slab starting at column tile
@@ -495,7 +497,7 @@ hipError_t launch_persistent_z(const BwdArgs& a, hipStream_t s) {
 }
 
 template <class T, bool WVH> hipError_t launch_persistent(const BwdArgs& a, hipStream_t s) {
-  return a.z_reg != 0.f ? launch_persistent_z<T, true, WVH>(a, s) : launch_persistent_z<T, false, WVH>(a, s);
+  return a.z_reg != 0.f || a.row_signs ? launch_persistent_z<T, true, WVH>(a, s) : launch_persistent_z<T, false, WVH>(a, s);
 }
 
 }  // namespace

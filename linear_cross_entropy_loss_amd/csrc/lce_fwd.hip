@@ -249,7 +249,10 @@ __global__ __launch_bounds__(64 * kMergeWaves) void fwd_rows_kernel(const FwdArg
   const bool exists = tok < rows;
   // packed rows: lse goes back to the token's own place; tokens that were dropped get 0 (as every token with an
   // ignored label does, below)
-  if (a.perm != nullptr && g == 1 && tok < a.N && a.y0[tok] == a.ignore_index) a.lse[tok] = 0.f;
+  if (a.perm != nullptr && g == 1 && tok < a.N && a.y0[tok] == a.ignore_index) {
+    a.lse[tok] = 0.f;
+    if (a.tok_logits != nullptr) a.tok_logits[tok] = 0.f;
+  }
   const int nslices = (int)(a.Vp / kChunkV);
 
   // Online (max, sum) merge of this group's slices, 8 at a time so that the loads of a
@@ -291,6 +294,11 @@ __global__ __launch_bounds__(64 * kMergeWaves) void fwd_rows_kernel(const FwdArg
     // packed) or not: a caller sees one thing.  (sh_lse keeps the value: logit_entropy is taken over valid rows only,
     // and the backward never looks at the lse of such a token.)
     if (exists) a.lse[a.perm != nullptr ? packed_token(a.perm, tok, a.N) : tok] = a.y[tok] != a.ignore_index ? lse : 0.f;
+    if (exists && a.tok_logits != nullptr) {
+      const int64_t yy = a.y[tok];
+      const float z = yy == a.ignore_index || yy == a.tok_other ? 0.f : yy >= 0 && yy < a.V ? a.tgt[tok] : __builtin_nanf("");
+      a.tok_logits[a.perm != nullptr ? packed_token(a.perm, tok, a.N) : tok] = z;
+    }
   }
   if (a.monitoring) {
     __syncthreads();
@@ -471,7 +479,7 @@ hipError_t launch_fwd_rows(const FwdArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_fwd_final(const FwdArgs& a, hipStream_t s) {
-  if (final_merge_blocks(a) != 0) return hipSuccess;
+  if (final_merge_blocks(a) != 0 || a.tok_logits != nullptr) return hipSuccess;  // (of single tokens nothing is summed)
   hipLaunchKernelGGL(fwd_final_kernel, dim3(1), dim3(64 * kMergeWaves), 0, s, a);
   return hipGetLastError();
 }

@@ -128,6 +128,10 @@ struct FwdArgs {
   float* tgt;        // [Np]          target logit (written for tokens whose label is a column of W)
   float* blk;        // [Np/64][8]    per-merge-block partial sums (doubles, seven of a block's eight)
   float* lse_rows;   // [Np] or null  lse of every row in the order the tile kernels see them (packed rows), whatever its label
+  // lce_token_logits (null in every other call): the logit of each token's own column, [N] -- 0 where the label is
+  // ignore_index or `tok_other`, NaN where it is any other that is no column
+  float* tok_logits;
+  int64_t tok_other;
 };
 
 struct BwdArgs {
@@ -223,6 +227,10 @@ struct BwdArgs {
   void* dw_plane_hi;
   int dw_acc;
   int vtail_all;  // the logit kernel for the tile column that straddles the end of the vocabulary takes every column
+  // lce_token_logits_backward: rows have upstream gradients of their own.  `lse` then holds lse - log |g_lse|, `y` -1 for no row, V where
+  // g_lse is positive and kNegativeRow where it is negative, and the kernels stage g_lse * softmax, the sign through the gain of z_reg;
+  // the label's column is launch_row_targets'.  n_valid is null there.
+  int row_signs;
 };
 
 // Element offset of block (row tile, column group) of a dz stage that is `vs` columns wide.
@@ -236,7 +244,7 @@ __host__ __device__ inline int64_t dz_block_offset(int64_t row_tile, int64_t gro
 // dz.  With no valid label at all every dz is zero and the factor is taken as 0, so both
 // gradients are exact zeros (what F.cross_entropy's backward gives for such a batch; the loss itself is NaN).
 __device__ __forceinline__ float final_factor_of(const BwdArgs& a) {
-  const int64_t n = a.n_valid[0];
+  const int64_t n = a.n_valid != nullptr ? a.n_valid[0] : 1;
   const float unscale = __builtin_bit_cast(float, (127 - a.dz_shift) << 23);  // 2^-dz_shift
   return n > 0 ? a.grad_out[0] * a.scale / (float)n * unscale : 0.f;
 }
@@ -515,6 +523,73 @@ hipError_t launch_soft_gradient(const BwdArgs& a, const SoftTargets& t, hipStrea
 hipError_t launch_soft_loss(const SoftTargets& t, const int64_t* y, const float* lse, int64_t V, const int64_t* n_valid, double* part,
                             float* loss, hipStream_t s);
 int soft_loss_groups();
+
+// Upstream gradients of each row (lce_tokens.hip): `lse` and `y` as BwdArgs::row_signs has them, of row perm[j] where the rows are packed
+// (perm not null).  With `normalise` the gradients are divided by *factor, the power of two that leaves |grad_lse| + |grad_logits| at
+// most 1 (else *factor = 1); rows whose label is ignore_index do not count.  part: kRowGradientParts floats.
+struct RowGradients {
+  const float* grad_lse;
+  const float* grad_logits;
+  const float* logits;  // of the labels' columns
+  const float* lse;
+  const int64_t* y;
+  int64_t N, V, ignore_index;
+  const int* perm;
+  int normalise;
+  float* row_lse;
+  int64_t* row_y;
+  float* factor;
+  float* part;
+};
+constexpr int kRowGradientParts = 64;
+constexpr int64_t kNegativeRow = -2;
+hipError_t launch_row_gradients(const RowGradients& g, hipStream_t s);
+// dz of the labels' columns of the slab that `a` describes, over what the kernels staged there.
+hipError_t launch_row_targets(const BwdArgs& a, const RowGradients& g, hipStream_t s);
+// out[i] = the column tokens[i] - start where that is one of V, -1 for ignore_index, V for another token of [0, size), V + 1 for what is none.
+hipError_t launch_token_labels(const int64_t* tokens, int64_t N, int64_t ignore_index, int64_t start, int64_t V, int64_t size, int64_t* out,
+                               hipStream_t s);
+
+// Numbers of 8 bits with a scale for each row, and logits from them (lce_int8.hip); strides ldq, ldw and ldx in bytes, multiples of 16.
+hipError_t launch_quantize_rows(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales,
+                                hipStream_t s);
+hipError_t launch_quantize_columns(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales,
+                                   hipStream_t s);
+struct Int8Args {
+  const signed char* x;
+  const signed char* w;
+  const float* x_scales;
+  const float* w_scales;
+  void* out;
+  int64_t N, V, ldx, ldw, ldo;
+  int H, K2;  // numbers in a row; pairs of them, a multiple of 8 (zeros behind the last number of a row of x)
+  int out_dtype;
+  float scale;
+  int num_cus, small_wgs, live;  // as in FwdArgs
+};
+hipError_t launch_int8_logits(const Int8Args& a, hipStream_t s);
+
+// Tensors scaled by their common norm (lce_clip.hip).  The kernels' arguments hold the tensors of one launch (of the 4 KiB that
+// they may take).
+struct ClipEntry {
+  const void* grad;
+  void* out;
+  int64_t n;
+  unsigned first;  // its first stretch among the launch's
+  short dtype, out_dtype;
+};
+constexpr int kClipEntries = 120;
+struct ClipBatch {
+  ClipEntry e[kClipEntries];
+  double* part;
+  int count, part0;  // part0: the launch's first partial sum
+  unsigned stretches;
+};
+int64_t clip_stretches(int64_t n);
+hipError_t launch_clip_norm(const ClipBatch& b, int grid, hipStream_t s);
+// (norm: null except for one of the launches)
+hipError_t launch_clip_scale(const ClipBatch& b, int grid, int parts, float max_norm, float divisor, const float* divisor_ptr, float* norm,
+                             hipStream_t s);
 
 // Selections from rows of logits (lce_select.hip).  A pointer that is not null has one setting for each row.
 struct Sampling {

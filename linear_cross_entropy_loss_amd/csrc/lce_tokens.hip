@@ -1,0 +1,126 @@
+// The logits of given tokens (lce_token_logits): what its two calls need beside the kernels of the loss.
+//
+// With z = scale * x W and lse = log sum exp z the gradients of a row, for upstream gradients g_lse and g_logit of its lse and of the
+// logit of its column y, are those of
+//     dz[v] = g_lse * exp(z[v] - lse) + g_logit * [v == y]
+// The kernels of the loss's backward stage +-exp(z - lse'), lse' = lse - log |g_lse|: no product more than with z-regularisation and no
+// register (a number of its own for each row, held over the last K tiles, put 50 to 100 registers of the dz kernels into memory).
+// lse' is rounded at 24 bits, which moves a probability by a factor of 1 +- 2^-19 at |lse'| < 32, as far as the rounding of its
+// exponent does.  The label's column is written over the stage afterwards, from the logit that the forward gave (row_targets_kernel).
+//
+// fp16: a stage has 30 binary places below 1 while upstream gradients are of any size (1 / rows, times a loss scale), so all are divided
+// by one power of two, which the dx and dW kernels multiply in again after their fp32 sums.
+//
+// All of it is a few numbers a row: bound by launches.
+#include "lce_gemm.h"
+#include "lce_internal.h"
+
+namespace lce {
+
+namespace {
+
+constexpr int kRowThreads = 256;
+
+__device__ float largest_of_workgroup(float m) {
+  __shared__ float sh[kRowThreads / 64];
+  for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = sh[0];
+  for (int i = 1; i < kRowThreads / 64; ++i) m = fmaxf(m, sh[i]);
+  return m;
+}
+
+// part[b] = the largest |g_lse| + |g_logit| of this workgroup's rows (NaN does not count; the rows it is in are NaN anyway).
+__global__ __launch_bounds__(kRowThreads) void row_gradient_max_kernel(const RowGradients g) {
+  float m = 0.f;
+  for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < g.N; i += (int64_t)gridDim.x * kRowThreads)
+    if (g.y[i] != g.ignore_index) m = fmaxf(m, fabsf(g.grad_lse[i]) + fabsf(g.grad_logits[i]));
+  m = largest_of_workgroup(m);
+  if (threadIdx.x == 0) g.part[blockIdx.x] = m;
+}
+
+__global__ __launch_bounds__(kRowThreads) void row_gradients_kernel(const RowGradients g, int parts) {
+  int e = 0;  // the factor is 2^e
+  if (parts > 0) {
+    const float m = largest_of_workgroup((int)threadIdx.x < parts ? g.part[threadIdx.x] : 0.f);
+    if (m > 0.f && m < INFINITY) {
+      (void)frexpf(m, &e);
+      e = e < -126 ? -126 : e > 127 ? 127 : e;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *g.factor = ldexpf(1.f, e);
+  for (int64_t j = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; j < g.N; j += (int64_t)gridDim.x * kRowThreads) {
+    const int64_t n = g.perm != nullptr ? packed_token(g.perm, j, g.N) : j;
+    const float gl = ldexpf(g.grad_lse[n], -e);
+    // (no gradient: exp(z - lse') is 0 whatever the logits.  Finite all the same: the kernels multiply it by a z_reg of 0.)
+    const float l = g.lse[n] - logf(fabsf(gl));
+    g.row_lse[j] = l > 1e30f ? 1e30f : l < -1e30f ? -1e30f : l;
+    g.row_y[j] = g.y[n] == g.ignore_index ? -1 : gl < 0.f ? kNegativeRow : g.V;
+  }
+}
+
+// The staged dz at the labels' columns of this slab: 2^shift * (g_lse * softmax + g_logit), rounded once.
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void row_targets_kernel(const BwdArgs a, const RowGradients g) {
+  const int64_t rows = packed_rows(a.n_rows, a.N);
+  for (int64_t j = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; j < rows; j += (int64_t)gridDim.x * kRowThreads) {
+    const int64_t n = g.perm != nullptr ? packed_token(g.perm, j, g.N) : j;
+    const int64_t yy = g.y[n], rel = yy - a.v0;
+    if (yy == g.ignore_index || yy < 0 || yy >= a.V || rel < 0 || rel >= a.vw) continue;
+    const float f = *g.factor;  // (quotients by a power of two are exact)
+    const float p = __expf(g.logits[n] - g.lse[n]);
+    const float d = ldexpf(fmaf(g.grad_lse[n] / f, p, g.grad_logits[n] / f), a.dz_shift);
+    const int64_t at = (j & (kTile - 1)) * 64 + (rel & 63);
+    unsigned short* dz = reinterpret_cast<unsigned short*>(a.dz);
+    if constexpr (is_pair<T>::value) {
+      dz += 2 * dz_block_offset(j / kTile, rel / 64, a.vs) + at;
+      dz[0] = to_bits<BF16>(d);
+      dz[kDzBlockElems] = to_bits<BF16>(bf16_lo(d));
+    } else {
+      dz[dz_block_offset(j / kTile, rel / 64, a.vs) + at] = to_bits<T>(d);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kRowThreads) void token_labels_kernel(const int64_t* tokens, int64_t N, int64_t ignore_index, int64_t start,
+                                                                   int64_t V, int64_t size, int64_t* out) {
+  for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < N; i += (int64_t)gridDim.x * kRowThreads) {
+    const int64_t t = tokens[i];
+    out[i] = t == ignore_index ? -1 : t < 0 || t >= size ? V + 1 : t >= start && t < start + V ? t - start : V;
+  }
+}
+
+unsigned row_groups(int64_t N, int64_t most) {
+  const int64_t n = (N + kRowThreads - 1) / kRowThreads;
+  return (unsigned)(n < most ? n : most);
+}
+
+}  // namespace
+
+hipError_t launch_row_gradients(const RowGradients& g, hipStream_t s) {
+  const int parts = g.normalise ? (int)row_groups(g.N, kRowGradientParts) : 0;
+  if (parts > 0) {
+    hipLaunchKernelGGL(row_gradient_max_kernel, dim3(parts), dim3(kRowThreads), 0, s, g);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(row_gradients_kernel, dim3(row_groups(g.N, 1024)), dim3(kRowThreads), 0, s, g, parts);
+  return hipGetLastError();
+}
+
+hipError_t launch_row_targets(const BwdArgs& a, const RowGradients& g, hipStream_t s) {
+  const dim3 grid(row_groups(a.N, 1024)), threads(kRowThreads);
+  if (a.x_dtype == DT_PAIR) hipLaunchKernelGGL(row_targets_kernel<BF16P>, grid, threads, 0, s, a, g);
+  else if (a.x_dtype == DT_F16) hipLaunchKernelGGL(row_targets_kernel<F16>, grid, threads, 0, s, a, g);
+  else hipLaunchKernelGGL(row_targets_kernel<BF16>, grid, threads, 0, s, a, g);
+  return hipGetLastError();
+}
+
+hipError_t launch_token_labels(const int64_t* tokens, int64_t N, int64_t ignore_index, int64_t start, int64_t V, int64_t size, int64_t* out,
+                               hipStream_t s) {
+  hipLaunchKernelGGL(token_labels_kernel, dim3(row_groups(N, 1024)), dim3(kRowThreads), 0, s, tokens, N, ignore_index, start, V, size, out);
+  return hipGetLastError();
+}
+
+}  // namespace lce

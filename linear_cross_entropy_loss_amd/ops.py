@@ -788,5 +788,19 @@ class LinearCrossEntropyLoss(torch.nn.Linear):
 
         return linear_distillation(x, self.weight, index, logits, temperature, self.logit_scale, self.N_chunk_size)
 
+    def log_probs(self, x, tokens):
+        """Log-probability of each row's token under ``x`` (``linear_token_logits``), with this module's weight, ignore_index, logit_scale
+        and N_chunk_size: float32, of the shape of ``tokens``, 0 where a token is ignore_index; differentiable."""
+        from .token_logits import linear_token_logits
+
+        logits, lse = linear_token_logits(x, self.weight, tokens, self.ignore_index, self.logit_scale, self.N_chunk_size)
+        return logits - lse
+
+    def quantize(self):
+        """This module's weight as it is now in 8 bits, for ``quantized_logits``."""
+        from .quantization import quantize_weight
+
+        return quantize_weight(self.weight)
+
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias=False"
