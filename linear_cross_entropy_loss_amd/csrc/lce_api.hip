@@ -1825,9 +1825,10 @@ int lce_quantize_rows(const void* src, int dtype, int64_t rows, int64_t cols, in
 
 int lce_quantize_columns(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* q, int64_t ldq, float* scales,
                          void* stream) {
-  const int rc = check_quantize(src, dtype, cols, rows, 0, ld, q, ldq, scales);
+  int rc = check_quantize(src, dtype, cols, rows, 0, ld, q, ldq, scales), num_cus = 0;
+  if (rc == LCE_OK) rc = current_num_cus(&num_cus, 0);
   if (rc != LCE_OK) return rc;
-  const hipError_t e = lce::launch_quantize_columns(src, dtype, rows, cols, ld, (signed char*)q, ldq, scales, (hipStream_t)stream);
+  const hipError_t e = lce::launch_quantize_columns(src, dtype, rows, cols, ld, (signed char*)q, ldq, scales, num_cus, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "quantize_columns");
   return LCE_OK;
 }

@@ -27,111 +27,396 @@ namespace {
 struct __attribute__((packed, aligned(2))) Piece {
   u32x4_t v;
 };
+// The same, of what is not read again.
+LCE_DEV u32x4_t load_once(const void* p) {
+  typedef u32x4_t __attribute__((aligned(2))) any_t;
+  return __builtin_nontemporal_load(reinterpret_cast<const any_t*>(p));
+}
 
 // ---------------------------------------------------------------------------
 // Quantising
 // ---------------------------------------------------------------------------
-template <class S> LCE_DEV float number(S v);
-template <> LCE_DEV float number<float>(float v) { return v; }
-template <> LCE_DEV float number<__bf16>(__bf16 v) { return (float)v; }
-template <> LCE_DEV float number<_Float16>(_Float16 v) { return (float)v; }
+// Elements as the kernels read them: 16 bytes at a time.
+template <int DT> struct Source {
+  static constexpr int kPer = 8;
+  typedef unsigned short S;
+  static LCE_DEV float get(S b) { return DT == DT_BF16 ? from_bits<BF16>(b) : from_bits<F16>(b); }
+};
+template <> struct Source<DT_F32> {
+  static constexpr int kPer = 4;
+  typedef float S;
+  static LCE_DEV float get(S f) { return f; }
+};
+// The piece at column c of a row of `cols`, zeros behind its end.
+template <int DT, bool ONCE = false> LCE_DEV u32x4_t load_piece(const typename Source<DT>::S* row, int c, int cols) {
+  constexpr int kPer = Source<DT>::kPer;
+  if (c + kPer <= cols) return ONCE ? load_once(row + c) : reinterpret_cast<const Piece*>(row + c)->v;
+  typename Source<DT>::S e[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) e[i] = c + i < cols ? row[c + i] : (typename Source<DT>::S)0;
+  u32x4_t v;
+  __builtin_memcpy(&v, e, 16);
+  return v;
+}
+template <int DT> LCE_DEV void numbers(u32x4_t v, float (&f)[Source<DT>::kPer]) {
+  typename Source<DT>::S e[Source<DT>::kPer];
+  __builtin_memcpy(e, &v, 16);
+#pragma unroll
+  for (int i = 0; i < Source<DT>::kPer; ++i) f[i] = Source<DT>::get(e[i]);
+}
+// Element k of a piece (k need not be known to the compiler).
+template <int DT> LCE_DEV float element(u32x4_t v, int k) {
+  const int i = DT == DT_F32 ? k : k >> 1;
+  const unsigned w = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
+  if constexpr (DT == DT_F32) return __builtin_bit_cast(float, w);
+  else return Source<DT>::get((unsigned short)(w >> (16 * (k & 1))));
+}
+LCE_DEV unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
+// The largest magnitudes of pieces, element by element, as bits (of 16-bit types two to a word: their order is that of the numbers).
+template <int DT> LCE_DEV u32x4_t larger_piece(u32x4_t a, u32x4_t v) {
+  if constexpr (DT == DT_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = larger(a[i], v[i] & 0x7fffffffu);
+  } else {
+    typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned was = a[i], now = v[i] & 0x7fff7fffu;  // (a bit cast of a vector's element itself is one of its first)
+      a[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, was), __builtin_bit_cast(u16x2_t, now)));
+    }
+  }
+  return a;
+}
+// One element's, as those of the float32 number.
+template <int DT> LCE_DEV unsigned magnitude(u32x4_t v, int i) { return __builtin_bit_cast(unsigned, element<DT>(v, i)); }
 
-// What a row's numbers are multiplied by, from the largest magnitude among them as bits (of which NaN and infinity are the largest).
+// The scale of a row, from the largest magnitude among its numbers as bits (of which NaN and infinity are the largest).
 struct RowScale {
-  float top, inverse;  // inverse: 127 / top, 0 for a row of zeros or one that is not finite
-  float scale;
-  bool tiny;           // 127 / top is no float32 number: the quotient is taken in doubles
+  float top, scale;
+  bool finite;
   LCE_DEV explicit RowScale(unsigned bits) {
-    const bool finite = bits < 0x7f800000u;
     top = __builtin_bit_cast(float, bits);
-    tiny = top < 1e-30f && bits != 0;
-    inverse = finite && bits != 0 && !tiny ? 127.f / top : 0.f;
+    finite = bits < 0x7f800000u;
     scale = finite ? (float)((double)top / 127.0) : __builtin_nanf("");
   }
 };
-// The whole number nearest to 127 v / top.  The product with the rounded inverse is off by less than 2^-15; within that of a border
-// the two sides are compared as 127 |v| and (k + 1/2) top, which doubles hold exactly.
-LCE_DEV int quantized(float v, const RowScale& r) {
-  if (r.tiny) return (int)rint((double)v * 127.0 / (double)r.top);
-  const float t = v * r.inverse;
-  float q = __builtin_rintf(t);
-  const float off = fabsf(t - q);
-  if (off > 0.49996f && r.inverse != 0.f) {
-    const float k = floorf(fabsf(t));
-    const double a = 127.0 * (double)fabsf(v), b = ((double)k + 0.5) * (double)r.top;
-    const float m = a > b || (a == b && ((int)k & 1)) ? k + 1.f : k;
-    q = copysignf(m, t);
+// The whole number nearest to 127 v / top, as the lowest byte of what byte_of returns: v times 127 / top, plus 3 * 2^22, whose last place
+// is 1.
+//
+// 16-bit types.  127 v and top have at most 18 and 11 bits, so a quotient Q that is not half way between two whole numbers is at
+// least Q * 2^-19 away from there, while the product with the rounded 127 / top is off by at most Q * 2^-23: rounded to 20 bits first it
+// is on the half way exactly where Q is, and on Q's side of it elsewhere.  (In bf16 every thousandth number is half its row's largest, which
+// is 63.5.)
+//
+// float32.  The product with a float below 127 / top and with one above, each rounded once: where both give the same, so does the
+// quotient; where they do not, one number in 10^5, `differ` is not 0 afterwards and exact_byte decides.
+//
+// Rows whose 127 / top is no ordinary number have 0 for both (a row of zeros), or go by exact_byte altogether (`odd`).
+struct Inverse {
+  float near, below, above;
+  bool odd;
+  LCE_DEV Inverse() {}
+  LCE_DEV explicit Inverse(const RowScale& r) {
+    odd = !r.finite || (r.top < 1e-30f && r.top > 0.f);
+    near = odd || r.top == 0.f ? 0.f : 127.f / r.top;
+    const unsigned bits = __builtin_bit_cast(unsigned, near);
+    below = near == 0.f ? 0.f : __builtin_bit_cast(float, bits - 1);
+    above = near == 0.f ? 0.f : __builtin_bit_cast(float, bits + 1);
   }
-  return (int)q;
+};
+constexpr float kWhole = 12582912.f;
+template <int DT> LCE_DEV unsigned byte_of(float v, const Inverse& i, unsigned& differ) {
+  if constexpr (DT == DT_F32) {
+    const unsigned a = __builtin_bit_cast(unsigned, fmaf(v, i.below, kWhole));
+    const unsigned b = __builtin_bit_cast(unsigned, fmaf(v, i.above, kWhole));
+    differ |= a ^ b;
+    return a;
+  } else {
+    const unsigned t = __builtin_bit_cast(unsigned, v * i.near);
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(float, (t + 8) & ~15u) + kWhole);
+  }
 }
-LCE_DEV unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+// By comparing 127 |v| with (k + 1/2) top, which doubles hold exactly.
+LCE_DEV unsigned exact_byte(float v, const RowScale& r) {
+  if (!r.finite) return 0u;
+  if (r.top < 1e-30f) return r.top > 0.f ? (unsigned)(int)rint((double)v * 127.0 / (double)r.top) : 0u;
+  const float t = fabsf(v) * (127.f / r.top), k = floorf(t);
+  if (fabsf(t - k - 0.5f) > 0.01f) return (unsigned)(int)copysignf(rintf(t), v);
+  const double a = 127.0 * (double)fabsf(v), b = ((double)k + 0.5) * (double)r.top;
+  return (unsigned)(int)copysignf(a > b || (a == b && ((int)k & 1)) ? k + 1.f : k, v);
+}
+// The lowest bytes of four, in their order.
+LCE_DEV unsigned four_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+  return lo | hi << 16;
+}
 
+// Rows.  WAVES waves to a row (one, of four rows to a workgroup, where that holds the row in registers and there are many; else
+// a workgroup); a row of up to 64 * WAVES * PIECES pieces is read once, a longer one twice.  131072 x 2048 bf16 136 us, 5.9 TB/s.
 constexpr int kQuantThreads = 256;
-// Rows, one workgroup each.
-template <class S>
-__global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const S* src, int64_t rows, int cols, int64_t ld, signed char* q, int64_t ldq,
+template <int DT> LCE_DEV void store_bytes(u32x4_t piece, const RowScale& s, const Inverse& inverse, signed char* to) {
+  constexpr int kPer = Source<DT>::kPer;
+  float f[kPer];
+  numbers<DT>(piece, f);
+  unsigned b[kPer], differ = inverse.odd;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) b[i] = byte_of<DT>(f[i], inverse, differ);
+  if (differ == 0) {
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) reinterpret_cast<unsigned*>(to)[i / 4] = four_bytes(b[i], b[i + 1], b[i + 2], b[i + 3]);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kPer; ++i) to[i] = (signed char)exact_byte(element<DT>(piece, i), s);
+  }
+}
+template <int DT, int WAVES, int PIECES>
+__global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void* src, int64_t rows, int cols, int64_t ld, signed char* q, int ldq,
                                                                       float* scales) {
+  typedef Source<DT> E;
+  constexpr int kStep = 64 * WAVES * E::kPer;
   __shared__ unsigned sh[kQuantThreads / 64];
-  const int64_t r = blockIdx.x;
-  const S* from = src + r * ld;
+  const int wave = threadIdx.x >> 6;
+  const int64_t r = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+  if (r >= rows) return;
+  const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const typename E::S* from = reinterpret_cast<const typename E::S*>(src) + r * ld;
+  const bool once = cols <= kStep * PIECES;
+  u32x4_t v[PIECES], tops = {0, 0, 0, 0};
+  for (int c0 = 0; c0 < cols; c0 += kStep * PIECES) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) v[i] = load_piece<DT, WAVES == 1>(from, c0 + i * kStep + t * E::kPer, cols);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) tops = larger_piece<DT>(tops, v[i]);
+  }
   unsigned top = 0;
-  for (int c = threadIdx.x; c < cols; c += kQuantThreads) {
-    const unsigned m = magnitude(number(from[c]));
-    top = m > top ? m : top;
-  }
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const unsigned o = (unsigned)__shfl_xor((int)top, d);
-    top = o > top ? o : top;
-  }
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
-  __syncthreads();
+  for (int k = 0; k < E::kPer; ++k) top = larger(top, magnitude<DT>(tops, k));
 #pragma unroll
-  for (int i = 0; i < kQuantThreads / 64; ++i) top = sh[i] > top ? sh[i] : top;
+  for (int d = 1; d < 64; d <<= 1) top = larger(top, (unsigned)__shfl_xor((int)top, d));
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) sh[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) top = larger(top, sh[i]);
+  }
   const RowScale s(top);
-  if (threadIdx.x == 0) scales[r] = s.scale;
-  for (int c = threadIdx.x; c < ldq; c += kQuantThreads) q[r * ldq + c] = c < cols && s.scale == s.scale ? (signed char)quantized(number(from[c]), s) : 0;
+  const Inverse inverse(s);
+  if (t == 0) scales[r] = s.scale;
+  signed char* to = q + r * ldq;
+  for (int c0 = 0; c0 < ldq; c0 += kStep * PIECES)
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int c = c0 + i * kStep + t * E::kPer;
+      if (c < ldq) store_bytes<DT>(once ? v[i] : load_piece<DT>(from, c, cols), s, inverse, to + c);
+    }
 }
 
-// Columns: a workgroup takes 64 of them, twice: for the largest magnitudes, then in tiles of 128 rows, which are turned in LDS.
+// Columns.  A workgroup of NT threads takes stripes of COLS of them, one after another.  It holds a stripe in registers -- kTiles * 4 pieces
+// to a thread -- until the largest magnitudes are known, and turns it in LDS, a tile of rows at a time, four rows of a piece to a
+// thread, so that q is written in stretches of 128 bytes and more; a tile's registers take the next stripe's as soon as it is in LDS.
+// The weight is read once.  Two neighbouring stripes, which may share lines, go to one XCD.
+// Bound by memory, 2048 x 131072 bf16 in 172 us, 4.7 TB/s read and written (the same without the quantising itself; reading alone 126).  Reading
+// the weight twice, an element to a load, took 625; twice with 16 bytes 300; held, without the next stripe under way, 204.
+constexpr int kTiles = 4;
+template <int DT, int NT, int COLS, bool ONCE>
+__global__ __launch_bounds__(NT, 4) void quantize_held_columns_kernel(const void* src, int rows, int64_t cols, int64_t ld, signed char* q, int ldq,
+                                                                      float* scales) {
+  typedef Source<DT> E;
+  constexpr int kPer = E::kPer, kPieces = COLS / kPer, kQuads = NT / kPieces;  // fours of rows in a tile
+  constexpr int kWords = kQuads + 2;  // of a line in LDS: the lanes of a wave write to different banks
+  __shared__ unsigned sh_top[COLS];
+  __shared__ Inverse sh_inverse[COLS];
+  __shared__ unsigned sh_q[2][COLS * kWords];
+  const int t = threadIdx.x, c = t % kPieces * kPer, quad = t / kPieces;
+  // (the last stripe ends with the last column: some columns are then done twice, alike)
+  const auto place = [&](int id) { return (((int64_t)(id >> 4) * 8 + (id & 7)) * 2 + (id >> 3 & 1)) * COLS; };
+  const auto stripe = [&](int id) { return place(id) < cols - COLS ? place(id) : cols - COLS; };
+  u32x4_t v[kTiles][4];
+  const unsigned mine = (unsigned)(((int64_t)quad * 4 * ld + c) * (int64_t)sizeof(typename E::S));  // of a thread in a tile: 32 bits
+  const auto load_tile = [&](int64_t c0, int u) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = u * kQuads * 4 + j;  // (uniform)
+      const char* from = reinterpret_cast<const char*>(reinterpret_cast<const typename E::S*>(src) + c0 + (int64_t)r * ld);
+      v[u][j] = u32x4_t{0, 0, 0, 0};
+      if (r + quad * 4 < rows) v[u][j] = ONCE ? load_once(from + mine) : reinterpret_cast<const Piece*>(from + mine)->v;
+    }
+  };
+  int id = blockIdx.x;
+  if (place(id) >= cols) return;
+  int64_t c0 = stripe(id);
+#pragma unroll
+  for (int u = 0; u < kTiles; ++u) load_tile(c0, u);
+  for (bool more = true; more; id += gridDim.x) {
+    more = place(id + (int)gridDim.x) < cols;  // (a workgroup's stripes come from left to right)
+    const int64_t next = more ? stripe(id + (int)gridDim.x) : 0;
+    if (t < COLS) sh_top[t] = 0;
+    __syncthreads();
+    u32x4_t tops = {0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tops = larger_piece<DT>(tops, v[u][j]);
+#pragma unroll
+    for (int d = kPieces; d < 64; d <<= 1) {
+      u32x4_t o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = (unsigned)__shfl_xor((int)tops[i], d);
+      tops = larger_piece<DT>(tops, o);
+    }
+    if ((t & 63) < kPieces) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) atomicMax(&sh_top[c + k], magnitude<DT>(tops, k));
+    }
+    __syncthreads();
+    if (t < COLS) {
+      const RowScale s(sh_top[t]);
+      sh_inverse[t] = Inverse(s);
+      scales[c0 + t] = s.scale;
+    }
+    __syncthreads();
+    Inverse inverse[kPer];
+    bool odd = false;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      inverse[k] = sh_inverse[c + k];
+      odd |= inverse[k].odd;
+    }
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u) {
+      const int r0 = u * kQuads * 4;
+      if (r0 >= ldq) break;
+      unsigned* tile = sh_q[u & 1];
+      unsigned differ = odd;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(v[u][j]));  // (or the compiler keeps the numbers of all tiles, in twice the registers)
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        unsigned b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = byte_of<DT>(element<DT>(v[u][j], k), inverse[k], differ);
+        tile[(c + k) * kWords + quad] = four_bytes(b[0], b[1], b[2], b[3]);
+      }
+      if (differ != 0) {
+#pragma unroll 1
+        for (int k = 0; k < kPer; ++k) {  // (rare)
+          const RowScale s(sh_top[c + k]);
+          unsigned b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = exact_byte(element<DT>(v[u][j], k), s);
+          tile[(c + k) * kWords + quad] = four_bytes(b[0], b[1], b[2], b[3]);
+        }
+      }
+      if (more) load_tile(next, u);
+      __syncthreads();  // (the one of the next tile parts this tile's readers from the writers of the one after it)
+      // 32 bytes of a line to a thread
+      for (int line = t / (kQuads / 8); line < COLS; line += NT / (kQuads / 8)) {
+        const int part = t % (kQuads / 8) * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4_t o;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = tile[line * kWords + part + h * 4 + i];
+          const int at = r0 + (part + h * 4) * 4;
+          if (at < ldq) *reinterpret_cast<u32x4_t*>(q + (c0 + line) * ldq + at) = o;
+        }
+      }
+    }
+    c0 = next;
+  }
+}
+
+// The same for columns that the registers do not hold: a stripe of 64 is read twice, for the largest magnitudes and then in tiles of
+// 128 rows.
 constexpr int kColTile = 64, kRowTile = 128, kLineWords = kRowTile / 4 + 1;
-template <class S>
-__global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const S* src, int rows, int64_t cols, int64_t ld, signed char* q,
-                                                                         int64_t ldq, float* scales) {
+template <int DT>
+__global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const void* src, int rows, int64_t cols, int64_t ld, signed char* q, int ldq,
+                                                                         float* scales) {
+  typedef Source<DT> E;
+  constexpr int kPer = E::kPer, kPieces = kColTile / kPer, kRowsAtOnce = kQuantThreads / kPieces;  // pieces of a row of the stripe
+  constexpr int kTurns = kRowTile / 4 / kRowsAtOnce;                                              // of four rows, to a tile
   __shared__ unsigned sh_top[kColTile];
+  __shared__ Inverse sh_inverse[kColTile];
   __shared__ unsigned sh_q[kColTile * kLineWords];
   const int t = threadIdx.x;
   const int64_t c0 = (int64_t)blockIdx.x * kColTile;
   const int width = cols - c0 < kColTile ? (int)(cols - c0) : kColTile;
+  const typename E::S* from = reinterpret_cast<const typename E::S*>(src) + c0;
   if (t < kColTile) sh_top[t] = 0;
   __syncthreads();
-  const int c = t & (kColTile - 1);
-  unsigned top = 0;
+  const int c = t % kPieces * kPer, r1 = t / kPieces;
+  u32x4_t tops = {0, 0, 0, 0};
+  constexpr int kFlight = 8;
   if (c < width)
-    for (int r = t / kColTile; r < rows; r += kQuantThreads / kColTile) {
-      const unsigned m = magnitude(number(src[r * ld + c0 + c]));
-      top = m > top ? m : top;
-    }
-  atomicMax(&sh_top[c], top);
-  __syncthreads();
-  const RowScale s(sh_top[c]);
-  if (t < width) scales[c0 + t] = s.scale;
-  for (int r0 = 0; r0 < ldq; r0 += kRowTile) {
-    // four rows of one column to a thread at a time
-    for (int i = t / kColTile; i < kRowTile / 4; i += kQuantThreads / kColTile) {
-      unsigned w = 0;
+    for (int r0 = r1; r0 < rows; r0 += kFlight * kRowsAtOnce) {
+      u32x4_t v[kFlight];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = r0 + 4 * i + k;
-        const int n = c < width && r < rows && s.scale == s.scale ? quantized(number(src[r * ld + c0 + c]), s) : 0;
-        w |= (unsigned)(n & 255) << (8 * k);
+      for (int i = 0; i < kFlight; ++i) {
+        const int r = r0 + i * kRowsAtOnce;
+        v[i] = load_piece<DT>(from + (int64_t)(r < rows ? r : r0) * ld, c, width);
       }
-      sh_q[c * kLineWords + i] = w;
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) tops = larger_piece<DT>(tops, v[i]);
     }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) atomicMax(&sh_top[c + k], magnitude<DT>(tops, k));
+  __syncthreads();
+  if (t < kColTile) {
+    const RowScale s(sh_top[t]);
+    sh_inverse[t] = Inverse(s);
+    if (t < width) scales[c0 + t] = s.scale;
+  }
+  __syncthreads();
+  Inverse inverse[kPer];
+  bool odd = false;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    inverse[k] = sh_inverse[c + k];
+    odd |= inverse[k].odd;
+  }
+  u32x4_t v[kTurns][4];
+  const auto load_tile = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + 4 * (i * kRowsAtOnce + r1) + j;
+        v[i][j] = c < width && r < rows ? load_piece<DT>(from + (int64_t)r * ld, c, width) : u32x4_t{0, 0, 0, 0};
+      }
+  };
+  load_tile(0);
+  for (int r0 = 0; r0 < ldq; r0 += kRowTile) {
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      float f[4][kPer];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) numbers<DT>(v[i][j], f[j]);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        unsigned b[4], differ = odd;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = byte_of<DT>(f[j][k], inverse[k], differ);
+        if (differ != 0) {
+          const RowScale s(sh_top[c + k]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = exact_byte(f[j][k], s);
+        }
+        sh_q[(c + k) * kLineWords + i * kRowsAtOnce + r1] = four_bytes(b[0], b[1], b[2], b[3]);
+      }
+    }
+    if (r0 + kRowTile < ldq) load_tile(r0 + kRowTile);
     __syncthreads();
-    for (int i = t; i < kColTile * (kRowTile / 4); i += kQuantThreads) {
-      const int line = i / (kRowTile / 4), word = i % (kRowTile / 4);
-      if (line < width && r0 + 4 * word < ldq) *reinterpret_cast<unsigned*>(q + (c0 + line) * ldq + r0 + 4 * word) = sh_q[line * kLineWords + word];
+    // 32 bytes of a line to a thread
+    const int line = t >> 2, part = (t & 3) * 8;
+    if (line < width) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4_t o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = sh_q[line * kLineWords + part + h * 4 + i];
+        const int at = r0 + (part + h * 4) * 4;
+        if (at < ldq) *reinterpret_cast<u32x4_t*>(q + (c0 + line) * ldq + at) = o;
+      }
     }
     __syncthreads();
   }
@@ -311,16 +596,42 @@ template <class T> hipError_t launch_product(const Int8Args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <class S>
+template <int DT>
 hipError_t quantize_rows(const void* src, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales, hipStream_t s) {
-  hipLaunchKernelGGL(quantize_rows_kernel<S>, dim3((unsigned)rows), dim3(kQuantThreads), 0, s, reinterpret_cast<const S*>(src), rows, (int)cols,
-                     ld, q, ldq, scales);
+  constexpr int kPer = Source<DT>::kPer;
+  const dim3 fours((unsigned)((rows + 3) / 4)), ones((unsigned)rows), threads(kQuantThreads);
+  const auto go = [&](auto kernel, dim3 grid) { hipLaunchKernelGGL(kernel, grid, threads, 0, s, src, rows, (int)cols, ld, q, (int)ldq, scales); };
+  if (rows < 1024 || cols > 64 * kPer * 8) go(quantize_rows_kernel<DT, 4, 32 / kPer>, ones);
+  else if (cols > 64 * kPer * 4) go(quantize_rows_kernel<DT, 1, 8>, fours);
+  else if (cols > 64 * kPer * 2) go(quantize_rows_kernel<DT, 1, 4>, fours);
+  else go(quantize_rows_kernel<DT, 1, 2>, fours);
   return hipGetLastError();
 }
-template <class S>
-hipError_t quantize_columns(const void* src, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales, hipStream_t s) {
-  hipLaunchKernelGGL(quantize_columns_kernel<S>, dim3((unsigned)((cols + kColTile - 1) / kColTile)), dim3(kQuantThreads), 0, s,
-                     reinterpret_cast<const S*>(src), (int)rows, cols, ld, q, ldq, scales);
+template <int DT, int NT, int COLS>
+hipError_t quantize_held_columns(const void* src, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales, int num_cus,
+                                 hipStream_t s) {
+  const int64_t stripes = pad_to((cols + COLS - 1) / COLS, 16);
+  const int64_t most = pad_to((int64_t)num_cus * (1024 / NT), 16);  // (as many workgroups as the compute units hold at a time)
+  const dim3 grid((unsigned)(stripes < most ? stripes : most));
+  // (past the caches where no two stripes share a line: 2048 x 131072 bf16 192 us, so 168; but 768 x 50257, whose stripes do, 31 and 39)
+  constexpr int kEs = DT == DT_F32 ? 4 : 2;
+  if (COLS * kEs % 128 == 0 && ld * kEs % 128 == 0 && reinterpret_cast<uintptr_t>(src) % 128 == 0)
+    hipLaunchKernelGGL((quantize_held_columns_kernel<DT, NT, COLS, true>), grid, dim3(NT), 0, s, src, (int)rows, cols, ld, q, (int)ldq, scales);
+  else
+    hipLaunchKernelGGL((quantize_held_columns_kernel<DT, NT, COLS, false>), grid, dim3(NT), 0, s, src, (int)rows, cols, ld, q, (int)ldq, scales);
+  return hipGetLastError();
+}
+template <int DT>
+hipError_t quantize_columns(const void* src, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales, int num_cus,
+                            hipStream_t s) {
+  constexpr int kRows = 4 * kTiles * Source<DT>::kPer;  // numbers that a thread holds
+  // (offsets within a tile of the rows have 32 bits)
+  const bool held = cols >= 64 && ld * (DT == DT_F32 ? 4 : 2) * 1024 < (int64_t)1 << 31;
+  if (held && rows <= 512 * kRows / 64) return quantize_held_columns<DT, 512, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+  if (held && rows <= 1024 * kRows / 64) return quantize_held_columns<DT, 1024, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+  if (held && rows <= 1024 * kRows / 32) return quantize_held_columns<DT, 1024, 32>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+  hipLaunchKernelGGL(quantize_columns_kernel<DT>, dim3((unsigned)((cols + kColTile - 1) / kColTile)), dim3(kQuantThreads), 0, s, src, (int)rows,
+                     cols, ld, q, (int)ldq, scales);
   return hipGetLastError();
 }
 
@@ -328,15 +639,15 @@ hipError_t quantize_columns(const void* src, int64_t rows, int64_t cols, int64_t
 
 hipError_t launch_quantize_rows(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales,
                                 hipStream_t s) {
-  return dtype == DT_BF16  ? quantize_rows<__bf16>(src, rows, cols, ld, q, ldq, scales, s)
-         : dtype == DT_F16 ? quantize_rows<_Float16>(src, rows, cols, ld, q, ldq, scales, s)
-                           : quantize_rows<float>(src, rows, cols, ld, q, ldq, scales, s);
+  return dtype == DT_BF16  ? quantize_rows<DT_BF16>(src, rows, cols, ld, q, ldq, scales, s)
+         : dtype == DT_F16 ? quantize_rows<DT_F16>(src, rows, cols, ld, q, ldq, scales, s)
+                           : quantize_rows<DT_F32>(src, rows, cols, ld, q, ldq, scales, s);
 }
 hipError_t launch_quantize_columns(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales,
-                                   hipStream_t s) {
-  return dtype == DT_BF16  ? quantize_columns<__bf16>(src, rows, cols, ld, q, ldq, scales, s)
-         : dtype == DT_F16 ? quantize_columns<_Float16>(src, rows, cols, ld, q, ldq, scales, s)
-                           : quantize_columns<float>(src, rows, cols, ld, q, ldq, scales, s);
+                                   int num_cus, hipStream_t s) {
+  return dtype == DT_BF16  ? quantize_columns<DT_BF16>(src, rows, cols, ld, q, ldq, scales, num_cus, s)
+         : dtype == DT_F16 ? quantize_columns<DT_F16>(src, rows, cols, ld, q, ldq, scales, num_cus, s)
+                           : quantize_columns<DT_F32>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
 }
 hipError_t launch_int8_logits(const Int8Args& a, hipStream_t s) {
   return a.out_dtype == DT_BF16 ? launch_product<BF16>(a, s) : a.out_dtype == DT_F16 ? launch_product<F16>(a, s) : launch_product<float>(a, s);

@@ -554,7 +554,7 @@ hipError_t launch_token_labels(const int64_t* tokens, int64_t N, int64_t ignore_
 hipError_t launch_quantize_rows(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales,
                                 hipStream_t s);
 hipError_t launch_quantize_columns(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales,
-                                   hipStream_t s);
+                                   int num_cus, hipStream_t s);
 struct Int8Args {
   const signed char* x;
   const signed char* w;
