@@ -37,6 +37,10 @@ def _check(grads, out, max_norm, divisor):
         raise ValueError(f"clip_gradients: divisor must be positive and finite in float32, got {divisor}")
 
 
+def _raise(rc, what):
+    _lib.raise_for_status(rc, what + ": tensors that are written share memory, or" if rc == _lib.LCE_EINVAL_ARG else what)
+
+
 @torch.compiler.disable
 @torch.no_grad()
 def clip_gradients(grads, max_norm, divisor=1.0, out=None):
@@ -65,6 +69,14 @@ def clip_gradients(grads, max_norm, divisor=1.0, out=None):
         grads, out = [grads[i] for i in kept], [out[i] for i in kept]
     max_norm = float(max_norm)
     divisor = divisor if isinstance(divisor, torch.Tensor) else float(divisor)
+    by_ptr = isinstance(divisor, torch.Tensor)
+    if grads and max_norm > 0 and isinstance(grads[0], torch.Tensor) and grads[0].is_cuda and (
+            grads[0].device.index == torch._C._cuda_getDevice()) and (by_ptr or _lib.F32_ZERO < divisor < _lib.F32_INF):
+        done = _lib.host().clip(grads, out, max_norm, 1.0 if by_ptr else divisor, divisor if by_ptr else None, _stream(grads[0].device))
+        if isinstance(done, torch.Tensor):
+            return done
+        if done is not None:
+            _raise(*done)
     _check(grads, out, max_norm, divisor)
     if not grads:
         raise ValueError("clip_gradients: there are no gradients")
@@ -87,10 +99,9 @@ def clip_gradients(grads, max_norm, divisor=1.0, out=None):
         _lib.raise_for_status(lib.lce_clip_workspace_bytes(tasks, len(tasks), ctypes.byref(b)), "clip_gradients")
         ws = torch.empty(b.value, dtype=torch.uint8, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        by_ptr = isinstance(divisor, torch.Tensor)
         rc = lib.lce_clip(tasks, len(tasks), max_norm, 1.0 if by_ptr else divisor, _ptr(divisor) if by_ptr else None, _ptr(norm), _ptr(ws),
                           b.value, _stream(dev))
-        _lib.raise_for_status(rc, "clip_gradients: outputs share memory, or" if rc == _lib.LCE_EINVAL_ARG else "clip_gradients")
+        _raise(rc, "clip_gradients")
         for o, to in late:
             o.copy_(to)
         torch.autograd.graph.increment_version(out)  # (written behind autograd's back)

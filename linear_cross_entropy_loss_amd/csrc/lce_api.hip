@@ -1222,7 +1222,7 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
     a.y = rows->row_y;
     a.ignore_index = -1;
     a.grad_out = rows->factor;
-    a.n_valid = nullptr;
+    a.n_valid = rows->one;
     // (normalised rows: |dz| <= 2, times 2^14 within fp16's range; probabilities stay normal down to 2^-28)
     a.dz_shift = rows->normalise ? 14 : 0;
   }
@@ -1736,7 +1736,7 @@ int plan_token_backward(const lce_problem* q, TokenPlan* t) {
   size_t o = align_up(t->b.total);
   t->row_lse = o; o += align_up((size_t)q->N * 4);
   t->row_y = o; o += align_up((size_t)q->N * 8);
-  t->part = o; o += align_up((size_t)(lce::kRowGradientParts + 1) * 4);
+  t->part = o; o += align_up((size_t)lce::kRowGradientParts * 4 + 16);
   t->bwd_total = o;
   return LCE_OK;
 }
@@ -1785,6 +1785,7 @@ int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w
   r.normalise = p->x_dtype == LCE_F16;
   r.row_lse = (float*)(base + t.row_lse); r.row_y = (int64_t*)(base + t.row_y);
   r.part = (float*)(base + t.part); r.factor = r.part + lce::kRowGradientParts;
+  r.one = (int64_t*)(r.factor + 2);
   return backward_impl(&q, t.b, x, w, y, lse, nullptr, nullptr, dx, dw, ws, stream, nullptr, &r);
 }
 
@@ -1866,8 +1867,13 @@ int lce_int8_logits(const void* x, int x_dtype, int64_t N, int64_t H, int64_t V,
   rc = current_num_cus(&a.num_cus, 0, &a.small_wgs);
   if (rc != LCE_OK) return rc;
   a.live = lce::live_bands(lce::padded_k(a.K2) * 2);
-  hipError_t e = lce::launch_quantize_rows(x, x_dtype, N, H, ldx, (signed char*)ws + f.q, f.ldx, (float*)((char*)ws + f.scales), s);
-  if (e != hipSuccess) return hip_fail(e, "quantize_rows");
+  hipError_t e = hipSuccess;
+  if (lce::int8_quantizes(a)) {
+    a.x_in = x; a.ldx_in = ldx; a.x_in_dtype = x_dtype;
+  } else {
+    e = lce::launch_quantize_rows(x, x_dtype, N, H, ldx, (signed char*)ws + f.q, f.ldx, (float*)((char*)ws + f.scales), s);
+    if (e != hipSuccess) return hip_fail(e, "quantize_rows");
+  }
   e = lce::launch_int8_logits(a, s);
   if (e != hipSuccess) return hip_fail(e, "int8_logits");
   return LCE_OK;

@@ -9,12 +9,15 @@
 // here: the functions return None before anything has been allocated or launched, and ops.py goes on as for any call, errors
 // included.  Device calls go to the current device and the stream that is handed over; allocations come from torch's caching
 // allocator, as the current stream's.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/Allocator.h>
+
+#include <vector>
 
 #include "../../include/lce.h"
 
@@ -38,6 +41,14 @@ struct Abi {
   decltype(&lce_distill) distill;
   decltype(&lce_top_logits) top_logits;
   decltype(&lce_sample) sample;
+  decltype(&lce_token_labels) token_labels;
+  decltype(&lce_token_logits_workspace_bytes) token_logits_workspace_bytes;
+  decltype(&lce_token_logits) token_logits;
+  decltype(&lce_token_logits_backward) token_logits_backward;
+  decltype(&lce_int8_logits_workspace_bytes) int8_logits_workspace_bytes;
+  decltype(&lce_int8_logits) int8_logits;
+  decltype(&lce_clip_workspace_bytes) clip_workspace_bytes;
+  decltype(&lce_clip) clip;
 } abi;
 
 template <class F> void bind_one(const py::dict& d, const char* name, F& f) { f = reinterpret_cast<F>(d[name].cast<uintptr_t>()); }
@@ -58,6 +69,14 @@ void bind(const py::dict& d) {
   bind_one(d, "lce_distill", abi.distill);
   bind_one(d, "lce_top_logits", abi.top_logits);
   bind_one(d, "lce_sample", abi.sample);
+  bind_one(d, "lce_token_labels", abi.token_labels);
+  bind_one(d, "lce_token_logits_workspace_bytes", abi.token_logits_workspace_bytes);
+  bind_one(d, "lce_token_logits", abi.token_logits);
+  bind_one(d, "lce_token_logits_backward", abi.token_logits_backward);
+  bind_one(d, "lce_int8_logits_workspace_bytes", abi.int8_logits_workspace_bytes);
+  bind_one(d, "lce_int8_logits", abi.int8_logits);
+  bind_one(d, "lce_clip_workspace_bytes", abi.clip_workspace_bytes);
+  bind_one(d, "lce_clip", abi.clip);
 }
 
 int dtype_code(at::ScalarType t) {
@@ -409,6 +428,156 @@ py::object sample_logits(const at::Tensor& logits, const at::Tensor& u, const py
   return py::cast(token);
 }
 
+// Logits of given tokens (token_logits.py): (logits, lse, x, w, w_layout, labels, ignore_index), as its _forward returns them; (status,
+// name) where the C ABI refused; None: not handled.
+py::object token_logits(const at::Tensor& x_in, const at::Tensor& At, const at::Tensor& tokens, int64_t ignore_index, double scale, int64_t n_chunk,
+                        int64_t vocab_start, int64_t vocab_size, int pack, bool copy_w, uintptr_t stream) {
+  Call c;
+  lce_problem& p = c.p;
+  if (!describe(x_in, At, false, c) || (c.w != kInPlace && !copy_w) || !plain(tokens) || tokens.scalar_type() != at::kLong ||
+      tokens.device() != x_in.device() || !tokens.is_contiguous() || tokens.numel() != p.N)
+    return py::none();
+  const bool piece = vocab_size != p.V;
+  p.ignore_index = piece ? -1 : ignore_index;
+  p.logit_scale = (float)scale;
+  p.n_chunk = n_chunk;
+  p.pack_rows = pack;
+  size_t bytes = 0;
+  if (abi.token_logits_workspace_bytes(&p, &bytes, nullptr) != LCE_OK) return py::none();
+
+  at::NoGradGuard no_grad;
+  const auto o = x_in.options().requires_grad(false);
+  const at::Tensor x = c.x != kInPlace ? rows_of(p.N, p.H, p.ldx, o) : x_in.dim() == 2 ? x_in : x_in.view({p.N, p.H});
+  const at::Tensor w = c.w != kInPlace ? rows_of(p.H, p.V, p.ldw, At.options().requires_grad(false)) : p.w_layout == LCE_W_VH ? At.t() : At;
+  const at::Tensor given = tokens.dim() == 1 ? tokens : tokens.view({p.N});
+  const at::Tensor labels = piece ? at::empty({p.N}, tokens.options()) : given;
+  const at::Tensor logits = at::empty(tokens.sizes(), o.dtype(at::kFloat)), lse = at::empty(tokens.sizes(), o.dtype(at::kFloat));
+  Workspace ws(bytes);
+  void* const s = reinterpret_cast<void*>(stream);
+  int rc = LCE_OK;
+  {
+    py::gil_scoped_release release;
+    if (c.x != kInPlace) rc = copy_rows(c.x, x_in, p.N, p.H, x, p.ldx, s);
+    if (rc == LCE_OK && c.w != kInPlace) rc = copy_rows(c.w, At, p.H, p.V, w, p.ldw, s);
+    if (rc == LCE_OK && piece)
+      rc = abi.token_labels((const int64_t*)given.data_ptr(), p.N, ignore_index, vocab_start, p.V, vocab_size, (int64_t*)labels.data_ptr(), s);
+    if (rc == LCE_OK)
+      rc = abi.token_logits(&p, x.data_ptr(), w.data_ptr(), (const int64_t*)labels.data_ptr(), piece ? p.V : ignore_index, (float*)logits.data_ptr(),
+                            (float*)lse.data_ptr(), ws.data.get(), bytes, s);
+  }
+  if (rc != LCE_OK) return py::make_tuple(rc, "linear_token_logits");
+  return py::make_tuple(logits, lse, x, w, p.w_layout, labels, p.ignore_index);
+}
+
+// Its gradients: (dx, dw), dense, dw as it is stored; (status, name, None) where the C ABI refused; None: not handled.
+py::object token_logits_backward(const at::Tensor& x, const at::Tensor& w, int layout, const at::Tensor& labels, const at::Tensor& logits,
+                                 const at::Tensor& lse, const at::Tensor& g_logits, const at::Tensor& g_lse, int64_t ignore_index, double scale,
+                                 int64_t n_chunk, int pack, bool need_dx, bool need_dw, uintptr_t stream) {
+  Call c;
+  lce_problem& p = c.p;
+  if (!(need_dx || need_dw) || w.dim() != 2) return py::none();
+  if (!describe(x, layout == LCE_W_VH ? w.t() : w, true, c) || c.w != kInPlace || p.w_layout != layout) return py::none();
+  for (const at::Tensor& t : {logits, lse, g_logits, g_lse})
+    if (!plain(t) || t.device() != x.device() || !t.is_contiguous() || t.scalar_type() != at::kFloat || t.numel() != p.N) return py::none();
+  if (!plain(labels) || labels.scalar_type() != at::kLong || labels.device() != x.device() || !labels.is_contiguous() || labels.numel() != p.N)
+    return py::none();
+  p.ignore_index = ignore_index;
+  p.logit_scale = (float)scale;
+  p.n_chunk = n_chunk;
+  p.pack_rows = pack;
+  size_t bytes = 0;
+  if (abi.token_logits_workspace_bytes(&p, nullptr, &bytes) != LCE_OK) return py::none();
+
+  at::NoGradGuard no_grad;
+  at::Tensor dx, dw;
+  if (need_dx) dx = rows_of(p.N, p.H, p.lddx, x.options().requires_grad(false));
+  if (need_dw) dw = rows_of(w.size(0), w.size(1), p.lddw, w.options().requires_grad(false));
+  Workspace ws(bytes);
+  int rc;
+  {
+    py::gil_scoped_release release;
+    rc = abi.token_logits_backward(&p, x.data_ptr(), w.data_ptr(), (const int64_t*)labels.data_ptr(), (const float*)logits.data_ptr(),
+                                   (const float*)lse.data_ptr(), (const float*)g_logits.data_ptr(), (const float*)g_lse.data_ptr(), ptr(dx),
+                                   ptr(dw), ws.data.get(), bytes, reinterpret_cast<void*>(stream));
+  }
+  if (rc != LCE_OK) return py::make_tuple(rc, "linear_token_logits", py::none());
+  if (need_dx) dx = dx.contiguous();
+  if (need_dw) dw = dw.contiguous();
+  return py::make_tuple(tensor_or_none(dx), tensor_or_none(dw));
+}
+
+// quantized_logits (quantization.py); (status, name) where the C ABI refused; None: not handled.
+py::object quantized_logits(const at::Tensor& x, const at::Tensor& values, const at::Tensor& scales, double scale, py::object dtype, uintptr_t stream) {
+  Rows r;
+  if (!describe_rows(x, r) || !plain(values) || !plain(scales) || values.scalar_type() != at::kChar || scales.scalar_type() != at::kFloat ||
+      values.device() != x.device() || scales.device() != x.device() || values.dim() != 2 || values.size(0) < 1 || values.size(1) != r.cols ||
+      values.stride(1) != 1 || values.stride(0) < r.cols || values.stride(0) % 16 != 0 || !aligned(values) || scales.dim() != 1 ||
+      scales.size(0) != values.size(0) || !scales.is_contiguous())
+    return py::none();
+  const at::ScalarType type = dtype.is_none() ? x.scalar_type() : reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+  const int code = dtype_code(type);
+  const int64_t V = values.size(0);
+  size_t bytes = 0;
+  if (code < 0 || abi.int8_logits_workspace_bytes(r.rows, r.cols, V, &bytes) != LCE_OK) return py::none();
+  at::NoGradGuard no_grad;
+  auto shape = x.sizes().vec();
+  shape.back() = V;
+  const at::Tensor out = at::empty(shape, x.options().dtype(type).requires_grad(false));
+  Workspace ws(bytes);
+  int rc;
+  {
+    py::gil_scoped_release release;
+    rc = abi.int8_logits(x.data_ptr(), r.dtype, r.rows, r.cols, V, r.ld, (const int8_t*)values.data_ptr(), values.stride(0),
+                         (const float*)scales.data_ptr(), (float)scale, out.data_ptr(), code, V, ws.data.get(), bytes,
+                         reinterpret_cast<void*>(stream));
+  }
+  if (rc != LCE_OK) return py::make_tuple(rc, "quantized_logits");
+  return py::cast(out);
+}
+
+// The norm that clip_gradients (clipping.py) returns; (status, name) where the C ABI refused; None: not handled.  grads, out: lists of the
+// same length; divisor_rows: None or a tensor with the divisor.
+py::object clip(const py::list& grads, const py::list& out, double max_norm, double divisor, const py::object& divisor_tensor, uintptr_t stream) {
+  const size_t n = grads.size();
+  if (n == 0 || out.size() != n) return py::none();
+  std::vector<lce_tensor> t(n);
+  at::TensorOptions options;
+  c10::Device device(c10::kCPU);
+  for (size_t i = 0; i < n; ++i) {
+    const py::handle gh = grads[i], oh = out[i];
+    if (!THPVariable_Check(gh.ptr()) || !THPVariable_Check(oh.ptr())) return py::none();
+    const at::Tensor &g = THPVariable_Unpack(gh.ptr()), &o = THPVariable_Unpack(oh.ptr());
+    if (!plain(g) || !plain(o) || g.sizes() != o.sizes() || g.strides() != o.strides() || !g.is_non_overlapping_and_dense()) return py::none();
+    if (i == 0) {
+      device = g.device();
+      options = g.options();
+    }
+    const int gd = dtype_code(g.scalar_type()), od = dtype_code(o.scalar_type());
+    if (g.device() != device || o.device() != device || gd < 0 || (od != gd && od != LCE_F32)) return py::none();
+    t[i] = {g.data_ptr(), o.data_ptr(), g.numel(), gd, od};
+  }
+  const float* by = nullptr;
+  if (!divisor_tensor.is_none()) {
+    const at::Tensor& d = THPVariable_Unpack(divisor_tensor.ptr());
+    if (!plain(d) || d.scalar_type() != at::kFloat || d.numel() != 1 || d.device() != device) return py::none();
+    by = (const float*)d.data_ptr();
+  }
+  size_t bytes = 0;
+  if (abi.clip_workspace_bytes(t.data(), (int64_t)n, &bytes) != LCE_OK) return py::none();
+  at::NoGradGuard no_grad;
+  const at::Tensor norm = at::empty({}, options.dtype(at::kFloat).requires_grad(false));
+  Workspace ws(bytes);
+  int rc;
+  {
+    py::gil_scoped_release release;
+    rc = abi.clip(t.data(), (int64_t)n, (float)max_norm, (float)divisor, by, (float*)norm.data_ptr(), ws.data.get(), bytes,
+                  reinterpret_cast<void*>(stream));
+  }
+  if (rc != LCE_OK) return py::make_tuple(rc, "clip_gradients");
+  for (size_t i = 0; i < n; ++i) THPVariable_Unpack(py::handle(out[i]).ptr()).unsafeGetTensorImpl()->bump_version();
+  return py::cast(norm);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_lce_host, m) {
@@ -418,4 +587,8 @@ PYBIND11_MODULE(_lce_host, m) {
   m.def("distill", &distill);
   m.def("top_logits", &top_logits);
   m.def("sample_logits", &sample_logits);
+  m.def("token_logits", &token_logits);
+  m.def("token_logits_backward", &token_logits_backward);
+  m.def("quantized_logits", &quantized_logits);
+  m.def("clip", &clip);
 }

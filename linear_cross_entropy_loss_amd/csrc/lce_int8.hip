@@ -574,7 +574,172 @@ template <class T> __global__ __launch_bounds__(kThreads, 2) void int8_small_ker
   logits_epilogue<T, 1>(a, acc, (int64_t)tp * kSmallTile, (int64_t)tq * kSmallTile + wave * kBlk, lds + wave * kWaveLds);
 }
 
+// ---------------------------------------------------------------------------
+// Few rows: a pass over the weight.  A wave takes 16 rows of it at a time, straight from memory to the registers that
+// v_mfma_i32_16x16x64_i8 reads (lane l: row l % 16, 16 bytes of K at 16 * (l / 16) of every 64), a group of kFlight loads ahead of the one
+// that is multiplied, across the ends of its rows too; the quantised rows of x lie in LDS in the order in which the lanes want them:
+// 16 bytes of K, row after row.  There are 1, 2, 4, 8 or 16 places for rows, or 32, which are two instructions to a load; lanes
+// beyond the places read the same rows again, and nobody stores what comes of it.
+// A small x (kFusedNumbers) is quantised by every workgroup for itself while its first loads of the weight are under way: one row of 2048
+// in 3 us less than a launch takes, eight in 5 more.
+// Bound by the weight's way from memory.  us, with x quantised, against the 128 x 128 tiles: 2048 x 131072 one row 50 / 58, 16 rows 55 / 58;
+// 4096 x 128256 one row 97 / 110, 16 rows 108 / 116, 32 rows 114 / 121 (2048 x 131072 61 / 59: not taken for short rows); 8192 x 32000 55 / 67.
+// Four loads in a group 50, 106 and 64 us for one row, twelve 55, 110 and 59; loads past the caches 53, 107 and 59.
+// ---------------------------------------------------------------------------
+constexpr int kStreamThreads = 512, kFlight = 8, kGroupBytes = 64 * kFlight;
+constexpr int kStreamLds = 150 * 1024;
+constexpr int64_t kFusedNumbers = 8192;
+LCE_DEV u32x4_t* place_of(char* lds, int byte, int n, int places) {
+  return reinterpret_cast<u32x4_t*>(lds + ((byte >> 4) * places + n) * 16 + (byte & 15));
+}
+template <int DT> LCE_DEV void quantize_into(const Int8Args& a, char* lds, int places, int depth, unsigned* sh_top, float* sh_scale, Inverse* sh_inverse) {
+  typedef Source<DT> E;
+  const int N = (int)a.N, t = threadIdx.x;
+  for (int n = 0; n < N; ++n) {
+    const typename E::S* row = reinterpret_cast<const typename E::S*>(a.x_in) + n * a.ldx_in;
+    u32x4_t tops = {0, 0, 0, 0};
+    for (int c = t * E::kPer; c < a.H; c += kStreamThreads * E::kPer) tops = larger_piece<DT>(tops, load_piece<DT>(row, c, a.H));
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < E::kPer; ++k) top = larger(top, magnitude<DT>(tops, k));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = larger(top, (unsigned)__shfl_xor((int)top, d));
+    if ((t & 63) == 0) atomicMax(&sh_top[n], top);
+  }
+  __syncthreads();
+  if (t < N) {
+    const RowScale s(sh_top[t]);
+    sh_scale[t] = s.scale * a.scale;
+    sh_inverse[t] = Inverse(s);
+  }
+  __syncthreads();
+  for (int n = 0; n < N; ++n) {
+    const typename E::S* row = reinterpret_cast<const typename E::S*>(a.x_in) + n * a.ldx_in;
+    const Inverse inverse = sh_inverse[n];
+    for (int c = t * E::kPer; c < depth; c += kStreamThreads * E::kPer) {
+      const u32x4_t piece = load_piece<DT>(row, c, a.H);
+      store_bytes<DT>(piece, RowScale(sh_top[n]), inverse, reinterpret_cast<signed char*>(place_of(lds, c, n, places)));
+    }
+  }
+}
+template <class T, int NB> __global__ __launch_bounds__(kStreamThreads, 4) void int8_stream_kernel(const Int8Args a, int places, int depth) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float sh_scale[32];
+  __shared__ unsigned sh_top[32];
+  __shared__ Inverse sh_inverse[32];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int blocks = (int)((a.V + 15) / 16), step = (int)gridDim.x * (kStreamThreads / 64);
+  const int groups = depth / kGroupBytes;
+  int block = wave * (int)gridDim.x + (int)blockIdx.x;  // (the last ones go to different compute units)
+  const unsigned mine = (unsigned)((lane & 15) * a.ldw + (lane >> 4) * 16);
+  const char* const end = reinterpret_cast<const char*>(weight_end(a));
+  u32x4_t w[2][kFlight];
+  // (of the last row nothing is read past its end; what is read of the next row behind the end of one meets zeros)
+  const auto load = [&](int buf, int b, int g) {
+    const char* base = reinterpret_cast<const char*>(a.w) + (int64_t)b * 16 * a.ldw + g * kGroupBytes;
+    const int64_t left = end - base;
+    const __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, left <= 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : (int)left, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) w[buf][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)mine + i * 64, 0, 0);
+  };
+  if (block < blocks) load(0, block, 0);
+  if (t < 32) sh_top[t] = 0;
+  __syncthreads();
+  if (a.x_in != nullptr) {
+    if (a.x_in_dtype == DT_BF16) quantize_into<DT_BF16>(a, lds, places, depth, sh_top, sh_scale, sh_inverse);
+    else if (a.x_in_dtype == DT_F16) quantize_into<DT_F16>(a, lds, places, depth, sh_top, sh_scale, sh_inverse);
+    else quantize_into<DT_F32>(a, lds, places, depth, sh_top, sh_scale, sh_inverse);
+  } else {
+    if (t < a.N) sh_scale[t] = a.x_scales[t] * a.scale;
+    const int pieces = depth / 16;
+    for (int i = t; i < pieces * (int)a.N; i += kStreamThreads) {
+      const int n = i / pieces, c = (i - n * pieces) * 16;
+      *place_of(lds, c, n, places) = c < 2 * a.K2 ? *reinterpret_cast<const u32x4_t*>(a.x + n * a.ldx + c) : u32x4_t{0, 0, 0, 0};
+    }
+  }
+  __syncthreads();
+  const int n = lane & 15, row = n & (places - 1);
+  const char* const from = lds + ((lane >> 4) * places + row) * 16;
+  i32x4_t acc[NB];
+  const auto multiply = [&](int buf, int g) {
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const i32x4_t x = *reinterpret_cast<const i32x4_t*>(from + (g * kFlight + i) * (64 * places) + b * 256);
+        acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, w[buf][i]), x, acc[b], 0, 0, 0);
+      }
+  };
+  // One block of rows, whose first group is in buffer FIRST; the next one's is in the other buffer afterwards where the groups are odd.
+  const auto rows16 = [&](auto first, int next) {
+    constexpr int F = decltype(first)::value;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = i32x4_t{0, 0, 0, 0};
+    int g = 0;
+    for (; g + 1 < groups; g += 2) {
+      load(1 - F, block, g + 1);
+      multiply(F, g);
+      if (g + 2 < groups) load(F, block, g + 2);
+      else if (next < blocks) load(F, next, 0);
+      multiply(1 - F, g + 1);
+    }
+    if (g < groups) {
+      if (next < blocks) load(1 - F, next, 0);
+      multiply(F, g);
+    }
+    // lane: rows 4 * (lane / 16) ... + 3 of the weight's, row `n` of x
+    const int64_t v = (int64_t)block * 16 + (lane >> 4) * 4;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (n + 16 * b < a.N) {
+        const float sx = sh_scale[n + 16 * b];
+        char* to = reinterpret_cast<char*>(a.out) + ((n + 16 * b) * a.ldo + v) * out_of<T>::kEs;
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = (float)acc[b][i] * sx * (v + i < a.V ? a.w_scales[v + i] : 0.f);
+        if constexpr (out_of<T>::kEs == 4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (v + i < a.V) reinterpret_cast<float*>(to)[i] = f[i];
+        } else if (v + 4 <= a.V && (reinterpret_cast<uintptr_t>(to) & 7) == 0) {
+          *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3])};
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (v + i < a.V) reinterpret_cast<unsigned short*>(to)[i] = to_bits<T>(f[i]);
+        }
+      }
+  };
+  const bool odd = (groups & 1) != 0;
+  for (; block < blocks; block += step) {
+    rows16(std::integral_constant<int, 0>(), block + step);
+    if (odd && (block += step) < blocks) rows16(std::integral_constant<int, 1>(), block + step);
+  }
+}
+
+// Places for rows of x, 0 where the kernel does not take the problem.
+int stream_places(const Int8Args& a, int* depth) {
+  *depth = (int)pad_to(a.H, kGroupBytes);
+  int places = 1;
+  while (places < a.N) places *= 2;
+  if (places == 32 && *depth < 3584) return 0;
+  return places <= 32 && (int64_t)places * *depth <= kStreamLds ? places : 0;
+}
+template <class T, int NB> hipError_t launch_stream(const Int8Args& a, int places, int depth, hipStream_t s) {
+  static LdsOptIn optin;
+  const hipError_t e = optin.ensure(reinterpret_cast<const void*>(int8_stream_kernel<T, NB>), kStreamLds);
+  if (e != hipSuccess) return e;
+  const int bytes = places * depth, per = bytes <= kStreamLds / 2 ? 2 : 1;
+  const int64_t groups = ((a.V + 15) / 16 + kStreamThreads / 64 - 1) / (kStreamThreads / 64);
+  const int64_t most = (int64_t)a.num_cus * per;
+  hipLaunchKernelGGL((int8_stream_kernel<T, NB>), dim3((unsigned)(groups < most ? groups : most)), dim3(kStreamThreads), bytes, s, a, places, depth);
+  return hipGetLastError();
+}
+
 template <class T> hipError_t launch_product(const Int8Args& a, hipStream_t s) {
+  int depth;
+  if (const int places = stream_places(a, &depth)) return places > 16 ? launch_stream<T, 2>(a, places, depth, s) : launch_stream<T, 1>(a, places, depth, s);
   if (few_logit_tiles(a.N, a.V, small_logit_ktiles(a.K2, 1), a.small_wgs)) {
     const int tiles_p = (int)((a.V + kSmallTile - 1) / kSmallTile), tiles_q = (int)((a.N + kSmallTile - 1) / kSmallTile);
     hipLaunchKernelGGL(int8_small_kernel<T>, dim3((unsigned)(tiles_p * tiles_q)), dim3(kThreads), kSmallLds, s, a, tiles_p, tiles_q);
@@ -648,6 +813,10 @@ hipError_t launch_quantize_columns(const void* src, int dtype, int64_t rows, int
   return dtype == DT_BF16  ? quantize_columns<DT_BF16>(src, rows, cols, ld, q, ldq, scales, num_cus, s)
          : dtype == DT_F16 ? quantize_columns<DT_F16>(src, rows, cols, ld, q, ldq, scales, num_cus, s)
                            : quantize_columns<DT_F32>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+}
+bool int8_quantizes(const Int8Args& a) {
+  int depth;
+  return a.N * a.H <= kFusedNumbers && stream_places(a, &depth) > 0;
 }
 hipError_t launch_int8_logits(const Int8Args& a, hipStream_t s) {
   return a.out_dtype == DT_BF16 ? launch_product<BF16>(a, s) : a.out_dtype == DT_F16 ? launch_product<F16>(a, s) : launch_product<float>(a, s);

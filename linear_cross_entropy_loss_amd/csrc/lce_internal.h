@@ -229,7 +229,7 @@ struct BwdArgs {
   int vtail_all;  // the logit kernel for the tile column that straddles the end of the vocabulary takes every column
   // lce_token_logits_backward: rows have upstream gradients of their own.  `lse` then holds lse - log |g_lse|, `y` -1 for no row, V where
   // g_lse is positive and kNegativeRow where it is negative, and the kernels stage g_lse * softmax, the sign through the gain of z_reg;
-  // the label's column is launch_row_targets'.  n_valid is null there.
+  // the label's column is launch_row_targets'.  grad_out and n_valid are a factor and 1 there.
   int row_signs;
 };
 
@@ -244,7 +244,7 @@ __host__ __device__ inline int64_t dz_block_offset(int64_t row_tile, int64_t gro
 // dz.  With no valid label at all every dz is zero and the factor is taken as 0, so both
 // gradients are exact zeros (what F.cross_entropy's backward gives for such a batch; the loss itself is NaN).
 __device__ __forceinline__ float final_factor_of(const BwdArgs& a) {
-  const int64_t n = a.n_valid != nullptr ? a.n_valid[0] : 1;
+  const int64_t n = a.n_valid[0];
   const float unscale = __builtin_bit_cast(float, (127 - a.dz_shift) << 23);  // 2^-dz_shift
   return n > 0 ? a.grad_out[0] * a.scale / (float)n * unscale : 0.f;
 }
@@ -539,6 +539,7 @@ struct RowGradients {
   float* row_lse;
   int64_t* row_y;
   float* factor;
+  int64_t* one;  // becomes 1
   float* part;
 };
 constexpr int kRowGradientParts = 64;
@@ -566,7 +567,12 @@ struct Int8Args {
   int out_dtype;
   float scale;
   int num_cus, small_wgs, live;  // as in FwdArgs
+  // null, or the rows themselves (row stride in elements), which the kernel quantises itself (int8_quantizes)
+  const void* x_in;
+  int64_t ldx_in;
+  int x_in_dtype;
 };
+bool int8_quantizes(const Int8Args& a);
 hipError_t launch_int8_logits(const Int8Args& a, hipStream_t s);
 
 // Tensors scaled by their common norm (lce_clip.hip).  The kernels' arguments hold the tensors of one launch (of the 4 KiB that

@@ -49,7 +49,10 @@ __global__ __launch_bounds__(kRowThreads) void row_gradients_kernel(const RowGra
       e = e < -126 ? -126 : e > 127 ? 127 : e;
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *g.factor = ldexpf(1.f, e);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *g.factor = ldexpf(1.f, e);
+    *g.one = 1;
+  }
   for (int64_t j = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; j < g.N; j += (int64_t)gridDim.x * kRowThreads) {
     const int64_t n = g.perm != nullptr ? packed_token(g.perm, j, g.N) : j;
     const float gl = ldexpf(g.grad_lse[n], -e);

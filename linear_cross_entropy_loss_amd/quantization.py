@@ -149,6 +149,13 @@ def quantized_logits(x, weight: Quantized, logit_scale: float = 1.0, dtype: Opti
     NaN or an infinity give NaN.
     """
     values, scales = weight
+    if not torch.compiler.is_compiling() and x.is_cuda and x.device.index == torch._C._cuda_getDevice() and (
+            _lib.F32_ZERO < logit_scale < _lib.F32_INF) and (dtype is None or isinstance(dtype, torch.dtype)):
+        done = _lib.host().quantized_logits(x, values, scales, logit_scale, dtype, _stream(x.device))
+        if isinstance(done, torch.Tensor):
+            return done
+        if done is not None:
+            _lib.raise_for_status(*done)
     if x.dim() < 1 or values.dim() != 2 or values.shape[1] != x.shape[-1]:
         raise ValueError(f"quantized_logits: x of shape {tuple(x.shape)} does not go with values of shape {tuple(values.shape)}")
     _check(x, "quantized_logits", x.shape[-1])

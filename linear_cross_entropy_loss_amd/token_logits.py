@@ -51,6 +51,13 @@ def _forward(x_in, At, tokens, ignore_index, logit_scale, N_chunk_size, vocab_st
     """(logits, lse) and what the backward reads: the views x and w, w's layout, the labels with their ignore_index."""
     ops._check_dtypes(x_in, At)
     V, dev = At.shape[1], x_in.device
+    if dev.index == torch._C._cuda_getDevice():
+        done = _lib.host().token_logits(x_in, At, tokens, ignore_index, logit_scale, N_chunk_size, vocab_start, vocab_size, pack,
+                                        "weight" in ops._copy_warned, _stream(dev))
+        if done is not None and len(done) == 2:
+            _lib.raise_for_status(*done)
+        if done is not None:
+            return done
     with _on_device(dev):
         x = ops._aligned_rows(x_in.reshape(-1, x_in.shape[-1]))
         layout = ops._weight_layout(At, x.dtype)
@@ -82,6 +89,14 @@ def _backward(x, w, layout, labels, logits, lse, g_logits, g_lse, ignore_index, 
     N, H = x.shape
     V = w.shape[0] if layout == _lib.W_VH else w.shape[1]
     dev = x.device
+    if dev.index == torch._C._cuda_getDevice():
+        done = _lib.host().token_logits_backward(x, w, layout, labels, logits, lse, g_logits, g_lse, ignore_index, logit_scale, N_chunk_size, pack,
+                                                 need_dx, need_dw, _stream(dev))
+        if done is not None:
+            if len(done) == 3:
+                _lib.raise_for_status(*done[:2])
+            dx, dw = done
+            return dx, dw.t() if layout == _lib.W_VH and dw is not None else dw
     with _on_device(dev):
         dx, dw = ops._alloc_grads(x, w, layout, N, H, V, need_dx, need_dw)
         if N == 0:
