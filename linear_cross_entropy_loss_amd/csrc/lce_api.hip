@@ -1972,6 +1972,10 @@ int lce_clip(const lce_tensor* t, int64_t count, float max_norm, float divisor, 
   lce::ClipBatch b;
   memset(&b, 0, sizeof(b));
   b.part = (double*)ws;
+  // What does not fit the 256 MB Infinity Cache between the two passes goes by it (lce_clip.hip).
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < count; ++i) bytes += t[i].n * (es_of(t[i].dtype) + (t[i].grad != t[i].out ? es_of(t[i].out_dtype) : 0));
+  b.once = bytes > (int64_t)256 << 20;
   const auto fill = [&](const ClipLaunch& l) {
     b.count = (int)(l.last - l.first);
     b.stretches = (unsigned)l.stretches;

@@ -17,9 +17,16 @@ constexpr int kClipThreads = 256;
 constexpr int kStretch = 8192;
 
 // 16 bytes at any 2-byte address: one load or store all the same.
-struct __attribute__((packed, aligned(2))) Piece {
-  u32x4_t v;
-};
+typedef u32x4_t __attribute__((aligned(2))) piece_t;
+template <bool ONCE> LCE_DEV u32x4_t load_piece(const void* p) {
+  const piece_t* q = reinterpret_cast<const piece_t*>(p);
+  return ONCE ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool ONCE> LCE_DEV void store_piece(void* p, u32x4_t v) {
+  piece_t* q = reinterpret_cast<piece_t*>(p);
+  if (ONCE) __builtin_nontemporal_store(v, q);
+  else *q = v;
+}
 
 template <int DT> struct Elem {
   static constexpr int kPer = 8;
@@ -45,7 +52,7 @@ LCE_DEV int entry_of(const ClipBatch& b, unsigned c) {
   return lo;
 }
 
-template <int DT> LCE_DEV void add_squares(const void* at, int n, double (&sum)[4]) {
+template <int DT, bool ONCE> LCE_DEV void add_squares(const void* at, int n, double (&sum)[4]) {
   typedef Elem<DT> E;
   constexpr int kStep = kClipThreads * E::kPer, kRounds = kStretch / kStep;
   const typename E::S* p = reinterpret_cast<const typename E::S*>(at);
@@ -53,7 +60,7 @@ template <int DT> LCE_DEV void add_squares(const void* at, int n, double (&sum)[
   if (n == kStretch) {
     u32x4_t v[kRounds];
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) v[r] = reinterpret_cast<const Piece*>(p + r * kStep + t * E::kPer)->v;
+    for (int r = 0; r < kRounds; ++r) v[r] = load_piece<ONCE>(p + r * kStep + t * E::kPer);
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       typename E::S e[E::kPer];
@@ -83,44 +90,56 @@ LCE_DEV double workgroup_sum(double v) {
   return v;
 }
 
-__global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(const ClipBatch b) {
+template <bool ONCE> __global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(const ClipBatch b) {
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
   for (unsigned c = blockIdx.x; c < b.stretches; c += gridDim.x) {
     const ClipEntry& e = b.e[entry_of(b, c)];
     const int64_t at = (int64_t)(c - e.first) * kStretch, left = e.n - at;
     const int n = left < kStretch ? (int)left : kStretch;
     const char* p = reinterpret_cast<const char*>(e.grad) + at * (e.dtype == DT_F32 ? 4 : 2);
-    if (e.dtype == DT_BF16) add_squares<DT_BF16>(p, n, sum);
-    else if (e.dtype == DT_F16) add_squares<DT_F16>(p, n, sum);
-    else add_squares<DT_F32>(p, n, sum);
+    if (e.dtype == DT_BF16) add_squares<DT_BF16, ONCE>(p, n, sum);
+    else if (e.dtype == DT_F16) add_squares<DT_F16, ONCE>(p, n, sum);
+    else add_squares<DT_F32, ONCE>(p, n, sum);
   }
   const double all = workgroup_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
   if (threadIdx.x == 0) b.part[b.part0 + blockIdx.x] = all;
 }
 
-template <int DT, int OUT> LCE_DEV void scale_stretch(const void* from, void* to, int n, float f) {
+// (16 bits to 32: 8 bytes of input to a lane, so that what a wave stores at a time lies together)
+template <int DT, int OUT, bool ONCE> LCE_DEV void scale_stretch(const void* from, void* to, int n, float f) {
   typedef Elem<DT> E;
   typedef Elem<OUT> O;
-  constexpr int kStep = kClipThreads * E::kPer, kRounds = kStretch / kStep;
+  constexpr int kPer = O::kPer, kStep = kClipThreads * kPer, kRounds = 8;
   const typename E::S* p = reinterpret_cast<const typename E::S*>(from);
   typename O::S* q = reinterpret_cast<typename O::S*>(to);
   const int t = threadIdx.x;
   if (n == kStretch) {
-    u32x4_t v[kRounds];
+    typedef u32x2_t __attribute__((aligned(2))) half_t;
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) v[r] = reinterpret_cast<const Piece*>(p + r * kStep + t * E::kPer)->v;
+    for (int r0 = 0; r0 < kStretch / kStep; r0 += kRounds) {
+      constexpr int kHere = kStretch / kStep < kRounds ? kStretch / kStep : kRounds;
+      u32x4_t v[kHere];
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      typename E::S e[E::kPer];
-      typename O::S o[E::kPer];
-      __builtin_memcpy(e, &v[r], 16);
+      for (int r = 0; r < kHere; ++r) {
+        const typename E::S* at = p + (r0 + r) * kStep + t * kPer;
+        if constexpr (E::kPer == kPer) {
+          v[r] = load_piece<ONCE>(at);
+        } else {
+          const half_t* h = reinterpret_cast<const half_t*>(at);
+          const u32x2_t w = ONCE ? __builtin_nontemporal_load(h) : *h;
+          v[r] = u32x4_t{w[0], w[1], 0, 0};
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < E::kPer; ++i) o[i] = O::put(E::get(e[i]) * f);
+      for (int r = 0; r < kHere; ++r) {
+        typename E::S e[16 / sizeof(typename E::S)];
+        typename O::S o[kPer];
+        __builtin_memcpy(e, &v[r], 16);
 #pragma unroll
-      for (int h = 0; h < E::kPer / O::kPer; ++h) {
-        Piece w;
-        __builtin_memcpy(&w.v, o + h * O::kPer, 16);
-        *reinterpret_cast<Piece*>(q + r * kStep + t * E::kPer + h * O::kPer) = w;
+        for (int i = 0; i < kPer; ++i) o[i] = O::put(E::get(e[i]) * f);
+        u32x4_t w;
+        __builtin_memcpy(&w, o, 16);
+        store_piece<ONCE>(q + (r0 + r) * kStep + t * kPer, w);
       }
     }
     return;
@@ -128,6 +147,7 @@ template <int DT, int OUT> LCE_DEV void scale_stretch(const void* from, void* to
   for (int i = t; i < n; i += kClipThreads) q[i] = O::put(E::get(p[i]) * f);
 }
 
+template <bool ONCE>
 __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipBatch b, int parts, float max_norm, float divisor, const float* divisor_ptr,
                                                                   float* norm_out) {
   double sum = 0.0;
@@ -147,11 +167,11 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipBatc
     const int n = left < kStretch ? (int)left : kStretch;
     const char* p = reinterpret_cast<const char*>(e.grad) + at * (e.dtype == DT_F32 ? 4 : 2);
     char* q = reinterpret_cast<char*>(e.out) + at * (e.out_dtype == DT_F32 ? 4 : 2);
-    if (e.dtype == DT_F32) scale_stretch<DT_F32, DT_F32>(p, q, n, factor);
-    else if (e.dtype == DT_BF16 && e.out_dtype == DT_F32) scale_stretch<DT_BF16, DT_F32>(p, q, n, factor);
-    else if (e.dtype == DT_BF16) scale_stretch<DT_BF16, DT_BF16>(p, q, n, factor);
-    else if (e.out_dtype == DT_F32) scale_stretch<DT_F16, DT_F32>(p, q, n, factor);
-    else scale_stretch<DT_F16, DT_F16>(p, q, n, factor);
+    if (e.dtype == DT_F32) scale_stretch<DT_F32, DT_F32, ONCE>(p, q, n, factor);
+    else if (e.dtype == DT_BF16 && e.out_dtype == DT_F32) scale_stretch<DT_BF16, DT_F32, ONCE>(p, q, n, factor);
+    else if (e.dtype == DT_BF16) scale_stretch<DT_BF16, DT_BF16, ONCE>(p, q, n, factor);
+    else if (e.out_dtype == DT_F32) scale_stretch<DT_F16, DT_F32, ONCE>(p, q, n, factor);
+    else scale_stretch<DT_F16, DT_F16, ONCE>(p, q, n, factor);
   }
 }
 
@@ -160,13 +180,14 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipBatc
 int64_t clip_stretches(int64_t n) { return (n + kStretch - 1) / kStretch; }
 
 hipError_t launch_clip_norm(const ClipBatch& b, int grid, hipStream_t s) {
-  hipLaunchKernelGGL(clip_norm_kernel, dim3(grid), dim3(kClipThreads), 0, s, b);
+  hipLaunchKernelGGL(b.once ? clip_norm_kernel<true> : clip_norm_kernel<false>, dim3(grid), dim3(kClipThreads), 0, s, b);
   return hipGetLastError();
 }
 
 hipError_t launch_clip_scale(const ClipBatch& b, int grid, int parts, float max_norm, float divisor, const float* divisor_ptr, float* norm,
                              hipStream_t s) {
-  hipLaunchKernelGGL(clip_scale_kernel, dim3(grid), dim3(kClipThreads), 0, s, b, parts, max_norm, divisor, divisor_ptr, norm);
+  hipLaunchKernelGGL(b.once ? clip_scale_kernel<true> : clip_scale_kernel<false>, dim3(grid), dim3(kClipThreads), 0, s, b, parts, max_norm,
+                     divisor, divisor_ptr, norm);
   return hipGetLastError();
 }
 

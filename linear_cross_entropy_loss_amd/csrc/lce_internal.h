@@ -590,6 +590,7 @@ struct ClipBatch {
   double* part;
   int count, part0;  // part0: the launch's first partial sum
   unsigned stretches;
+  int once;  // loads and stores past the caches
 };
 int64_t clip_stretches(int64_t n);
 hipError_t launch_clip_norm(const ClipBatch& b, int grid, hipStream_t s);
