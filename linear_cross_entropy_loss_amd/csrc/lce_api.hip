@@ -173,7 +173,8 @@ bool fwd_reads_f32(const lce_problem* p) {
          p->ldw < ((int64_t)1 << 22) && p->max_workgroups <= 0;
 }
 
-FwdPlan plan_fwd(const lce_problem* p) {
+// (`half`: fp32 tensors as fp16 pairs, of which there is always a copy)
+FwdPlan plan_fwd(const lce_problem* p, bool half = false) {
   FwdPlan f;
   const size_t Np = (size_t)lce::padded_tokens(p->N), Vp = (size_t)lce::padded_vocab(p->V);
   f.nc = fwd_chunk_rows(p);
@@ -193,7 +194,7 @@ FwdPlan plan_fwd(const lce_problem* p) {
   // in one launch; no difference at H = 2048, where x stays in the cache).
   // (fp32 activations reach the tile kernels as bf16 pairs, twice as wide)
   if ((size_t)f.nc * (size_t)(parts_of(p) * p->H) * 2 > ((size_t)128 << 20) && f.vs > 32768) f.vs = 32768;
-  if (p->w_dtype == LCE_F32 && !fwd_reads_f32(p)) {
+  if (p->w_dtype == LCE_F32 && (half || !fwd_reads_f32(p))) {
     // slab copies of at most 256 MiB (at least one tile column)
     const int64_t hw = parts_of(p) * p->H;  // rows of the copy
     int64_t cols = ((int64_t)256 << 20) / (hw * 2) / 256 * 256;
@@ -856,17 +857,20 @@ int current_num_cus(int* out, int cap, int* small_wgs = nullptr) {
 }
 
 // Body of lce_forward; `ws` is the caller's workspace or the library's static scratch.
-// (`tok_logits`, `tok_other`: as in FwdArgs; out5 and n_valid may then be left unwritten)
+// (`tok_logits`, `tok_other`, `pair`: as in FwdArgs; out5 and n_valid may then be left unwritten)
 int forward_impl(const lce_problem* p, const void* x, const void* w, const int64_t* y, float* lse, float* out5,
-                 int64_t* n_valid, void* ws, size_t ws_bytes, void* stream, float* tok_logits = nullptr, int64_t tok_other = 0) {
+                 int64_t* n_valid, void* ws, size_t ws_bytes, void* stream, float* tok_logits = nullptr, int64_t tok_other = 0,
+                 const float* pair = nullptr) {
   int rc = check(p, false);
   if (rc != LCE_OK) return rc;
   if (!x || !w || !y || !lse || !out5 || !n_valid) return LCE_EINVAL_ARG;
   if (misaligned(x) || misaligned(w)) return LCE_EINVAL_ARG;
-  const FwdPlan f = plan_fwd(p);
+  const bool half = pair != nullptr;
+  const FwdPlan f = plan_fwd(p, half);
   if (!ws || ws_bytes < f.total || misaligned(ws)) return LCE_EWORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   char* base = (char*)ws;
+  const int compute = half ? (int)lce::DT_HALF_PAIR : compute_dtype(p);
 
   lce::FwdArgs a;
   memset(&a, 0, sizeof(a));
@@ -878,7 +882,7 @@ int forward_impl(const lce_problem* p, const void* x, const void* w, const int64
   a.ignore_index = p->ignore_index;
   a.scale = p->logit_scale; a.z_reg = p->z_reg; a.monitoring = p->monitoring ? 1 : 0;
   a.lse = lse; a.out5 = out5; a.n_valid = n_valid;
-  a.tok_logits = tok_logits; a.tok_other = tok_other;
+  a.tok_logits = tok_logits; a.tok_other = tok_other; a.pair = pair;
   a.part_lse = (float*)(base + f.part_lse);
   a.part_max = (float*)(base + f.part_max);
   a.part_pz = (float*)(base + f.part_pz);
@@ -910,7 +914,7 @@ int forward_impl(const lce_problem* p, const void* x, const void* w, const int64
         if (e != hipSuccess) return hip_fail(e, "compact_labels");
       }
       e = x32 ? lce::launch_gather_rows_split((const float*)x, p->ldx, p->H, a.perm, a.n_rows, p->N, base + k.xc,
-                                              k.ldxc, nullptr, nullptr, a.num_cus, s)
+                                              k.ldxc, nullptr, nullptr, a.num_cus, s, pair)
               : lce::launch_gather_rows(x, p->ldx * 2, p->H * 2, a.perm, a.n_rows, p->N, base + k.xc, k.ldxc * 2, nullptr, nullptr,
                                         a.num_cus, s);
       if (e != hipSuccess) return hip_fail(e, "gather_rows");
@@ -918,7 +922,7 @@ int forward_impl(const lce_problem* p, const void* x, const void* w, const int64
     if (x32) {  // the tile kernels read the copy in bf16 pairs, whether or not rows were dropped
       a.x = a.xc;
       a.ldx = a.ldxc;
-      a.x_dtype = lce::DT_PAIR;
+      a.x_dtype = compute;
       a.x_lo = a.ldxc / 2;
     }
   }
@@ -933,14 +937,14 @@ int forward_impl(const lce_problem* p, const void* x, const void* w, const int64
         lce::FwdArgs t = a;
         t.v0 = v0;
         t.vw = p->V - v0 < f.vs ? p->V - v0 : f.vs;
-        if (p->w_dtype == LCE_F32 && !fwd_reads_f32(p)) {
+        if (p->w_dtype == LCE_F32 && (half || !fwd_reads_f32(p))) {
           const int64_t ld16 = a.w_vh ? p->H : lce::pad_to(t.vw, 256);
           e = a.w_vh ? lce::launch_convert_w_rows((const float*)w, p->ldw, p->H, v0, t.vw, base + f.w16, ld16,
-                                                  compute_dtype(p), s)
+                                                  compute, s)
                      : lce::launch_convert_w_slab((const float*)w, p->ldw, p->H, v0, t.vw, base + f.w16, ld16,
-                                                  compute_dtype(p), s);
+                                                  compute, s, pair);
           if (e != hipSuccess) return hip_fail(e, "convert_w");
-          t.w = base + f.w16; t.ldw = ld16; t.w_dtype = compute_dtype(p); t.wv0 = v0; t.Vw = t.vw;
+          t.w = base + f.w16; t.ldw = ld16; t.w_dtype = compute; t.wv0 = v0; t.Vw = t.vw;
         } else {
           t.wv0 = 0; t.Vw = p->V;
         }
@@ -1186,6 +1190,9 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
   // Tokens with an ignored label have dz == 0: the kernels run on the other rows only, packed to the front.
   const PackPlan& k = b.pack;
   const bool pack = b.pack_on, x32 = p->x_dtype == LCE_F32;
+  const float* const pair = rows != nullptr ? rows->pair : nullptr;
+  const int compute = pair != nullptr ? (int)lce::DT_HALF_PAIR : compute_dtype(p);
+  a.pair = pair;
   const int64_t dxes = p->dx_dtype == LCE_F32 ? 4 : 2;
   a.xc = base + k.xc;
   a.ldxc = k.ldxc;
@@ -1207,7 +1214,7 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
     }
     float* lse_c = pack ? (float*)(base + b.lse_c) : nullptr;
     e = x32 ? lce::launch_gather_rows_split((const float*)x, p->ldx, p->H, perm, a.n_rows, p->N, base + k.xc, k.ldxc,
-                                            pack ? lse : nullptr, lse_c, a.num_cus, s)
+                                            pack ? lse : nullptr, lse_c, a.num_cus, s, pair)
             : lce::launch_gather_rows(x, p->ldx * 2, p->H * 2, perm, a.n_rows, p->N, base + k.xc, k.ldxc * 2, lse, lse_c,
                                       a.num_cus, s);
     if (e != hipSuccess) return hip_fail(e, "gather_rows");
@@ -1229,7 +1236,7 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
   if (x32) {  // fp32 activations reach the tile kernels as copies in bf16 pairs, whether or not rows were dropped
     a.x = a.xc;
     a.ldx = a.ldxc;
-    a.x_dtype = lce::DT_PAIR;
+    a.x_dtype = compute;
     a.x_lo = a.ldxc / 2;
   }
   a.dz_rows = a.Np;  // rows of the dz stage (BwdArgs::dz)
@@ -1245,12 +1252,12 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
       // dz and dx of this slab read a 16-bit copy of its columns of the fp32 weight
       if ((ph & LCE_PHASE_BWD_DZ) || (dx && (ph & LCE_PHASE_BWD_DX))) {
         e = a.w_vh ? lce::launch_convert_w_rows((const float*)w, p->ldw, p->H, a.v0, a.vw, base + b.w16, p->H,
-                                                compute_dtype(p), s)
+                                                compute, s)
                    : lce::launch_convert_w_slab((const float*)w, p->ldw, p->H, a.v0, a.vw, base + b.w16, a.vs,
-                                                compute_dtype(p), s);
+                                                compute, s, pair);
         if (e != hipSuccess) return hip_fail(e, "convert_w");
       }
-      a.w = base + b.w16; a.ldw = a.w_vh ? p->H : a.vs; a.w_dtype = compute_dtype(p); a.wv0 = a.v0; a.Vw = a.vw;
+      a.w = base + b.w16; a.ldw = a.w_vh ? p->H : a.vs; a.w_dtype = compute; a.wv0 = a.v0; a.Vw = a.vw;
     } else {
       a.wv0 = 0; a.Vw = p->V;
     }
@@ -1283,10 +1290,12 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
       if (e != hipSuccess) return hip_fail(e, "bwd_grads_small");
       continue;
     }
+    if (rows != nullptr) a.grad_out = rows->factor + 1;
     if (want_dx) {
       e = lce::launch_bwd_dx(a, s);
       if (e != hipSuccess) return hip_fail(e, "bwd_dx");
     }
+    if (rows != nullptr) a.grad_out = rows->factor + 2;
     if (want_dw) {
       e = lce::launch_bwd_dw(a, s);
       if (e != hipSuccess) return hip_fail(e, "bwd_dw");
@@ -1709,8 +1718,8 @@ namespace {
 // What the calls for single tokens keep behind the workspace of the loss's own forward and backward.
 struct TokenPlan {
   BwdPlan b;
-  size_t fwd, fwd_total;                   // forward: out5 and n_valid, which nobody reads
-  size_t row_lse, row_y, part, bwd_total;  // backward: lce::RowGradients; its factor behind the parts
+  size_t fwd, fwd_pair, fwd_total;         // forward: out5 and n_valid, which nobody reads; scales of fp16 pairs and what they are made of
+  size_t row_lse, row_y, part, pair, bwd_total;  // backward: lce::RowGradients; its factor behind the parts
 };
 
 int check_tokens(const lce_problem* p, bool backward) {
@@ -1726,9 +1735,11 @@ lce_problem token_problem(const lce_problem* p) {
   return q;
 }
 
+constexpr size_t kPairBytes = 256 + (size_t)lce::kPairParts * 4;
 size_t plan_token_forward(const lce_problem* p, TokenPlan* t) {
-  t->fwd = align_up(plan_fwd(p).total);
-  return t->fwd_total = t->fwd + 256;
+  t->fwd = align_up(plan_fwd(p, splits(p)).total);
+  t->fwd_pair = t->fwd + 256;
+  return t->fwd_total = t->fwd_pair + (splits(p) ? kPairBytes : 0);
 }
 int plan_token_backward(const lce_problem* q, TokenPlan* t) {
   const int rc = plan_bwd(q, &t->b);
@@ -1736,7 +1747,8 @@ int plan_token_backward(const lce_problem* q, TokenPlan* t) {
   size_t o = align_up(t->b.total);
   t->row_lse = o; o += align_up((size_t)q->N * 4);
   t->row_y = o; o += align_up((size_t)q->N * 8);
-  t->part = o; o += align_up((size_t)lce::kRowGradientParts * 4 + 16);
+  t->part = o; o += align_up((size_t)lce::kRowGradientParts * 4 + 32);
+  t->pair = o; o += splits(q) ? kPairBytes : 0;
   t->bwd_total = o;
   return LCE_OK;
 }
@@ -1762,8 +1774,17 @@ int lce_token_logits(const lce_problem* p, const void* x, const void* w, const i
   if (!logits) return LCE_EINVAL_ARG;
   TokenPlan t;
   if (!ws || ws_bytes < plan_token_forward(p, &t)) return LCE_EWORKSPACE;
+  if (misaligned(ws)) return LCE_EWORKSPACE;
+  if (!x || !w || !y || !lse || misaligned(x) || misaligned(w)) return LCE_EINVAL_ARG;
   char* const out = (char*)ws + t.fwd;
-  return forward_impl(p, x, w, y, lse, (float*)out, (int64_t*)(out + 128), ws, t.fwd, stream, logits, other);
+  float* pair = nullptr;
+  if (splits(p)) {
+    pair = (float*)((char*)ws + t.fwd_pair);
+    const hipError_t e = lce::launch_pair_scales((const float*)x, p->ldx, p->N, p->H, y, p->ignore_index, (const float*)w, p->ldw, p->V, pair,
+                                                 pair + 64, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "pair_scales");
+  }
+  return forward_impl(p, x, w, y, lse, (float*)out, (int64_t*)(out + 128), ws, t.fwd, stream, logits, other, pair);
 }
 
 int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w, const int64_t* y, const float* logits, const float* lse,
@@ -1782,10 +1803,17 @@ int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w
   memset(&r, 0, sizeof(r));
   r.grad_lse = grad_lse; r.grad_logits = grad_logits; r.logits = logits; r.lse = lse; r.y = y;
   r.N = p->N; r.V = p->V; r.ignore_index = p->ignore_index;
-  r.normalise = p->x_dtype == LCE_F16;
+  r.normalise = p->x_dtype != LCE_BF16;
   r.row_lse = (float*)(base + t.row_lse); r.row_y = (int64_t*)(base + t.row_y);
   r.part = (float*)(base + t.part); r.factor = r.part + lce::kRowGradientParts;
-  r.one = (int64_t*)(r.factor + 2);
+  r.one = (int64_t*)(r.factor + 4);
+  if (splits(p)) {
+    float* const pair = (float*)(base + t.pair);
+    const hipError_t e = lce::launch_pair_scales((const float*)x, p->ldx, p->N, p->H, y, p->ignore_index, (const float*)w, p->ldw, p->V, pair,
+                                                 pair + 64, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "pair_scales");
+    r.pair = pair;
+  }
   return backward_impl(&q, t.b, x, w, y, lse, nullptr, nullptr, dx, dw, ws, stream, nullptr, &r);
 }
 

@@ -712,6 +712,7 @@ hipError_t launch_bwd_dw(const BwdArgs& a, hipStream_t s) {
   if (a.x_dtype == DT_BF16) return a.w_vh ? launch_persistent<BF16, true>(a, s) : launch_persistent<BF16, false>(a, s);
   if (a.x_dtype == DT_F16) return a.w_vh ? launch_persistent<F16, true>(a, s) : launch_persistent<F16, false>(a, s);
   if (a.x_dtype == DT_PAIR && a.dw_dtype == DT_F32 && !a.w_vh) return launch_persistent<BF16P, false>(a, s);
+  if (a.x_dtype == DT_HALF_PAIR && a.dw_dtype == DT_F32 && !a.w_vh && a.dw_acc == 0) return launch_persistent<F16P, false>(a, s);
   return hipErrorInvalidValue;
 }
 

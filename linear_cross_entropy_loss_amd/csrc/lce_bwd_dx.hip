@@ -347,6 +347,7 @@ hipError_t launch_bwd_dx(const BwdArgs& a, hipStream_t s) {
   if (a.x_dtype == DT_BF16 && a.w_dtype == DT_BF16) return launch_persistent<BF16>(a, s);
   if (a.x_dtype == DT_F16 && a.w_dtype == DT_F16) return launch_persistent<F16>(a, s);
   if (a.x_dtype == DT_PAIR && a.w_dtype == DT_PAIR && !a.w_vh) return launch_persistent<BF16P>(a, s);
+  if (a.x_dtype == DT_HALF_PAIR && a.w_dtype == DT_HALF_PAIR && !a.w_vh) return launch_persistent<F16P>(a, s);
   return hipErrorInvalidValue;
 }
 

@@ -81,7 +81,7 @@ LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const flo
   typedef typename elem_of<T>::type E;
   const int lane = opaque_tid() & 63;
   const int half = lane >> 5;
-  const float c1 = a.scale * kLog2e;
+  const float c1 = scale_of<T>(a) * kLog2e;
   // columns of this wave's slice that exist: nq whole runs of 8, then `cut` more columns
   const int64_t left = a.v0 + a.vw - slice_v0;
   const int vrem = VTAIL ? (int)(left < 0 ? 0 : (left > kWaveTile ? kWaveTile : left)) : kWaveTile;
@@ -192,7 +192,7 @@ LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const flo
         for (int part = 0; part < (SPLIT && !KEEP ? 2 : KEEP ? 0 : 1); ++part) {
           if (part == 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = bf16_lo(d[i]);
+            for (int i = 0; i < 8; ++i) d[i] = part_lo<T>(d[i]);
           }
           const unsigned x0 = pack2<T>(d[0], d[1]), x1 = pack2<T>(d[2], d[3]);
           const unsigned y0 = pack2<T>(d[4], d[5]), y1 = pack2<T>(d[6], d[7]);
@@ -313,7 +313,7 @@ LCE_DEV void dz_epilogue_impl(const BwdArgs& a, const int (&pf_y)[NQ], const flo
       const float tv = p - __builtin_bit_cast(float, (127 + a.dz_shift) << 23);  // the one, times 2^dz_shift
       E* at = row + (yl >> 6) * grp + qb * (kBlk * kGroup) + (yl & (kGroup - 1));
       *reinterpret_cast<unsigned short*>(at) = to_bits<T>(tv);
-      if (SPLIT) *reinterpret_cast<unsigned short*>(at + kDzBlockElems) = to_bits<T>(bf16_lo(tv));
+      if (SPLIT) *reinterpret_cast<unsigned short*>(at + kDzBlockElems) = to_bits<T>(part_lo<T>(tv));
     }
   }
 }
@@ -513,6 +513,7 @@ hipError_t launch_bwd_dz(const BwdArgs& a, hipStream_t s) {
   if (a.x_dtype == DT_F16 && a.w_dtype == DT_F16) return launch_persistent<F16, false>(a, s);
   // (an fp32 weight arrives here as a copy in the compute type, fp32 activations as bf16 pairs)
   if (a.x_dtype == DT_PAIR && a.w_dtype == DT_PAIR) return launch_persistent<BF16P, false>(a, s);
+  if (a.x_dtype == DT_HALF_PAIR && a.w_dtype == DT_HALF_PAIR && a.row_signs) return launch_persistent_z<F16P, true, false>(a, s);
   return hipErrorInvalidValue;
 }
 

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kThreads, 2) void grads_small_kernel(const BwdArgs 
   __syncthreads();
   float* part = nseg > 1 ? g.part + ((is_dx ? 0 : (int64_t)g.dx_blocks) + (int64_t)tile * nseg + seg) * (kSmallTile * kSmallTile) : nullptr;
   float* sum = !is_dx || (a.first && a.last) ? nullptr : a.dx_acc;
-  const float coef = final_factor_of(a);
+  const float coef = is_dx ? gradient_factor<T, kPairDx>(a) : gradient_factor<T, kPairDw>(a);
   const bool h_rows = !is_dx && !WVH;
   const int64_t qv = q0 + (is_dx ? 0 : a.v0), row0 = h_rows ? h0 : qv, col0 = h_rows ? qv : h0;
 #pragma unroll 2
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void grads_tail_kernel(const BwdArgs a, const 
   const float* part = g.part + ((is_dx ? 0 : (int64_t)g.dx_blocks) + (int64_t)tile * nseg) * (kSmallTile * kSmallTile);
   const int64_t h0 = (int64_t)tp * kSmallTile, q0 = (int64_t)tq * kSmallTile + (is_dx ? 0 : a.v0);
   float* sum = !is_dx || (a.first && a.last) ? nullptr : a.dx_acc;
-  const float coef = final_factor_of(a);
+  const float coef = is_dx ? gradient_factor<T, kPairDx>(a) : gradient_factor<T, kPairDw>(a);
   const bool h_rows = !is_dx && !WVH;
   const int64_t row0 = h_rows ? h0 : q0, col0 = h_rows ? q0 : h0;
   constexpr int kQuads = kSmallTile * kSmallTile / 4 / kTailParts;
@@ -195,6 +195,7 @@ hipError_t launch_bwd_grads_small(const BwdArgs& a, const SmallGrads& g, bool wa
   if (a.x_dtype == DT_BF16 && a.w_dtype == DT_BF16) return launch_small<BF16, false>(a, g, want_dx, want_dw, s);
   if (a.x_dtype == DT_F16 && a.w_dtype == DT_F16) return launch_small<F16, false>(a, g, want_dx, want_dw, s);
   if (a.x_dtype == DT_PAIR && a.w_dtype == DT_PAIR && a.dw_dtype == DT_F32) return launch_small<BF16P, false>(a, g, want_dx, want_dw, s);
+  if (a.x_dtype == DT_HALF_PAIR && a.w_dtype == DT_HALF_PAIR && a.dw_dtype == DT_F32 && !a.w_vh) return launch_small<F16P, false>(a, g, want_dx, want_dw, s);
   return hipErrorInvalidValue;
 }
 

@@ -181,9 +181,10 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const char* x, int64_t
 // long (a multiple of 8, zero-padded).  One workgroup per packed row (grid-stride), 8 elements to a thread: two 16-byte loads,
 // two 16-byte stores; the run that the end of a row cuts is read element by element.  Bound by memory traffic, 4 bytes read and
 // 4 written per element.
+template <class T>
 __global__ __launch_bounds__(256) void gather_rows_split_kernel(const float* x, int64_t ldx, int64_t H, const int* perm,
                                                                 const int64_t* n_rows, int64_t N, unsigned short* xc,
-                                                                int64_t part, const float* lse, float* lse_c) {
+                                                                int64_t part, const float* lse, float* lse_c, const float* pair) {
   const int64_t rows = n_rows != nullptr ? packed_rows(n_rows, N) : N;
   for (int64_t j = blockIdx.x; j < rows; j += gridDim.x) {
     const int64_t src = perm != nullptr ? packed_token(perm, j, N) : j;
@@ -203,11 +204,16 @@ __global__ __launch_bounds__(256) void gather_rows_split_kernel(const float* x, 
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = k + i < H ? s[k + i] : 0.f;
       }
+      if constexpr (is_half_pair<T>::value) {
+        const float f = pair[0];  // (kPairX)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= f;
+      }
       u32x4_t hi, lo;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        hi[i] = pack2<BF16>(v[2 * i], v[2 * i + 1]);
-        lo[i] = pack2<BF16>(bf16_lo(v[2 * i]), bf16_lo(v[2 * i + 1]));
+        hi[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+        lo[i] = pack2<T>(part_lo<T>(v[2 * i]), part_lo<T>(v[2 * i + 1]));
       }
       *reinterpret_cast<u32x4_t*>(c + k) = hi;
       *reinterpret_cast<u32x4_t*>(c + part + k) = lo;
@@ -326,10 +332,10 @@ hipError_t launch_stand_in(const int64_t* y, int64_t N, int64_t ignore_index, fl
 
 hipError_t launch_gather_rows_split(const float* x, int64_t ldx, int64_t H, const int* perm, const int64_t* n_rows,
                                     int64_t N, void* xc, int64_t ldxc, const float* lse, float* lse_c, int num_cus,
-                                    hipStream_t s) {
+                                    hipStream_t s, const float* pair) {
   if (ldxc % 16 != 0) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(gather_rows_split_kernel, dim3(row_grid(N, num_cus)), dim3(256), 0, s, x, ldx, H, perm, n_rows, N,
-                     reinterpret_cast<unsigned short*>(xc), ldxc / 2, lse, lse_c);
+  hipLaunchKernelGGL((pair != nullptr ? gather_rows_split_kernel<F16P> : gather_rows_split_kernel<BF16P>), dim3(row_grid(N, num_cus)), dim3(256), 0, s, x,
+                     ldx, H, perm, n_rows, N, reinterpret_cast<unsigned short*>(xc), ldxc / 2, lse, lse_c, pair);
   return hipGetLastError();
 }
 

@@ -105,7 +105,7 @@ template <class T, bool VTAIL, bool KMASK, bool WVH, bool MON> struct FwdProblem
       const int64_t tok = a.row0 + (int64_t)etq * kTile + (wave >> 1) * kWaveTile + qb * kBlk + (lane & 31);
       const int64_t yy = pf_y[qb], rel = yy - slice_v0;
       const bool here = yy != a.ignore_index && rel >= 0 && rel < kWaveTile && ((rel >> 2) & 1) == (lane >> 5);
-      fwd_store_target(a, acc, tok, qb, here ? (int)rel : -1);
+      fwd_store_target<T, kNB>(a, acc, tok, qb, here ? (int)rel : -1);
     }
   }
   LCE_DEV void epilogue(int tile, f32x16_t (&acc)[kNB][kNB], char*) const {
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_small_kernel(const FwdArgs a,
     const int lane = threadIdx.x & 63;
     const int64_t tok = a.row0 + tw + (lane & 31), yy = tok < rows ? a.y[tok] : a.ignore_index, rel = yy - slice_v0;
     const bool here = yy != a.ignore_index && rel >= 0 && rel < kWaveTile && ((rel >> 2) & 1) == (lane >> 5);
-    fwd_store_target<1>(a, acc, tok, 0, here ? (int)rel : -1);
+    fwd_store_target<T, 1>(a, acc, tok, 0, here ? (int)rel : -1);
   } else {
     fwd_epilogue<T, true, MON, 1>(a, rows, acc, slice_v0, tw);
   }
@@ -421,7 +421,7 @@ template <class T, bool WVH, bool MON> hipError_t launch_persistent(const FwdArg
     if (a.H <= kNarrowHidden && a.small_wgs > 0 && a.w_dtype != DT_F32) return launch_fwd_narrow(a, rows, s);
   }
   if (a.w_dtype == DT_F32) {  // read as it is (fwd_reads_f32)
-    if constexpr (is_pair<T>::value && MON) {
+    if constexpr ((is_pair<T>::value && MON) || is_half_pair<T>::value) {
       return hipErrorInvalidValue;
     } else {
       const int tiles_p = (int)(pad_to(a.vw, kTile) / kSmallTile), tiles_q = (int)((rows + kSmallTile - 1) / kSmallTile);
@@ -447,7 +447,8 @@ template <class T, bool WVH, bool MON> hipError_t launch_persistent(const FwdArg
 }
 
 template <class T, bool WVH> hipError_t launch_layout(const FwdArgs& a, hipStream_t s) {
-  return a.monitoring ? launch_persistent<T, WVH, true>(a, s) : launch_persistent<T, WVH, false>(a, s);
+  if constexpr (is_half_pair<T>::value) return launch_persistent<T, WVH, false>(a, s);
+  else return a.monitoring ? launch_persistent<T, WVH, true>(a, s) : launch_persistent<T, WVH, false>(a, s);
 }
 
 }  // namespace
@@ -459,6 +460,7 @@ hipError_t launch_fwd_tiles(const FwdArgs& a, hipStream_t s) {
   if (a.x_dtype == DT_BF16 && as_x) return a.w_vh ? launch_layout<BF16, true>(a, s) : launch_layout<BF16, false>(a, s);
   if (a.x_dtype == DT_F16 && as_x) return a.w_vh ? launch_layout<F16, true>(a, s) : launch_layout<F16, false>(a, s);
   if (a.x_dtype == DT_PAIR && as_x && !a.w_vh) return launch_layout<BF16P, false>(a, s);
+  if (a.x_dtype == DT_HALF_PAIR && a.w_dtype == DT_HALF_PAIR && !a.w_vh) return launch_layout<F16P, false>(a, s);
   return hipErrorInvalidValue;
 }
 

@@ -34,7 +34,7 @@ LCE_DEV void fwd_epilogue(const FwdArgs& a, int64_t rows, f32x16_t (&acc)[kNB][N
   const int nq = vrem >> 3, cut = vrem & 7;
   const int mine = cut - 4 * (lane >> 5);  // elements of this lane's quad of the cut run that exist (<= 0: none)
 
-  const float c1 = a.scale * kLog2e;
+  const float c1 = scale_of<T>(a) * kLog2e;
   const int64_t slice = slice_v0 / kChunkV;
 #pragma unroll
   for (int qb = 0; qb < NQ; ++qb) {
@@ -70,7 +70,7 @@ LCE_DEV void fwd_epilogue(const FwdArgs& a, int64_t rows, f32x16_t (&acc)[kNB][N
           for (int j = 0; j < 4; ++j) m = j < mine ? fmaxf(m, acc[pb][qb][rq * 4 + j]) : m;
         }
     m = fmaxf(m, __shfl_xor(m, 32));
-    m *= a.scale;  // logit_scale > 0, so max commutes with the scaling
+    m *= scale_of<T>(a);  // logit_scale > 0, so max commutes with the scaling
     const float mo = m * kLog2e;
     float s = 0.f, pz = 0.f, sq = 0.f;
     if (MON) {
@@ -82,7 +82,7 @@ LCE_DEV void fwd_epilogue(const FwdArgs& a, int64_t rows, f32x16_t (&acc)[kNB][N
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float e = fast_exp2(fmaf(acc[pb][qb][rq * 4 + j], c1, -mo));
-              const float z = acc[pb][qb][rq * 4 + j] * a.scale;
+              const float z = acc[pb][qb][rq * 4 + j] * scale_of<T>(a);
               s += e;
               pz = fmaf(e, z, pz);
               sq = fmaf(z, z, sq);
@@ -91,7 +91,7 @@ LCE_DEV void fwd_epilogue(const FwdArgs& a, int64_t rows, f32x16_t (&acc)[kNB][N
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float e = fast_exp2(fmaf(acc[pb][qb][rq * 4 + j], c1, -mo));
-              const float z = acc[pb][qb][rq * 4 + j] * a.scale;
+              const float z = acc[pb][qb][rq * 4 + j] * scale_of<T>(a);
               s += j < mine ? e : 0.f;
               pz = j < mine ? fmaf(e, z, pz) : pz;
               sq = j < mine ? fmaf(z, z, sq) : sq;
@@ -132,7 +132,7 @@ LCE_DEV void fwd_epilogue(const FwdArgs& a, int64_t rows, f32x16_t (&acc)[kNB][N
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (pb == want_pb && r == want_r) zt = acc[pb][qb][r];
-      a.tgt[tok] = zt * a.scale;
+      a.tgt[tok] = zt * scale_of<T>(a);
     }
   }
 }
@@ -141,7 +141,7 @@ LCE_DEV void fwd_epilogue(const FwdArgs& a, int64_t rows, f32x16_t (&acc)[kNB][N
 // The logit of the target column, written by the one lane that holds it (rare: a wave holds the target of
 // one token in a thousand at a vocabulary of 131072).  `yl`: the column inside this wave's 128-wide slice if
 // this lane's half holds it, else -1.
-template <int NQ>
+template <class T, int NQ>
 LCE_DEV void fwd_store_target(const FwdArgs& a, f32x16_t (&acc)[kNB][NQ], int64_t tok, int qb, int yl) {
   if (yl >= 0) {
     const int want = (yl >> 5) * 16 + ((yl >> 3) & 3) * 4 + (yl & 3);  // (block, register) index
@@ -155,7 +155,7 @@ LCE_DEV void fwd_store_target(const FwdArgs& a, f32x16_t (&acc)[kNB][NQ], int64_
         asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(acc[pb][qb][r]));
         if (want == pb * 16 + r) zt = v;
       }
-    a.tgt[tok] = zt * a.scale;
+    a.tgt[tok] = zt * scale_of<T>(a);
   }
 }
 
@@ -175,9 +175,9 @@ struct FwdColumnState {
 // Slot 0..15 of block column QB: the running (max, sum) of this lane's 64 values -- and, MON, the two monitoring
 // sums, which leave the arithmetic on (max, sum) as it is, so that the loss does not depend on the monitoring flag
 // bit for bit.  The exponentials of a slot are added up in the next one, when they are there.
-template <int QB, bool MON, int NQ>
+template <class T, int QB, bool MON, int NQ>
 LCE_DEV void fwd_slot_sum(const FwdArgs& a, FwdColumnState& st, f32x16_t (&acc)[kNB][NQ], int slot) {
-  const float c1 = a.scale * kLog2e;
+  const float c1 = scale_of<T>(a) * kLog2e;
   const int c = slot >> 3, sub = slot & 7;  // chunk c: accumulator blocks 2c, 2c + 1, slots 8c .. 8c + 7
   if (slot > 0) {
     st.s += (st.e[0] + st.e[1]) + (st.e[2] + st.e[3]);
@@ -185,7 +185,7 @@ LCE_DEV void fwd_slot_sum(const FwdArgs& a, FwdColumnState& st, f32x16_t (&acc)[
       const int prev = 4 * ((slot - 1) & 7);  // (the chunk of the previous slot is still in st.v)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float z = st.v[prev + r] * a.scale;
+        const float z = st.v[prev + r] * scale_of<T>(a);
         st.pz = fmaf(st.e[r], z, st.pz);
         st.sq = fmaf(z, z, st.sq);
       }
@@ -216,7 +216,7 @@ LCE_DEV void fwd_slot_sum(const FwdArgs& a, FwdColumnState& st, f32x16_t (&acc)[
     if (MON) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float z = st.v[28 + r] * a.scale;
+        const float z = st.v[28 + r] * scale_of<T>(a);
         st.pz = fmaf(st.e[r], z, st.pz);
         st.sq = fmaf(z, z, st.sq);
       }
@@ -225,9 +225,9 @@ LCE_DEV void fwd_slot_sum(const FwdArgs& a, FwdColumnState& st, f32x16_t (&acc)[
 }
 // After slot 15: the other half of the slice.  Leaves the slice's max (unscaled) in st.m, its sum of exp2 in st.s
 // and, MON, the slice's monitoring sums in st.pz, st.sq.
-template <bool MON>
+template <class T, bool MON>
 LCE_DEV void fwd_merge_halves(const FwdArgs& a, FwdColumnState& st) {
-  const float c1 = a.scale * kLog2e;
+  const float c1 = scale_of<T>(a) * kLog2e;
   // after the swaps both lanes of a pair hold the lower lane's value in [0] and the upper lane's in [1]
   const unsigned mb = __builtin_bit_cast(unsigned, st.m), sb = __builtin_bit_cast(unsigned, st.s);
   const auto mm = __builtin_amdgcn_permlane32_swap(mb, mb, false, false);
@@ -252,9 +252,9 @@ LCE_DEV void fwd_merge_halves(const FwdArgs& a, FwdColumnState& st) {
 // tw: first token row of the wave inside this launch's chunk (like slice_v0 uniform over the wave).
 template <class T, int QB, bool MON, int NQ>
 LCE_DEV void fwd_epilogue_slot(const FwdArgs& a, FwdColumnState& st, f32x16_t (&acc)[kNB][NQ], int64_t slice_v0, int64_t tw, int slot) {
-  fwd_slot_sum<QB, MON, NQ>(a, st, acc, slot);
+  fwd_slot_sum<T, QB, MON, NQ>(a, st, acc, slot);
   if (slot == 15) {
-    fwd_merge_halves<MON>(a, st);
+    fwd_merge_halves<T, MON>(a, st);
     // one store per token and partial: the upper lanes get an offset that the range check of the buffer store drops
     const int lane = threadIdx.x & 63;
     const int64_t o = slice_v0 / kChunkV * a.nc + tw + QB * kBlk;
@@ -263,9 +263,9 @@ LCE_DEV void fwd_epilogue_slot(const FwdArgs& a, FwdColumnState& st, f32x16_t (&
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(base + o, 0, kBlk * 4, 0x00020000);
       __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, voff, 0, 0);
     };
-    store(a.part_lse, fmaf(st.m, a.scale, fast_log(st.s)));
+    store(a.part_lse, fmaf(st.m, scale_of<T>(a), fast_log(st.s)));
     if (MON) {
-      store(a.part_max, st.m * a.scale);
+      store(a.part_max, st.m * scale_of<T>(a));
       store(a.part_pz, st.pz / st.s);
       store(a.part_sq, st.sq);
     }

@@ -50,13 +50,18 @@ constexpr int kMainloopLds = 2 * kStageBytes;      // double buffered: 128 KiB
 struct BF16 {};
 struct F16 {};
 struct BF16P {};  // fp32 values as bf16 pairs (below)
+struct F16P {};   // the same as fp16 pairs, scaled (below)
 template <class T> struct is_pair { static constexpr bool value = false; };
 template <> struct is_pair<BF16P> { static constexpr bool value = true; };
+template <> struct is_pair<F16P> { static constexpr bool value = true; };
+template <class T> struct is_half_pair { static constexpr bool value = false; };
+template <> struct is_half_pair<F16P> { static constexpr bool value = true; };
 
 template <class T> struct elem_of;
 template <> struct elem_of<BF16> { typedef __bf16 type; };
 template <> struct elem_of<F16> { typedef _Float16 type; };
 template <> struct elem_of<BF16P> { typedef __bf16 type; };
+template <> struct elem_of<F16P> { typedef _Float16 type; };
 
 template <class T> LCE_DEV f32x16_t mfma32(s16x8_t a, s16x8_t b, f32x16_t c);
 template <> LCE_DEV f32x16_t mfma32<BF16>(s16x8_t a, s16x8_t b, f32x16_t c) {
@@ -68,6 +73,7 @@ template <> LCE_DEV f32x16_t mfma32<F16>(s16x8_t a, s16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
                                                 __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
+template <> LCE_DEV f32x16_t mfma32<F16P>(s16x8_t a, s16x8_t b, f32x16_t c) { return mfma32<F16>(a, b, c); }
 
 // float -> 16-bit compute type, round to nearest even, returned as raw bits.
 template <class T> LCE_DEV unsigned short to_bits(float f) {
@@ -92,6 +98,10 @@ LCE_DEV float bf16_hi(float v) {
   return __builtin_bit_cast(float, (unsigned)to_bits<BF16>(v) << 16);
 }
 LCE_DEV float bf16_lo(float v) { return v - bf16_hi(v); }  // exact in fp32; rounded to bf16 when stored
+// Pairs of fp16 (lce_token_logits) carry 22 bits in the same space and the same three products, where the numbers lie in fp16's
+// range: every operand is multiplied by a power of two that brings its largest number to 2^13 ... 2^14 (launch_pair_scales), and a number
+// is then off by 2^-23 of itself or by 2^-39 of the largest, whichever is more.
+template <class T> LCE_DEV float part_lo(float v) { return v - (float)(typename elem_of<T>::type)v; }
 
 // threadIdx.x behind an optimisation barrier.  Epilogues that run inside a
 // persistent tile loop derive their per-lane indices from this, so that the

@@ -30,6 +30,18 @@
 
 namespace lce {
 
+// Factor of the sums that are logits, and of those that are gradients where one launch has both: what the operands of an fp16 pair were
+// multiplied by goes out again.  (The kernels of dx or dW alone find it in BwdArgs::grad_out: they have no register for it.)
+enum { kPairX = 0, kPairW, kPairLogits, kPairDx, kPairDw, kPairScales };
+template <class T, class Args> LCE_DEV float scale_of(const Args& a) {
+  if constexpr (is_half_pair<T>::value) return a.scale * a.pair[kPairLogits];
+  else return a.scale;
+}
+template <class T, int OF> LCE_DEV float gradient_factor(const BwdArgs& a) {
+  if constexpr (is_half_pair<T>::value) return final_factor_of(a) * a.pair[OF];
+  else return final_factor_of(a);
+}
+
 // Register staging of one operand tile of CHUNKS * 32 rows or columns: CHUNKS chunks of 8 elements (one 16-byte register quad)
 // per thread.
 // Operands are always 16-bit in memory: fp32 activations and weights are rounded to the compute type by

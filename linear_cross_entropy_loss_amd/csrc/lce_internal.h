@@ -11,8 +11,8 @@
 namespace lce {
 
 enum { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
-// Compute type of fp32 tensors inside the library: bf16 pairs (lce_gemm.h).
-enum { DT_PAIR = 3 };
+// Compute types of fp32 tensors inside the library: bf16 pairs, fp16 pairs (lce_gemm.h).
+enum { DT_PAIR = 3, DT_HALF_PAIR = 4 };
 
 // The tile kernels use more dynamic LDS than a kernel gets by default and have to opt in
 // (hipFuncAttributeMaxDynamicSharedMemorySize): once per kernel and device, not before every launch.  One object
@@ -49,7 +49,7 @@ constexpr int64_t padded_k(int64_t H) { return pad_to(H, 128) < 256 ? 256 : pad_
 // Pairs: three K tiles for each of these 64-wide ones, so two of them are enough
 constexpr int64_t padded_k_pair(int64_t H) { return pad_to(H, 128); }
 // Matrix products per K tile of the compute type.
-constexpr int products_of(int dtype) { return dtype == DT_PAIR ? 3 : 1; }
+constexpr int products_of(int dtype) { return dtype == DT_PAIR || dtype == DT_HALF_PAIR ? 3 : 1; }
 // K tiles of the logit contraction on 128 x 128 tiles, which need no four of them (N=8192, H=128, V=8192: 60 us with four, 47 with two).
 __host__ __device__ constexpr int64_t small_logit_ktiles(int64_t H, int products) { return products * (pad_to(H, 128) / 64); }
 
@@ -132,6 +132,7 @@ struct FwdArgs {
   // ignore_index or `tok_other`, NaN where it is any other that is no column
   float* tok_logits;
   int64_t tok_other;
+  const float* pair;  // DT_HALF_PAIR: launch_pair_scales
 };
 
 struct BwdArgs {
@@ -231,6 +232,7 @@ struct BwdArgs {
   // g_lse is positive and kNegativeRow where it is negative, and the kernels stage g_lse * softmax, the sign through the gain of z_reg;
   // the label's column is launch_row_targets'.  grad_out and n_valid are a factor and 1 there.
   int row_signs;
+  const float* pair;  // DT_HALF_PAIR: launch_pair_scales
 };
 
 // Element offset of block (row tile, column group) of a dz stage that is `vs` columns wide.
@@ -276,9 +278,9 @@ hipError_t launch_scale_two(const ScaleTask& t0, const ScaleTask& t1, const floa
 hipError_t launch_bwd_dx(const BwdArgs& a, hipStream_t s);
 hipError_t launch_bwd_dw(const BwdArgs& a, hipStream_t s);
 // dst[h][c] = 16-bit rounding of src[h * ld + v0 + c] for c < vw, 0 for vw <= c < dst_ld; h < H.
-// compute_dtype: DT_BF16, DT_F16 or DT_PAIR: dst then has 2 H rows, [bf16 hi ; bf16 lo] of the fp32 values.
+// compute_dtype: DT_BF16, DT_F16 or a pair: dst then has 2 H rows, [hi ; lo] of the fp32 values (`pair`: DT_HALF_PAIR's scales).
 hipError_t launch_convert_w_slab(const float* src, int64_t ld, int64_t H, int64_t v0, int64_t vw, void* dst,
-                                 int64_t dst_ld, int compute_dtype, hipStream_t s);
+                                 int64_t dst_ld, int compute_dtype, hipStream_t s, const float* pair = nullptr);
 // The same for a weight stored (V, H) row-major (H a multiple of 8): rows [v0, v0 + vw) go to dst[vw][dst_ld].
 hipError_t launch_convert_w_rows(const float* src, int64_t ld, int64_t H, int64_t v0, int64_t vw, void* dst,
                                  int64_t dst_ld, int compute_dtype, hipStream_t s);
@@ -326,7 +328,7 @@ hipError_t launch_gather_rows(const void* x, int64_t ldx_bytes, int64_t row_byte
 // order).  Strides in elements; rows of x on 16-byte boundaries.
 hipError_t launch_gather_rows_split(const float* x, int64_t ldx, int64_t H, const int* perm, const int64_t* n_rows,
                                     int64_t N, void* xc, int64_t ldxc, const float* lse, float* lse_c, int num_cus,
-                                    hipStream_t s);
+                                    hipStream_t s, const float* pair = nullptr);
 // dx[perm[j]] = dxc[j] for j < *n_rows (skipped when dxc is null) and dx[i] = 0 for every token i with
 // y[i] == ignore_index, in 8-byte pieces covering row_bytes; nothing when *n_rows == N.
 hipError_t launch_scatter_rows(const void* dxc, int64_t lddxc_bytes, const int* perm, const int64_t* n_rows,
@@ -526,7 +528,7 @@ int soft_loss_groups();
 
 // Upstream gradients of each row (lce_tokens.hip): `lse` and `y` as BwdArgs::row_signs has them, of row perm[j] where the rows are packed
 // (perm not null).  With `normalise` the gradients are divided by *factor, the power of two that leaves |grad_lse| + |grad_logits| at
-// most 1 (else *factor = 1); rows whose label is ignore_index do not count.  part: kRowGradientParts floats.
+// most 1 (else 1); rows whose label is ignore_index do not count.  part: kRowGradientParts floats.
 struct RowGradients {
   const float* grad_lse;
   const float* grad_logits;
@@ -538,8 +540,9 @@ struct RowGradients {
   int normalise;
   float* row_lse;
   int64_t* row_y;
-  float* factor;
-  int64_t* one;  // becomes 1
+  float* factor;  // [3]: for the staged rows, and with the scales of an fp16 pair for dx and dW where they are apart
+  int64_t* one;   // becomes 1
+  const float* pair;  // BwdArgs::pair
   float* part;
 };
 constexpr int kRowGradientParts = 64;
@@ -547,6 +550,11 @@ constexpr int64_t kNegativeRow = -2;
 hipError_t launch_row_gradients(const RowGradients& g, hipStream_t s);
 // dz of the labels' columns of the slab that `a` describes, over what the kernels staged there.
 hipError_t launch_row_targets(const BwdArgs& a, const RowGradients& g, hipStream_t s);
+// pair[kPairScales] (lce_gemm3.h) for fp32 rows x of kept labels and a weight (H, V); numbers that are not finite do not count.  part:
+// kPairParts floats.
+constexpr int kPairParts = 1024;
+hipError_t launch_pair_scales(const float* x, int64_t ldx, int64_t N, int64_t H, const int64_t* y, int64_t ignore_index, const float* w, int64_t ldw,
+                              int64_t V, float* pair, float* part, hipStream_t s);
 // out[i] = the column tokens[i] - start where that is one of V, -1 for ignore_index, V for another token of [0, size), V + 1 for what is none.
 hipError_t launch_token_labels(const int64_t* tokens, int64_t N, int64_t ignore_index, int64_t start, int64_t V, int64_t size, int64_t* out,
                                hipStream_t s);

@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_narrow_kernel(const FwdArgs a
       for (int slot = 0; slot < 16; ++slot) fwd_epilogue_slot<T, 0, MON, 1>(a, st, acc, slice_v0, tw, slot);
       const int64_t rel = yy - slice_v0;
       const bool here = yy != a.ignore_index && rel >= 0 && rel < kNarrowTile && ((rel >> 2) & 1) == (lane >> 5);
-      fwd_store_target<1>(a, acc, tok, 0, here ? (int)rel : -1);
+      fwd_store_target<T, 1>(a, acc, tok, 0, here ? (int)rel : -1);
     } else {
       fwd_epilogue<T, true, MON, 1>(a, rows, acc, slice_v0, tw);
     }

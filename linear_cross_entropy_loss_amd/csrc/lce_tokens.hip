@@ -8,11 +8,14 @@
 // lse' is rounded at 24 bits, which moves a probability by a factor of 1 +- 2^-19 at |lse'| < 32, as far as the rounding of its
 // exponent does.  The label's column is written over the stage afterwards, from the logit that the forward gave (row_targets_kernel).
 //
-// fp16: a stage has 30 binary places below 1 while upstream gradients are of any size (1 / rows, times a loss scale), so all are divided
+// fp16, and fp32 as fp16 pairs: a stage has 30 binary places below 1 while upstream gradients are of any size (1 / rows, times a loss scale), so all are divided
 // by one power of two, which the dx and dW kernels multiply in again after their fp32 sums.
 //
-// All of it is a few numbers a row: bound by launches.
-#include "lce_gemm.h"
+// All of that is a few numbers a row: bound by launches.
+//
+// fp32 tensors: fp16 pairs (lce_gemm.h) instead of the loss's bf16 ones, for products 22 bits wide.  N=2048, H=1024, V=16384, errors of dx and
+// dW against fp64, relative to their norms: PAIRERR.  Their scales cost one more pass over the weight (pair_max_kernel).
+#include "lce_gemm3.h"
 #include "lce_internal.h"
 
 namespace lce {
@@ -50,7 +53,10 @@ __global__ __launch_bounds__(kRowThreads) void row_gradients_kernel(const RowGra
     }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    *g.factor = ldexpf(1.f, e);
+    const float f = ldexpf(1.f, e);
+    g.factor[0] = f;
+    g.factor[1] = g.pair != nullptr ? f * g.pair[kPairDx] : f;
+    g.factor[2] = g.pair != nullptr ? f * g.pair[kPairDw] : f;
     *g.one = 1;
   }
   for (int64_t j = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; j < g.N; j += (int64_t)gridDim.x * kRowThreads) {
@@ -78,8 +84,8 @@ __global__ __launch_bounds__(kRowThreads) void row_targets_kernel(const BwdArgs 
     unsigned short* dz = reinterpret_cast<unsigned short*>(a.dz);
     if constexpr (is_pair<T>::value) {
       dz += 2 * dz_block_offset(j / kTile, rel / 64, a.vs) + at;
-      dz[0] = to_bits<BF16>(d);
-      dz[kDzBlockElems] = to_bits<BF16>(bf16_lo(d));
+      dz[0] = to_bits<T>(d);
+      dz[kDzBlockElems] = to_bits<T>(part_lo<T>(d));
     } else {
       dz[dz_block_offset(j / kTile, rel / 64, a.vs) + at] = to_bits<T>(d);
     }
@@ -91,6 +97,65 @@ __global__ __launch_bounds__(kRowThreads) void token_labels_kernel(const int64_t
   for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < N; i += (int64_t)gridDim.x * kRowThreads) {
     const int64_t t = tokens[i];
     out[i] = t == ignore_index ? -1 : t < 0 || t >= size ? V + 1 : t >= start && t < start + V ? t - start : V;
+  }
+}
+
+// part[b] = the largest finite magnitude of this workgroup's pieces: of kept rows of x (the first x_groups workgroups) or of the weight.
+constexpr int64_t kScalePiece = 4096;  // numbers of a row that a workgroup looks at at a time
+__global__ __launch_bounds__(kRowThreads) void pair_max_kernel(const float* x, int64_t ldx, int64_t N, int64_t H, const int64_t* y, int64_t ignore_index,
+                                                               const float* w, int64_t ldw, int64_t V, int x_groups, float* part) {
+  const bool of_x = (int)blockIdx.x < x_groups;
+  const float* t = of_x ? x : w;
+  const int64_t rows = of_x ? N : H, cols = of_x ? H : V, ld = of_x ? ldx : ldw, per = (cols + kScalePiece - 1) / kScalePiece;
+  const int64_t first = of_x ? blockIdx.x : blockIdx.x - x_groups, step = of_x ? x_groups : (int)gridDim.x - x_groups;
+  float m = 0.f;
+  for (int64_t i = first; i < rows * per; i += step) {
+    const int64_t r = i / per, c0 = (i - r * per) * kScalePiece;
+    if (of_x && y[r] == ignore_index) continue;
+    const float* row = t + r * ld;
+#pragma unroll
+    for (int k = 0; k < kScalePiece / (4 * kRowThreads); ++k) {
+      const int64_t c = c0 + (k * kRowThreads + (int)threadIdx.x) * 4;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (c + 4 <= cols) {
+        const f32x4_t q = *reinterpret_cast<const f32x4_t*>(row + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = q[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < cols) v[j] = row[c + j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = fabsf(v[j]);
+        m = a < INFINITY && a > m ? a : m;
+      }
+    }
+  }
+  m = largest_of_workgroup(m);
+  if (threadIdx.x == 0) part[blockIdx.x] = m;
+}
+__global__ __launch_bounds__(kRowThreads) void pair_scales_kernel(const float* part, int x_groups, int groups, float* pair) {
+  __shared__ int exponent[2];
+  for (int of = 0; of < 2; ++of) {
+    float m = 0.f;
+    for (int i = (of == 0 ? 0 : x_groups) + threadIdx.x; i < (of == 0 ? x_groups : groups); i += kRowThreads) m = fmaxf(m, part[i]);
+    m = largest_of_workgroup(m);
+    if (threadIdx.x == 0) {
+      int e = 0;
+      if (m > 0.f) (void)frexpf(m, &e);
+      e = 14 - e;  // the largest becomes 2^13 ... 2^14
+      exponent[of] = m > 0.f ? (e > 60 ? 60 : e) : 0;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    pair[kPairX] = ldexpf(1.f, exponent[0]);
+    pair[kPairW] = ldexpf(1.f, exponent[1]);
+    pair[kPairLogits] = ldexpf(1.f, -exponent[0] - exponent[1]);
+    pair[kPairDx] = ldexpf(1.f, -exponent[1]);
+    pair[kPairDw] = ldexpf(1.f, -exponent[0]);
   }
 }
 
@@ -114,9 +179,20 @@ hipError_t launch_row_gradients(const RowGradients& g, hipStream_t s) {
 
 hipError_t launch_row_targets(const BwdArgs& a, const RowGradients& g, hipStream_t s) {
   const dim3 grid(row_groups(a.N, 1024)), threads(kRowThreads);
-  if (a.x_dtype == DT_PAIR) hipLaunchKernelGGL(row_targets_kernel<BF16P>, grid, threads, 0, s, a, g);
+  if (a.x_dtype == DT_HALF_PAIR) hipLaunchKernelGGL(row_targets_kernel<F16P>, grid, threads, 0, s, a, g);
   else if (a.x_dtype == DT_F16) hipLaunchKernelGGL(row_targets_kernel<F16>, grid, threads, 0, s, a, g);
   else hipLaunchKernelGGL(row_targets_kernel<BF16>, grid, threads, 0, s, a, g);
+  return hipGetLastError();
+}
+
+hipError_t launch_pair_scales(const float* x, int64_t ldx, int64_t N, int64_t H, const int64_t* y, int64_t ignore_index, const float* w, int64_t ldw,
+                              int64_t V, float* pair, float* part, hipStream_t s) {
+  const int64_t px = N * ((H + kScalePiece - 1) / kScalePiece), pw = H * ((V + kScalePiece - 1) / kScalePiece);
+  const int x_groups = (int)(px < kPairParts / 4 ? px : kPairParts / 4), w_groups = (int)(pw < kPairParts * 3 / 4 ? pw : kPairParts * 3 / 4);
+  hipLaunchKernelGGL(pair_max_kernel, dim3(x_groups + w_groups), dim3(kRowThreads), 0, s, x, ldx, N, H, y, ignore_index, w, ldw, V, x_groups, part);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(pair_scales_kernel, dim3(1), dim3(kRowThreads), 0, s, part, x_groups, x_groups + w_groups, pair);
   return hipGetLastError();
 }
 
