@@ -6,6 +6,10 @@
 // The contraction is that of the loss's logit kernels (lce_gemm3.h, lce_gemm_small.h) with v_mfma_i32_32x32x32_i8 in the place of the 16-bit
 // instruction: both take 16 bytes of K of each lane, so that an operand of 8-bit numbers is staged, swizzled and read as one of
 // half as many 16-bit numbers, in the same time for twice the K.  Sums are exact in 32 bits (127^2 * 2^17 < 2^31).
+// Bound by the matrix cores' power from some 500 rows on: 2048 rows of 4096 x 32000 in 220 us, 2.4 POP/s, the rate of a large library product of
+// 8-bit numbers here (2.1 to 2.4), and less than twice that of 16-bit ones, whose K tiles take 1.2 us, not 1.9.  256 rows of 4096 x 128256, where
+// weight and matrix cores ask for as much, 166 us: 1.6 POP/s beside 3.6 TB/s.  (A second set of registers for the weight's K tiles, two
+// ahead: 173 us, the loads are not what it waits for; 128 x 128 tiles 186.)
 #include "lce_gemm_small.h"
 #include "lce_internal.h"
 
@@ -580,15 +584,16 @@ template <class T> __global__ __launch_bounds__(kThreads, 2) void int8_small_ker
 // that is multiplied, across the ends of its rows too; the quantised rows of x lie in LDS in the order in which the lanes want them:
 // 16 bytes of K, row after row.  There are 1, 2, 4, 8 or 16 places for rows, or 32, which are two instructions to a load; lanes
 // beyond the places read the same rows again, and nobody stores what comes of it.
-// A small x (kFusedNumbers) is quantised by every workgroup for itself while its first loads of the weight are under way: one row of 2048
-// in 3 us less than a launch takes, eight in 5 more.
+// One or two short rows (kFusedRows, kFusedNumbers) are quantised by every workgroup for itself while its first loads of the weight are under
+// way: one row of 2048 in 3 us less than a launch takes.  (More rows, which it takes one after another: 8 of 2048 5 us more than the
+// launch, 16 of 256 13.)
 // Bound by the weight's way from memory.  us, with x quantised, against the 128 x 128 tiles: 2048 x 131072 one row 50 / 58, 16 rows 55 / 58;
 // 4096 x 128256 one row 97 / 110, 16 rows 108 / 116, 32 rows 114 / 121 (2048 x 131072 61 / 59: not taken for short rows); 8192 x 32000 55 / 67.
 // Four loads in a group 50, 106 and 64 us for one row, twelve 55, 110 and 59; loads past the caches 53, 107 and 59.
 // ---------------------------------------------------------------------------
 constexpr int kStreamThreads = 512, kFlight = 8, kGroupBytes = 64 * kFlight;
 constexpr int kStreamLds = 150 * 1024;
-constexpr int64_t kFusedNumbers = 8192;
+constexpr int64_t kFusedRows = 2, kFusedNumbers = 16384;
 LCE_DEV u32x4_t* place_of(char* lds, int byte, int n, int places) {
   return reinterpret_cast<u32x4_t*>(lds + ((byte >> 4) * places + n) * 16 + (byte & 15));
 }
@@ -816,7 +821,7 @@ hipError_t launch_quantize_columns(const void* src, int dtype, int64_t rows, int
 }
 bool int8_quantizes(const Int8Args& a) {
   int depth;
-  return a.N * a.H <= kFusedNumbers && stream_places(a, &depth) > 0;
+  return a.N <= kFusedRows && a.N * a.H <= kFusedNumbers && stream_places(a, &depth) > 0;
 }
 hipError_t launch_int8_logits(const Int8Args& a, hipStream_t s) {
   return a.out_dtype == DT_BF16 ? launch_product<BF16>(a, s) : a.out_dtype == DT_F16 ? launch_product<F16>(a, s) : launch_product<float>(a, s);
