@@ -61,8 +61,9 @@ template <int CHUNKS> struct StageRegs {
 // SGPRs) points at the current K tile, each thread contributes one 32-bit byte
 // offset, and the stride between a thread's 8 chunks is a scalar offset, so a
 // load costs one instruction and no vector address arithmetic.
-// KMASK = false compiles the K mask out, for launches whose K tiles cover the K extent exactly.
-template <class T, class SrcT, bool KC, bool KMASK, int CHUNKS = 8> struct Stager3 {
+// KMASK = false compiles the K mask out, for launches whose K tiles cover the K extent exactly.  AUX: cache policy of the loads (2:
+// streaming).
+template <class T, class SrcT, bool KC, bool KMASK, int CHUNKS = 8, int AUX = 0> struct Stager3 {
   static_assert(sizeof(SrcT) == 2, "operands are staged as 16-bit data");
   static constexpr int kEs = (int)sizeof(SrcT);
   typedef StageRegs<CHUNKS> Regs;
@@ -144,7 +145,7 @@ template <class T, class SrcT, bool KC, bool KMASK, int CHUNKS = 8> struct Stage
         __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)range, 0x00020000);
 #pragma unroll
     for (int i = i0; i < i1; ++i)
-      r.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)voff_cur, (int)(i * iter_stride), 0);
+      r.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)voff_cur, (int)(i * iter_stride), AUX);
   }
   LCE_DEV void store(const Regs& r, char* tile, int i0, int i1) const {
     constexpr int step = KC ? 32 * 128 : kRowsAtOnce * kRowPieces * 16;
@@ -225,8 +226,8 @@ template <class T> LCE_DEV int logit_ktiles(int64_t H) {
 //        that the pipeline does not touch until the next barrier it issues
 //        itself -- the epilogue must end with all its LDS traffic complete
 //        (a __syncthreads() if it used scratch).
-template <class T, class PSrc, bool P_KC, class QSrc, bool Q_KC, class Problem> struct Pipe3 {
-  typedef Stager3<T, PSrc, P_KC, Problem::kKMask> PStager;
+template <class T, class PSrc, bool P_KC, class QSrc, bool Q_KC, class Problem, int P_AUX = 0> struct Pipe3 {
+  typedef Stager3<T, PSrc, P_KC, Problem::kKMask, 8, P_AUX> PStager;
   typedef Stager3<T, QSrc, Q_KC, Problem::kKMask> QStager;
   typedef typename PStager::Regs PRegs;
   typedef typename QStager::Regs QRegs;

@@ -96,13 +96,13 @@ template <class T, bool KC, int CHUNKS> struct StagerF32 {
 // epilogues do not need a slice of the vocabulary in one wave and whose fragment reads are then four for four products.
 // Q_BLOCKED, SWAP: Problem::kQBlocked and kSwapAB of Pipe3.
 template <class T, bool P_KC, bool Q_KC = true, bool Q_BLOCKED = false, int NP = 4, int NQ = 1, bool SWAP = false,
-          bool P_F32 = false> struct SmallPipe {
+          bool P_F32 = false, int P_AUX = 0> struct SmallPipe {
   static_assert(NP * NQ == kNB, "four accumulator blocks to a wave");
   typedef typename elem_of<T>::type E;
   static constexpr bool kSplit = is_pair<T>::value;
   static constexpr bool kQRowBlocks = Q_BLOCKED && !Q_KC;
   static constexpr int kWavesP = kNB / NP;
-  typedef typename std::conditional<P_F32, StagerF32<T, P_KC, 4>, Stager3<T, E, P_KC, true, 4>>::type PStager;
+  typedef typename std::conditional<P_F32, StagerF32<T, P_KC, 4>, Stager3<T, E, P_KC, true, 4, P_AUX>>::type PStager;
   typedef Stager3<T, E, Q_KC, true, 4> QStager;
   PStager ps;
   QStager qs;

@@ -7,9 +7,9 @@
 // instruction: both take 16 bytes of K of each lane, so that an operand of 8-bit numbers is staged, swizzled and read as one of
 // half as many 16-bit numbers, in the same time for twice the K.  Sums are exact in 32 bits (127^2 * 2^17 < 2^31).
 // Bound by the matrix cores' power from some 500 rows on: 2048 rows of 4096 x 32000 in 220 us, 2.4 POP/s, the rate of a large library product of
-// 8-bit numbers here (2.1 to 2.4), and less than twice that of 16-bit ones, whose K tiles take 1.2 us, not 1.9.  256 rows of 4096 x 128256, where
-// weight and matrix cores ask for as much, 166 us: 1.6 POP/s beside 3.6 TB/s.  (A second set of registers for the weight's K tiles, two
-// ahead: 173 us, the loads are not what it waits for; 128 x 128 tiles 186.)
+// 8-bit numbers here (2.1 to 2.4), and less than twice that of 16-bit ones, whose K tiles take 1.2 us, not 1.9 (the clock is at 1.7 of 2.4 GHz
+// then, the matrix cores busy for 66 % of it).  256 rows of 4096 x 128256, where weight and matrix cores ask for as much, 155 us: 1.7 POP/s beside
+// 3.8 TB/s.  (A second set of registers for the weight's K tiles, two ahead, loses 5 %, the loads are not what it waits for; 128 x 128 tiles 186.)
 #include "lce_gemm_small.h"
 #include "lce_internal.h"
 
@@ -521,6 +521,9 @@ LCE_DEV void logits_epilogue(const Int8Args& a, f32x16_t (&acc)[kNB][NQ], int64_
 // (of the last row no more is read than the 4 bytes that hold its last number; whatever lies behind a row's last one meets zeros)
 LCE_DEV const signed char* weight_end(const Int8Args& a) { return a.w + (a.V - 1) * a.ldw + ((a.H + 3) & ~3); }
 
+// The weight streams past the rows of x, which should stay in L2: 256 rows of 4096 x 128256 166 to 155 us, of 2048 x 131072 90 to 84, 2048 of
+// 4096 x 32000 1 %.
+constexpr int kWeightAux = 2;
 template <class T, bool KMASK> struct Int8Problem {
   typedef short E;
   static constexpr bool kKMask = KMASK;
@@ -560,17 +563,17 @@ template <class T, bool KMASK> __global__ __launch_bounds__(kThreads) void int8_
   extern __shared__ __attribute__((aligned(16))) char lds[];
   typedef Int8Problem<T, KMASK> Problem;
   Problem prob(a);
-  Pipe3<I8, short, true, short, true, Problem> pipe(prob);
+  Pipe3<I8, short, true, short, true, Problem, kWeightAux> pipe(prob);
   pipe.run(a.ldw / 2, a.ldx / 2, (int)(padded_k(a.K2) / kBK), lds, (int)blockIdx.x);
 }
 
 // The same on 128 x 128 tiles, one workgroup each, for problems with few tiles.
 static_assert(4 * kWaveLds <= kSmallLds, "the pieces fit where the stages were");
-template <class T> __global__ __launch_bounds__(kThreads, 2) void int8_small_kernel(const Int8Args a, int tiles_p, int tiles_q) {
+template <class T, int AUX> __global__ __launch_bounds__(kThreads, 2) void int8_small_kernel(const Int8Args a, int tiles_p, int tiles_q) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   int tp, tq;
   tile_coords((int)blockIdx.x, (int)gridDim.x, tiles_p, tiles_q, 8, 8, tp, tq);
-  SmallPipe<I8, true> pipe;
+  SmallPipe<I8, true, true, false, 4, 1, false, false, AUX> pipe;
   f32x16_t acc[kNB][1];
   pipe.run(a.w + (int64_t)tp * kSmallTile * a.ldw, weight_end(a), a.ldw / 2, a.x + (int64_t)tq * kSmallTile * a.ldx,
            a.x + (a.N - 1) * a.ldx + 2 * a.K2, a.ldx / 2, a.K2, (int)small_logit_ktiles(a.K2, 1), 0, 0, lds, acc);
@@ -582,17 +585,17 @@ template <class T> __global__ __launch_bounds__(kThreads, 2) void int8_small_ker
 // Few rows: a pass over the weight.  A wave takes 16 rows of it at a time, straight from memory to the registers that
 // v_mfma_i32_16x16x64_i8 reads (lane l: row l % 16, 16 bytes of K at 16 * (l / 16) of every 64), a group of kFlight loads ahead of the one
 // that is multiplied, across the ends of its rows too; the quantised rows of x lie in LDS in the order in which the lanes want them:
-// 16 bytes of K, row after row.  There are 1, 2, 4, 8 or 16 places for rows, or 32, which are two instructions to a load; lanes
-// beyond the places read the same rows again, and nobody stores what comes of it.
+// 16 bytes of K, row after row.  There are 1, 2, 4, 8 or 16 places for rows; lanes beyond the places read the same rows again, and
+// nobody stores what comes of it.
 // One or two short rows (kFusedRows, kFusedNumbers) are quantised by every workgroup for itself while its first loads of the weight are under
 // way: one row of 2048 in 3 us less than a launch takes.  (More rows, which it takes one after another: 8 of 2048 5 us more than the
 // launch, 16 of 256 13.)
-// Bound by the weight's way from memory.  us, with x quantised, against the 128 x 128 tiles: 2048 x 131072 one row 50 / 58, 16 rows 55 / 58;
-// 4096 x 128256 one row 97 / 110, 16 rows 108 / 116, 32 rows 114 / 121 (2048 x 131072 61 / 59: not taken for short rows); 8192 x 32000 55 / 67.
-// Four loads in a group 50, 106 and 64 us for one row, twelve 55, 110 and 59; loads past the caches 53, 107 and 59.
+// Bound by the weight's way from memory.  us, x quantised too, against the 128 x 128 tiles: 2048 x 131072 one row 47 / 52, 4096 x 128256 95 / 105,
+// 8192 x 32000 52 / 63; with x quantised before, 8 rows of 2048 x 131072 53 / 49, 4096 x 128256 104 / 102, 8192 x 32000 57 / 63.
+// Four loads in a group 50, 106 and 64 us for one row, twelve 55, 110 and 59; loads past the caches 53, 107 and 59 (half a line at a time).
 // ---------------------------------------------------------------------------
 constexpr int kStreamThreads = 512, kFlight = 8, kGroupBytes = 64 * kFlight;
-constexpr int kStreamLds = 150 * 1024;
+constexpr int kStreamLds = 150 * 1024, kStreamRows = 16;
 constexpr int64_t kFusedRows = 2, kFusedNumbers = 16384;
 LCE_DEV u32x4_t* place_of(char* lds, int byte, int n, int places) {
   return reinterpret_cast<u32x4_t*>(lds + ((byte >> 4) * places + n) * 16 + (byte & 15));
@@ -627,11 +630,11 @@ template <int DT> LCE_DEV void quantize_into(const Int8Args& a, char* lds, int p
     }
   }
 }
-template <class T, int NB> __global__ __launch_bounds__(kStreamThreads, 4) void int8_stream_kernel(const Int8Args a, int places, int depth) {
+template <class T> __global__ __launch_bounds__(kStreamThreads, 4) void int8_stream_kernel(const Int8Args a, int places, int depth) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ float sh_scale[32];
-  __shared__ unsigned sh_top[32];
-  __shared__ Inverse sh_inverse[32];
+  __shared__ float sh_scale[kStreamRows];
+  __shared__ unsigned sh_top[kStreamRows];
+  __shared__ Inverse sh_inverse[kStreamRows];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int blocks = (int)((a.V + 15) / 16), step = (int)gridDim.x * (kStreamThreads / 64);
   const int groups = depth / kGroupBytes;
@@ -649,7 +652,7 @@ template <class T, int NB> __global__ __launch_bounds__(kStreamThreads, 4) void 
     for (int i = 0; i < kFlight; ++i) w[buf][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)mine + i * 64, 0, 0);
   };
   if (block < blocks) load(0, block, 0);
-  if (t < 32) sh_top[t] = 0;
+  if (t < kStreamRows) sh_top[t] = 0;
   __syncthreads();
   if (a.x_in != nullptr) {
     if (a.x_in_dtype == DT_BF16) quantize_into<DT_BF16>(a, lds, places, depth, sh_top, sh_scale, sh_inverse);
@@ -666,21 +669,18 @@ template <class T, int NB> __global__ __launch_bounds__(kStreamThreads, 4) void 
   __syncthreads();
   const int n = lane & 15, row = n & (places - 1);
   const char* const from = lds + ((lane >> 4) * places + row) * 16;
-  i32x4_t acc[NB];
+  i32x4_t acc;
   const auto multiply = [&](int buf, int g) {
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i)
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const i32x4_t x = *reinterpret_cast<const i32x4_t*>(from + (g * kFlight + i) * (64 * places) + b * 256);
-        acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, w[buf][i]), x, acc[b], 0, 0, 0);
-      }
+    for (int i = 0; i < kFlight; ++i) {
+      const i32x4_t x = *reinterpret_cast<const i32x4_t*>(from + (g * kFlight + i) * (64 * places));
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, w[buf][i]), x, acc, 0, 0, 0);
+    }
   };
   // One block of rows, whose first group is in buffer FIRST; the next one's is in the other buffer afterwards where the groups are odd.
   const auto rows16 = [&](auto first, int next) {
     constexpr int F = decltype(first)::value;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = i32x4_t{0, 0, 0, 0};
+    acc = i32x4_t{0, 0, 0, 0};
     int g = 0;
     for (; g + 1 < groups; g += 2) {
       load(1 - F, block, g + 1);
@@ -695,26 +695,24 @@ template <class T, int NB> __global__ __launch_bounds__(kStreamThreads, 4) void 
     }
     // lane: rows 4 * (lane / 16) ... + 3 of the weight's, row `n` of x
     const int64_t v = (int64_t)block * 16 + (lane >> 4) * 4;
+    if (n < a.N) {
+      const float sx = sh_scale[n];
+      char* to = reinterpret_cast<char*>(a.out) + (n * a.ldo + v) * out_of<T>::kEs;
+      float f[4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (n + 16 * b < a.N) {
-        const float sx = sh_scale[n + 16 * b];
-        char* to = reinterpret_cast<char*>(a.out) + ((n + 16 * b) * a.ldo + v) * out_of<T>::kEs;
-        float f[4];
+      for (int i = 0; i < 4; ++i) f[i] = (float)acc[i] * sx * (v + i < a.V ? a.w_scales[v + i] : 0.f);
+      if constexpr (out_of<T>::kEs == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = (float)acc[b][i] * sx * (v + i < a.V ? a.w_scales[v + i] : 0.f);
-        if constexpr (out_of<T>::kEs == 4) {
+        for (int i = 0; i < 4; ++i)
+          if (v + i < a.V) reinterpret_cast<float*>(to)[i] = f[i];
+      } else if (v + 4 <= a.V && (reinterpret_cast<uintptr_t>(to) & 7) == 0) {
+        *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3])};
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (v + i < a.V) reinterpret_cast<float*>(to)[i] = f[i];
-        } else if (v + 4 <= a.V && (reinterpret_cast<uintptr_t>(to) & 7) == 0) {
-          *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3])};
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (v + i < a.V) reinterpret_cast<unsigned short*>(to)[i] = to_bits<T>(f[i]);
-        }
+        for (int i = 0; i < 4; ++i)
+          if (v + i < a.V) reinterpret_cast<unsigned short*>(to)[i] = to_bits<T>(f[i]);
       }
+    }
   };
   const bool odd = (groups & 1) != 0;
   for (; block < blocks; block += step) {
@@ -723,31 +721,34 @@ template <class T, int NB> __global__ __launch_bounds__(kStreamThreads, 4) void 
   }
 }
 
-// Places for rows of x, 0 where the kernel does not take the problem.
-int stream_places(const Int8Args& a, int* depth) {
+// Whether the kernel takes the problem: one or two rows that it quantises itself, or a few long ones (see above; at 4096 the two are even).
+constexpr int kStreamDepth = 6144;
+bool fuses(const Int8Args& a) { return a.N <= kFusedRows && a.N * a.H <= kFusedNumbers; }
+bool streams(const Int8Args& a, int* places, int* depth) {
   *depth = (int)pad_to(a.H, kGroupBytes);
-  int places = 1;
-  while (places < a.N) places *= 2;
-  if (places == 32 && *depth < 3584) return 0;
-  return places <= 32 && (int64_t)places * *depth <= kStreamLds ? places : 0;
+  *places = 1;
+  while (*places < a.N && *places < 2 * kStreamRows) *places *= 2;
+  return *places <= kStreamRows && (int64_t)*places * *depth <= kStreamLds && (fuses(a) || *depth >= kStreamDepth);
 }
-template <class T, int NB> hipError_t launch_stream(const Int8Args& a, int places, int depth, hipStream_t s) {
+template <class T> hipError_t launch_stream(const Int8Args& a, int places, int depth, hipStream_t s) {
   static LdsOptIn optin;
-  const hipError_t e = optin.ensure(reinterpret_cast<const void*>(int8_stream_kernel<T, NB>), kStreamLds);
+  const hipError_t e = optin.ensure(reinterpret_cast<const void*>(int8_stream_kernel<T>), kStreamLds);
   if (e != hipSuccess) return e;
   const int bytes = places * depth, per = bytes <= kStreamLds / 2 ? 2 : 1;
   const int64_t groups = ((a.V + 15) / 16 + kStreamThreads / 64 - 1) / (kStreamThreads / 64);
   const int64_t most = (int64_t)a.num_cus * per;
-  hipLaunchKernelGGL((int8_stream_kernel<T, NB>), dim3((unsigned)(groups < most ? groups : most)), dim3(kStreamThreads), bytes, s, a, places, depth);
+  hipLaunchKernelGGL(int8_stream_kernel<T>, dim3((unsigned)(groups < most ? groups : most)), dim3(kStreamThreads), bytes, s, a, places, depth);
   return hipGetLastError();
 }
 
 template <class T> hipError_t launch_product(const Int8Args& a, hipStream_t s) {
-  int depth;
-  if (const int places = stream_places(a, &depth)) return places > 16 ? launch_stream<T, 2>(a, places, depth, s) : launch_stream<T, 1>(a, places, depth, s);
+  int places, depth;
+  if (streams(a, &places, &depth)) return launch_stream<T>(a, places, depth, s);
   if (few_logit_tiles(a.N, a.V, small_logit_ktiles(a.K2, 1), a.small_wgs)) {
     const int tiles_p = (int)((a.V + kSmallTile - 1) / kSmallTile), tiles_q = (int)((a.N + kSmallTile - 1) / kSmallTile);
-    hipLaunchKernelGGL(int8_small_kernel<T>, dim3((unsigned)(tiles_p * tiles_q)), dim3(kThreads), kSmallLds, s, a, tiles_p, tiles_q);
+    // (a single row of tiles: nobody reads a tile of the weight again.  37 rows of 4096 x 128256 121 to 112 us; but 192 of 8192 x 32000 85 to 107)
+    hipLaunchKernelGGL((tiles_q == 1 ? int8_small_kernel<T, kWeightAux> : int8_small_kernel<T, 0>), dim3((unsigned)(tiles_p * tiles_q)), dim3(kThreads),
+                       kSmallLds, s, a, tiles_p, tiles_q);
     return hipGetLastError();
   }
   const int64_t tiles = (a.V + kTile - 1) / kTile * ((a.N + kTile - 1) / kTile);
@@ -820,8 +821,8 @@ hipError_t launch_quantize_columns(const void* src, int dtype, int64_t rows, int
                            : quantize_columns<DT_F32>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
 }
 bool int8_quantizes(const Int8Args& a) {
-  int depth;
-  return a.N <= kFusedRows && a.N * a.H <= kFusedNumbers && stream_places(a, &depth) > 0;
+  int places, depth;
+  return fuses(a) && streams(a, &places, &depth);
 }
 hipError_t launch_int8_logits(const Int8Args& a, hipStream_t s) {
   return a.out_dtype == DT_BF16 ? launch_product<BF16>(a, s) : a.out_dtype == DT_F16 ? launch_product<F16>(a, s) : launch_product<float>(a, s);
