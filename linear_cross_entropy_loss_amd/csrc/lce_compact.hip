@@ -207,7 +207,11 @@ __global__ __launch_bounds__(256) void gather_rows_split_kernel(const float* x, 
       if constexpr (is_half_pair<T>::value) {
         const float f = pair[0];  // (kPairX)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= f;
+        for (int i = 0; i < 8; ++i) {
+          // (more than the largest of the rows that count: a row that does not, which must not become an infinity, for 0 times that is NaN)
+          const bool outside = fabsf(v[i]) < INFINITY && fabsf(v[i] * f) > 32768.f;
+          v[i] = outside ? 0.f : v[i] * f;
+        }
       }
       u32x4_t hi, lo;
 #pragma unroll

@@ -8,7 +8,6 @@ counterpart in the reference.)
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -128,6 +127,7 @@ class TokenLogitsImplementation(torch.autograd.Function):
         return logits, lse
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logits, g_lse):
         x, w, labels, logits, lse = ctx.saved_tensors
         layout, ignore, logit_scale, N_chunk_size, pack = ctx.lce_cfg
@@ -206,15 +206,18 @@ def linear_token_logits(x, At, tokens, ignore_index: int = -100, logit_scale: fl
         At: weight (H, V) with the strides that ``linear_cross_entropy`` takes: of x's dtype, or float32 under 16-bit x.
         tokens: (...) torch.long.
         ignore_index: a token that marks a row as not wanted (prompts, padding): it is not computed, both results are 0 and
-            it has no gradient, whatever the upstream gradient is there.
+            it has no gradient, whatever the upstream gradient is there.  (What x holds there is to be finite: where few rows
+            are marked they stay in the products, times zero.)
         N_chunk_size: as of ``LinearCrossEntropyLoss``.
         vocab_start, vocab_size: where ``At`` is one piece of a vocabulary, the token that its first column stands for and the number
             of all tokens.  A token of another piece has a logit of 0 here, so that the sum of the pieces' logits and the
             ``logsumexp`` of their lse are those of the whole.
 
     A token that is none (negative or beyond the vocabulary, and not ``ignore_index``) has a NaN logit.  Arithmetic as of
-    ``linear_cross_entropy``: 16-bit gradients come from a dz that was rounded to the type, float32 tensors are multiplied as pairs of
-    bfloat16; float16's dz is held to a 2^-28 of the largest row's upstream gradient.
+    ``linear_cross_entropy``: 16-bit gradients come from a dz that was rounded to the type, float32 tensors are multiplied as
+    pairs of float16 under one power of two for each of x, weight and dz, and hold 22 bits (``linear_cross_entropy``: pairs of
+    bfloat16, 16 bits) or 2^-39 of the largest element there; float16's dz is held to 2^-38 of the largest row's upstream gradient.
+    The gradients are not differentiable in their turn.
     """
     _check_inputs(x, At, tokens)
     V, ignore_index, logit_scale = At.shape[1], int(ignore_index), float(logit_scale)
