@@ -14,8 +14,8 @@ def _dense(t):
 
 
 def _check(grads, out, max_norm, divisor):
-    if not max_norm > 0:
-        raise ValueError(f"clip_gradients: max_norm must be positive, got {max_norm}")
+    if not max_norm > _lib.F32_ZERO:
+        raise ValueError(f"clip_gradients: max_norm must be positive in float32, got {max_norm}")
     if len(out) != len(grads):
         raise ValueError(f"clip_gradients: {len(grads)} gradients and {len(out)} outputs")
     for g, o in zip(grads, out):
@@ -70,7 +70,7 @@ def clip_gradients(grads, max_norm, divisor=1.0, out=None):
     max_norm = float(max_norm)
     divisor = divisor if isinstance(divisor, torch.Tensor) else float(divisor)
     by_ptr = isinstance(divisor, torch.Tensor)
-    if grads and max_norm > 0 and isinstance(grads[0], torch.Tensor) and grads[0].is_cuda and (
+    if grads and max_norm > _lib.F32_ZERO and isinstance(grads[0], torch.Tensor) and grads[0].is_cuda and (
             grads[0].device.index == torch._C._cuda_getDevice()) and (by_ptr or _lib.F32_ZERO < divisor < _lib.F32_INF):
         done = _lib.host().clip(grads, out, max_norm, 1.0 if by_ptr else divisor, divisor if by_ptr else None, _stream(grads[0].device))
         if isinstance(done, torch.Tensor):

@@ -119,7 +119,8 @@ def _op_quantized_logits(x: torch.Tensor, values: torch.Tensor, scales: torch.Te
     if rows.stride(1) != 1 and H > 1:
         rows = rows.contiguous()
     with _on_device(dev):
-        if (values.stride(1) != 1 and H > 1) or values.stride(0) % 16 != 0 or values.data_ptr() % 16 != 0:
+        if (values.stride(1) != 1 and H > 1) or values.stride(0) % 16 != 0 or values.data_ptr() % 16 != 0 or not (
+                H <= values.stride(0) <= 2 * _lib.INT8_DEPTH):
             ops._warn_copy_once("8-bit weight", values, "rows must be contiguous and start on 16-byte boundaries")
             copy, _ = _empty(V, H, dev)
             values = copy.copy_(values)

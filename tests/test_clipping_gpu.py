@@ -160,3 +160,19 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     assert torch.equal(torch.stack(got), torch.stack(norms))
     assert all(torch.equal(a, b) for s, w in zip(sets, want) for a, b in zip(s, w))
+
+
+def test_offsets_past_32_bits():
+    from linear_cross_entropy_loss_amd import clip_gradients
+
+    n = (1 << 31) + 12345
+    g = torch.full((n,), 2.0 ** -8, dtype=BF16, device="cuda")
+    g[-1] = 3.0
+    print(f"clip {n}", flush=True)
+    norm = math.sqrt((n - 1) * 2.0 ** -16 + 9.0)
+    got = clip_gradients(g, 0.5)
+    assert abs(float(got) - norm) <= 2.0 ** -23 * norm
+    for at, was in ((0, 2.0 ** -8), (n - 2, 2.0 ** -8), (n - 1, 3.0)):
+        want = was * 0.5 / norm
+        assert abs(float(g[at]) - want) <= (2.0 ** -23 + 2.0 ** -8) * want
+    assert torch.equal(g[:-1].min(), g[:-1].max())

@@ -170,7 +170,7 @@ def test_clip_gradients_arguments():
     from linear_cross_entropy_loss_amd import clip_gradients
 
     x = torch.zeros(3)
-    for bad in (dict(max_norm=0.0), dict(max_norm=-1.0), dict(max_norm=math.nan), dict(max_norm=1.0, out=[])):
+    for bad in (dict(max_norm=0.0), dict(max_norm=1e-50), dict(max_norm=-1.0), dict(max_norm=math.nan), dict(max_norm=1.0, out=[])):
         with pytest.raises(ValueError):
             clip_gradients([x], **bad)
     with pytest.raises(ValueError, match="no gradients"):

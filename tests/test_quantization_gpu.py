@@ -219,3 +219,51 @@ def test_compiled_and_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, quantized_logits(x, quantize_weight(At)))
+
+
+def test_offsets_past_32_bits():
+    """A result of more than 2^31 numbers, and a weight of more than 2^31 bytes: the rows at either end are those that are computed alone."""
+    from linear_cross_entropy_loss_amd import quantize_weight, quantized_logits
+    from linear_cross_entropy_loss_amd.quantization import Quantized
+
+    x = torch.randn(17000, 64, device="cuda").to(BF16)
+    w = quantize_weight(torch.randn(64, 131000, device="cuda").to(BF16))
+    print("quantized_logits 17000 x 131000", flush=True)
+    z = quantized_logits(x, w)
+    for rows in (slice(0, 3), slice(16300, 16500), slice(16999, 17000)):
+        assert torch.equal(z[rows], quantized_logits(x[rows], w))
+    del z
+    H, V = 16400, 131500  # (V, H) int8: 2.16e9 bytes
+    for N in (1, 5, 40, 300):
+        print(f"quantized_logits {N} x {H} x {V}", flush=True)
+        values = torch.randint(-127, 128, (V, H), dtype=torch.int8, device="cuda")
+        scales = torch.rand(V, device="cuda")
+        x = torch.randn(N, H, device="cuda").to(BF16)
+        z = quantized_logits(x, Quantized(values, scales), dtype=F32)
+        for cols in (slice(0, 100), slice(V - 600, V)):
+            assert torch.equal(z[:, cols], quantized_logits(x, Quantized(values[cols], scales[cols]), dtype=F32))
+
+
+def test_many_columns_and_rows_past_32_bits():
+    from linear_cross_entropy_loss_amd import quantize_rows, quantize_weight
+
+    At = torch.empty(16400, 131500, dtype=BF16, device="cuda").normal_()
+    print("quantize_weight 16400 x 131500", flush=True)
+    got = quantize_weight(At)
+    for cols in (slice(0, 50), slice(131000, 131500)):
+        check_numbers(quantize_rows(At[:, cols].t()), At[:, cols].t())
+        assert torch.equal(got.values[cols], quantize_rows(At[:, cols].t()).values)
+    At = At[:, :131072]
+    check_numbers(quantize_rows(At[-3:]), At[-3:])
+    assert torch.equal(quantize_rows(At).values[-3:], quantize_rows(At[-3:]).values)
+
+
+def test_values_that_share_rows_are_copied():
+    from linear_cross_entropy_loss_amd import quantized_logits
+    from linear_cross_entropy_loss_amd.quantization import Quantized
+
+    x = torch.randn(5, 96, device="cuda").to(BF16)
+    row = torch.randint(-127, 128, (1, 96), dtype=torch.int8, device="cuda")
+    scales = torch.rand(70, device="cuda")
+    got = quantized_logits(x, Quantized(row.expand(70, 96), scales))
+    assert torch.equal(got, quantized_logits(x, Quantized(row.repeat(70, 1), scales)))
