@@ -45,6 +45,8 @@ struct Abi {
   decltype(&lce_token_logits_workspace_bytes) token_logits_workspace_bytes;
   decltype(&lce_token_logits) token_logits;
   decltype(&lce_token_logits_backward) token_logits_backward;
+  decltype(&lce_quantize_rows) quantize_rows;
+  decltype(&lce_quantize_columns) quantize_columns;
   decltype(&lce_int8_logits_workspace_bytes) int8_logits_workspace_bytes;
   decltype(&lce_int8_logits) int8_logits;
   decltype(&lce_clip_workspace_bytes) clip_workspace_bytes;
@@ -73,6 +75,8 @@ void bind(const py::dict& d) {
   bind_one(d, "lce_token_logits_workspace_bytes", abi.token_logits_workspace_bytes);
   bind_one(d, "lce_token_logits", abi.token_logits);
   bind_one(d, "lce_token_logits_backward", abi.token_logits_backward);
+  bind_one(d, "lce_quantize_rows", abi.quantize_rows);
+  bind_one(d, "lce_quantize_columns", abi.quantize_columns);
   bind_one(d, "lce_int8_logits_workspace_bytes", abi.int8_logits_workspace_bytes);
   bind_one(d, "lce_int8_logits", abi.int8_logits);
   bind_one(d, "lce_clip_workspace_bytes", abi.clip_workspace_bytes);
@@ -506,6 +510,39 @@ py::object token_logits_backward(const at::Tensor& x, const at::Tensor& w, int l
   return py::make_tuple(tensor_or_none(dx), tensor_or_none(dw));
 }
 
+// What quantize_rows and, of the columns of a matrix, quantize_weight (quantization.py) return, the values with rows of `ldq` bytes; (status,
+// name, None) where the C ABI refused; None: not handled.
+py::object quantize(const at::Tensor& t, bool columns, int64_t ldq, uintptr_t stream) {
+  Rows r;
+  if (!describe_rows(t, r) || r.rows < 1 || (columns && t.dim() != 2)) return py::none();
+  const int64_t depth = columns ? r.rows : r.cols, others = columns ? r.cols : r.rows;
+  at::NoGradGuard no_grad;
+  const auto o = t.options().requires_grad(false);
+  auto shape = t.sizes().vec();
+  if (columns) std::swap(shape[0], shape[1]);
+  std::vector<int64_t> strides(shape.size());
+  strides.back() = 1;
+  int64_t n = ldq;
+  for (int i = (int)shape.size() - 2; i >= 0; --i) {
+    strides[i] = n;
+    n *= shape[i];
+  }
+  // (whole rows of memory, of which the values are the first `depth` of each)
+  const at::Tensor values = at::empty({others, ldq}, o.dtype(at::kChar)).as_strided(shape, strides);
+  shape.pop_back();
+  const at::Tensor scales = at::empty(shape, o.dtype(at::kFloat));
+  int rc;
+  {
+    py::gil_scoped_release release;
+    rc = columns ? abi.quantize_columns(t.data_ptr(), r.dtype, depth, others, r.ld, (int8_t*)values.data_ptr(), ldq, (float*)scales.data_ptr(),
+                                        reinterpret_cast<void*>(stream))
+                 : abi.quantize_rows(t.data_ptr(), r.dtype, others, depth, r.ld, (int8_t*)values.data_ptr(), ldq, (float*)scales.data_ptr(),
+                                     reinterpret_cast<void*>(stream));
+  }
+  if (rc != LCE_OK) return py::make_tuple(rc, columns ? "quantize_weight" : "quantize_rows", py::none());
+  return py::make_tuple(values, scales);
+}
+
 // quantized_logits (quantization.py); (status, name) where the C ABI refused; None: not handled.
 py::object quantized_logits(const at::Tensor& x, const at::Tensor& values, const at::Tensor& scales, double scale, py::object dtype, uintptr_t stream) {
   Rows r;
@@ -589,6 +626,7 @@ PYBIND11_MODULE(_lce_host, m) {
   m.def("sample_logits", &sample_logits);
   m.def("token_logits", &token_logits);
   m.def("token_logits_backward", &token_logits_backward);
+  m.def("quantize", &quantize);
   m.def("quantized_logits", &quantized_logits);
   m.def("clip", &clip);
 }

@@ -55,6 +55,7 @@ template <> struct Source<DT_F32> {
 template <int DT, bool ONCE = false> LCE_DEV u32x4_t load_piece(const typename Source<DT>::S* row, int c, int cols) {
   constexpr int kPer = Source<DT>::kPer;
   if (c + kPer <= cols) return ONCE ? load_once(row + c) : reinterpret_cast<const Piece*>(row + c)->v;
+  if (c >= cols) return u32x4_t{0, 0, 0, 0};
   typename Source<DT>::S e[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) e[i] = c + i < cols ? row[c + i] : (typename Source<DT>::S)0;
@@ -156,7 +157,9 @@ LCE_DEV unsigned four_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
 }
 
 // Rows.  WAVES waves to a row (one, of four rows to a workgroup, where that holds the row in registers and there are many; else
-// a workgroup); a row of up to 64 * WAVES * PIECES pieces is read once, a longer one twice.  131072 x 2048 bf16 136 us, 5.9 TB/s.
+// a workgroup), or LANES lanes of a wave where it is short; a row of up to LANES * WAVES * PIECES pieces is read once, a longer one twice.
+// 131072 x 2048 bf16 136 us, 5.9 TB/s; 200000 x 256 by 16 lanes 30 us, 5.1 TB/s, by 64 92; 65133 x 672 fp16 29 and 40.  (The piece that a row's end cuts
+// as the row's last 16 bytes, shifted, not element by element: 5 % more.)
 constexpr int kQuantThreads = 256;
 template <int DT> LCE_DEV void store_bytes(u32x4_t piece, const RowScale& s, const Inverse& inverse, signed char* to) {
   constexpr int kPer = Source<DT>::kPer;
@@ -173,16 +176,17 @@ template <int DT> LCE_DEV void store_bytes(u32x4_t piece, const RowScale& s, con
     for (int i = 0; i < kPer; ++i) to[i] = (signed char)exact_byte(element<DT>(piece, i), s);
   }
 }
-template <int DT, int WAVES, int PIECES>
+template <int DT, int WAVES, int PIECES, int LANES = 64>
 __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void* src, int64_t rows, int cols, int64_t ld, signed char* q, int ldq,
                                                                       float* scales) {
   typedef Source<DT> E;
-  constexpr int kStep = 64 * WAVES * E::kPer;
+  static_assert(WAVES == 1 || LANES == 64, "lanes of one wave, or whole waves");
+  constexpr int kStep = LANES * WAVES * E::kPer;
   __shared__ unsigned sh[kQuantThreads / 64];
   const int wave = threadIdx.x >> 6;
-  const int64_t r = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+  const int64_t r = WAVES == 1 ? (int64_t)blockIdx.x * (kQuantThreads / LANES) + threadIdx.x / LANES : (int64_t)blockIdx.x;
   if (r >= rows) return;
-  const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const int t = WAVES == 1 ? threadIdx.x & (LANES - 1) : threadIdx.x;
   const typename E::S* from = reinterpret_cast<const typename E::S*>(src) + r * ld;
   const bool once = cols <= kStep * PIECES;
   u32x4_t v[PIECES], tops = {0, 0, 0, 0};
@@ -196,7 +200,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void
 #pragma unroll
   for (int k = 0; k < E::kPer; ++k) top = larger(top, magnitude<DT>(tops, k));
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = larger(top, (unsigned)__shfl_xor((int)top, d));
+  for (int d = 1; d < LANES; d <<= 1) top = larger(top, (unsigned)__shfl_xor((int)top, d));
   if constexpr (WAVES > 1) {
     if ((threadIdx.x & 63) == 0) sh[wave] = top;
     __syncthreads();
@@ -770,12 +774,14 @@ template <class T> hipError_t launch_product(const Int8Args& a, hipStream_t s) {
 template <int DT>
 hipError_t quantize_rows(const void* src, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales, hipStream_t s) {
   constexpr int kPer = Source<DT>::kPer;
-  const dim3 fours((unsigned)((rows + 3) / 4)), ones((unsigned)rows), threads(kQuantThreads);
+  const dim3 sixteens((unsigned)((rows + 15) / 16)), fours((unsigned)((rows + 3) / 4)), ones((unsigned)rows), threads(kQuantThreads);
   const auto go = [&](auto kernel, dim3 grid) { hipLaunchKernelGGL(kernel, grid, threads, 0, s, src, rows, (int)cols, ld, q, (int)ldq, scales); };
   if (rows < 1024 || cols > 64 * kPer * 8) go(quantize_rows_kernel<DT, 4, 32 / kPer>, ones);
   else if (cols > 64 * kPer * 4) go(quantize_rows_kernel<DT, 1, 8>, fours);
   else if (cols > 64 * kPer * 2) go(quantize_rows_kernel<DT, 1, 4>, fours);
-  else go(quantize_rows_kernel<DT, 1, 2>, fours);
+  else if (cols > 16 * kPer * 4) go(quantize_rows_kernel<DT, 1, 8, 16>, sixteens);
+  else if (cols > 16 * kPer * 2) go(quantize_rows_kernel<DT, 1, 4, 16>, sixteens);
+  else go(quantize_rows_kernel<DT, 1, 2, 16>, sixteens);
   return hipGetLastError();
 }
 template <int DT, int NT, int COLS>

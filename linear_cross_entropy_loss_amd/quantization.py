@@ -88,6 +88,17 @@ def _(At):
     return At.new_empty_strided((V, H), _strides((V, H)), dtype=torch.int8), At.new_empty((V,), dtype=torch.float32)
 
 
+def _quantize(t, columns):
+    depth = t.shape[0] if columns else t.shape[-1]
+    if not torch.compiler.is_compiling() and t.device.index == torch._C._cuda_getDevice():
+        done = _lib.host().quantize(t, columns, _row_bytes(depth), _stream(t.device))
+        if done is not None and len(done) == 3:
+            _lib.raise_for_status(*done[:2])
+        if done is not None:
+            return Quantized(*done)
+    return Quantized(*(_op_quantize_columns if columns else _op_quantize_rows)(t.detach()))
+
+
 def quantize_rows(t) -> Quantized:
     """Each row of ``t`` (..., H) in 8 bits: ``scales = max |t| / 127`` over the row, ``values`` the whole numbers nearest to
     ``127 * t / max |t|``, of two the even one.
@@ -96,7 +107,7 @@ def quantize_rows(t) -> Quantized:
     a scale of NaN.
     """
     _check(t, "quantize_rows", t.shape[-1] if t.dim() else 0)
-    return Quantized(*_op_quantize_rows(t.detach()))
+    return _quantize(t, False)
 
 
 def quantize_weight(At) -> Quantized:
@@ -106,10 +117,9 @@ def quantize_weight(At) -> Quantized:
     if At.dim() != 2 or At.shape[1] < 1:
         raise ValueError(f"quantize_weight: weight must be 2-D with shape (in_features, out_features), got {tuple(At.shape)}")
     _check(At, "quantize_weight", At.shape[0])
-    At = At.detach()
     if At.stride(1) == 1 or At.shape[1] == 1:
-        return Quantized(*_op_quantize_columns(At))
-    return Quantized(*_op_quantize_rows(At.t()))
+        return _quantize(At, True)
+    return _quantize(At.t(), False)
 
 
 @torch.library.custom_op("lce_amd::quantized_logits", mutates_args=(), device_types="cuda")
