@@ -28,8 +28,11 @@ bool is16(int d) { return d == LCE_BF16 || d == LCE_F16; }
 
 // A flag in the route of the problems that lce_distill plans: a row has several targets, which are put into the staged dz.
 constexpr int kSoftTargets = 1 << 30;
+// Another, in those of lce_token_logits_backward: a row has upstream gradients of its own.
+constexpr int kOwnGradients = 1 << 29;
 bool soft(const lce_problem* p) { return (p->route & kSoftTargets) != 0; }
-int route_of(const lce_problem* p) { return p->route & ~(LCE_ROUTE_EXACT_SUMS | LCE_ROUTE_KEEP_LOGITS | kSoftTargets); }
+bool flagged(const lce_problem* p) { return (p->route & (kSoftTargets | kOwnGradients)) != 0; }
+int route_of(const lce_problem* p) { return p->route & ~(LCE_ROUTE_EXACT_SUMS | LCE_ROUTE_KEEP_LOGITS | kSoftTargets | kOwnGradients); }
 
 // The last plan of a kind that this thread made.  A call asks for its plan up to three times (whether the route covers the
 // problem, the workspace, the launches), and a training step for the same one as the step before; a plan follows from the
@@ -56,7 +59,7 @@ template <class Plan> struct LastPlan {
 constexpr int64_t kTileLimit = ((int64_t)1 << 31) / 256;  // bytes of a row
 
 int check(const lce_problem* p, bool backward) {
-  if (!p || soft(p)) return LCE_EINVAL_ARG;  // (the flag is set after the check)
+  if (!p || flagged(p)) return LCE_EINVAL_ARG;  // (the flags are set after the check)
   if (p->N <= 0 || p->H <= 0 || p->V <= 0 || p->n_chunk <= 0) return LCE_EINVAL_SHAPE;
   // Any N, H, V; only the row strides are constrained (below).
   if (p->N > (int64_t)1 << 30 || p->V > (int64_t)1 << 30 || p->H > (int64_t)1 << 20) return LCE_EINVAL_SHAPE;
@@ -527,7 +530,7 @@ struct FusedPlan {
 // 2.56, 1280 3.12 / 3.17, 1536 3.53 / 3.53, 2048 4.41 / 4.32; N=16384, V=131072 stored (V, H), H=768 9.46 / 10.13, 1024
 // 11.85 / 12.30, 1536 17.57 / 17.58; fp16, N=8192, V=50304, H=768 2.15 / 2.28, 1024 2.65 / 2.73, 1536 3.78 / 3.74.
 // (Several targets a row: each would have its slice of the stage rewritten, so they are put in after the pass.)
-bool factors_in_gradients(const lce_problem* p) { return lce::padded_hidden(p->H) <= 1024 && !soft(p); }
+bool factors_in_gradients(const lce_problem* p) { return lce::padded_hidden(p->H) <= 1024 && !flagged(p); }
 
 bool plan_fused_with(const lce_problem* p, bool lo8, bool settled, int64_t most_chunks, FusedPlan* f);
 constexpr int64_t kMostChunks = 1024;  // (lce_compact.hip counts the rows of so many)
@@ -1222,6 +1225,9 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
   if (rows != nullptr) {
     // gradients of each row in the place of one upstream gradient
     rows->perm = pack ? (const int*)(base + k.perm) : nullptr;
+    // (normalised rows: |dz| <= 2, times 2^14 within fp16's range; probabilities stay normal down to 2^-28)
+    a.dz_shift = rows->dz_shift = rows->normalise ? 14 : 0;
+    if (!b.narrow) rows->row_value = nullptr;
     const hipError_t e = lce::launch_row_gradients(*rows, s);
     if (e != hipSuccess) return hip_fail(e, "row_gradients");
     a.row_signs = 1;
@@ -1230,8 +1236,7 @@ int backward_impl(const lce_problem* p, const BwdPlan& b, const void* x, const v
     a.ignore_index = -1;
     a.grad_out = rows->factor;
     a.n_valid = rows->one;
-    // (normalised rows: |dz| <= 2, times 2^14 within fp16's range; probabilities stay normal down to 2^-28)
-    a.dz_shift = rows->normalise ? 14 : 0;
+    a.row_value = rows->row_value;
   }
   if (x32) {  // fp32 activations reach the tile kernels as copies in bf16 pairs, whether or not rows were dropped
     a.x = a.xc;
@@ -1719,7 +1724,7 @@ namespace {
 struct TokenPlan {
   BwdPlan b;
   size_t fwd, fwd_pair, fwd_total;         // forward: out5 and n_valid, which nobody reads; scales of fp16 pairs and what they are made of
-  size_t row_lse, row_y, part, pair, bwd_total;  // backward: lce::RowGradients; its factor behind the parts
+  size_t row_lse, row_y, row_value, part, pair, bwd_total;  // backward: lce::RowGradients; its factor behind the parts
 };
 
 int check_tokens(const lce_problem* p, bool backward) {
@@ -1728,10 +1733,10 @@ int check_tokens(const lce_problem* p, bool backward) {
   return p->monitoring || p->z_reg != 0.f || p->phases || !(p->logit_scale < INFINITY) ? LCE_EINVAL_ARG : LCE_OK;
 }
 
-// The problem as the planner of the backward sees it: dz is staged (rows have numbers of their own), as for distillation.
+// The problem as the planner of the backward sees it.
 lce_problem token_problem(const lce_problem* p) {
   lce_problem q = *p;
-  q.route = kSoftTargets;
+  q.route = kOwnGradients;
   return q;
 }
 
@@ -1747,6 +1752,7 @@ int plan_token_backward(const lce_problem* q, TokenPlan* t) {
   size_t o = align_up(t->b.total);
   t->row_lse = o; o += align_up((size_t)q->N * 4);
   t->row_y = o; o += align_up((size_t)q->N * 8);
+  t->row_value = o; o += t->b.narrow ? align_up((size_t)q->N * 4) : 0;
   t->part = o; o += align_up((size_t)lce::kRowGradientParts * 4 + 32);
   t->pair = o; o += splits(q) ? kPairBytes : 0;
   t->bwd_total = o;
@@ -1804,7 +1810,7 @@ int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w
   r.grad_lse = grad_lse; r.grad_logits = grad_logits; r.logits = logits; r.lse = lse; r.y = y;
   r.N = p->N; r.V = p->V; r.ignore_index = p->ignore_index;
   r.normalise = p->x_dtype != LCE_BF16;
-  r.row_lse = (float*)(base + t.row_lse); r.row_y = (int64_t*)(base + t.row_y);
+  r.row_lse = (float*)(base + t.row_lse); r.row_y = (int64_t*)(base + t.row_y); r.row_value = (float*)(base + t.row_value);
   r.part = (float*)(base + t.part); r.factor = r.part + lce::kRowGradientParts;
   r.one = (int64_t*)(r.factor + 4);
   if (splits(p)) {

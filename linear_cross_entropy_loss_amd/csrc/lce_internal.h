@@ -230,8 +230,10 @@ struct BwdArgs {
   int vtail_all;  // the logit kernel for the tile column that straddles the end of the vocabulary takes every column
   // lce_token_logits_backward: rows have upstream gradients of their own.  `lse` then holds lse - log |g_lse|, `y` -1 for no row, V where
   // g_lse is positive and kNegativeRow where it is negative, and the kernels stage g_lse * softmax, the sign through the gain of z_reg;
-  // the label's column is launch_row_targets'.  grad_out and n_valid are a factor and 1 there.
+  // the label's column is launch_row_targets'.  grad_out and n_valid are a factor and 1 there.  launch_bwd_narrow, which stages nothing,
+  // has the label in `y`, and sign and label's dz of a row in row_value (pack_row_value).
   int row_signs;
+  const float* row_value;
   const float* pair;  // DT_HALF_PAIR: launch_pair_scales
 };
 
@@ -540,11 +542,23 @@ struct RowGradients {
   int normalise;
   float* row_lse;
   int64_t* row_y;
+  float* row_value;  // BwdArgs::row_value, or null: `y` and `lse` are for kernels that stage dz
+  int dz_shift;      // BwdArgs::dz_shift
   float* factor;  // [3]: for the staged rows, and with the scales of an fp16 pair for dx and dW where they are apart
   int64_t* one;   // becomes 1
   const float* pair;  // BwdArgs::pair
   float* part;
 };
+// What the kernel without a stage needs of a row besides: the sign of g_lse in the sign's place, and 2^dz_shift * dz at the label, whose
+// own sign takes the lowest bit (dz is rounded to 16 bits afterwards).
+__device__ __forceinline__ float pack_row_value(float d, bool negative) {
+  const unsigned b = __builtin_bit_cast(unsigned, d);
+  return __builtin_bit_cast(float, (b & 0x7ffffffeu) | b >> 31 | (negative ? 0x80000000u : 0u));
+}
+__device__ __forceinline__ float unpack_row_value(float v) {
+  const unsigned b = __builtin_bit_cast(unsigned, v);
+  return __builtin_bit_cast(float, (b & 0x7ffffffeu) | b << 31);
+}
 constexpr int kRowGradientParts = 64;
 constexpr int64_t kNegativeRow = -2;
 hipError_t launch_row_gradients(const RowGradients& g, hipStream_t s);

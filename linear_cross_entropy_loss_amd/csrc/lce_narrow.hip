@@ -238,20 +238,28 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_narrow_kernel(const FwdArgs a
 // dz of a wave's S: 128 streaming rows x 32 stationary rows, in place.  dx: the stationary row is a token, with its scalars in this lane,
 // the streaming ones are columns from v0 on; dW: the other way round, the tokens' scalars in LDS.
 constexpr int kNoColumn = -0x7fffffff;
+// What an exponential is multiplied by: 1, the factor of z-regularisation, the sign of a row's own upstream gradient (BwdArgs::row_value,
+// with dz at the label; 1 + 2 z_reg lse is not used then).  8520 x 64 x 32768 with half of the rows dropped, forward and backward of given
+// tokens: 346 us, 591 where dz is staged; 1335 x 115 x 37248 171 and 156.
+enum RowGain { kNoGain, kRegGain, kOwnGain };
 // (label: kNoColumn where there is no column to look for)
-LCE_DEV void narrow_scalars(const BwdArgs& a, int64_t rows, int64_t tok, float& nlse, float& gain, int& label) {
+template <RowGain GAIN> LCE_DEV void narrow_scalars(const BwdArgs& a, int64_t rows, int64_t tok, float& nlse, float& gain, int& label) {
   const int64_t yy = tok < rows ? a.y[tok] : a.ignore_index;
   const bool valid = yy != a.ignore_index;
   const float l = valid ? a.lse[tok] : 0.f;
   nlse = valid ? fmaf(-l, kLog2e, (float)a.dz_shift) : -INFINITY;
-  gain = 1.f + 2.f * a.z_reg * l;
-  if (a.dz_shift != 0) gain = fminf(fmaxf(gain, -63.f), 63.f);  // (as in lce_bwd_dz.hip)
+  if (GAIN == kOwnGain) {
+    gain = valid ? a.row_value[tok] : 0.f;
+  } else {
+    gain = 1.f + 2.f * a.z_reg * l;
+    if (a.dz_shift != 0) gain = fminf(fmaxf(gain, -63.f), 63.f);  // (as in lce_bwd_dz.hip)
+  }
   label = valid && yy >= 0 && yy < a.V ? (int)yy : kNoColumn;
 }
 
 // The gradient of one 128-row tile of the stationary matrix over streaming tiles [first, last): acc[hb], rows h along registers,
 // stationary rows along lanes.  rows: the tokens that are worked on, all of x's or the packed ones.
-template <class T, bool WVH, bool DW, bool ZREG, int KT>
+template <class T, bool WVH, bool DW, RowGain GAIN, int KT>
 LCE_DEV void narrow_gradient(const BwdArgs& a, int64_t rows, int wave, int tile, int first, int last, char* lds, f32x16_t (&acc)[2 * KT]) {
   typedef typename elem_of<T>::type E;
   constexpr bool TRANS = !DW && !WVH;  // the streaming matrix is W stored (H, V)
@@ -274,7 +282,7 @@ LCE_DEV void narrow_gradient(const BwdArgs& a, int64_t rows, int wave, int tile,
     const int64_t c = (int64_t)tc * kNarrowTile;
     if (DW) {
       next.load(x + c * ldx, x_end, 0);
-      narrow_scalars(a, rows, c + (tid & (kNarrowTile - 1)), nlse, gain, label);
+      narrow_scalars<GAIN>(a, rows, c + (tid & (kNarrowTile - 1)), nlse, gain, label);
     } else {
       next.load(w + (WVH ? c * a.ldw : c), w_end, a.Vw - c);
     }
@@ -319,7 +327,7 @@ LCE_DEV void narrow_gradient(const BwdArgs& a, int64_t rows, int wave, int tile,
     for (int r = 0; r < 16; ++r) acc[hb][r] = 0.f;
   if (first >= last) return;
   fetch(first);
-  if (!DW) narrow_scalars(a, rows, rw + (lane & 31), nlse, gain, label);
+  if (!DW) narrow_scalars<GAIN>(a, rows, rw + (lane & 31), nlse, gain, label);
   put(0);
   __syncthreads();
   for (int tc = first; tc < last; ++tc) {
@@ -358,13 +366,14 @@ LCE_DEV void narrow_gradient(const BwdArgs& a, int64_t rows, int wave, int tile,
             f32x4_t nl, ga;
             if (DW) {
               nl = *reinterpret_cast<const f32x4_t*>(scal + c0);
-              if (ZREG) ga = *reinterpret_cast<const f32x4_t*>(scal + kNarrowTile + c0);
+              if (GAIN != kNoGain) ga = *reinterpret_cast<const f32x4_t*>(scal + kNarrowTile + c0);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float z = s[i][0][(g + h2) * 4 + j];
               float e = __builtin_amdgcn_exp2f(fmaf(z, c1, DW ? nl[j] : nlse));
-              if (ZREG) e *= DW ? ga[j] : gain;
+              if (GAIN == kRegGain) e *= DW ? ga[j] : gain;
+              if (GAIN == kOwnGain) e = copysignf(e, DW ? ga[j] : gain);
               d[4 * h2 + j] = e;
             }
             if (GENERAL) {
@@ -373,11 +382,15 @@ LCE_DEV void narrow_gradient(const BwdArgs& a, int64_t rows, int wave, int tile,
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   const float lj = la[j];
-                  d[4 * h2 + j] = __builtin_bit_cast(int, lj) == my_v ? d[4 * h2 + j] - one : d[4 * h2 + j];
+                  const float at = GAIN == kOwnGain ? unpack_row_value(ga[j]) : d[4 * h2 + j] - one;
+                  d[4 * h2 + j] = __builtin_bit_cast(int, lj) == my_v ? at : d[4 * h2 + j];
                 }
               } else if (!kOneCopy || hit) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d[4 * h2 + j] = rel == c0 + j ? d[4 * h2 + j] - one : d[4 * h2 + j];
+                for (int j = 0; j < 4; ++j) {
+                  const float at = GAIN == kOwnGain ? unpack_row_value(gain) : d[4 * h2 + j] - one;
+                  d[4 * h2 + j] = rel == c0 + j ? at : d[4 * h2 + j];
+                }
               }
             }
             if (GENERAL && !DW && (!kOneCopy || cols < kNarrowTile)) {
@@ -441,7 +454,7 @@ template <class T, bool WVH> LCE_DEV void narrow_out(const BwdArgs& a, int64_t r
   }
 }
 
-template <class T, bool WVH, bool ZREG, int KT>
+template <class T, bool WVH, RowGain GAIN, int KT>
 __global__ __launch_bounds__(kThreads, 2) void grads_narrow_kernel(const BwdArgs a, const SmallGrads g) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const bool in_first = (int)blockIdx.x < g.first_span, dw = in_first == (g.dw_first != 0);
@@ -455,8 +468,8 @@ __global__ __launch_bounds__(kThreads, 2) void grads_narrow_kernel(const BwdArgs
   const int first = (int)((int64_t)stream * seg / nseg), last = (int)((int64_t)stream * (seg + 1) / nseg);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16_t acc[2 * KT];
-  if (dw) narrow_gradient<T, WVH, true, ZREG, KT>(a, rows, wave, tile, first, last, lds, acc);
-  else narrow_gradient<T, WVH, false, ZREG, KT>(a, rows, wave, tile, first, last, lds, acc);
+  if (dw) narrow_gradient<T, WVH, true, GAIN, KT>(a, rows, wave, tile, first, last, lds, acc);
+  else narrow_gradient<T, WVH, false, GAIN, KT>(a, rows, wave, tile, first, last, lds, acc);
   const int lane = narrow_tid(0), r = wave * kBlk + (lane & 31), hq = 4 * (lane >> 5);
   float* part = nseg > 1 ? g.part + ((dw ? (int64_t)g.dx_blocks : 0) + (int64_t)tile * nseg + seg) * (kNarrowTile * kBK * KT) : nullptr;
   const float coef = final_factor_of(a);
@@ -514,19 +527,17 @@ template <class T, bool WVH, int KT> hipError_t launch_grads(const BwdArgs& a, S
   const int64_t grid = g.first_span + (g.dw_first ? dx_items : dw_items);
   if (grid <= 0) return hipSuccess;
   hipError_t e;
-  if (a.z_reg != 0.f) {
+  const auto go = [&](auto gain) {
     static LdsOptIn optin;
-    auto kern = grads_narrow_kernel<T, WVH, true, KT>;
-    e = optin.ensure(reinterpret_cast<const void*>(kern), narrow_lds<KT>());
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(kThreads), narrow_lds<KT>(), s, a, g);
-  } else {
-    static LdsOptIn optin;
-    auto kern = grads_narrow_kernel<T, WVH, false, KT>;
-    e = optin.ensure(reinterpret_cast<const void*>(kern), narrow_lds<KT>());
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(kThreads), narrow_lds<KT>(), s, a, g);
-  }
+    auto kern = grads_narrow_kernel<T, WVH, decltype(gain)::value, KT>;
+    const hipError_t set = optin.ensure(reinterpret_cast<const void*>(kern), narrow_lds<KT>());
+    if (set == hipSuccess) hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(kThreads), narrow_lds<KT>(), s, a, g);
+    return set;
+  };
+  e = a.row_signs        ? go(std::integral_constant<RowGain, kOwnGain>())
+      : a.z_reg != 0.f ? go(std::integral_constant<RowGain, kRegGain>())
+                       : go(std::integral_constant<RowGain, kNoGain>());
+  if (e != hipSuccess) return e;
   e = hipGetLastError();
   const int64_t dx_tails = g.dx_nseg > 1 ? tok : 0, tails = dx_tails + (g.dw_nseg > 1 ? voc : 0);
   if (e != hipSuccess || tails == 0) return e;
@@ -565,7 +576,7 @@ hipError_t launch_fwd_narrow(const FwdArgs& a, int64_t rows, hipStream_t s) {
 }
 
 hipError_t launch_bwd_narrow(const BwdArgs& a, const SmallGrads& g, bool want_dx, bool want_dw, hipStream_t s) {
-  if (a.H > kNarrowHidden || a.w_dtype != a.x_dtype || a.perm_always || a.dxc != nullptr || a.v0 != 0 || a.wv0 != 0 || a.vw != a.V ||
+  if (a.H > kNarrowHidden || a.w_dtype != a.x_dtype || a.perm_always || (a.row_signs && a.row_value == nullptr) || a.dxc != nullptr || a.v0 != 0 || a.wv0 != 0 || a.vw != a.V ||
       ((g.dx_nseg > 1 || g.dw_nseg > 1) && g.part == nullptr))
     return hipErrorInvalidValue;
   if (a.x_dtype == DT_BF16) return a.w_vh ? launch_grads_kt<BF16, true>(a, g, want_dx, want_dw, s) : launch_grads_kt<BF16, false>(a, g, want_dx, want_dw, s);

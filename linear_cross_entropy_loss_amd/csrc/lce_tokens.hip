@@ -6,7 +6,8 @@
 // The kernels of the loss's backward stage +-exp(z - lse'), lse' = lse - log |g_lse|: no product more than with z-regularisation and no
 // register (a number of its own for each row, held over the last K tiles, put 50 to 100 registers of the dz kernels into memory).
 // lse' is rounded at 24 bits, which moves a probability by a factor of 1 +- 2^-19 at |lse'| < 32, as far as the rounding of its
-// exponent does.  The label's column is written over the stage afterwards, from the logit that the forward gave (row_targets_kernel).
+// exponent does.  The label's column is written over the stage afterwards, from the logit that the forward gave (row_targets_kernel); the
+// kernel for few hidden indices, which stages nothing, puts it in as it goes (lce_narrow.hip).
 //
 // fp16, and fp32 as fp16 pairs: a stage has 30 binary places below 1 while upstream gradients are of any size (1 / rows, times a loss
 // scale), so all are divided by one power of two, which the dx and dW kernels multiply in again after their fp32 sums.
@@ -45,6 +46,11 @@ __global__ __launch_bounds__(kRowThreads) void row_gradient_max_kernel(const Row
   if (threadIdx.x == 0) g.part[blockIdx.x] = m;
 }
 
+// 2^shift * dz at a label.
+__device__ float target(float g_lse, float g_logit, float logit, float lse, int shift) {
+  return ldexpf(fmaf(g_lse, __expf(logit - lse), g_logit), shift);
+}
+
 __global__ __launch_bounds__(kRowThreads) void row_gradients_kernel(const RowGradients g, int parts) {
   int e = 0;  // the factor is 2^e
   if (parts > 0) {
@@ -67,7 +73,13 @@ __global__ __launch_bounds__(kRowThreads) void row_gradients_kernel(const RowGra
     // (no gradient: exp(z - lse') is 0 whatever the logits.  Finite all the same: the kernels multiply it by a z_reg of 0.)
     const float l = g.lse[n] - logf(fabsf(gl));
     g.row_lse[j] = l > 1e30f ? 1e30f : l < -1e30f ? -1e30f : l;
-    g.row_y[j] = g.y[n] == g.ignore_index ? -1 : gl < 0.f ? kNegativeRow : g.V;
+    const int64_t yy = g.y[n];
+    if (g.row_value == nullptr) {
+      g.row_y[j] = yy == g.ignore_index ? -1 : gl < 0.f ? kNegativeRow : g.V;
+    } else {
+      g.row_y[j] = yy == g.ignore_index ? -1 : yy >= 0 && yy < g.V ? yy : g.V;
+      g.row_value[j] = pack_row_value(target(gl, ldexpf(g.grad_logits[n], -e), g.logits[n], g.lse[n], g.dz_shift), gl < 0.f);
+    }
   }
 }
 
@@ -80,8 +92,7 @@ __global__ __launch_bounds__(kRowThreads) void row_targets_kernel(const BwdArgs 
     const int64_t yy = g.y[n], rel = yy - a.v0;
     if (yy == g.ignore_index || yy < 0 || yy >= a.V || rel < 0 || rel >= a.vw) continue;
     const float f = *g.factor;  // (quotients by a power of two are exact)
-    const float p = __expf(g.logits[n] - g.lse[n]);
-    const float d = ldexpf(fmaf(g.grad_lse[n] / f, p, g.grad_logits[n] / f), a.dz_shift);
+    const float d = target(g.grad_lse[n] / f, g.grad_logits[n] / f, g.logits[n], g.lse[n], a.dz_shift);
     const int64_t at = (j & (kTile - 1)) * 64 + (rel & 63);
     unsigned short* dz = reinterpret_cast<unsigned short*>(a.dz);
     if constexpr (is_pair<T>::value) {

@@ -349,3 +349,14 @@ def test_second_derivatives_are_refused():
     (dx,) = torch.autograd.grad((logits - lse).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.float().sum().backward()
+
+
+@pytest.mark.pack_auto
+@pytest.mark.parametrize("dtype, w_dtype", [(BF16, None), (F16, None), (BF16, F32)], ids=str)
+@pytest.mark.parametrize("N, H, V, drop", [(3000, 128, 17000, 0.5), (1300, 64, 9001, 0.0), (5000, 40, 777, 0.1)])
+def test_few_hidden_indices(N, H, V, drop, dtype, w_dtype):
+    """Without a stage of dz, and where many rows are dropped on packed ones."""
+    check(make(N, H, V, dtype, seed=N, drop=drop, w_dtype=w_dtype))
+    check(make(N, H, V, dtype, seed=N, drop=drop, w_dtype=w_dtype), tied=True, scale=0.5)
+    if w_dtype is None:
+        check(make(N, H, V, dtype, seed=N, drop=drop, pieces=2), first=V, size=2 * V)
