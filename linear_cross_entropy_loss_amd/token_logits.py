@@ -219,12 +219,21 @@ def linear_token_logits(x, At, tokens, ignore_index: int = -100, logit_scale: fl
     bfloat16, 16 bits) or 2^-39 of the largest element there; float16's dz is held to 2^-38 of the largest row's upstream gradient.
     The gradients are not differentiable in their turn.
     """
-    _check_inputs(x, At, tokens)
-    V, ignore_index, logit_scale = At.shape[1], int(ignore_index), float(logit_scale)
+    compiling = torch.compiler.is_compiling()
+    if At.dim() != 2:
+        _check_inputs(x, At, tokens)
+    V, ignore_index, logit_scale = At.shape[-1], int(ignore_index), float(logit_scale)
     vocab_start = int(vocab_start)
     vocab_size = vocab_start + V if vocab_size is None else int(vocab_size)
+    if not compiling and x.is_cuda and x.device.index == torch._C._cuda_getDevice() and not torch.is_autocast_enabled("cuda") and (
+            _lib.F32_ZERO < logit_scale < _lib.F32_INF) and 0 <= vocab_start <= vocab_size - V:
+        done = _lib.host().differentiable_token_logits(x, At, tokens, ignore_index, logit_scale, int(N_chunk_size), vocab_start, vocab_size,
+                                                       ops._pack_mode(), "weight" in ops._copy_warned, _stream(x.device))
+        if done is not None:
+            return done
+    _check_inputs(x, At, tokens)
     _check_numbers(V, vocab_start, vocab_size, logit_scale)
-    if not torch.compiler.is_compiling():
+    if not compiling:
         return TokenLogitsImplementation.apply(x, At, tokens, ignore_index, logit_scale, int(N_chunk_size), vocab_start, vocab_size)
     return _op_token_logits(ops._autocast_x(x, At), At, tokens, ignore_index, logit_scale, int(N_chunk_size), vocab_start, vocab_size,
                             ops._pack_mode())
