@@ -17,7 +17,7 @@
 //
 // fp32 tensors: fp16 pairs (lce_gemm.h) instead of the loss's bf16 ones, for products 22 bits wide.  N=2048, H=1024, V=16384, errors of dx and
 // dW against fp64, relative to their norms: 3.4e-7, of bf16 pairs 4.4e-6 (a float32 library product and its softmax: 2.2e-6).  Their scales
-// cost one more pass over the weight and x in each direction (pair_max_kernel, 21 of some 470 us).
+// cost one more pass over the weight and x in each direction (pair_max_kernel, 17 of some 460 us).
 #include "lce_gemm3.h"
 #include "lce_internal.h"
 
@@ -114,36 +114,49 @@ __global__ __launch_bounds__(kRowThreads) void token_labels_kernel(const int64_t
 }
 
 // part[b] = the largest finite magnitude of this workgroup's pieces: of kept rows of x (the first x_groups workgroups) or of the weight.
-constexpr int64_t kScalePiece = 4096;  // numbers of a row that a workgroup looks at at a time
+constexpr int64_t kScalePiece = 4 * kRowThreads;  // numbers of a row that a workgroup looks at at a time, four such in flight
 __global__ __launch_bounds__(kRowThreads) void pair_max_kernel(const float* x, int64_t ldx, int64_t N, int64_t H, const int64_t* y, int64_t ignore_index,
                                                                const float* w, int64_t ldw, int64_t V, int x_groups, float* part) {
   const bool of_x = (int)blockIdx.x < x_groups;
   const float* t = of_x ? x : w;
   const int64_t rows = of_x ? N : H, cols = of_x ? H : V, ld = of_x ? ldx : ldw, per = (cols + kScalePiece - 1) / kScalePiece;
-  const int64_t first = of_x ? blockIdx.x : blockIdx.x - x_groups, step = of_x ? x_groups : (int)gridDim.x - x_groups;
+  const int64_t first = 4 * (of_x ? blockIdx.x : blockIdx.x - x_groups), step = 4 * (of_x ? x_groups : (int64_t)gridDim.x - x_groups);
+  const int64_t step_r = step / per, step_c = step - step_r * per;
   float m = 0.f;
-  for (int64_t i = first; i < rows * per; i += step) {
-    const int64_t r = i / per, c0 = (i - r * per) * kScalePiece;
-    if (of_x && y[r] == ignore_index) continue;
-    const float* row = t + r * ld;
+  for (int64_t r = first / per, c = first - r * per; r < rows;) {
+    int64_t rk = r, ck = c;
+    f32x4_t q[4];
 #pragma unroll
-    for (int k = 0; k < kScalePiece / (4 * kRowThreads); ++k) {
-      const int64_t c = c0 + (k * kRowThreads + (int)threadIdx.x) * 4;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (c + 4 <= cols) {
-        const f32x4_t q = *reinterpret_cast<const f32x4_t*>(row + c);
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = ck * kScalePiece + (int)threadIdx.x * 4;
+      q[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (rk < rows && !(of_x && y[rk] == ignore_index)) {
+        const float* from = t + rk * ld + at;
+        if (at + 4 <= cols) {
+          q[k] = *reinterpret_cast<const f32x4_t*>(from);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = q[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < cols) v[j] = row[c + j];
+          for (int j = 0; j < 4; ++j)
+            if (at + j < cols) q[k][j] = from[j];
+        }
       }
+      if (++ck == per) {
+        ck = 0;
+        ++rk;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float a = fabsf(v[j]);
+        const float a = fabsf(q[k][j]);
         m = a < INFINITY && a > m ? a : m;
       }
+    r += step_r;
+    c += step_c;
+    if (c >= per) {
+      c -= per;
+      ++r;
     }
   }
   m = largest_of_workgroup(m);
@@ -200,7 +213,7 @@ hipError_t launch_row_targets(const BwdArgs& a, const RowGradients& g, hipStream
 
 hipError_t launch_pair_scales(const float* x, int64_t ldx, int64_t N, int64_t H, const int64_t* y, int64_t ignore_index, const float* w, int64_t ldw,
                               int64_t V, float* pair, float* part, hipStream_t s) {
-  const int64_t px = N * ((H + kScalePiece - 1) / kScalePiece), pw = H * ((V + kScalePiece - 1) / kScalePiece);
+  const int64_t px = (N * ((H + kScalePiece - 1) / kScalePiece) + 3) / 4, pw = (H * ((V + kScalePiece - 1) / kScalePiece) + 3) / 4;
   const int x_groups = (int)(px < kPairParts / 4 ? px : kPairParts / 4), w_groups = (int)(pw < kPairParts * 3 / 4 ? pw : kPairParts * 3 / 4);
   hipLaunchKernelGGL(pair_max_kernel, dim3(x_groups + w_groups), dim3(kRowThreads), 0, s, x, ldx, N, H, y, ignore_index, w, ldw, V, x_groups, part);
   const hipError_t e = hipGetLastError();
