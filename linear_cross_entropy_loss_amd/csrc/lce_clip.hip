@@ -7,7 +7,7 @@
 // float32), one partial sum to a workgroup; in the second every workgroup adds up all partial sums, in the same order, and scales.
 // The list of tensors travels in the kernels' arguments: nothing is copied to the device, and a captured launch holds its own.
 //
-// Bound by memory beyond some MiB, by the two launches below (13 us for 2.7M float32).  470M bf16 to float32: 660 us for 3.76 GB, 5.7 TB/s (the norm 6.2
+// Bound by memory beyond some MiB, by the two launches below (13 us for 0.16M float32).  470M bf16 to float32: 660 us for 3.76 GB, 5.7 TB/s (the norm 6.2
 // to 6.3 TB/s, what reading alone reaches here; a copy of as much 5.3).
 // ONCE: tensors that together do not fit the 256 MiB Infinity Cache go past it (loads and stores that are not kept): 739 to 660 us.
 // Smaller ones the second launch finds there.
