@@ -572,10 +572,17 @@ struct TokenLogits : public torch::autograd::Function<TokenLogits> {
     const auto saved = ctx->get_saved_variables();
     auto& d = ctx->saved_data;
     const int layout = (int)d["layout"].toInt();
+    // (hooks on saved tensors may bring them back with other strides)
+    const auto rows = [](const at::Tensor& t) {
+      if (t.stride(1) == 1 && t.stride(0) % row_multiple(t.scalar_type()) == 0 && t.stride(0) >= t.size(1) && aligned(t)) return t;
+      at::NoGradGuard no_grad;
+      at::Tensor copy = rows_of(t.size(0), t.size(1), padded_cols(t.size(1), t.scalar_type()), t.options().requires_grad(false));
+      return copy.copy_(t);
+    };
     const at::Tensor g_logits = g[0].contiguous(), g_lse = g[1].contiguous();
     at::Tensor dx, dw;
     int rc = LCE_OK;
-    const bool handled = run_tokens_backward(saved[0], saved[1], layout, saved[2], saved[3], saved[4], g_logits, g_lse,
+    const bool handled = run_tokens_backward(rows(saved[0]), rows(saved[1]), layout, saved[2].contiguous(), saved[3].contiguous(), saved[4].contiguous(), g_logits, g_lse,
                                              d["ignore_index"].toInt(), d["scale"].toDouble(), d["n_chunk"].toInt(), (int)d["pack"].toInt(),
                                              ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                              reinterpret_cast<void*>((uintptr_t)d["stream"].toInt()), dx, dw, rc);

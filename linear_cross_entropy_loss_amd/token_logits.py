@@ -130,6 +130,7 @@ class TokenLogitsImplementation(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_logits, g_lse):
         x, w, labels, logits, lse = ctx.saved_tensors
+        x, w = ops._aligned_rows(x), ops._aligned_rows(w)  # (hooks on saved tensors may bring them back with other strides)
         layout, ignore, logit_scale, N_chunk_size, pack = ctx.lce_cfg
         dx, dw = _backward(x, w, layout, labels, logits, lse, g_logits, g_lse, ignore, logit_scale, N_chunk_size, pack,
                            ctx.needs_input_grad[0], ctx.needs_input_grad[1])

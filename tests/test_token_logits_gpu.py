@@ -360,3 +360,37 @@ def test_few_hidden_indices(N, H, V, drop, dtype, w_dtype):
     check(make(N, H, V, dtype, seed=N, drop=drop, w_dtype=w_dtype), tied=True, scale=0.5)
     if w_dtype is None:
         check(make(N, H, V, dtype, seed=N, drop=drop, pieces=2), first=V, size=2 * V)
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("N, H, V", [(37, 67, 131), (40, 64, 512)])
+def test_saved_tensors_kept_on_the_host(N, H, V, tied):
+    """Rows that were copied to wider ones come back dense."""
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    def run(*args, **kw):
+        with torch.autograd.graph.save_on_cpu():
+            return linear_token_logits(*args, **kw)
+
+    check(make(N, H, V, BF16, seed=11), run=run, tied=tied)
+    with torch.autocast("cuda", dtype=BF16):  # (the Function in Python)
+        check(make(N, H, V, BF16, seed=11), run=run, tied=tied)
+
+
+def test_upstream_gradients_that_are_missing_or_expanded():
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    x, w, tokens, *_ = (t.cuda() for t in make(60, 72, 500, BF16, seed=13))
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    logits, lse = linear_token_logits(x.view(3, 20, 72), w, tokens.view(3, 20), ignore_index=IGNORE)
+    zero, one = torch.zeros_like(lse), torch.ones_like(lse)
+    for got, up in ((logits.sum(), (one, zero)), (lse.sum(), (zero, one)), ((logits - lse).mean(), (one / 60, -one / 60))):
+        a = torch.autograd.grad(got, (x, w), retain_graph=True)
+        b = torch.autograd.grad((logits, lse), (x, w), up, retain_graph=True)
+        assert all(torch.equal(i, j) for i, j in zip(a, b))
+    with pytest.raises(RuntimeError):  # (changed between the passes)
+        x.data_ptr()
+        with torch.no_grad():
+            x.add_(1)
+        torch.autograd.grad(lse.sum(), x)
