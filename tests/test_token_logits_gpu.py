@@ -394,3 +394,62 @@ def test_upstream_gradients_that_are_missing_or_expanded():
         with torch.no_grad():
             x.add_(1)
         torch.autograd.grad(lse.sum(), x)
+
+
+@pytest.mark.pack_auto  # (the recomputation may run in a thread of autograd's, which has the library's own choice)
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_under_a_checkpoint(reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    def run(x, At, tokens, **kw):
+        return checkpoint(lambda a, b: linear_token_logits(a, b, tokens, **kw), x, At, use_reentrant=reentrant)
+
+    inputs = make(50, 72, 600, BF16, seed=17)
+    if not reentrant:
+        check(inputs, run=run)
+        return
+    x, w, tokens, g_logits, g_lse = (t.cuda() for t in inputs)  # (that one gives gradients to leaves only)
+    grads = []
+    for f in (run, linear_token_logits):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w)]
+        torch.autograd.backward(f(*leaves, tokens, ignore_index=IGNORE), (g_logits, g_lse))
+        grads.append([t.grad for t in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.pack_auto  # (a setting of packing is a thread's own)
+def test_calls_from_several_threads_and_streams():
+    """Forward and backward of four threads at once, each on a stream of its own: what each gives alone."""
+    import threading
+
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    sizes = [(64, 256, 4096), (300, 128, 5000), (513, 72, 999), (128, 512, 9000)]
+    cases = [tuple(t.cuda() for t in make(*s, BF16, seed=i)) for i, s in enumerate(sizes)]
+
+    def step(x, w, tokens, g_logits, g_lse):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        out = linear_token_logits(x, w, tokens, ignore_index=IGNORE)
+        return (*out, *torch.autograd.grad(out, (x, w), (g_logits, g_lse)))
+
+    alone = [[t.detach().clone() for t in step(*c)] for c in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = step(*cases[i])
+            stream.synchronize()
+        if not all(torch.equal(a, b) for a, b in zip(got, alone[i])):
+            failed.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
