@@ -507,19 +507,23 @@ int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_
  *           number: logit NaN, no gradient by it.  lce_token_labels makes them.
  *   logits, lse   N floats each: out; the backward takes them as the forward gave them
  *   grad_logits, grad_lse   N floats each
+ *   scales  NULL, or room for LCE_PAIR_SCALES floats in the forward, which the backward of the same x, w and y takes: under fp32 tensors it
+ *           then need not look for the largest numbers again (others: not touched)
  *   dx, dw  out, at least one of them
  *
  * lce_token_labels: labels[i] = tokens[i] - vocab_start where that is one of V columns, -1 where tokens[i] is ignore_index, V where
  * it is another token of a vocabulary of vocab_size, V + 1 where it is none (for the two calls: ignore_index -1, other V).
  * 0 <= vocab_start <= vocab_size - V, 0 <= N <= 2^30.
  */
+#define LCE_PAIR_SCALES 8
 int lce_token_labels(const int64_t* tokens, int64_t N, int64_t ignore_index, int64_t vocab_start, int64_t V, int64_t vocab_size,
                      int64_t* labels, void* stream);
 int lce_token_logits_workspace_bytes(const lce_problem* p, size_t* fwd_bytes, size_t* bwd_bytes);
-int lce_token_logits(const lce_problem* p, const void* x, const void* w, const int64_t* y, int64_t other, float* logits, float* lse, void* ws,
-                     size_t ws_bytes, void* stream);
+int lce_token_logits(const lce_problem* p, const void* x, const void* w, const int64_t* y, int64_t other, float* logits, float* lse,
+                     float* scales, void* ws, size_t ws_bytes, void* stream);
 int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w, const int64_t* y, const float* logits, const float* lse,
-                              const float* grad_logits, const float* grad_lse, void* dx, void* dw, void* ws, size_t ws_bytes, void* stream);
+                              const float* grad_logits, const float* grad_lse, const float* scales, void* dx, void* dw, void* ws, size_t ws_bytes,
+                              void* stream);
 
 /*
  * Numbers of 8 bits with a scale for each row: t[r][c] = q[r][c] * scales[r], scales[r] = max_c |t[r][c]| / 127, q the whole number

@@ -193,8 +193,8 @@ def load():
     f32, cint = ctypes.c_float, ctypes.c_int
     lib.lce_token_labels.argtypes = [vp, i64, i64, i64, i64, i64, vp, vp]
     lib.lce_token_logits_workspace_bytes.argtypes = [P, ctypes.POINTER(sz), ctypes.POINTER(sz)]
-    lib.lce_token_logits.argtypes = [P, vp, vp, vp, i64, vp, vp, vp, sz, vp]
-    lib.lce_token_logits_backward.argtypes = [P] + [vp] * 10 + [sz, vp]
+    lib.lce_token_logits.argtypes = [P, vp, vp, vp, i64, vp, vp, vp, vp, sz, vp]
+    lib.lce_token_logits_backward.argtypes = [P] + [vp] * 11 + [sz, vp]
     lib.lce_quantize_rows.argtypes = [vp, cint, i64, i64, i64, vp, i64, vp, vp]
     lib.lce_quantize_columns.argtypes = lib.lce_quantize_rows.argtypes
     lib.lce_int8_logits_workspace_bytes.argtypes = [i64, i64, i64, ctypes.POINTER(sz)]

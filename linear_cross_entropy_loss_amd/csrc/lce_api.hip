@@ -1773,8 +1773,8 @@ int lce_token_logits_workspace_bytes(const lce_problem* p, size_t* fwd_bytes, si
   return rc;
 }
 
-int lce_token_logits(const lce_problem* p, const void* x, const void* w, const int64_t* y, int64_t other, float* logits, float* lse, void* ws,
-                     size_t ws_bytes, void* stream) {
+int lce_token_logits(const lce_problem* p, const void* x, const void* w, const int64_t* y, int64_t other, float* logits, float* lse,
+                     float* scales, void* ws, size_t ws_bytes, void* stream) {
   const int rc = check_tokens(p, false);
   if (rc != LCE_OK) return rc;
   if (!logits) return LCE_EINVAL_ARG;
@@ -1785,16 +1785,18 @@ int lce_token_logits(const lce_problem* p, const void* x, const void* w, const i
   char* const out = (char*)ws + t.fwd;
   float* pair = nullptr;
   if (splits(p)) {
-    pair = (float*)((char*)ws + t.fwd_pair);
+    float* const part = (float*)((char*)ws + t.fwd_pair);
+    pair = scales ? scales : part;
     const hipError_t e = lce::launch_pair_scales((const float*)x, p->ldx, p->N, p->H, y, p->ignore_index, (const float*)w, p->ldw, p->V, pair,
-                                                 pair + 64, (hipStream_t)stream);
+                                                 part + 64, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "pair_scales");
   }
   return forward_impl(p, x, w, y, lse, (float*)out, (int64_t*)(out + 128), ws, t.fwd, stream, logits, other, pair);
 }
 
 int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w, const int64_t* y, const float* logits, const float* lse,
-                              const float* grad_logits, const float* grad_lse, void* dx, void* dw, void* ws, size_t ws_bytes, void* stream) {
+                              const float* grad_logits, const float* grad_lse, const float* scales, void* dx, void* dw, void* ws, size_t ws_bytes,
+                              void* stream) {
   int rc = check_tokens(p, true);
   if (rc != LCE_OK) return rc;
   if (!x || !w || !y || !logits || !lse || !grad_logits || !grad_lse || !(dx || dw)) return LCE_EINVAL_ARG;
@@ -1813,7 +1815,9 @@ int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w
   r.row_lse = (float*)(base + t.row_lse); r.row_y = (int64_t*)(base + t.row_y); r.row_value = (float*)(base + t.row_value);
   r.part = (float*)(base + t.part); r.factor = r.part + lce::kRowGradientParts;
   r.one = (int64_t*)(r.factor + 4);
-  if (splits(p)) {
+  if (splits(p) && scales) {
+    r.pair = scales;
+  } else if (splits(p)) {
     float* const pair = (float*)(base + t.pair);
     const hipError_t e = lce::launch_pair_scales((const float*)x, p->ldx, p->N, p->H, y, p->ignore_index, (const float*)w, p->ldw, p->V, pair,
                                                  pair + 64, (hipStream_t)stream);

@@ -443,6 +443,7 @@ struct TokenCall {
   void* stream;
   int rc = LCE_OK;
   at::Tensor logits, lse, x, w, labels;
+  at::Tensor scales;  // of float32 tensors, for the backward
 };
 
 // False: no ordinary call.
@@ -476,6 +477,7 @@ void run_tokens(const at::Tensor& x_in, const at::Tensor& At, const at::Tensor& 
   t.labels = t.piece ? at::empty({p.N}, tokens.options()) : given;
   t.logits = at::empty(tokens.sizes(), o.dtype(at::kFloat));
   t.lse = at::empty(tokens.sizes(), o.dtype(at::kFloat));
+  if (p.x_dtype == LCE_F32) t.scales = at::empty({LCE_PAIR_SCALES}, o);
   Workspace ws(t.bytes);
   if (c.x != kInPlace) t.rc = copy_rows(c.x, x_in, p.N, p.H, t.x, p.ldx, t.stream);
   if (t.rc == LCE_OK && c.w != kInPlace) t.rc = copy_rows(c.w, At, p.H, p.V, t.w, p.ldw, t.stream);
@@ -484,7 +486,7 @@ void run_tokens(const at::Tensor& x_in, const at::Tensor& At, const at::Tensor& 
                             t.stream);
   if (t.rc == LCE_OK)
     t.rc = abi.token_logits(&p, t.x.data_ptr(), t.w.data_ptr(), (const int64_t*)t.labels.data_ptr(), t.piece ? p.V : t.ignore_index,
-                            (float*)t.logits.data_ptr(), (float*)t.lse.data_ptr(), ws.data.get(), t.bytes, t.stream);
+                            (float*)t.logits.data_ptr(), (float*)t.lse.data_ptr(), (float*)ptr(t.scales), ws.data.get(), t.bytes, t.stream);
 }
 
 // (logits, lse, x, w, w_layout, labels, ignore_index), as _forward of token_logits.py returns them; (status, name) where the C ABI refused; None:
@@ -504,7 +506,8 @@ py::object token_logits(const at::Tensor& x_in, const at::Tensor& At, const at::
 // The gradients, dense, dw as it is stored.  False: not handled, nothing is launched.
 bool run_tokens_backward(const at::Tensor& x, const at::Tensor& w, int layout, const at::Tensor& labels, const at::Tensor& logits,
                          const at::Tensor& lse, const at::Tensor& g_logits, const at::Tensor& g_lse, int64_t ignore_index, double scale,
-                         int64_t n_chunk, int pack, bool need_dx, bool need_dw, void* stream, at::Tensor& dx, at::Tensor& dw, int& rc) {
+                         const at::Tensor& scales, int64_t n_chunk, int pack, bool need_dx, bool need_dw, void* stream, at::Tensor& dx,
+                         at::Tensor& dw, int& rc) {
   Call c;
   lce_problem& p = c.p;
   if (!(need_dx || need_dw) || w.dim() != 2) return false;
@@ -525,7 +528,8 @@ bool run_tokens_backward(const at::Tensor& x, const at::Tensor& w, int layout, c
   if (need_dw) dw = rows_of(w.size(0), w.size(1), p.lddw, w.options().requires_grad(false));
   Workspace ws(bytes);
   rc = abi.token_logits_backward(&p, x.data_ptr(), w.data_ptr(), (const int64_t*)labels.data_ptr(), (const float*)logits.data_ptr(),
-                                 (const float*)lse.data_ptr(), (const float*)g_logits.data_ptr(), (const float*)g_lse.data_ptr(), ptr(dx), ptr(dw),
+                                 (const float*)lse.data_ptr(), (const float*)g_logits.data_ptr(), (const float*)g_lse.data_ptr(), (const float*)ptr(scales),
+                                 ptr(dx), ptr(dw),
                                  ws.data.get(), bytes, stream);
   if (rc != LCE_OK) return true;
   if (need_dx) dx = dx.contiguous();
@@ -542,7 +546,7 @@ py::object token_logits_backward(const at::Tensor& x, const at::Tensor& w, int l
   bool handled;
   {
     py::gil_scoped_release release;
-    handled = run_tokens_backward(x, w, layout, labels, logits, lse, g_logits, g_lse, ignore_index, scale, n_chunk, pack, need_dx, need_dw,
+    handled = run_tokens_backward(x, w, layout, labels, logits, lse, g_logits, g_lse, ignore_index, scale, at::Tensor(), n_chunk, pack, need_dx, need_dw,
                                   reinterpret_cast<void*>(stream), dx, dw, rc);
   }
   if (!handled) return py::none();
@@ -557,7 +561,7 @@ struct TokenLogits : public torch::autograd::Function<TokenLogits> {
                                                 const at::Tensor& tokens, TokenCall* t) {
     run_tokens(x_in, At, tokens, *t);
     TORCH_CHECK(t->rc == LCE_OK, "linear_token_logits: status ", t->rc);
-    ctx->save_for_backward({t->x, t->w, t->labels, t->logits, t->lse});
+    ctx->save_for_backward({t->x, t->w, t->labels, t->logits, t->lse, t->scales});
     const lce_problem& p = t->c.p;
     ctx->saved_data["layout"] = (int64_t)p.w_layout;
     ctx->saved_data["ignore_index"] = p.ignore_index;
@@ -583,7 +587,7 @@ struct TokenLogits : public torch::autograd::Function<TokenLogits> {
     at::Tensor dx, dw;
     int rc = LCE_OK;
     const bool handled = run_tokens_backward(rows(saved[0]), rows(saved[1]), layout, saved[2].contiguous(), saved[3].contiguous(), saved[4].contiguous(), g_logits, g_lse,
-                                             d["ignore_index"].toInt(), d["scale"].toDouble(), d["n_chunk"].toInt(), (int)d["pack"].toInt(),
+                                             d["ignore_index"].toInt(), d["scale"].toDouble(), saved[5], d["n_chunk"].toInt(), (int)d["pack"].toInt(),
                                              ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                              reinterpret_cast<void*>((uintptr_t)d["stream"].toInt()), dx, dw, rc);
     TORCH_CHECK(handled && rc == LCE_OK, "linear_token_logits: status ", rc);

@@ -17,7 +17,7 @@
 //
 // fp32 tensors: fp16 pairs (lce_gemm.h) instead of the loss's bf16 ones, for products 22 bits wide.  N=2048, H=1024, V=16384, errors of dx and
 // dW against fp64, relative to their norms: 3.4e-7, of bf16 pairs 4.4e-6 (a float32 library product and its softmax: 2.2e-6).  Their scales
-// cost one more pass over the weight and x in each direction (pair_max_kernel, 17 of some 460 us).
+// cost one more pass over the weight and x (pair_max_kernel, 17 us of a forward and backward of 910; 930 where the backward has no scales).
 #include "lce_gemm3.h"
 #include "lce_internal.h"
 

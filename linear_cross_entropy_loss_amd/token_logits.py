@@ -76,7 +76,7 @@ def _forward(x_in, At, tokens, ignore_index, logit_scale, N_chunk_size, vocab_st
         prob = _problem(x, w, layout, V, ignore_index, logit_scale, N_chunk_size, pack)
         nbytes = _lib.token_logits_workspace_bytes(prob, False)  # (checks the problem)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        rc = _lib.load().lce_token_logits(ctypes.byref(prob), _ptr(x), _ptr(w), _ptr(labels), other, _ptr(logits), _ptr(lse), _ptr(ws), nbytes,
+        rc = _lib.load().lce_token_logits(ctypes.byref(prob), _ptr(x), _ptr(w), _ptr(labels), other, _ptr(logits), _ptr(lse), None, _ptr(ws), nbytes,
                                           _stream(dev))
         _lib.raise_for_status(rc, "linear_token_logits")
         del ws
@@ -105,7 +105,7 @@ def _backward(x, w, layout, labels, logits, lse, g_logits, g_lse, ignore_index, 
             nbytes = _lib.token_logits_workspace_bytes(prob, True)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             rows = [t.detach().to(device=dev, dtype=torch.float32).reshape(-1).contiguous() for t in (logits, lse, g_logits, g_lse)]
-            rc = _lib.load().lce_token_logits_backward(ctypes.byref(prob), _ptr(x), _ptr(w), _ptr(labels), *map(_ptr, rows), _ptr(dx), _ptr(dw),
+            rc = _lib.load().lce_token_logits_backward(ctypes.byref(prob), _ptr(x), _ptr(w), _ptr(labels), *map(_ptr, rows), None, _ptr(dx), _ptr(dw),
                                                        _ptr(ws), nbytes, _stream(dev))
             _lib.raise_for_status(rc, "linear_token_logits")
             del ws

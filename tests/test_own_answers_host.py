@@ -53,23 +53,23 @@ def test_token_logits_problems(lib, kw, status):
     f, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
     p = ctypes.byref(_prob(**kw))
     assert lib.lce_token_logits_workspace_bytes(p, ctypes.byref(f), ctypes.byref(b)) == status
-    assert lib.lce_token_logits(p, PTR, PTR, PTR, 0, PTR, PTR, PTR, BIG, None) == status
-    assert lib.lce_token_logits_backward(p, *[PTR] * 9, PTR, BIG, None) == status
+    assert lib.lce_token_logits(p, PTR, PTR, PTR, 0, PTR, PTR, None, PTR, BIG, None) == status
+    assert lib.lce_token_logits_backward(p, *[PTR] * 7, None, PTR, PTR, PTR, BIG, None) == status
 
 
 def test_token_logits_arguments(lib):
     p = ctypes.byref(_prob())
     f, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
     assert lib.lce_token_logits_workspace_bytes(p, ctypes.byref(f), ctypes.byref(b)) == 0
-    good = [PTR, PTR, PTR, 0, PTR, PTR, PTR]
+    good = [PTR, PTR, PTR, 0, PTR, PTR, None, PTR]
     for i in (0, 1, 2, 4, 5):
         assert lib.lce_token_logits(p, *[None if i == j else g for j, g in enumerate(good)], BIG, None) == ARG, i
     assert lib.lce_token_logits(p, *good[:-1], None, BIG, None) == WORKSPACE
     assert lib.lce_token_logits(p, *good, f.value - 1, None) == WORKSPACE
     for i in range(7):
-        assert lib.lce_token_logits_backward(p, *[None if i == j else PTR for j in range(9)], PTR, BIG, None) == ARG, i
-    assert lib.lce_token_logits_backward(p, *[PTR] * 7, None, None, PTR, BIG, None) == ARG
-    assert lib.lce_token_logits_backward(p, *[PTR] * 9, PTR, b.value - 1, None) == WORKSPACE
+        assert lib.lce_token_logits_backward(p, *[None if i == j else PTR for j in range(7)], None, PTR, PTR, PTR, BIG, None) == ARG, i
+    assert lib.lce_token_logits_backward(p, *[PTR] * 7, None, None, None, PTR, BIG, None) == ARG
+    assert lib.lce_token_logits_backward(p, *[PTR] * 7, None, PTR, PTR, PTR, b.value - 1, None) == WORKSPACE
     # the backward stages dz within the scratch bound of the loss (N_chunk_size * V * 4) wherever the narrowest split fits
     for N, H, V, chunk in ((16384, 768, 50264, 4096), (4096, 64, 32768, 1024)):
         q = _prob(N=N, H=H, V=V, ldx=H, ldw=V, lddx=H, lddw=V, n_chunk=chunk)
