@@ -97,7 +97,7 @@ def draw(rng):
             case = _int8(size(1, 4096, 1), size(64, 8192, 64), size(1000, 262144, 128), dtype, tied=rng.random() < 0.4,
                          fresh=rng.random() < 0.3, scale=rng.choice([1.0, 1.0, 0.5]))
         else:
-            case = _clip(size(16, 4096, 16), size(256, 131072, 128), rng.randint(0, 8), dtype, rng.choice([dtype, "f32"]),
+            case = _clip(size(16, 4096, 16), size(256, 131072, 128), rng.randint(0, 24), dtype, rng.choice([dtype, "f32"]),
                          norm=rng.choice([0.5, 2.0, 4.0, 100.0]), divisor=LOSS_SCALE if dtype == "f16" else 1.0)
         if _cost(case) <= most[what]:
             return case
