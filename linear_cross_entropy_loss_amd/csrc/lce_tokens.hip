@@ -68,17 +68,19 @@ __global__ __launch_bounds__(kRowThreads) void row_gradients_kernel(const RowGra
     *g.one = 1;
   }
   for (int64_t j = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; j < g.N; j += (int64_t)gridDim.x * kRowThreads) {
-    const int64_t n = g.perm != nullptr ? packed_token(g.perm, j, g.N) : j;
-    const float gl = ldexpf(g.grad_lse[n], -e);
-    // (no gradient: exp(z - lse') is 0 whatever the logits.  Finite all the same: the kernels multiply it by a z_reg of 0.)
+    const int64_t n = g.perm != nullptr ? packed_token(g.perm, j, g.N) : j, yy = g.y[n];
+    // (a row that does not count may hold any upstream gradient, NaN too, and its numbers are finite all the same: the kernels multiply its
+    // dz of 0 by a factor made of them)
+    const bool counts = yy != g.ignore_index;
+    const float gl = counts ? ldexpf(g.grad_lse[n], -e) : 0.f;
+    // (no gradient: exp(z - lse') is 0 whatever the logits.  Finite as well, for a z_reg of 0 is multiplied by it.)
     const float l = g.lse[n] - logf(fabsf(gl));
-    g.row_lse[j] = l > 1e30f ? 1e30f : l < -1e30f ? -1e30f : l;
-    const int64_t yy = g.y[n];
+    g.row_lse[j] = !counts ? 0.f : l > 1e30f ? 1e30f : l < -1e30f ? -1e30f : l;
     if (g.row_value == nullptr) {
-      g.row_y[j] = yy == g.ignore_index ? -1 : gl < 0.f ? kNegativeRow : g.V;
+      g.row_y[j] = !counts ? -1 : gl < 0.f ? kNegativeRow : g.V;
     } else {
-      g.row_y[j] = yy == g.ignore_index ? -1 : yy >= 0 && yy < g.V ? yy : g.V;
-      g.row_value[j] = pack_row_value(target(gl, ldexpf(g.grad_logits[n], -e), g.logits[n], g.lse[n], g.dz_shift), gl < 0.f);
+      g.row_y[j] = !counts ? -1 : yy >= 0 && yy < g.V ? yy : g.V;
+      g.row_value[j] = counts ? pack_row_value(target(gl, ldexpf(g.grad_logits[n], -e), g.logits[n], g.lse[n], g.dz_shift), gl < 0.f) : 0.f;
     }
   }
 }
