@@ -215,7 +215,8 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int c = c0 + i * kStep + t * E::kPer;
-      if (c < ldq) store_bytes<DT>(once ? v[i] : load_piece<DT>(from, c, cols), s, inverse, to + c);
+      // (behind what is held there are zeros only, as far as a wide ldq reaches)
+      if (c < ldq) store_bytes<DT>(once && c0 == 0 ? v[i] : load_piece<DT>(from, c, cols), s, inverse, to + c);
     }
 }
 

@@ -1,0 +1,55 @@
+"""Clipping where calls go wrong easily: norms at the end of float32, and tensors that have no memory of their own."""
+import math
+
+import pytest
+import torch
+
+pytestmark = [pytest.mark.gpu, pytest.mark.pack_auto]
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_a_norm_beyond_float32_is_infinite_and_nothing_is_clipped(dtype):
+    from linear_cross_entropy_loss_amd import clip_gradients
+
+    for to in (None, F32):
+        for divisor in (1.0, torch.ones((), device="cuda")):
+            g = [torch.full((9001,), 3e38, device="cuda").to(dtype), torch.full((5,), -2.0, device="cuda").to(dtype)]
+            was = [t.clone() for t in g]
+            out = None if to is None else [torch.zeros_like(t, dtype=to) for t in g]
+            assert float(clip_gradients(g, 1.0, divisor, out)) == math.inf
+            assert all(torch.equal(a.float(), b.float()) for a, b in zip(g if out is None else out, was))
+    # by the divisor alone: a norm of 2^127 and one of 2^128, which is no float32
+    for divisor, clipped in ((0.5, True), (2.0 ** -2, False)):
+        g = torch.full((4,), 2.0 ** 125, device="cuda", dtype=dtype)
+        norm = float(clip_gradients(g, 2.0, divisor))
+        assert norm == (2.0 ** 126 / divisor if clipped else math.inf)
+        assert (g == (1.0 if clipped else 2.0 ** 125 / divisor)).all()
+
+
+class Wrapped(torch.Tensor):
+    """A tensor whose numbers are another's, as those of sharded tensors are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        inner = [a.inner if isinstance(a, Wrapped) else a for a in args]
+        return func(*inner, **(kwargs or {}))
+
+
+def test_tensors_without_memory_of_their_own_are_refused():
+    from linear_cross_entropy_loss_amd import clip_gradients
+
+    plain = torch.ones(10, device="cuda")
+    sharded = Wrapped(torch.ones(10, device="cuda"))
+    for grads, out in (([sharded], None), ([plain, sharded], None), ([plain], [sharded]), ([sharded], [plain])):
+        with pytest.raises(ValueError, match="no memory of their own"):
+            clip_gradients(grads, 1.0, out=out)
+    assert (plain == 1).all() and (sharded.inner == 1).all()

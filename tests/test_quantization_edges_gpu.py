@@ -1,0 +1,43 @@
+"""Numbers of 8 bits where calls go wrong easily: through the C interface with row strides of the caller's own choice, with more rows than one
+launch takes, and with weights that were not laid out here."""
+import pytest
+import torch
+
+pytestmark = [pytest.mark.gpu, pytest.mark.pack_auto]
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def quantize(call, src, depth, others, ld, ldq):
+    """lce_quantize_rows or lce_quantize_columns into rows of ldq bytes that hold 77, between two rows that stay as they are."""
+    from linear_cross_entropy_loss_amd import _lib
+
+    lib = _lib.load()
+    room = torch.full((others + 2, ldq), 77, dtype=torch.int8, device="cuda")
+    scales = torch.full((others + 2,), 5.0, device="cuda")
+    rows, cols = (others, depth) if call == "lce_quantize_rows" else (depth, others)
+    rc = getattr(lib, call)(src.data_ptr(), _lib.dtype_code(src.dtype), rows, cols, ld, room[1:].data_ptr(), ldq, scales[1:].data_ptr(),
+                            torch.cuda.current_stream().cuda_stream)
+    _lib.raise_for_status(rc, call)
+    assert (room[0] == 77).all() and (room[-1] == 77).all() and scales[0] == 5.0 and scales[-1] == 5.0
+    return room[1:-1], scales[1:-1]
+
+
+def strides(depth):
+    least = -(-depth // 16) * 16
+    return sorted({least, least + 16, 2 * least + 512, 4096, 9008, 1 << 18} - set(range(0, least, 16)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("rows", [3, 1500])
+@pytest.mark.parametrize("cols", [1, 17, 100, 300, 700, 1000, 2100, 5000])
+def test_rows_of_any_stride(rows, cols, dtype):
+    from linear_cross_entropy_loss_amd import quantize_rows
+
+    t = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows + cols)).to(dtype).cuda()
+    want = quantize_rows(t)
+    for ldq in strides(cols):
+        print(f"lce_quantize_rows {rows} {cols} {dtype} ldq {ldq}", flush=True)
+        q, scales = quantize("lce_quantize_rows", t, cols, rows, cols, ldq)
+        assert torch.equal(q[:, :cols], want.values) and torch.equal(scales, want.scales)
+        assert not q[:, cols:].any()
