@@ -805,11 +805,13 @@ hipError_t quantize_columns(const void* src, int64_t rows, int64_t cols, int64_t
   constexpr int kRows = 4 * kTiles * Source<DT>::kPer;  // numbers that a thread holds
   // (offsets within a tile of the rows have 32 bits)
   const bool held = cols >= 64 && ld * (DT == DT_F32 ? 4 : 2) * 1024 < (int64_t)1 << 31;
+  // (what a workgroup holds of a column has to reach to the end of a row of q, zeros behind the last number included)
+  const auto holds = [&](int nt, int columns) { return held && ldq <= nt * kRows / columns; };
   // (smaller workgroups, more stripes under way: 64 x 100000 bf16 13 us, 21 in workgroups of 512; not to the full: 500 x 65536 27, 24)
-  if (held && rows <= 128 * kRows / 64) return quantize_held_columns<DT, 256, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
-  if (held && rows <= 512 * kRows / 64) return quantize_held_columns<DT, 512, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
-  if (held && rows <= 1024 * kRows / 64) return quantize_held_columns<DT, 1024, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
-  if (held && rows <= 1024 * kRows / 32) return quantize_held_columns<DT, 1024, 32>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+  if (rows <= 128 * kRows / 64 && holds(256, 64)) return quantize_held_columns<DT, 256, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+  if (holds(512, 64)) return quantize_held_columns<DT, 512, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+  if (holds(1024, 64)) return quantize_held_columns<DT, 1024, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
+  if (holds(1024, 32)) return quantize_held_columns<DT, 1024, 32>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
   hipLaunchKernelGGL(quantize_columns_kernel<DT>, dim3((unsigned)((cols + kColTile - 1) / kColTile)), dim3(kQuantThreads), 0, s, src, (int)rows,
                      cols, ld, q, (int)ldq, scales);
   return hipGetLastError();

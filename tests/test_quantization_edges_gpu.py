@@ -41,3 +41,18 @@ def test_rows_of_any_stride(rows, cols, dtype):
         q, scales = quantize("lce_quantize_rows", t, cols, rows, cols, ldq)
         assert torch.equal(q[:, :cols], want.values) and torch.equal(scales, want.scales)
         assert not q[:, cols:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("others", [5, 64, 130])
+@pytest.mark.parametrize("depth", [1, 64, 100, 200, 300, 1000, 1100, 2100, 4097])
+def test_columns_of_any_stride(depth, others, dtype):
+    from linear_cross_entropy_loss_amd import quantize_weight
+
+    At = torch.randn(depth, others, generator=torch.Generator().manual_seed(depth + others)).to(dtype).cuda()
+    want = quantize_weight(At)
+    for ldq in strides(depth):
+        print(f"lce_quantize_columns {depth} {others} {dtype} ldq {ldq}", flush=True)
+        q, scales = quantize("lce_quantize_columns", At, depth, others, others, ldq)
+        assert torch.equal(q[:, :depth], want.values) and torch.equal(scales, want.scales)
+        assert not q[:, depth:].any()
