@@ -654,8 +654,8 @@ py::object quantized_logits(const at::Tensor& x, const at::Tensor& values, const
   Rows r;
   if (!describe_rows(x, r) || !plain(values) || !plain(scales) || values.scalar_type() != at::kChar || scales.scalar_type() != at::kFloat ||
       values.device() != x.device() || scales.device() != x.device() || values.dim() != 2 || values.size(0) < 1 || values.size(1) != r.cols ||
-      values.stride(1) != 1 || values.stride(0) < r.cols || values.stride(0) % 16 != 0 || !aligned(values) || scales.dim() != 1 ||
-      scales.size(0) != values.size(0) || !scales.is_contiguous())
+      values.stride(1) != 1 || values.stride(0) < r.cols || values.stride(0) > 2 * LCE_INT8_DEPTH || values.stride(0) % 16 != 0 ||
+      !aligned(values) || scales.dim() != 1 || scales.size(0) != values.size(0) || !scales.is_contiguous())
     return py::none();
   const at::ScalarType type = dtype.is_none() ? x.scalar_type() : reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
   const int code = dtype_code(type);

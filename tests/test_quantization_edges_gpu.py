@@ -56,3 +56,15 @@ def test_columns_of_any_stride(depth, others, dtype):
         q, scales = quantize("lce_quantize_columns", At, depth, others, others, ldq)
         assert torch.equal(q[:, :depth], want.values) and torch.equal(scales, want.scales)
         assert not q[:, depth:].any()
+
+
+@pytest.mark.parametrize("N", [1, 5, 40, 300])
+def test_values_of_rows_wider_than_the_library_takes_are_copied(N):
+    from linear_cross_entropy_loss_amd import Quantized, quantize_weight, quantized_logits
+
+    x = torch.randn(N, 100, device="cuda").to(BF16)
+    weight = quantize_weight(torch.randn(100, 333, device="cuda").to(BF16))
+    for ld in ((1 << 18), (1 << 18) + 16, 1 << 20):
+        wide = torch.full((333, ld), 99, dtype=torch.int8, device="cuda")
+        wide[:, :100] = weight.values
+        assert torch.equal(quantized_logits(x, Quantized(wide[:, :100], weight.scales)), quantized_logits(x, weight))
