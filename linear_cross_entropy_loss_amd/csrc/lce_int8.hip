@@ -772,18 +772,29 @@ template <class T> hipError_t launch_product(const Int8Args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Workgroups of one launch, which has fewer than 2^32 threads: more rows or columns take several, one after another.
+constexpr int64_t kMostGroups = (int64_t)1 << 22;
+
 template <int DT>
 hipError_t quantize_rows(const void* src, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales, hipStream_t s) {
   constexpr int kPer = Source<DT>::kPer;
-  const dim3 sixteens((unsigned)((rows + 15) / 16)), fours((unsigned)((rows + 3) / 4)), ones((unsigned)rows), threads(kQuantThreads);
-  const auto go = [&](auto kernel, dim3 grid) { hipLaunchKernelGGL(kernel, grid, threads, 0, s, src, rows, (int)cols, ld, q, (int)ldq, scales); };
-  if (rows < 1024 || cols > 64 * kPer * 8) go(quantize_rows_kernel<DT, 4, 32 / kPer>, ones);
-  else if (cols > 64 * kPer * 4) go(quantize_rows_kernel<DT, 1, 8>, fours);
-  else if (cols > 64 * kPer * 2) go(quantize_rows_kernel<DT, 1, 4>, fours);
-  else if (cols > 16 * kPer * 4) go(quantize_rows_kernel<DT, 1, 8, 16>, sixteens);
-  else if (cols > 16 * kPer * 2) go(quantize_rows_kernel<DT, 1, 4, 16>, sixteens);
-  else go(quantize_rows_kernel<DT, 1, 2, 16>, sixteens);
-  return hipGetLastError();
+  // (`per` rows to a workgroup)
+  const auto go = [&](auto kernel, int64_t per) {
+    for (int64_t r = 0; r < rows; r += kMostGroups * per) {
+      const int64_t n = rows - r < kMostGroups * per ? rows - r : kMostGroups * per;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((n + per - 1) / per)), dim3(kQuantThreads), 0, s,
+                         reinterpret_cast<const typename Source<DT>::S*>(src) + r * ld, n, (int)cols, ld, q + r * ldq, (int)ldq, scales + r);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  };
+  if (rows < 1024 || cols > 64 * kPer * 8) return go(quantize_rows_kernel<DT, 4, 32 / kPer>, 1);
+  if (cols > 64 * kPer * 4) return go(quantize_rows_kernel<DT, 1, 8>, 4);
+  if (cols > 64 * kPer * 2) return go(quantize_rows_kernel<DT, 1, 4>, 4);
+  if (cols > 16 * kPer * 4) return go(quantize_rows_kernel<DT, 1, 8, 16>, 16);
+  if (cols > 16 * kPer * 2) return go(quantize_rows_kernel<DT, 1, 4, 16>, 16);
+  return go(quantize_rows_kernel<DT, 1, 2, 16>, 16);
 }
 template <int DT, int NT, int COLS>
 hipError_t quantize_held_columns(const void* src, int64_t rows, int64_t cols, int64_t ld, signed char* q, int64_t ldq, float* scales, int num_cus,
@@ -812,9 +823,14 @@ hipError_t quantize_columns(const void* src, int64_t rows, int64_t cols, int64_t
   if (holds(512, 64)) return quantize_held_columns<DT, 512, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
   if (holds(1024, 64)) return quantize_held_columns<DT, 1024, 64>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
   if (holds(1024, 32)) return quantize_held_columns<DT, 1024, 32>(src, rows, cols, ld, q, ldq, scales, num_cus, s);
-  hipLaunchKernelGGL(quantize_columns_kernel<DT>, dim3((unsigned)((cols + kColTile - 1) / kColTile)), dim3(kQuantThreads), 0, s, src, (int)rows,
-                     cols, ld, q, (int)ldq, scales);
-  return hipGetLastError();
+  for (int64_t c = 0; c < cols; c += kMostGroups * kColTile) {
+    const int64_t n = cols - c < kMostGroups * kColTile ? cols - c : kMostGroups * kColTile;
+    hipLaunchKernelGGL(quantize_columns_kernel<DT>, dim3((unsigned)((n + kColTile - 1) / kColTile)), dim3(kQuantThreads), 0, s,
+                       reinterpret_cast<const typename Source<DT>::S*>(src) + c, (int)rows, n, ld, q + c * ldq, (int)ldq, scales + c);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace

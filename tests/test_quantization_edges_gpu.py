@@ -68,3 +68,36 @@ def test_values_of_rows_wider_than_the_library_takes_are_copied(N):
         wide = torch.full((333, ld), 99, dtype=torch.int8, device="cuda")
         wide[:, :100] = weight.values
         assert torch.equal(quantized_logits(x, Quantized(wide[:, :100], weight.scales)), quantized_logits(x, weight))
+
+
+def windows(n):
+    """Rows at both ends and around every 2^21-th."""
+    at = {0, n - 40} | {i - 20 for i in range(1 << 21, n - 40, 1 << 21)}
+    return [slice(i, i + 40) for i in sorted(at)]
+
+
+# (a launch has fewer than 2^32 threads: 16, 64 and 256 of them to a row, by its length)
+@pytest.mark.parametrize("rows, cols, dtype", [((1 << 28) + 77, 8, BF16), ((1 << 26) + 77, 520, F32), ((1 << 24) + 77, 2100, F32)], ids=str)
+def test_more_rows_than_a_launch_takes(rows, cols, dtype):
+    """Rows that begin one number after another: a source that fits."""
+    from linear_cross_entropy_loss_amd import quantize_rows
+
+    src = torch.randn(rows + cols - 1, device="cuda", dtype=F32).to(dtype)
+    ldq = -(-cols // 16) * 16
+    print(f"lce_quantize_rows {rows} {cols} {dtype}", flush=True)
+    q, scales = quantize("lce_quantize_rows", src, cols, rows, 1, ldq)
+    for part in windows(rows):
+        want = quantize_rows(src[part.start:part.stop + cols - 1].unfold(0, cols, 1))
+        assert torch.equal(q[part, :cols], want.values) and torch.equal(scales[part], want.scales) and not q[part, cols:].any()
+
+
+def test_more_columns_than_a_launch_takes():
+    from linear_cross_entropy_loss_amd import quantize_rows
+
+    cols = 1 << 30
+    src = torch.empty(cols, device="cuda", dtype=BF16).normal_()
+    print(f"lce_quantize_columns 1 {cols}", flush=True)
+    q, scales = quantize("lce_quantize_columns", src, 1, cols, cols, 16)
+    for part in windows(cols)[::16] + windows(cols)[-1:]:
+        want = quantize_rows(src[part, None])
+        assert torch.equal(q[part, :1], want.values) and torch.equal(scales[part], want.scales) and not q[part, 1:].any()
