@@ -557,7 +557,8 @@ int lce_int8_logits(const void* x, int x_dtype, int64_t N, int64_t H, int64_t V,
  * The norm of many tensors together, and the tensors scaled to at most that of max_norm:
  *   *norm = sqrt(sum over all of them of g^2) / divisor,   out = g * min(1, max_norm / *norm) / divisor
  * squares and their sum in doubles, in a fixed order; the factor rounded to fp32, each product to out's type.  A norm that is not
- * finite leaves min(...) at 1: the caller looks at *norm.  No counterpart in the reference.  From version 1100 on.
+ * finite, or beyond float32, as *norm says, leaves min(...) at 1: the caller looks at *norm.  No counterpart in the reference.  From
+ * version 1100 on.
  *   t        `count` tensors (host memory, read during the call), n elements each, dense, at any element boundary; grad: in; out: of
  *            dtype or LCE_F32, may be grad itself; an `out` may overlap no other tensor's memory.  0 <= count <= 2^20
  *   max_norm > 0 (infinity: no limit);  divisor_ptr: a device pointer to 1 float, or NULL: the number `divisor` > 0

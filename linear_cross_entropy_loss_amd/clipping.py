@@ -48,7 +48,7 @@ def clip_gradients(grads, max_norm, divisor=1.0, out=None):
     their device.
 
     With ``norm = sqrt(sum of all squares) / divisor`` every element becomes ``g * min(1, max_norm / norm) / divisor``.  A norm that
-    is not finite (an overflow of float16) leaves ``min(...)`` at 1: look at the norm before the step is taken.
+    is not finite (an overflow of float16), or beyond float32, leaves ``min(...)`` at 1: look at the norm before the step is taken.
 
     Args:
         grads: a tensor or an iterable of them: bfloat16, float16 and float32, mixed at will, on one device.  None is passed over.

@@ -159,8 +159,8 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipBatc
   for (int i = threadIdx.x; i < parts; i += kClipThreads) sum += b.part[i];
   const double d = divisor_ptr != nullptr ? (double)*divisor_ptr : (double)divisor;
   const double norm = sqrt(workgroup_sum(sum)) / d;
-  // (not finite: nothing is clipped, and whoever reads the norm knows)
-  const double f = (norm > (double)max_norm && norm < (double)INFINITY ? (double)max_norm / norm : 1.0) / d;
+  // (not finite, as the float32 number that the caller sees: nothing is clipped, and whoever reads the norm knows)
+  const double f = (norm > (double)max_norm && (float)norm < INFINITY ? (double)max_norm / norm : 1.0) / d;
   const float factor = (float)f;
   if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   // (from the last stretch to the first: those that the first launch read last are still in the Infinity Cache)
