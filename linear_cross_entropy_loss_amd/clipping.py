@@ -30,6 +30,9 @@ def _check(grads, out, max_norm, divisor):
             raise ValueError("clip_gradients: all tensors must be on the same device")
         if o.shape != g.shape or (o.dtype != g.dtype and o.dtype != torch.float32):
             raise ValueError(f"clip_gradients: a gradient of shape {tuple(g.shape)} and {g.dtype} cannot go to {tuple(o.shape)} and {o.dtype}")
+        if g.numel() > 0 and not (g.data_ptr() and o.data_ptr()):
+            raise ValueError("clip_gradients: tensors that have no memory of their own (sharded ones, wrappers of others) are not supported: "
+                             "hand over what they hold here")
     if isinstance(divisor, torch.Tensor):
         if divisor.dtype != torch.float32 or divisor.numel() != 1 or (grads and divisor.device != grads[0].device):
             raise ValueError("clip_gradients: divisor must be a number, or a float32 tensor with one on the gradients' device")
@@ -52,6 +55,7 @@ def clip_gradients(grads, max_norm, divisor=1.0, out=None):
 
     Args:
         grads: a tensor or an iterable of them: bfloat16, float16 and float32, mixed at will, on one device.  None is passed over.
+            The norm is that of these tensors: nothing is added up over processes.
         max_norm: positive; infinity scales by the divisor alone.
         divisor: the factor that the loss was multiplied by (a loss scale, a number of accumulated steps): a positive number, or a
             float32 tensor with one.

@@ -26,3 +26,30 @@ def test_a_norm_beyond_float32_is_infinite_and_nothing_is_clipped(dtype):
         norm = float(clip_gradients(g, 2.0, divisor))
         assert norm == (2.0 ** 126 / divisor if clipped else math.inf)
         assert (g == (1.0 if clipped else 2.0 ** 125 / divisor)).all()
+
+
+class Wrapped(torch.Tensor):
+    """A tensor whose numbers are another's, as those of sharded tensors are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        inner = [a.inner if isinstance(a, Wrapped) else a for a in args]
+        return func(*inner, **(kwargs or {}))
+
+
+def test_tensors_without_memory_of_their_own_are_refused():
+    from linear_cross_entropy_loss_amd import clip_gradients
+
+    plain = torch.ones(10, device="cuda")
+    sharded = Wrapped(torch.ones(10, device="cuda"))
+    for grads, out in (([sharded], None), ([plain, sharded], None), ([plain], [sharded]), ([sharded], [plain])):
+        with pytest.raises(ValueError, match="no memory of their own"):
+            clip_gradients(grads, 1.0, out=out)
+    assert (plain == 1).all() and (sharded.inner == 1).all()
