@@ -33,6 +33,9 @@ def _check(grads, out, max_norm, divisor):
         if g.numel() > 0 and not (g.data_ptr() and o.data_ptr()):
             raise ValueError("clip_gradients: tensors that have no memory of their own (sharded ones, wrappers of others) are not supported: "
                              "hand over what they hold here")
+    # (of dense tensors the library looks for shared memory; of others, two that begin with the same number are seen here)
+    if len({o.data_ptr() for o in out if o.numel() > 0}) != sum(o.numel() > 0 for o in out):
+        raise ValueError("clip_gradients: tensors that are written share memory")
     if isinstance(divisor, torch.Tensor):
         if divisor.dtype != torch.float32 or divisor.numel() != 1 or (grads and divisor.device != grads[0].device):
             raise ValueError("clip_gradients: divisor must be a number, or a float32 tensor with one on the gradients' device")

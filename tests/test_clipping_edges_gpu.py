@@ -53,3 +53,18 @@ def test_tensors_without_memory_of_their_own_are_refused():
         with pytest.raises(ValueError, match="no memory of their own"):
             clip_gradients(grads, 1.0, out=out)
     assert (plain == 1).all() and (sharded.inner == 1).all()
+
+
+def test_the_same_tensor_twice_is_refused():
+    from linear_cross_entropy_loss_amd import clip_gradients
+
+    a = torch.ones(20, 30, device="cuda")
+    for grads in ([a, a], [a, a[:, ::2]], [a[:, ::2], a[:, ::2]], [a[:, ::2], a[::2, ::2]]):
+        with pytest.raises(ValueError, match="share memory"):
+            clip_gradients(grads, 1.0)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_gradients([torch.ones_like(a), torch.ones_like(a)], 1.0, out=[a.t().t(), a])
+    assert (a == 1).all()
+    clip_gradients([a[:, ::2], a[:, 1::2]], 1.0)  # (side by side)
+    norm = math.sqrt(600.0)
+    assert ((a * norm - 1).abs() <= 2.0 ** -22).all()
