@@ -27,6 +27,8 @@ namespace {
 
 // The C ABI's functions, by the addresses that the loader of the library gives (bind).
 struct Abi {
+  decltype(&lce_strerror) strerror;
+  decltype(&lce_last_hip_error) last_hip_error;
   decltype(&lce_check_problem) check_problem;
   decltype(&lce_workspace_bytes) workspace_bytes;
   decltype(&lce_forward) forward;
@@ -57,6 +59,8 @@ struct Abi {
 
 template <class F> void bind_one(const py::dict& d, const char* name, F& f) { f = reinterpret_cast<F>(d[name].cast<uintptr_t>()); }
 void bind(const py::dict& d) {
+  bind_one(d, "lce_strerror", abi.strerror);
+  bind_one(d, "lce_last_hip_error", abi.last_hip_error);
   bind_one(d, "lce_check_problem", abi.check_problem);
   bind_one(d, "lce_workspace_bytes", abi.workspace_bytes);
   bind_one(d, "lce_forward", abi.forward);
@@ -560,7 +564,7 @@ struct TokenLogits : public torch::autograd::Function<TokenLogits> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x_in, const at::Tensor& At,
                                                 const at::Tensor& tokens, TokenCall* t) {
     run_tokens(x_in, At, tokens, *t);
-    TORCH_CHECK(t->rc == LCE_OK, "linear_token_logits: status ", t->rc);
+    TORCH_CHECK(t->rc == LCE_OK, "linear_token_logits");  // (differentiable_token_logits has the status)
     ctx->save_for_backward({t->x, t->w, t->labels, t->logits, t->lse, t->scales});
     const lce_problem& p = t->c.p;
     ctx->saved_data["layout"] = (int64_t)p.w_layout;
@@ -590,7 +594,8 @@ struct TokenLogits : public torch::autograd::Function<TokenLogits> {
                                              d["ignore_index"].toInt(), d["scale"].toDouble(), saved[5], d["n_chunk"].toInt(), (int)d["pack"].toInt(),
                                              ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                              reinterpret_cast<void*>((uintptr_t)d["stream"].toInt()), dx, dw, rc);
-    TORCH_CHECK(handled && rc == LCE_OK, "linear_token_logits: status ", rc);
+    TORCH_CHECK(handled, "linear_token_logits: upstream gradients or saved tensors that are no dense tensors of the forward's device and sizes");
+    TORCH_CHECK(rc == LCE_OK, "linear_token_logits: ", abi.strerror(rc), rc == LCE_EHIP ? ": " : "", rc == LCE_EHIP ? abi.last_hip_error() : "");
     if (dx.defined()) dx = dx.view(d["shape"].toIntVector());
     if (dw.defined() && layout == LCE_W_VH) dw = dw.t();
     torch::autograd::variable_list out = {dx, dw};
@@ -603,7 +608,7 @@ struct TokenLogits : public torch::autograd::Function<TokenLogits> {
   }
 };
 
-// linear_token_logits: (logits, lse); None: not handled.
+// linear_token_logits: (logits, lse); (status, name, None) where the C ABI refused; None: not handled.
 py::object differentiable_token_logits(const at::Tensor& x_in, const at::Tensor& At, const at::Tensor& tokens, int64_t ignore_index, double scale,
                                        int64_t n_chunk, int64_t vocab_start, int64_t vocab_size, int pack, bool copy_w, uintptr_t stream) {
   TokenCall t;
@@ -611,8 +616,13 @@ py::object differentiable_token_logits(const at::Tensor& x_in, const at::Tensor&
   torch::autograd::variable_list out;
   {
     py::gil_scoped_release release;
-    out = TokenLogits::apply(x_in, At, tokens, &t);
+    try {
+      out = TokenLogits::apply(x_in, At, tokens, &t);
+    } catch (const c10::Error&) {
+      if (t.rc == LCE_OK) throw;
+    }
   }
+  if (t.rc != LCE_OK) return py::make_tuple(t.rc, "linear_token_logits", py::none());
   return py::make_tuple(out[0], out[1]);
 }
 

@@ -230,6 +230,8 @@ def linear_token_logits(x, At, tokens, ignore_index: int = -100, logit_scale: fl
             _lib.F32_ZERO < logit_scale < _lib.F32_INF) and 0 <= vocab_start <= vocab_size - V:
         done = _lib.host().differentiable_token_logits(x, At, tokens, ignore_index, logit_scale, int(N_chunk_size), vocab_start, vocab_size,
                                                        ops._pack_mode(), "weight" in ops._copy_warned, _stream(x.device))
+        if done is not None and len(done) == 3:
+            _lib.raise_for_status(*done[:2])
         if done is not None:
             return done
     _check_inputs(x, At, tokens)

@@ -52,3 +52,29 @@ def test_objective_that_is_nan_on_padding():
     x.grad = module.weight.grad = None
     module.log_probs(x, tokens).backward(advantage)
     assert torch.equal(x.grad, want[0]) and torch.equal(module.weight.grad, want[1])
+
+
+def test_a_launch_that_fails_names_its_error():
+    """The library's own functions stand aside for two that return LCE_EHIP, as a failed launch does."""
+    from linear_cross_entropy_loss_amd import _lib, linear_token_logits
+
+    host, lib = _lib.host(), _lib.load()
+    table = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _lib.EXPORTS}
+    vp, i64, size = ctypes.c_void_p, ctypes.c_int64, ctypes.c_size_t
+    forward = ctypes.CFUNCTYPE(ctypes.c_int, vp, vp, vp, vp, i64, vp, vp, vp, vp, size, vp)(lambda *_: _lib.LCE_EHIP)
+    backward = ctypes.CFUNCTYPE(ctypes.c_int, *[vp] * 12, size, vp)(lambda *_: _lib.LCE_EHIP)
+    x, w, tokens, g_logits, g_lse = (t.cuda() for t in make(40, 64, 300, BF16, seed=9))
+    x.requires_grad_(True)
+    text = f"linear_token_logits: {lib.lce_strerror(_lib.LCE_EHIP).decode()}: "
+    out = linear_token_logits(x, w, tokens, IGNORE)
+    try:
+        host.bind({**table, "lce_token_logits": ctypes.cast(forward, vp).value, "lce_token_logits_backward": ctypes.cast(backward, vp).value})
+        with pytest.raises(RuntimeError) as failed:
+            linear_token_logits(x, w, tokens, IGNORE)
+        assert str(failed.value).startswith(text)
+        with pytest.raises(RuntimeError) as failed:
+            torch.autograd.grad(out, x, (g_logits, g_lse), retain_graph=True)
+        assert str(failed.value).startswith(text)
+    finally:
+        host.bind(table)
+    torch.autograd.grad(out, x, (g_logits, g_lse))
