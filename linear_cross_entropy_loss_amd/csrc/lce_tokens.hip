@@ -174,16 +174,19 @@ __global__ __launch_bounds__(kRowThreads) void pair_scales_kernel(const float* p
       int e = 0;
       if (m > 0.f) (void)frexpf(m, &e);
       e = 14 - e;  // the largest becomes 2^13 ... 2^14
-      exponent[of] = m > 0.f ? (e > 60 ? 60 : e) : 0;
+      exponent[of] = m > 0.f ? (e > 120 ? 120 : e) : 0;
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    pair[kPairX] = ldexpf(1.f, exponent[0]);
-    pair[kPairW] = ldexpf(1.f, exponent[1]);
-    pair[kPairLogits] = ldexpf(1.f, -exponent[0] - exponent[1]);
-    pair[kPairDx] = ldexpf(1.f, -exponent[1]);
-    pair[kPairDw] = ldexpf(1.f, -exponent[0]);
+    // (the logits' factor stays a number of float32 with all its bits, times any logit_scale above 2^-6)
+    const int more = exponent[0] + exponent[1] - 120;
+    const int ex = exponent[0] - (more > 0 ? (more + 1) / 2 : 0), ew = exponent[1] - (more > 0 ? more / 2 : 0);
+    pair[kPairX] = ldexpf(1.f, ex);
+    pair[kPairW] = ldexpf(1.f, ew);
+    pair[kPairLogits] = ldexpf(1.f, -ex - ew);
+    pair[kPairDx] = ldexpf(1.f, -ew);
+    pair[kPairDw] = ldexpf(1.f, -ex);
   }
 }
 

@@ -78,3 +78,90 @@ def test_a_launch_that_fails_names_its_error():
     finally:
         host.bind(table)
     torch.autograd.grad(out, x, (g_logits, g_lse))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+def test_slabs_of_other_types(dtype, packing):
+    from linear_cross_entropy_loss_amd import _lib
+    from linear_cross_entropy_loss_amd.token_logits import _problem
+
+    N, H, V, n_chunk = 3000, 256, 8192, 512
+    inputs = make(N, H, V, dtype, seed=3)
+    prob = _problem(inputs[0], inputs[1], _lib.W_HV, V, IGNORE, 1.0, n_chunk, 0)
+    # (less than a dz of all columns takes: there is more than one slab)
+    assert _lib.token_logits_workspace_bytes(prob, True) < N * V * dtype.itemsize
+    check(inputs, n_chunk=n_chunk, scale=0.7)
+
+
+@pytest.mark.parametrize("N, H, V", [(1, 64, 1000), (40, 64, 999), (130, 33, 515), (2100, 320, 20000)])
+def test_float32_tied_weight(N, H, V):
+    check(make(N, H, V, F32, seed=9), tied=True)
+    check(make(N, H, V, F32, seed=9, pieces=2), tied=True, first=V, size=2 * V)
+
+
+@pytest.mark.parametrize("rows", [(), (1,), (1, 1, 1), (5, 1)])
+def test_rows_of_any_shape(rows):
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    x, w, tokens, g_logits, g_lse = (t.cuda() for t in make(5, 72, 300, BF16, seed=2, drop=0.0))
+    n = math.prod(rows)
+    leaf = x[:n].reshape(*rows, 72).requires_grad_(True)
+    logits, lse = linear_token_logits(leaf, w, tokens[:n].view(rows))
+    assert logits.shape == lse.shape == torch.Size(rows)
+    (dx,) = torch.autograd.grad((logits, lse), leaf, (g_logits[:n].view(rows), g_lse[:n].view(rows)))
+    flat = x[:n].clone().requires_grad_(True)
+    out = linear_token_logits(flat, w, tokens[:n])
+    (want,) = torch.autograd.grad(out, flat, (g_logits[:n], g_lse[:n]))
+    assert torch.equal(logits.view(-1), out[0]) and torch.equal(lse.view(-1), out[1])
+    assert dx.shape == leaf.shape and torch.equal(dx.view(-1, 72), want)
+
+
+@pytest.mark.parametrize("size, w_size", [(2.0 ** -44, 2.0 ** 42), (2.0 ** -70, 2.0 ** 68), (2.0 ** -100, 2.0 ** 98), (2.0 ** 60, 2.0 ** -62),
+                                          (2.0 ** -60, 2.0 ** -20), (2.0 ** -20, 2.0 ** -60)])
+def test_float32_numbers_of_any_size(size, w_size):
+    """Pairs are off by 2^-23 of a number or, as the largest of a tensor is multiplied to at least 2^13 and the lower number of a pair is a
+    multiple of 2^-24, by 2^-38 of the largest: in each number of x, which a logit has |w| times over and dW |dz| times, and in each of w."""
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    N, H, V = 70, 136, 600
+    x, w, tokens, g_logits, g_lse = (t.cuda() for t in make(N, H, V, F32, seed=21))
+    x, w = (x * size).requires_grad_(True), (w * w_size).requires_grad_(True)
+    print(f"token_logits float32 x of {size} w of {w_size}", flush=True)
+    logits, lse = linear_token_logits(x, w, tokens, IGNORE)
+    dx, dw = torch.autograd.grad((logits, lse), (x, w), (g_logits, g_lse))
+    want, (mag, mag_dx, mag_dw, w_sum, x_sum) = oracle(x.detach(), w.detach(), tokens, g_logits, g_lse, 1.0, 0)
+    xd, wd = x.detach().double().abs(), w.detach().double().abs()
+    tol_z = ((H + 2) * 2.0 ** -24 + 2.0 ** -21) * mag + 2.0 ** -38 * (xd.max() * wd.sum(0).max() + wd.max() * xd.sum(1).max())
+    assert ((logits.double() - want[0]).abs() <= tol_z).all()
+    assert ((lse.double() - want[1]).abs() <= tol_z + 2.0 ** -18 * (1 + want[1].abs())).all()
+    live = tokens != IGNORE
+    up = float((g_logits.abs() + g_lse.abs())[live].max())
+    p_off = 2.0 ** -15 + 4 * float(tol_z.max())  # (of a softmax: exponent and lse each off by tol_z; e^2t - 1 <= 4 t for t below 1/2)
+    assert p_off < 2.0 ** -10
+    # (dz has steps of 2^-38 of the largest upstream gradients, rounded up to a power of two; magnitudes of all dz: at most 2 of them a row)
+    for g, r, m, terms, edge in ((dx, want[2], mag_dx, V, 2.0 ** -37 * up * w_sum[None, :] + 2.0 ** -38 * wd.max() * 2 * up),
+                                 (dw, want[3], mag_dw, N, 2.0 ** -37 * up * x_sum[:, None] + 2.0 ** -38 * xd.max() * 2 * up * live.sum())):
+        tol = (2.0 ** -21 + p_off + terms * 2.0 ** -24) * m + 2.0 ** -24 * r.abs() + edge
+        assert ((g.double() - r).abs() <= tol).all(), float(((g.double() - r).abs() / tol).max())
+
+
+def test_function_transforms_and_forward_mode_are_refused():
+    import torch.autograd.forward_ad as fwAD
+    from torch.func import grad, jvp, vmap
+
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    x, w, tokens, *_ = (t.cuda() for t in make(40, 64, 300, BF16, seed=9, drop=0.0))
+
+    def total(x):
+        logits, lse = linear_token_logits(x, w, tokens)
+        return (logits - lse).sum()
+
+    with pytest.raises(RuntimeError):
+        grad(total)(x)
+    with pytest.raises(RuntimeError):
+        jvp(total, (x,), (x,))
+    with pytest.raises(RuntimeError):
+        vmap(lambda x: linear_token_logits(x[None], w, tokens[:1])[0])(x)
+    with fwAD.dual_level(), pytest.raises(RuntimeError):
+        total(fwAD.make_dual(x, x))
