@@ -30,6 +30,8 @@ def _check(grads, out, max_norm, divisor):
             raise ValueError("clip_gradients: all tensors must be on the same device")
         if o.shape != g.shape or (o.dtype != g.dtype and o.dtype != torch.float32):
             raise ValueError(f"clip_gradients: a gradient of shape {tuple(g.shape)} and {g.dtype} cannot go to {tuple(o.shape)} and {o.dtype}")
+        if o.is_inference() and not torch.is_inference_mode_enabled():
+            raise RuntimeError("clip_gradients: tensors of inference mode cannot be changed outside it")
         if g.numel() > 0 and not (g.data_ptr() and o.data_ptr()):
             raise ValueError("clip_gradients: tensors that have no memory of their own (sharded ones, wrappers of others) are not supported: "
                              "hand over what they hold here")

@@ -18,6 +18,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/Allocator.h>
+#include <c10/core/InferenceMode.h>
 
 #include <vector>
 
@@ -701,6 +702,7 @@ py::object clip(const py::list& grads, const py::list& out, double max_norm, dou
     if (!THPVariable_Check(gh.ptr()) || !THPVariable_Check(oh.ptr())) return py::none();
     const at::Tensor &g = THPVariable_Unpack(gh.ptr()), &o = THPVariable_Unpack(oh.ptr());
     if (!plain(g) || !plain(o) || g.sizes() != o.sizes() || g.strides() != o.strides() || !g.is_non_overlapping_and_dense()) return py::none();
+    if (o.is_inference() && !c10::InferenceMode::is_enabled()) return py::none();
     if (i == 0) {
       device = g.device();
       options = g.options();

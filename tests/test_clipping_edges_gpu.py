@@ -68,3 +68,23 @@ def test_the_same_tensor_twice_is_refused():
     clip_gradients([a[:, ::2], a[:, 1::2]], 1.0)  # (side by side)
     norm = math.sqrt(600.0)
     assert ((a * norm - 1).abs() <= 2.0 ** -22).all()
+
+
+def test_tensors_of_inference_mode():
+    """Outside that mode torch refuses to change them; so does this, before anything is written."""
+    from linear_cross_entropy_loss_amd import clip_gradients
+
+    with torch.inference_mode():
+        given = torch.randn(5000, device="cuda")
+        dense, strided = given.clone(), given.clone().view(50, 100)[:, ::2]
+        want = [t.clone() for t in (dense, strided)]
+        for t, was in zip((dense, strided), want):
+            out = torch.empty_like(t)
+            assert float(clip_gradients(t, 1.0)) == float(clip_gradients(was, 1.0, out=out)) > 1
+            assert torch.equal(t, out)
+    kept = [t.clone() for t in (dense, strided)]
+    for t, was in zip((dense, strided), kept):
+        with pytest.raises(RuntimeError, match="inference"):
+            clip_gradients(t, 0.5)
+        assert torch.equal(t, was)
+        assert abs(float(clip_gradients(t, 0.5, out=torch.zeros(t.shape, device="cuda"))) - 1) <= 2.0 ** -20  # (only read)
