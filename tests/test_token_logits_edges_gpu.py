@@ -165,3 +165,36 @@ def test_function_transforms_and_forward_mode_are_refused():
         vmap(lambda x: linear_token_logits(x[None], w, tokens[:1])[0])(x)
     with fwAD.dual_level(), pytest.raises(RuntimeError):
         total(fwAD.make_dual(x, x))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("N, H, V", [(1, 200, 1000), (1, 64, 999), (16, 264, 3001), (64, 1000, 4097), (200, 2048, 5000)])
+def test_float32_weight_under_few_rows(N, H, V, tied, dtype):
+    check(make(N, H, V, dtype, seed=N, w_dtype=F32), tied=tied)
+
+
+def test_captured_backward_of_many_tiles():
+    """Packed rows and several slabs in a graph, replayed between eager steps of the same operator."""
+    from linear_cross_entropy_loss_amd import linear_token_logits
+
+    inputs = [t.cuda() for t in make(2100, 320, 20001, F32, seed=5, drop=0.4)]
+
+    def step(x, w, tokens, g_logits, g_lse):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        out = linear_token_logits(x, w, tokens, IGNORE, N_chunk_size=512)
+        return tuple(t.detach() for t in out) + torch.autograd.grad(out, (x, w), (g_logits, g_lse))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(*inputs)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*inputs)
+    for seed in range(3):
+        for t, fresh in zip(inputs, make(2100, 320, 20001, F32, seed=30 + seed, drop=0.3)):
+            t.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step(*inputs)))
