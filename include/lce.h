@@ -501,7 +501,7 @@ int lce_sample(const void* logits, int dtype, int64_t rows, int64_t cols, int64_
  * pieces' and the logit the sum of theirs.  By the kernels, in the scratch and with the arithmetic of lce_forward and of a
  * lce_backward that stages dz; an fp16 stage is scaled by the largest |grad_lse| + |grad_logits|.
  *
- *   p       as for those calls; monitoring, z_reg and phases are 0, route is not looked at
+ *   p       as for those calls; monitoring, z_reg and phases are 0, route is one that those calls take and has no effect
  *   y       N labels: a column; p->ignore_index: a row that is not computed, logit and lse 0, without gradients, whatever
  *           grad_logits and grad_lse hold there; `other`: a column of another piece, logit 0 and no gradient by it; any other
  *           number: logit NaN, no gradient by it.  lce_token_labels makes them.
@@ -536,7 +536,9 @@ int lce_token_logits_backward(const lce_problem* p, const void* x, const void* w
  * 1 <= rows, cols; the length of what gets one scale is at most LCE_INT8_DEPTH, the other at most 2^30.
  *
  * lce_int8_logits: out[n][v] = logit_scale * sx[n] * w_scales[v] * sum_h qx[n][h] * w[v][h] for v < V, with qx, sx of the rows of x,
- * which are quantised on the way: the sum in whole numbers, exact; the product with the scales in fp32, rounded once to out's type.
+ * which are quantised on the way: the sum in whole numbers, exact, then one fp32 number; (sum * (sx * logit_scale)) * w_scales in fp32; the
+ * result in out's type.  Off by at most 2^-21 of itself and half a step of that type, as long as the two products before the last
+ * are normal numbers of fp32 or zero.
  *   x       (N, H), any row stride, at any element boundary
  *   w       (V, H) as the calls above give it, ldw a multiple of 16; what lies behind the end of a row has no effect, and of the last row
  *           nothing is read past the 4 bytes that hold its last number

@@ -6,7 +6,7 @@
 // The contraction is that of the loss's logit kernels (lce_gemm3.h, lce_gemm_small.h) with v_mfma_i32_32x32x32_i8 in the place of the 16-bit
 // instruction: both take 16 bytes of K of each lane, so that an operand of 8-bit numbers is staged, swizzled and read as one of
 // half as many 16-bit numbers, in the same time for twice the K.  Sums are exact in 32 bits (127^2 * 2^17 < 2^31).
-// Bound by the matrix cores' power from some 500 rows on: 2048 rows of 4096 x 32000 in 220 us, 2.4 POP/s, the rate of a large library product of
+// Bound by the matrix cores' power from some 500 rows on: 2048 rows of 4096 x 32000 in 236 us, 2.3 POP/s, the rate of a large library product of
 // 8-bit numbers here (2.1 to 2.4), and less than twice that of 16-bit ones, whose K tiles take 1.2 us, not 1.9 (the clock is at 1.7 of 2.4 GHz
 // then, the matrix cores busy for 66 % of it).  256 rows of 4096 x 128256, where weight and matrix cores ask for as much, 155 us: 1.7 POP/s beside
 // 3.8 TB/s.  (A second set of registers for the weight's K tiles, two ahead, loses 5 %, the loads are not what it waits for; 128 x 128 tiles 186.)

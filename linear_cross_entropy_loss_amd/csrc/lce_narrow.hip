@@ -239,8 +239,10 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_narrow_kernel(const FwdArgs a
 // the streaming ones are columns from v0 on; dW: the other way round, the tokens' scalars in LDS.
 constexpr int kNoColumn = -0x7fffffff;
 // What an exponential is multiplied by: 1, the factor of z-regularisation, the sign of a row's own upstream gradient (BwdArgs::row_value,
-// with dz at the label; 1 + 2 z_reg lse is not used then).  8520 x 64 x 32768 with half of the rows dropped, forward and backward of given
-// tokens: 346 us, 591 where dz is staged; 1335 x 115 x 37248 171 and 156.
+// with dz at the label; 1 + 2 z_reg lse is not used then).  Forward and backward of given tokens in bf16, us, here / where dz is staged: 8520 x 64 x
+// 32768 with half of the rows dropped 322 / 540, 16384 x 128 x 8192 310 / 328, 4096 x 128 x 32768 233 / 261, 2000 x 128 x 37248 150 / 178; but
+// 1335 x 128 x 37248 155 / 138, 1335 x 115 163 / 148, 1024 x 128 x 50304 144 / 125.  The plan (plan_narrow) knows no such line: this form is taken
+// wherever it fits, 10 to 15 % late for some thousand rows and fewer at H near 128.
 enum RowGain { kNoGain, kRegGain, kOwnGain };
 // (label: kNoColumn where there is no column to look for)
 template <RowGain GAIN> LCE_DEV void narrow_scalars(const BwdArgs& a, int64_t rows, int64_t tok, float& nlse, float& gain, int& label) {

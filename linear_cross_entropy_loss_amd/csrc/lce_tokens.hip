@@ -12,12 +12,13 @@
 // fp16, and fp32 as fp16 pairs: a stage has 30 binary places below 1 while upstream gradients are of any size (1 / rows, times a loss
 // scale), so all are divided by one power of two, which the dx and dW kernels multiply in again after their fp32 sums.
 //
-// All of that is a few numbers a row: bound by launches, 3 to 5 us each.  The products around it run at the loss's rate: 12288 rows of 4096 x 128256
-// with their backward in 19.8 ms, 1.31 PFLOP/s of 8 N H V operations (a large library product here: 1.38).
+// All of that is a few numbers a row: bound by launches, 2 to 5 us each.  The products around it run at the loss's rate: 12288 rows of 2048 x 131072
+// with their backward in 19.5 ms, 1.35 PFLOP/s of 8 N H V operations, of 4096 x 128256 in 37.2 ms, 1.39 (a large library product here: 1.38).
 //
 // fp32 tensors: fp16 pairs (lce_gemm.h) instead of the loss's bf16 ones, for products 22 bits wide.  N=2048, H=1024, V=16384, errors of dx and
 // dW against fp64, relative to their norms: 3.4e-7, of bf16 pairs 4.4e-6 (a float32 library product and its softmax: 2.2e-6).  Their scales
-// cost one more pass over the weight and x (pair_max_kernel, 17 us of a forward and backward of 910; 930 where the backward has no scales).
+// cost one more pass over the weight and x (pair_max_kernel 20 us, pair_scales_kernel 5, of a forward and backward of 910; 930 where the backward
+// has no scales).
 #include "lce_gemm3.h"
 #include "lce_internal.h"
 

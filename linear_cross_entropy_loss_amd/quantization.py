@@ -156,8 +156,9 @@ def quantized_logits(x, weight: Quantized, logit_scale: float = 1.0, dtype: Opti
     """``logit_scale * x @ At`` (..., V) from the 8-bit copy of ``At`` that ``quantize_weight`` gives, the rows of ``x`` quantised alike.
 
     ``x``: hidden states (..., H), bfloat16, float16 or float32, any strides.  ``dtype``: of the result, any of these; that of x unless
-    given.  The sums of products are exact; they are multiplied by the scales in float32 and rounded once.  Rows and columns with a
-    NaN or an infinity give NaN.
+    given.  The sums of products are exact; made float32 and multiplied by the scales there, they are off by at most 2^-21 of themselves
+    (where x's scale times ``logit_scale``, and that times the sum, are normal numbers of float32) before they are rounded to ``dtype``.  Rows
+    and columns with a NaN or an infinity give NaN.
     """
     values, scales = weight
     if not torch.compiler.is_compiling() and x.is_cuda and x.device.index == torch._C._cuda_getDevice() and (
