@@ -217,8 +217,9 @@ def linear_token_logits(x, At, tokens, ignore_index: int = -100, logit_scale: fl
     A token that is none (negative or beyond the vocabulary, and not ``ignore_index``) has a NaN logit.  Arithmetic as of
     ``linear_cross_entropy``: 16-bit gradients come from a dz that was rounded to the type, float32 tensors are multiplied as
     pairs of float16 under one power of two for each of x, weight and dz, and hold 22 bits (``linear_cross_entropy``: pairs of
-    bfloat16, 16 bits) or 2^-39 of the largest element there (as long as that is at least 2^-106, and x's times the weight's at least
-    2^-92: below, steps grow beside the elements); float16's dz is held to 2^-38 of the largest row's upstream gradient.
+    bfloat16, 16 bits) or 2^-39 of the largest element there (as long as that is at least 2^-106, and the product of any two of x's, the
+    weight's and the upstream gradients' at least 2^-92: below, steps grow beside the elements); float16's dz is held to 2^-38 of the largest row's
+    upstream gradient.
     The gradients are not differentiable in their turn.
     """
     compiling = torch.compiler.is_compiling()
